@@ -345,6 +345,71 @@ tcaspmm_status tcaspmm_spmm_csr_noalloc(const int32_t *d_row_ptr, const int32_t 
                                         int64_t M, int64_t K, int64_t nnz, const void *dB, int64_t ldb, float *dC,
                                         int64_t ldc, int64_t N, tcaspmm_dtype dt, void *stream);
 
+/* ------------------------------------- dense operators around the product
+ * What a block around a fixed A trains and serves beside it: layer norm over the
+ * product's inputs or outputs, and low-rank adapters beside the product.  They
+ * take matrices in device memory of the current device, allocate nothing, launch
+ * on `stream` (capturable) and share no state, so calls may overlap on any
+ * streams and from any threads as long as no output or workspace of one is used
+ * by another.  Sums are fp32 and their order is fixed: results are
+ * bit-identical from run to run.  No counterpart in the reference. */
+
+/* Layer norm of the rows x cols matrix X: of each row (dim 1: a node's features,
+ * the layout of a graph product's C) or of each column (dim 0: a token's
+ * features, the layout of a pruned weight's B).  Per vector x of n elements:
+ *     mean = sum x / n,  rstd = 1 / sqrt(sum (x - mean)^2 / n + eps)
+ *     y = weight * (x - mean) * rstd + bias
+ * X has x_dt, Y is stored as y_dt, weight and bias (n elements each, NULL = 1 and
+ * 0) have p_dt.  mean and rstd: one fp32 per vector for the backward pass, or
+ * both NULL.  Y may be X itself (same ld and type).  TCASPMM_TF32 is fp32 here. */
+tcaspmm_status tcaspmm_layer_norm(const void *dX, int64_t ldx, tcaspmm_dtype x_dt, void *dY, int64_t ldy,
+                                  tcaspmm_dtype y_dt, const void *weight, const void *bias, tcaspmm_dtype p_dt,
+                                  float *mean, float *rstd, int64_t rows, int64_t cols, int dim, double eps,
+                                  void *stream);
+/* Bytes of device scratch tcaspmm_layer_norm_backward needs on the current device. */
+size_t tcaspmm_layer_norm_backward_workspace(int64_t rows, int64_t cols, int dim);
+/* Gradients: dX (x_dt), dweight = sum over vectors of dY * xhat and dbias = sum of
+ * dY (p_dt, n elements; written as zeros when there is no vector).  Any of the
+ * three may be NULL.  mean and rstd are the forward pass's; workspace is at least
+ * tcaspmm_layer_norm_backward_workspace bytes, 16-byte aligned. */
+tcaspmm_status tcaspmm_layer_norm_backward(const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt, const void *dX,
+                                           int64_t ldx, tcaspmm_dtype x_dt, const float *mean, const float *rstd,
+                                           const void *weight, tcaspmm_dtype p_dt, void *dDX, int64_t lddx,
+                                           void *dweight, void *dbias, int64_t rows, int64_t cols, int dim,
+                                           void *workspace, size_t workspace_bytes, void *stream);
+
+/* `count` low-rank adapters of rank R <= 256 for an M x K product: adapter a is
+ * scale[a] * up[a] * down[a] with down[a] R x K and up[a] M x R, row-major,
+ * contiguous, in dt.  Column t of X and C belongs to adapter index[t]; an index
+ * outside [0, count) means no adapter.  index holds index_bytes = 4 or 8 bytes
+ * per column, or is NULL (adapter 0 for every column); scale is one fp32 per
+ * adapter, or NULL (1). */
+typedef struct tcaspmm_adapters {
+    const void *down; /* count x R x K */
+    const void *up;   /* count x M x R */
+    const void *index;
+    const float *scale;
+    int64_t count, rank, M, K;
+    tcaspmm_dtype dt; /* of down, up and X */
+    int index_bytes;
+} tcaspmm_adapters;
+
+/* Y[:, t] = base[:, t] + scale[a] * up[a] * (down[a] * X[:, t]), a = index[t];
+ * Y = base where column t has no adapter.  X is K x N in dt; base (M x N, or NULL
+ * = 0: usually the C of an execute call) and Y are in y_dt, and Y may be base
+ * itself.  dH: the R x N fp32 intermediate scale * down * X (contiguous; zeros
+ * where there is no adapter) for the backward pass, or NULL. */
+tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *dX, int64_t ldx, int64_t N, const void *dBase,
+                            int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, float *dH, void *stream);
+/* Gradients from dY (dy_dt: fp32 or dt): dX = base + scale * down^T (up^T dY) in
+ * dt, with dBase an fp32 K x N matrix (usually A^T dY) or NULL; ddown and dup in
+ * dt, zeros for adapters without columns.  Any of the three may be NULL.  dH is
+ * the forward pass's (for dup); dP is R x N floats of scratch (for dX and ddown). */
+tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt,
+                                     const void *dX, int64_t ldx, int64_t N, const float *dH, const float *dBase,
+                                     int64_t ldbase, void *dDX, int64_t lddx, void *ddown, void *dup, float *dP,
+                                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -594,3 +594,6 @@ def cublas_gemm(A_dense, B, Cout, dt, warmup: int = 5, iters: int = 10, stream=N
     _check(baselines().tcaspmm_cublas_gemm(_ptr(A_dense), _ptr(B), _ptr(Cout), M, N, K, int(as_dtype(dt)), warmup,
                                            iters, _stream_handle(stream), C.byref(ms)))
     return ms.value
+
+
+from .dense import layer_norm, layer_norm_backward, lora, lora_backward  # noqa: E402,F401

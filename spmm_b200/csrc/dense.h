@@ -1,0 +1,60 @@
+// Shared by the dense operators around a sparse product (norm.cu, lora.cu): element access by type, argument checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "internal.h"
+
+namespace tca {
+
+tcaspmm_status cuda_fail(cudaError_t e, const char *what);
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Element i of an array whose type is known at run time (0 fp32, 1 fp16, 2 bf16): the same branch for every thread.
+// 16-bit elements are loaded as integers: the header's own __ldg of a 16-bit float is an assembly statement without side
+// effects, which the compiler may execute ahead of the branch that guards it (seen as a read through a NULL weight).
+__device__ __forceinline__ float load_as(const void *p, int type, long long i)
+{
+    if (type == 0) return __ldg((const float *)p + i);
+    if (type == 1) return __half2float(__ushort_as_half(__ldg((const unsigned short *)p + i)));
+    return __bfloat162float(__ushort_as_bfloat16(__ldg((const unsigned short *)p + i)));
+}
+__device__ __forceinline__ void store_as(void *p, int type, long long i, float v)
+{
+    if (type == 0)
+        ((float *)p)[i] = v;
+    else if (type == 1)
+        ((__half *)p)[i] = __float2half_rn(v);
+    else
+        ((__nv_bfloat16 *)p)[i] = __float2bfloat16_rn(v);
+}
+
+// Type code of the kernels; TF32 is fp32 storage.
+inline int type_code(tcaspmm_dtype dt) { return dt == TCASPMM_F16 ? 1 : dt == TCASPMM_BF16 ? 2 : 0; }
+
+// Calls f(T{}) with the element type of code 0, 1 or 2.
+template <typename F>
+inline tcaspmm_status with_type(int code, F &&f)
+{
+    if (code == 0) return f(float{});
+    if (code == 1) return f(__half{});
+    return f(__nv_bfloat16{});
+}
+
+// A matrix argument: an inner extent of `cols`, a leading dimension of `ld`, and a pointer unless it is empty.
+inline bool matrix_ok(const void *p, int64_t rows, int64_t cols, int64_t ld)
+{
+    return ld >= cols && (p != nullptr || rows == 0 || cols == 0);
+}
+
+}  // namespace tca

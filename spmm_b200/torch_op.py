@@ -15,17 +15,25 @@ are treated as constants (the graph does not train).
     Y = torch.ops.tcaspmm.spmm_fused(crow, col, val, X, row_scale, bias, relu, out_dtype)
 
 applies the plan's fused epilogue (row scale, bias, ReLU, fp32/fp16/bf16 output) in
-the same kernels; its backward gives dX (through A^T) and d(bias).  There is no CPU or
+the same kernels; its backward gives dX (through A^T) and d(bias).
+
+    Y = torch_op.spmm_lora(crow, col, val, X, down, up, index, scale)
+    Y = torch_op.lora(X, down, up, index, scale, base)
+    Y = torch_op.layer_norm(X, weight, bias, eps, dim, out_dtype)
+
+are what trains around a fixed A: low-rank adapters beside the product, chosen per column
+of X, and layer norm of rows or columns (``torch.ops.tcaspmm.spmm_lora``, ``lora`` and
+``layer_norm`` also return what their backward passes read).  There is no CPU or
 PyTorch fallback: without the library or a CUDA device the ops raise.
 """
 from __future__ import annotations
 
-from typing import Dict, Optional, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
 
-from . import CSR, Epilogue, Plan, as_dtype
+from . import CSR, Epilogue, Plan, as_dtype, dense
 
 
 class _Entry:
@@ -198,13 +206,241 @@ def _backward_fused(ctx, grad):
 spmm_fused.register_autograd(_backward_fused, setup_context=_setup_fused)
 
 
+# ------------------------------------------- layer norm and low-rank adapters
+def _needed(t: torch.Tensor, wanted: bool) -> Optional[torch.Tensor]:
+    return t if wanted else None
+
+
+@torch.library.custom_op("tcaspmm::layer_norm", mutates_args=())
+def _layer_norm(X: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float, dim: int,
+                out_dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return dense.layer_norm(X, weight, bias, eps, dim, out_dtype, stats=True)
+
+
+@_layer_norm.register_fake
+def _(X, weight, bias, eps, dim, out_dtype):
+    vecs = X.new_empty(X.shape[1 - dim % 2], dtype=torch.float32)
+    return torch.empty(X.shape, dtype=out_dtype, device=X.device), vecs, torch.empty_like(vecs)
+
+
+@torch.library.custom_op("tcaspmm::layer_norm_backward", mutates_args=())
+def _layer_norm_backward(dY: torch.Tensor, X: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                         weight: Optional[torch.Tensor], dim: int, needed: List[bool],
+                         param_dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dX, dweight, dbias); an empty tensor for what is not needed."""
+    got = dense.layer_norm_backward(dY, X, mean, rstd, weight, dim, need_input=needed[0], need_weight=needed[1],
+                                    need_bias=needed[2], param_dtype=param_dtype)
+    return tuple(X.new_empty(0) if t is None else t for t in got)
+
+
+@_layer_norm_backward.register_fake
+def _(dY, X, mean, rstd, weight, dim, needed, param_dtype):
+    p = torch.empty(X.shape[dim], dtype=param_dtype, device=X.device)
+    return tuple(t if n else X.new_empty(0)
+                 for t, n in zip((torch.empty(X.shape, dtype=X.dtype, device=X.device), p, torch.empty_like(p)), needed))
+
+
+def _setup_norm(ctx, inputs, output):
+    X, weight, bias, _, dim, _ = inputs
+    _, mean, rstd = output
+    ctx.mark_non_differentiable(mean, rstd)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(X, weight, mean, rstd)
+    ctx.dim = dim
+    p = weight if weight is not None else bias
+    ctx.param_dtype = p.dtype if p is not None else torch.float32
+
+
+def _backward_norm(ctx, dY, *_):
+    if dY is None:
+        return (None,) * 6
+    X, weight, mean, rstd = ctx.saved_tensors
+    needed = [bool(n) for n in ctx.needs_input_grad[:3]]
+    got = torch.ops.tcaspmm.layer_norm_backward(dY, X, mean, rstd, weight, ctx.dim, needed, ctx.param_dtype)
+    return (*(_needed(t, n) for t, n in zip(got, needed)), None, None, None)
+
+
+_layer_norm.register_autograd(_backward_norm, setup_context=_setup_norm)
+
+
+def layer_norm(X: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, dim: int = 1, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """spmm_b200.layer_norm with gradients for X, weight and bias: the norm of each row (dim=1, a node's features) or
+    each column (dim=0, a token's features) of X, stored as out_dtype (default: X's type)."""
+    return torch.ops.tcaspmm.layer_norm(X, weight, bias, eps, dim, X.dtype if out_dtype is None else out_dtype)[0]
+
+
+def _lora_grads(ctx, dY, base, needed):
+    """(dX, ddown, dup) of the adapters from what the forward pass saved."""
+    X, down, up, index, scale, H = ctx.saved_tensors[-6:]
+    if dY.dtype not in (torch.float32, X.dtype):
+        dY = dY.float()
+    got = torch.ops.tcaspmm.lora_backward(dY, X, down, up, H, index, scale, base, needed)
+    return tuple(_needed(t, n) for t, n in zip(got, needed))
+
+
+def _refuse_scale(ctx, at: int) -> None:
+    if ctx.needs_input_grad[at]:
+        raise ValueError("the adapters' scale is a constant: it has no gradient")
+
+
+@torch.library.custom_op("tcaspmm::lora", mutates_args=())
+def _lora(X: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: Optional[torch.Tensor],
+          scale: Optional[torch.Tensor], base: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    return dense.lora(X, down, up, index, scale, base, hidden=True)
+
+
+@_lora.register_fake
+def _(X, down, up, index, scale, base):
+    shape = (up.shape[1], X.shape[1])
+    return (torch.empty(shape, dtype=torch.float32 if base is None else base.dtype, device=X.device),
+            torch.empty((down.shape[1], X.shape[1]), dtype=torch.float32, device=X.device))
+
+
+@torch.library.custom_op("tcaspmm::lora_backward", mutates_args=())
+def _lora_backward(dY: torch.Tensor, X: torch.Tensor, down: torch.Tensor, up: torch.Tensor, H: torch.Tensor,
+                   index: Optional[torch.Tensor], scale: Optional[torch.Tensor], base: Optional[torch.Tensor],
+                   needed: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dX (+ base), ddown, dup); an empty tensor for what is not needed."""
+    got = dense.lora_backward(dY, X, down, up, H, index, scale, base, need_input=needed[0], need_down=needed[1],
+                              need_up=needed[2])
+    return tuple(X.new_empty(0) if t is None else t for t in got)
+
+
+@_lora_backward.register_fake
+def _(dY, X, down, up, H, index, scale, base, needed):
+    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else X.new_empty(0)
+                 for t, n in zip((X, down, up), needed))
+
+
+def _setup_lora(ctx, inputs, output):
+    X, down, up, index, scale, base = inputs
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(X, down, up, index, scale, output[1])
+
+
+def _backward_lora(ctx, dY, *_):
+    _refuse_scale(ctx, 4)
+    if dY is None:
+        return (None,) * 6
+    needed = [bool(n) for n in ctx.needs_input_grad[:3]]
+    grads = _lora_grads(ctx, dY, None, needed) if any(needed) else (None, None, None)
+    return (*grads, None, None, dY if ctx.needs_input_grad[5] else None)
+
+
+_lora.register_autograd(_backward_lora, setup_context=_setup_lora)
+
+
+def lora(X: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: Optional[torch.Tensor] = None,
+         scale: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """spmm_b200.lora with gradients for X, down, up and base: base + scale[a] * up[a] @ (down[a] @ X[:, t]) for every
+    column t, a = index[t] (None = adapter 0, outside [0, L) = no adapter)."""
+    return torch.ops.tcaspmm.lora(X, down, up, index, scale, base)[0]
+
+
+@torch.library.custom_op("tcaspmm::spmm_lora", mutates_args=())
+def _spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torch.Tensor, down: torch.Tensor,
+               up: torch.Tensor, index: Optional[torch.Tensor],
+               scale: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(A @ X with each column's adapter beside it, the adapters' H): the plan's product, then the adapters in place."""
+    M = crow.shape[0] - 1
+    if tuple(up.shape[1:2]) != (M,):
+        raise ValueError(f"up must have shape (L, {M}, R), not {tuple(up.shape)}")
+    Y = spmm(crow, col, val, X)
+    return dense.lora(X, down, up, index, scale, Y, out=Y, hidden=True)
+
+
+@_spmm_lora.register_fake
+def _(crow, col, val, X, down, up, index, scale):
+    return (X.new_empty((crow.shape[0] - 1, X.shape[1]), dtype=torch.float32),
+            X.new_empty((down.shape[1], X.shape[1]), dtype=torch.float32))
+
+
+def _setup_spmm_lora(ctx, inputs, output):
+    crow, col, val, X, down, up, index, scale = inputs
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(crow, col, val, X, down, up, index, scale, output[1])
+
+
+def _backward_spmm_lora(ctx, dY, *_):
+    _refuse_scale(ctx, 7)
+    if dY is None:
+        return (None,) * 8
+    crow, col, val, X = ctx.saved_tensors[:4]
+    needed = [bool(n) for n in ctx.needs_input_grad[3:6]]
+    base = torch.ops.tcaspmm.spmm_t(crow, col, val, dY.to(X.dtype), X.shape[0]) if needed[0] else None
+    grads = _lora_grads(ctx, dY, base, needed) if any(needed) else (None, None, None)
+    return (None, None, None, *grads, None, None)
+
+
+_spmm_lora.register_autograd(_backward_spmm_lora, setup_context=_setup_spmm_lora)
+
+
+def spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torch.Tensor, down: torch.Tensor,
+              up: torch.Tensor, index: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A @ X + each column's low-rank adapter, fp32: a frozen pruned weight with the adapters that train (or serve)
+    beside it.  Gradients for X, down and up."""
+    return torch.ops.tcaspmm.spmm_lora(crow, col, val, X, down, up, index, scale)[0]
+
+
+class LayerNorm(torch.nn.Module):
+    """Layer norm over `features` elements of each row (dim=1) or each column (dim=0) of a matrix."""
+
+    def __init__(self, features: int, dim: int = 1, eps: float = 1e-5, affine: bool = True, bias: bool = True,
+                 out_dtype: Optional[torch.dtype] = None, device=None, dtype: torch.dtype = torch.float32):
+        super().__init__()
+        self.features, self.dim, self.eps, self.out_dtype = features, dim, eps, out_dtype
+        self.weight = torch.nn.Parameter(torch.ones(features, device=device, dtype=dtype)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(features, device=device, dtype=dtype)) if affine and bias else None
+
+    def forward(self, X: torch.Tensor) -> torch.Tensor:
+        if X.dim() == 2 and X.shape[self.dim] != self.features:
+            raise ValueError(f"X must have {self.features} elements along dim {self.dim}, not {X.shape[self.dim]}")
+        return layer_norm(X, self.weight, self.bias, self.eps, self.dim, self.out_dtype)
+
+
+class LowRankAdapters(torch.nn.Module):
+    """`count` adapters of one rank beside an M x K product: down starts at N(0, 1/K), up at zero, so that every adapter
+    starts as no change; each is scaled by alpha / rank."""
+
+    def __init__(self, count: int, rank: int, M: int, K: int, alpha: Optional[float] = None, device=None,
+                 dtype: torch.dtype = torch.float32):
+        super().__init__()
+        self.down = torch.nn.Parameter(torch.randn(count, rank, K, device=device).div_(max(K, 1) ** 0.5).to(dtype))
+        self.up = torch.nn.Parameter(torch.zeros(count, M, rank, device=device, dtype=dtype))
+        s = 1.0 if alpha is None else alpha / rank
+        self.register_buffer("scale", torch.full((count,), s, device=device, dtype=torch.float32))
+
+    def forward(self, X: torch.Tensor, base: Optional[torch.Tensor] = None,
+                index: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return lora(X, self.down, self.up, index, self.scale, base)
+
+
+class AdaptedProduct(torch.nn.Module):
+    """Y = A @ X + each column's adapter: a frozen sparse weight A in CSR with the adapters beside it."""
+
+    def __init__(self, crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, adapters: LowRankAdapters):
+        super().__init__()
+        self.register_buffer("crow", crow)
+        self.register_buffer("col", col)
+        self.register_buffer("val", val)
+        self.adapters = adapters
+
+    def forward(self, X: torch.Tensor, index: Optional[torch.Tensor] = None) -> torch.Tensor:
+        a = self.adapters
+        return spmm_lora(self.crow, self.col, self.val, X, a.down, a.up, index, a.scale)
+
+
 class GCNAggregate(torch.nn.Module):
     """Y = relu?(row_scale * (A_hat @ X) + bias) with a fixed adjacency A_hat in CSR (the GCN /
-    GraphSAGE-mean propagation step); without row_scale, bias or relu it is plain A_hat @ X."""
+    GraphSAGE-mean propagation step); without row_scale, bias or relu it is plain A_hat @ X.  With a
+    norm (LayerNorm over the features), Y = relu?(norm(row_scale * (A_hat @ X) + bias))."""
 
     def __init__(self, crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor,
                  row_scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
-                 relu: bool = False):
+                 relu: bool = False, norm: Optional[LayerNorm] = None):
         super().__init__()
         self.register_buffer("crow", crow)
         self.register_buffer("col", col)
@@ -212,9 +448,16 @@ class GCNAggregate(torch.nn.Module):
         self.register_buffer("row_scale", row_scale)
         self.bias = bias
         self.relu = relu
+        self.norm = norm
 
     def forward(self, X: torch.Tensor) -> torch.Tensor:
-        if self.row_scale is None and self.bias is None and not self.relu:
+        if self.norm is not None:
+            Y = self.norm(self._aggregate(X, False))
+            return torch.relu(Y) if self.relu else Y
+        return self._aggregate(X, self.relu)
+
+    def _aggregate(self, X: torch.Tensor, relu: bool) -> torch.Tensor:
+        if self.row_scale is None and self.bias is None and not relu:
             return torch.ops.tcaspmm.spmm(self.crow, self.col, self.val, X)
         return torch.ops.tcaspmm.spmm_fused(self.crow, self.col, self.val, X, self.row_scale, self.bias,
-                                            self.relu, torch.float32)
+                                            relu, torch.float32)
