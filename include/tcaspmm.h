@@ -361,7 +361,7 @@ tcaspmm_status tcaspmm_spmm_csr_noalloc(const int32_t *d_row_ptr, const int32_t 
  *     y = weight * (x - mean) * rstd + bias
  * X has x_dt, Y is stored as y_dt, weight and bias (n elements each, NULL = 1 and
  * 0) have p_dt.  mean and rstd: one fp32 per vector for the backward pass, or
- * both NULL.  Y may be X itself (same ld and type).  TCASPMM_TF32 is fp32 here. */
+ * both NULL.  TCASPMM_TF32 is fp32 here. */
 tcaspmm_status tcaspmm_layer_norm(const void *dX, int64_t ldx, tcaspmm_dtype x_dt, void *dY, int64_t ldy,
                                   tcaspmm_dtype y_dt, const void *weight, const void *bias, tcaspmm_dtype p_dt,
                                   float *mean, float *rstd, int64_t rows, int64_t cols, int dim, double eps,

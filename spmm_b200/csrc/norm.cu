@@ -1,63 +1,212 @@
-// Layer norm, forward and backward, over the rows' elements (dim 1: a node's features, the layout of a graph product's C)
-// or the columns' (dim 0: a token's features, the layout of a pruned weight's B).
-//
-//   mean = sum x / n    rstd = 1 / sqrt(sum (x - mean)^2 / n + eps)    xh = (x - mean) rstd    y = w xh + b
-//   g = w dy            dx = rstd (g - mean(g) - xh mean(g xh))        dw = sum dy xh          db = sum dy
-#include <algorithm>
-#include <climits>
+// Layer norm: the forward kernels, the join of the weight gradient's parts and the C entries.
 #include <cmath>
+#include <mutex>
 
-#include "dense.h"
+#include "norm.cuh"
 
 namespace tca {
-namespace {
 
-struct NormParams {
-    const void *X;
-    long long ldx;
-    void *Y;
-    long long ldy;
-    int yt;
-    const void *w, *b;  // one per feature, type pt, or NULL
-    int pt;
-    float *mean, *rstd;  // one per vector, or NULL
-    long long vecs, n;   // vectors normalised, their length
-    float eps;
-};
+tcaspmm_status norm_backward_f32(const NormGradParams &p, int dim, long long *parts, cudaStream_t st);
+tcaspmm_status norm_backward_f16(const NormGradParams &p, int dim, long long *parts, cudaStream_t st);
+tcaspmm_status norm_backward_bf16(const NormGradParams &p, int dim, long long *parts, cudaStream_t st);
 
-struct NormGradParams {
-    const void *dY;
-    long long lddy;
-    int dyt;
-    const void *X;
-    long long ldx;
-    const float *mean, *rstd;
-    const void *w;
-    int pt;
-    void *dX;
-    long long lddx;
-    void *dw, *db;  // type pt (fp32 without a weight), or NULL
-    long long vecs, n;
-};
-
-// Sum over the block's threads, the same in all of them.  `s` holds a float per warp.
-__device__ float block_sum(float v, float *s)
+// SMs of the current device, 148 when it cannot be asked.
+int sm_count()
 {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    const int warps = blockDim.x >> 5;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.0f;
-    for (int i = 0; i < warps; ++i) t += s[i];
-    return t;
+    static std::mutex mu;
+    static int known[64] = {};
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!known[dev] && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev] = n;
+    return known[dev] ? known[dev] : 148;
 }
 
-// One block per vector; element i of vector v lies at v * sv + i * si.
-template <typename T>
-__global__ void __launch_bounds__(256) norm_fwd(const NormParams p, long long sv, long long si, long long yv, long long yi)
+namespace {
+
+// A row's elements are dealt to its threads VEC at a time, NCH times; a thread's elements are the same in every row.
+template <typename T, int VEC, int NCH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_rows_fwd(const NormParams p, int lanes)
 {
-    __shared__ float s[8];
+    constexpr bool KEEP = VEC * NCH <= 8;  // weights stay in registers
+    __shared__ float s[2][1][32];
+    const int tpr = BLOCK ? (int)blockDim.x : lanes;
+    const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
+    const int per = BLOCK ? 1 : (int)blockDim.x / lanes;
+    const long long first = (long long)blockIdx.x * per + (BLOCK ? 0 : (int)threadIdx.x / lanes);
+    const long long step = (long long)gridDim.x * per;
+    const float inv = 1.0f / (float)p.n;
+    float w[KEEP ? VEC * NCH : 1], b[KEEP ? VEC * NCH : 1];
+    if (KEEP) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long long i = ((long long)c * tpr + t) * VEC;
+            if (i < p.n) {
+                load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, w + c * VEC);
+                load_params<VEC>(p.b, p.pt, p.pvec, i, 0.0f, b + c * VEC);
+            }
+        }
+    }
+    Pack<T, VEC> x[NCH], next[NCH];
+    auto fetch = [&](long long row, Pack<T, VEC> (&to)[NCH]) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long long i = ((long long)c * tpr + t) * VEC;
+            if (row < p.vecs && i < p.n)
+                to[c].load((const T *)p.X + row * p.ldx + i);
+            else
+                to[c].zero();
+        }
+    };
+    fetch(first, x);
+    // Every thread of a warp (block) takes the same number of turns: rows past the end are read as zeros and not written.
+    const long long turns = (p.vecs - (long long)blockIdx.x * per + step - 1) / step;
+    for (long long k = 0; k < turns; ++k) {
+        const long long row = first + k * step;
+        fetch(row + step, next);
+        float a[1] = {0.0f};
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[0] += x[c].get(e);
+        row_sum<BLOCK>(a, lanes, s[0]);
+        const float mean = a[0] * inv;
+        a[0] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+            if (((long long)c * tpr + t) * VEC < p.n) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float d = x[c].get(e) - mean;
+                    a[0] += d * d;
+                }
+            }
+        row_sum<BLOCK>(a, lanes, s[1]);
+        const float rstd = 1.0f / sqrtf(a[0] * inv + p.eps);
+        if (row < p.vecs) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const long long i = ((long long)c * tpr + t) * VEC;
+                if (i < p.n) {
+                    float y[VEC], ww[VEC], bb[VEC];
+                    if (!KEEP) {
+                        load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
+                        load_params<VEC>(p.b, p.pt, p.pvec, i, 0.0f, bb);
+                    }
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        y[e] = (x[c].get(e) - mean) * rstd * (KEEP ? w[c * VEC + e] : ww[e]) + (KEEP ? b[c * VEC + e] : bb[e]);
+                    store_vec<VEC>(p.Y, p.yt, row * p.ldy + i, y);
+                }
+            }
+            if (t == 0 && p.mean) {
+                p.mean[row] = mean;
+                p.rstd[row] = rstd;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) x[c] = next[c];
+    }
+}
+
+template <typename T, int VEC, int NCH>
+__global__ void __launch_bounds__(STRIP_THREADS) norm_cols_fwd(const NormParams p, const Strip q)
+{
+    __shared__ float s[1][STRIP_WARPS][STRIP_MAX];
+    __shared__ float sums[2][STRIP_MAX];  // this block's sum of x, then of squared differences from its own mean
+    __shared__ float fin[2][STRIP_MAX];   // the strip's mean and rstd
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int width = q.lpr * VEC, at = (threadIdx.x & (q.lpr - 1)) * VEC;
+    const long long col = (long long)(blockIdx.x / ranks) * width + at;
+    const long long r0 = min(p.n, rank * q.per_block), r1 = min(p.n, r0 + q.per_block);
+    const int lane_row = threadIdx.x >> q.shift, rows = STRIP_THREADS >> q.shift;
+    Pack<T, VEC> x[NCH];
+    float v[1][VEC] = {};
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long long r = r0 + lane_row + c * rows;
+        if (r < r1 && col < p.vecs)
+            x[c].load((const T *)p.X + r * p.ldx + col);
+        else
+            x[c].zero();
+    }
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[0][e] += x[c].get(e);
+    strip_sum(v, q.lpr, s, sums);
+    const float inv = r1 > r0 ? 1.0f / (float)(r1 - r0) : 0.0f;
+    float m[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        m[e] = sums[0][at + e] * inv;
+        v[0][e] = 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+        if (r0 + lane_row + c * rows < r1) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = x[c].get(e) - m[e];
+                v[0][e] += d * d;
+            }
+        }
+    strip_sum(v, q.lpr, s, sums + 1);
+    cluster.sync();
+    // Blocks' sums joined: sum (x - mean)^2 = sum over blocks of its own about its mean + rows (its mean - mean)^2.
+    if ((int)threadIdx.x < width) {
+        const int j = threadIdx.x;
+        float total = 0.0f, sq = 0.0f;
+        for (int k = 0; k < ranks; ++k) total += cluster.map_shared_rank(&sums[0][0], k)[j];
+        const float mean = total / (float)p.n;
+        for (int k = 0; k < ranks; ++k) {
+            const float *o = cluster.map_shared_rank(&sums[0][0], k);
+            const long long cnt = min(p.n, (k + 1) * q.per_block) - min(p.n, k * q.per_block);
+            if (cnt > 0) {
+                const float d = o[j] * (1.0f / (float)cnt) - mean;
+                sq += o[STRIP_MAX + j] + (float)cnt * d * d;
+            }
+        }
+        fin[0][j] = mean;
+        fin[1][j] = 1.0f / sqrtf(sq / (float)p.n + p.eps);
+    }
+    __syncthreads();
+    float mean[VEC], rstd[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        mean[e] = fin[0][at + e];
+        rstd[e] = fin[1][at + e];
+    }
+    if (col < p.vecs) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long long r = r0 + lane_row + c * rows;
+            if (r < r1) {
+                const float w = p.w ? load_as(p.w, p.pt, r) : 1.0f, b = p.b ? load_as(p.b, p.pt, r) : 0.0f;
+                float y[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) y[e] = (x[c].get(e) - mean[e]) * rstd[e] * w + b;
+                store_vec<VEC>(p.Y, p.yt, r * p.ldy + col, y);
+            }
+        }
+        if (p.mean && rank == 0 && lane_row == 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                p.mean[col + e] = mean[e];
+                p.rstd[col + e] = rstd[e];
+            }
+        }
+    }
+    cluster.sync();  // a block's sums are read by the others until here
+}
+
+// One block per vector, read three times: for vectors too long for the registers of a block (rows) or a cluster (columns).
+// Element i of vector v lies at v * sv + i * si.
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_long_fwd(const NormParams p, long long sv, long long si, long long yv, long long yi)
+{
+    __shared__ float s[32];
     for (long long v = blockIdx.x; v < p.vecs; v += gridDim.x) {
         const T *x = (const T *)p.X + v * sv;
         float a = 0.0f;
@@ -81,57 +230,54 @@ __global__ void __launch_bounds__(256) norm_fwd(const NormParams p, long long sv
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) norm_bwd(const NormGradParams p, long long sv, long long si, long long gv, long long gi,
-                                                long long dv, long long di)
+// dw (y = 0) and db (y = 1): the parts of each feature added in a fixed order, 32 features a block.
+__global__ void __launch_bounds__(1024) norm_join(const float *part, long long parts, long long n, void *dw, void *db, int type)
 {
-    __shared__ float s[8];
-    for (long long v = blockIdx.x; v < p.vecs; v += gridDim.x) {
-        const T *x = (const T *)p.X + v * sv;
-        const float mean = p.mean[v], rstd = p.rstd[v];
-        float a = 0.0f, c = 0.0f;
-        for (long long i = threadIdx.x; i < p.n; i += blockDim.x) {
-            const float g = load_as(p.dY, p.dyt, v * gv + i * gi) * (p.w ? load_as(p.w, p.pt, i) : 1.0f);
-            a += g;
-            c += g * ((to_float(x[i * si]) - mean) * rstd);
-        }
-        a = block_sum(a, s) / (float)p.n;
-        c = block_sum(c, s) / (float)p.n;
-        for (long long i = threadIdx.x; i < p.n; i += blockDim.x) {
-            const float g = load_as(p.dY, p.dyt, v * gv + i * gi) * (p.w ? load_as(p.w, p.pt, i) : 1.0f);
-            const float xh = (to_float(x[i * si]) - mean) * rstd;
-            ((T *)p.dX)[v * dv + i * di] = from_float<T>(rstd * (g - a - xh * c));
-        }
-    }
+    __shared__ float s[32][33];
+    void *out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const long long i = (long long)blockIdx.x * 32 + x;
+    float a = 0.0f;
+    if (i < n)
+        for (long long k = y; k < parts; k += 32) a += part[(blockIdx.y * parts + k) * n + i];
+    s[y][x] = a;
+    __syncthreads();
+    a = s[x][y];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+    const long long j = (long long)blockIdx.x * 32 + y;
+    if (x == 0 && j < n) store_as(out, type, j, a);
 }
 
-// One block per feature: its weight's and bias's gradients over all vectors.
-template <typename T>
-__global__ void __launch_bounds__(256) norm_wgrad(const NormGradParams p, long long sv, long long si, long long gv, long long gi)
+template <typename T, int VEC>
+tcaspmm_status forward(const NormParams &p, int dim, cudaStream_t st)
 {
-    __shared__ float s[8];
-    for (long long i = blockIdx.x; i < p.n; i += gridDim.x) {
-        float a = 0.0f, c = 0.0f;
-        for (long long v = threadIdx.x; v < p.vecs; v += blockDim.x) {
-            const float dy = load_as(p.dY, p.dyt, v * gv + i * gi);
-            a += dy * ((to_float(((const T *)p.X)[v * sv + i * si]) - p.mean[v]) * p.rstd[v]);
-            c += dy;
+    if (dim == 1) {
+        const RowPlan r = plan_rows(p.n, VEC, FWD_MOST, 1024);
+        if (r.nch) {
+            const long long per = r.lanes ? 256 / r.lanes : 1;
+            // Blocks an SM holds: at most 64 registers a thread up to 8 elements (2048 threads at 1), 128 above.
+            const long long fit = !r.lanes ? std::max(1, 1024 / r.threads) : r.nch * VEC > 8 ? 2 : r.nch * VEC > 4 ? 4 : 8;
+            const unsigned grid = blocks_of(std::min(ceil_div(p.vecs, per), fit * sm_count()));
+            return with_chunks<FWD_MOST / VEC>(r.nch, [&](auto nch) {
+                if (r.lanes)
+                    norm_rows_fwd<T, VEC, nch.value, false><<<grid, 256, 0, st>>>(p, r.lanes);
+                else
+                    norm_rows_fwd<T, VEC, nch.value, true><<<grid, r.threads, 0, st>>>(p, 32);
+                return launched("layer_norm launch");
+            });
         }
-        a = block_sum(a, s);
-        c = block_sum(c, s);
-        if (threadIdx.x == 0) {
-            if (p.dw) store_as(p.dw, p.pt, i, a);
-            if (p.db) store_as(p.db, p.pt, i, c);
-        }
+    } else {
+        constexpr int MOST = VEC == 1 ? STRIP_ROWS_ONE : STRIP_ROWS_VEC;
+        const StripPlan s = plan_strips(p.n, p.vecs, VEC, MOST, sm_count());
+        if (s.ranks && s.strips * s.ranks <= INT_MAX)
+            return with_chunks<MOST>(s.nch, [&](auto nch) {
+                return launch_cluster(norm_cols_fwd<T, VEC, nch.value>, s.strips * s.ranks, s.ranks, st, p, s.q);
+            });
     }
-}
-
-unsigned blocks_of(long long n) { return (unsigned)std::min<long long>(n, INT_MAX); }
-
-tcaspmm_status launched(const char *what)
-{
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, what);
+    norm_long_fwd<T><<<blocks_of(p.vecs), 1024, 0, st>>>(p, dim ? p.ldx : 1, dim ? 1 : p.ldx, dim ? p.ldy : 1, dim ? 1 : p.ldy);
+    return launched("layer_norm launch");
 }
 
 }  // namespace
@@ -156,21 +302,28 @@ extern "C" tcaspmm_status tcaspmm_layer_norm(const void *dX, int64_t ldx, tcaspm
     const long long vecs = dim == 1 ? rows : cols, n = dim == 1 ? cols : rows;
     if (vecs == 0) return TCASPMM_OK;
     if (n == 0) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: the normalised dimension is empty");
-    const NormParams p{dX, ldx, dY, ldy, type_code(y_dt), weight, bias, type_code(p_dt), mean, rstd, vecs, n, (float)eps};
-    return with_type(type_code(x_dt), [&](auto t) {
+    const int xt = type_code(x_dt), yt = type_code(y_dt), pt = type_code(p_dt);
+    NormParams p{dX, ldx, dY, ldy, yt, weight, bias, pt, 0, mean, rstd, vecs, n, (float)eps};
+    return with_type(xt, [&](auto t) {
         using T = decltype(t);
-        norm_fwd<T><<<blocks_of(vecs), 256, 0, (cudaStream_t)stream>>>(p, dim ? ldx : 1, dim ? 1 : ldx, dim ? ldy : 1,
-                                                                        dim ? 1 : ldy);
-        return launched("layer_norm launch");
+        constexpr int VEC = 16 / (int)sizeof(T);
+        p.pvec = aligned(weight, 0, pt, VEC) && aligned(bias, 0, pt, VEC);
+        if (cols % VEC == 0 && aligned(dX, ldx, xt, VEC) && aligned(dY, ldy, yt, VEC))
+            return forward<T, VEC>(p, dim, (cudaStream_t)stream);
+        return forward<T, 1>(p, dim, (cudaStream_t)stream);
     });
 }
 
 extern "C" size_t tcaspmm_layer_norm_backward_workspace(int64_t rows, int64_t cols, int dim)
 {
-    (void)rows;
-    (void)cols;
-    (void)dim;
-    return 0;
+    if (rows <= 0 || cols <= 0) return 0;
+    const long long n = dim == 1 ? cols : rows, vecs = dim == 1 ? rows : cols;
+    // Rows: ROW_PARTS blocks an SM, or LONG_PARTS.  Columns: a strip for every 32 columns up to 4096 rows; longer ones have
+    // strips of at least 131072 / rows columns rounded down to a power of two (plan_strips, elements one by one or by vectors).
+    long long width = 32;
+    while (width > 1 && width * n > 131072) width /= 2;
+    const long long parts = dim == 1 ? std::max<long long>((long long)ROW_PARTS * sm_count(), LONG_PARTS) : ceil_div(vecs, width);
+    return (size_t)(2 * std::min(parts, std::max<long long>(vecs, 1)) * n) * sizeof(float);
 }
 
 extern "C" tcaspmm_status tcaspmm_layer_norm_backward(const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt, const void *dX,
@@ -191,18 +344,20 @@ extern "C" tcaspmm_status tcaspmm_layer_norm_backward(const void *dDY, int64_t l
     const long long vecs = dim == 1 ? rows : cols, n = dim == 1 ? cols : rows;
     if (n == 0) return vecs == 0 ? TCASPMM_OK : fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: the normalised dimension is empty");
     if (vecs > 0 && (!mean || !rstd)) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: mean and rstd are needed");
-    if (workspace_bytes < tcaspmm_layer_norm_backward_workspace(rows, cols, dim))
-        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: workspace of %zu bytes is too small", workspace_bytes);
-    (void)workspace;
-    const NormGradParams p{dDY, lddy, type_code(dy_dt), dX, ldx, mean, rstd, weight, type_code(p_dt), dDX, lddx, dweight, dbias,
-                           vecs, n};
+    const bool params = dweight || dbias;
+    const size_t need = params ? tcaspmm_layer_norm_backward_workspace(rows, cols, dim) : 0;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: a workspace of %zu bytes, 16-byte aligned, is needed", need);
     const cudaStream_t st = (cudaStream_t)stream;
-    const long long sv = dim ? ldx : 1, si = dim ? 1 : ldx, gv = dim ? lddy : 1, gi = dim ? 1 : lddy;
-    return with_type(type_code(x_dt), [&](auto t) {
-        using T = decltype(t);
-        if (dDX && vecs > 0)
-            norm_bwd<T><<<blocks_of(vecs), 256, 0, st>>>(p, sv, si, gv, gi, dim ? lddx : 1, dim ? 1 : lddx);
-        if (dweight || dbias) norm_wgrad<T><<<blocks_of(n), 256, 0, st>>>(p, sv, si, gv, gi);
-        return launched("layer_norm_backward launch");
-    });
+    const int xt = type_code(x_dt), gt = type_code(dy_dt), pt = type_code(p_dt);
+    NormGradParams p{dDY, lddy, gt, dX, ldx, mean, rstd, weight, pt, 0, dDX, lddx, params ? (float *)workspace : nullptr, vecs, n};
+    long long parts = 0;
+    if (vecs > 0 && (dDX || params)) {
+        const auto run = xt == 0 ? norm_backward_f32 : xt == 1 ? norm_backward_f16 : norm_backward_bf16;
+        const tcaspmm_status s = run(p, dim, &parts, st);
+        if (s != TCASPMM_OK) return s;
+    }
+    if (!params) return TCASPMM_OK;
+    norm_join<<<dim3(blocks_of(ceil_div(n, 32)), 2), 1024, 0, st>>>((const float *)workspace, parts, n, dweight, dbias, pt);
+    return launched("layer_norm_backward launch");
 }

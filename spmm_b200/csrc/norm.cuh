@@ -1,0 +1,342 @@
+// Shared parts of layer norm (norm.cu, norm_grad.cuh): the mathematics, the split of the work, launches.
+//
+// Layer norm, forward and backward, over the rows' elements (dim 1: a node's features, the layout of a graph product's C)
+// or the columns' (dim 0: a token's features, the layout of a pruned weight's B).
+//
+//   mean = sum x / n    rstd = 1 / sqrt(sum (x - mean)^2 / n + eps)    xh = (x - mean) rstd    y = w xh + b
+//   g = w dy            dx = rstd (g - mean(g) - xh mean(g xh))        dw = sum dy xh          db = sum dy
+//
+// Every pass is bound by memory: the vector is read once, held in registers as it came, and summed twice there (the mean
+// first, then the squared differences from it, so that a large mean costs no precision).  Rows: a part of a warp, a warp or a
+// block per row, whichever leaves a thread at most 16 elements.  Columns: a cluster of up to 8
+// blocks shares a strip of 32-64 columns, each block holds a part of the strip's rows, and the blocks exchange their sums
+// through distributed shared memory, so that reads stay coalesced along the rows.  The weight's gradient is summed by each
+// thread over the vectors it meets (its features stay the same), by block through shared memory, and over the blocks by a
+// second kernel, in a fixed order.
+#pragma once
+
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <type_traits>
+
+#include <cooperative_groups.h>
+
+#include "dense.h"
+
+namespace cg = cooperative_groups;
+
+namespace tca {
+
+int sm_count();  // SMs of the current device (norm.cu)
+
+struct NormParams {
+    const void *X;
+    long long ldx;
+    void *Y;
+    long long ldy;
+    int yt;
+    const void *w, *b;  // one per feature, type pt, or NULL
+    int pt;
+    int pvec;            // w and b allow vector loads
+    float *mean, *rstd;  // one per vector, or NULL
+    long long vecs, n;   // vectors normalised, their length
+    float eps;
+};
+
+struct NormGradParams {
+    const void *dY;
+    long long lddy;
+    int dyt;
+    const void *X;
+    long long ldx;
+    const float *mean, *rstd;
+    const void *w;
+    int pt;
+    int pvec;
+    void *dX;  // or NULL
+    long long lddx;
+    float *part;  // partial weight (then bias) gradients, one row of n per part, or NULL
+    long long vecs, n;
+};
+
+namespace {
+
+// ------------------------------------------------------------------ vectors of elements
+template <int BYTES> struct Bits;
+template <> struct Bits<2> { using type = unsigned short; };
+template <> struct Bits<4> { using type = unsigned; };
+template <> struct Bits<8> { using type = uint2; };
+template <> struct Bits<16> { using type = uint4; };
+
+// VEC elements of type T as they lie in memory (at most 16 bytes).
+template <typename T, int VEC>
+struct Pack {
+    typename Bits<sizeof(T) * VEC>::type bits;
+    __device__ void load(const T *p) { bits = __ldg(reinterpret_cast<const decltype(bits) *>(p)); }
+    __device__ void zero() { bits = {}; }
+    __device__ float get(int i) const
+    {
+        T v[VEC];
+        memcpy(v, &bits, sizeof bits);
+        return to_float(v[i]);
+    }
+};
+
+template <int VEC, typename T>
+__device__ __forceinline__ void store_pack(T *p, const float (&v)[VEC])
+{
+    constexpr int PER = sizeof(T) * VEC > 16 ? 16 / (int)sizeof(T) : VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; k += PER) {
+        T t[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) t[i] = from_float<T>(v[k + i]);
+        typename Bits<sizeof(T) * PER>::type bits;
+        memcpy(&bits, t, sizeof bits);
+        *reinterpret_cast<decltype(bits) *>(p + k) = bits;
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_vec(void *p, int type, long long i, const float (&v)[VEC])
+{
+    if (type == 0)
+        store_pack<VEC>((float *)p + i, v);
+    else if (type == 1)
+        store_pack<VEC>((__half *)p + i, v);
+    else
+        store_pack<VEC>((__nv_bfloat16 *)p + i, v);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_pack(const T *p, float *v)
+{
+    constexpr int PER = sizeof(T) * VEC > 16 ? 16 / (int)sizeof(T) : VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; k += PER) {
+        Pack<T, PER> t;
+        t.load(p + k);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[k + i] = t.get(i);
+    }
+}
+
+// Parameters i .. i + VEC - 1; `dflt` without a parameter.
+template <int VEC>
+__device__ __forceinline__ void load_params(const void *p, int type, int pvec, long long i, float dflt, float *v)
+{
+    if (!p) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = dflt;
+    } else if (!pvec) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = load_as(p, type, i + k);
+    } else if (type == 0) {
+        load_pack<float, VEC>((const float *)p + i, v);
+    } else if (type == 1) {
+        load_pack<__half, VEC>((const __half *)p + i, v);
+    } else {
+        load_pack<__nv_bfloat16, VEC>((const __nv_bfloat16 *)p + i, v);
+    }
+}
+
+// ------------------------------------------------------------------ rows
+// Sum over a row's threads: `lanes` neighbours of a warp, or (BLOCK) the whole block through `s`, a float per warp.  Calls
+// alternate between two such arrays, so one barrier a call is enough.
+template <bool BLOCK, int COUNT>
+__device__ __forceinline__ void row_sum(float (&v)[COUNT], int lanes, float (*s)[32])
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        if (BLOCK || o < lanes) {
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) v[k] += __shfl_xor_sync(~0u, v[k], o);
+        }
+    if (BLOCK) {
+        const int warps = (int)(blockDim.x >> 5), lane = threadIdx.x & 31;
+#pragma unroll
+        for (int k = 0; k < COUNT; ++k)
+            if (lane == 0) s[k][threadIdx.x >> 5] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < COUNT; ++k) {
+            float t = lane < warps ? s[k][lane] : 0.0f;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+            v[k] = t;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ columns
+constexpr int STRIP_THREADS = 512;
+constexpr int STRIP_WARPS = STRIP_THREADS / 32;
+constexpr int STRIP_MAX = 64;  // columns of a strip at most
+
+// Sums over the block's rows of COUNT values for each of a thread's VEC columns, into `out`, one per column of the strip.
+// Threads of a warp whose numbers agree modulo `lpr` hold the same columns.
+template <int COUNT, int VEC>
+__device__ __forceinline__ void strip_sum(float (&v)[COUNT][VEC], int lpr, float (*s)[STRIP_WARPS][STRIP_MAX], float (*out)[STRIP_MAX])
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        if (o >= lpr) {
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[k][e] += __shfl_xor_sync(~0u, v[k][e], o);
+        }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane < lpr) {
+#pragma unroll
+        for (int k = 0; k < COUNT; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s[k][warp][lane * VEC + e] = v[k][e];
+    }
+    __syncthreads();
+    const int width = lpr * VEC;
+    for (int j = threadIdx.x; j < COUNT * width; j += STRIP_THREADS) {
+        const int k = j / width, c = j - k * width;
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < STRIP_WARPS; ++i) t += s[k][i][c];
+        out[k][c] = t;
+    }
+    __syncthreads();
+}
+
+struct Strip {
+    int lpr, shift;       // threads along a row of the strip (a power of two), its logarithm
+    long long per_block;  // rows of a block
+};
+
+// ------------------------------------------------------------------ vectors of any length
+// Sum over the block's threads, the same in all of them.  `s` holds a float per warp.
+__device__ float block_sum(float v, float *s)
+{
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    const int warps = blockDim.x >> 5;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float t = 0.0f;
+    for (int i = 0; i < warps; ++i) t += s[i];
+    return t;
+}
+
+// ------------------------------------------------------------------ launches
+unsigned blocks_of(long long n) { return (unsigned)std::min<long long>(n, INT_MAX); }
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+int size_of(int type) { return type == 0 ? 4 : 2; }
+
+tcaspmm_status launched(const char *what)
+{
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, what);
+}
+
+// Rows of `n` elements start where VEC-element loads and stores (at most 16 bytes each) may.
+bool aligned(const void *p, long long ld, int type, int vec)
+{
+    const int bytes = std::min(16, vec * size_of(type));
+    return !p || ((uintptr_t)p % bytes == 0 && ld * size_of(type) % bytes == 0);
+}
+
+// How rows of n elements are dealt to threads: `nch` chunks of vec elements for each of `lanes` threads of a warp, or of the
+// `threads` of a block (lanes 0).  nch 0: too long.
+struct RowPlan {
+    int nch, lanes, threads;
+};
+
+// A warp takes a row of up to 32 x `most` elements, below that the smallest power of two of lanes; a block longer ones.
+RowPlan plan_rows(long long n, int vec, int most, int threads_most)
+{
+    const long long chunks = ceil_div(n, vec);
+    const int cap = most / vec;
+    if (chunks <= 32 * cap) {
+        int lanes = 1;
+        while (lanes < 32 && lanes < chunks) lanes *= 2;
+        int nch = 1;
+        while ((long long)nch * lanes < chunks) nch *= 2;
+        return {nch, lanes, 256};
+    }
+    if (chunks > (long long)threads_most * cap) return {0, 0, 0};
+    int nch = cap;
+    while (nch > 1 && ceil_div(chunks, nch / 2) <= 256) nch /= 2;
+    return {nch, 0, (int)(ceil_div(ceil_div(chunks, nch), 32) * 32)};
+}
+
+// How columns are dealt to clusters: strips of lpr x vec columns, `ranks` blocks a strip, nch rows a thread.  ranks 0: too long.
+struct StripPlan {
+    int nch, ranks;
+    Strip q;
+    long long strips;
+};
+
+StripPlan plan_strips(long long n, long long vecs, int vec, int most, int sms)
+{
+    // The widest strip of up to 64 columns (32 without vectors) whose rows fit in 8 blocks, narrower for fewer columns.
+    int lpr = vec == 1 ? 32 : STRIP_MAX / vec;
+    while (lpr > 1 && (lpr / 2) * vec >= vecs) lpr /= 2;
+    while (lpr > 1 && n > 8ll * most * (STRIP_THREADS / lpr)) lpr /= 2;
+    const int rows = STRIP_THREADS / lpr;
+    if (n > 8ll * most * rows) return {};
+    const long long strips = ceil_div(vecs, (long long)lpr * vec);
+    int ranks = 1;
+    while (n > (long long)ranks * most * rows) ranks *= 2;
+    while (ranks < 8 && strips * ranks < sms && n > (long long)ranks * rows) ranks *= 2;  // idle SMs take a share
+    const long long per = ceil_div(n, ranks);
+    int nch = 1;
+    while ((long long)nch * rows < per) nch *= 2;
+    int shift = 0;
+    while ((1 << shift) < lpr) ++shift;
+    return {nch, ranks, {lpr, shift, per}, strips};
+}
+
+template <typename... Args>
+tcaspmm_status launch_cluster(void (*kernel)(Args...), long long blocks, int ranks, cudaStream_t st, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(STRIP_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, "layer_norm launch");
+}
+
+// Calls f with the compile-time chunk count.
+template <int MOST, typename F>
+tcaspmm_status with_chunks(int nch, F &&f)
+{
+    if (nch <= 1) return f(std::integral_constant<int, 1>{});
+    if constexpr (MOST >= 2)
+        if (nch == 2) return f(std::integral_constant<int, 2>{});
+    if constexpr (MOST >= 4)
+        if (nch == 4) return f(std::integral_constant<int, 4>{});
+    if constexpr (MOST >= 8)
+        if (nch == 8) return f(std::integral_constant<int, 8>{});
+    if constexpr (MOST >= 16)
+        if (nch == 16) return f(std::integral_constant<int, 16>{});
+    if constexpr (MOST >= 32)
+        if (nch == 32) return f(std::integral_constant<int, 32>{});
+    return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: no kernel for %d chunks", nch);
+}
+
+constexpr int FWD_MOST = 16;       // elements of a row a thread holds, forward
+constexpr int BWD_MOST = 16;       // backward, where the sums of both gradients sit beside them
+constexpr int STRIP_ROWS_VEC = 8;  // vectors of a column strip a thread holds
+constexpr int STRIP_ROWS_ONE = 32; // elements, where rows do not allow vectors
+
+// Parts the weight gradient's sums come in: blocks of the backward kernel over rows, strips over columns.
+constexpr int ROW_PARTS = 4;
+constexpr int LONG_PARTS = 64;
+
+}  // namespace
+}  // namespace tca

@@ -1,0 +1,360 @@
+// The backward kernels of layer norm and their launch, instantiated by the type of X in norm_grad_*.cu.
+#pragma once
+
+#include "norm.cuh"
+
+namespace tca {
+namespace {
+
+template <typename T, typename G, int VEC, int NCH, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p, int lanes)
+{
+    constexpr bool BLOCK = THREADS != 256;
+    constexpr bool KEEP = VEC * NCH <= 8 || THREADS == 512;
+    __shared__ float s[2][2][32];
+    extern __shared__ float sum[];  // !BLOCK: a block's partial gradients, added warp by warp
+    const int tpr = BLOCK ? (int)blockDim.x : lanes;
+    const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
+    const int per = BLOCK ? 1 : (int)blockDim.x / lanes;
+    const long long first = (long long)blockIdx.x * per + (BLOCK ? 0 : (int)threadIdx.x / lanes);
+    const long long step = (long long)gridDim.x * per;
+    const float inv = 1.0f / (float)p.n;
+    float w[KEEP ? VEC * NCH : 1], dw[VEC * NCH], db[VEC * NCH];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long long i = ((long long)c * tpr + t) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) dw[c * VEC + e] = db[c * VEC + e] = 0.0f;
+        if (KEEP && i < p.n) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, w + c * VEC);
+    }
+    Pack<T, VEC> x[NCH], nx[NCH];
+    Pack<G, VEC> g[NCH], ng[NCH];
+    float mean, rstd, nmean, nrstd;
+    auto fetch = [&](long long row, Pack<T, VEC> (&tx)[NCH], Pack<G, VEC> (&tg)[NCH], float &m, float &r) {
+        const bool in = row < p.vecs;
+        m = in ? __ldg(p.mean + row) : 0.0f;
+        r = in ? __ldg(p.rstd + row) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long long i = ((long long)c * tpr + t) * VEC;
+            if (in && i < p.n) {
+                tx[c].load((const T *)p.X + row * p.ldx + i);
+                tg[c].load((const G *)p.dY + row * p.lddy + i);
+            } else {
+                tx[c].zero();
+                tg[c].zero();
+            }
+        }
+    };
+    fetch(first, x, g, mean, rstd);
+    const long long turns = (p.vecs - (long long)blockIdx.x * per + step - 1) / step;
+    for (long long k = 0; k < turns; ++k) {
+        const long long row = first + k * step;
+        fetch(row + step, nx, ng, nmean, nrstd);
+        float a[2] = {0.0f, 0.0f};
+        const bool in = row < p.vecs;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long long i = ((long long)c * tpr + t) * VEC;
+            if (in && i < p.n) {
+                float ww[VEC];
+                if (!KEEP) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float dy = g[c].get(e), xh = (x[c].get(e) - mean) * rstd;
+                    const float v = dy * (KEEP ? w[c * VEC + e] : ww[e]);
+                    a[0] += v;
+                    a[1] += v * xh;
+                    dw[c * VEC + e] += dy * xh;
+                    db[c * VEC + e] += dy;
+                }
+            }
+        }
+        if (p.dX) {
+            row_sum<BLOCK>(a, lanes, s[k & 1]);
+            const float c1 = a[0] * inv, c2 = a[1] * inv;
+            if (in) {
+#pragma unroll
+                for (int c = 0; c < NCH; ++c) {
+                    const long long i = ((long long)c * tpr + t) * VEC;
+                    if (i < p.n) {
+                        float d[VEC], ww[VEC];
+                        if (!KEEP) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const float xh = (x[c].get(e) - mean) * rstd;
+                            d[e] = rstd * (g[c].get(e) * (KEEP ? w[c * VEC + e] : ww[e]) - c1 - xh * c2);
+                        }
+                        store_pack<VEC>((T *)p.dX + row * p.lddx + i, d);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            x[c] = nx[c];
+            g[c] = ng[c];
+        }
+        mean = nmean;
+        rstd = nrstd;
+    }
+    if (!p.part) return;
+    float *pw = p.part + (long long)blockIdx.x * p.n, *pb = pw + (long long)gridDim.x * p.n;
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const long long i = ((long long)c * tpr + t) * VEC + e;
+                if (i < p.n) {
+                    pw[i] = dw[c * VEC + e];
+                    pb[i] = db[c * VEC + e];
+                }
+            }
+    } else {
+        // The groups of `lanes` threads add up in turn: within a warp by shuffles, then the warps one after another.
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            if (o >= lanes) {
+#pragma unroll
+                for (int j = 0; j < VEC * NCH; ++j) {
+                    dw[j] += __shfl_xor_sync(~0u, dw[j], o);
+                    db[j] += __shfl_xor_sync(~0u, db[j], o);
+                }
+            }
+        const int width = lanes * VEC * NCH;
+        for (int k = 0; k < (int)(blockDim.x >> 5); ++k) {
+            if ((int)(threadIdx.x >> 5) == k && (int)(threadIdx.x & 31) < lanes) {
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int i = (c * lanes + t) * VEC + e;
+                        sum[i] = (k ? sum[i] : 0.0f) + dw[c * VEC + e];
+                        sum[width + i] = (k ? sum[width + i] : 0.0f) + db[c * VEC + e];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
+            pw[i] = sum[i];
+            pb[i] = sum[width + i];
+        }
+    }
+}
+
+template <typename T, typename G, int VEC, int NCH>
+__global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradParams p, const Strip q)
+{
+    __shared__ float s[2][STRIP_WARPS][STRIP_MAX];
+    __shared__ float sums[2][STRIP_MAX];
+    __shared__ float fin[2][STRIP_MAX];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int width = q.lpr * VEC, at = (threadIdx.x & (q.lpr - 1)) * VEC;
+    const long long strip = blockIdx.x / ranks, strips = gridDim.x / ranks;
+    const long long col = strip * width + at;
+    const bool in = col < p.vecs;
+    const long long r0 = min(p.n, rank * q.per_block), r1 = min(p.n, r0 + q.per_block);
+    const int lane_row = threadIdx.x >> q.shift, rows = STRIP_THREADS >> q.shift;
+    Pack<T, VEC> x[NCH];
+    Pack<G, VEC> g[NCH];
+    float w[NCH];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long long r = r0 + lane_row + c * rows;
+        w[c] = 1.0f;
+        if (r < r1 && in) {
+            x[c].load((const T *)p.X + r * p.ldx + col);
+            g[c].load((const G *)p.dY + r * p.lddy + col);
+            if (p.w) w[c] = load_as(p.w, p.pt, r);
+        } else {
+            x[c].zero();
+            g[c].zero();
+        }
+    }
+    float mean[VEC], rstd[VEC], v[2][VEC] = {};
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        mean[e] = in ? __ldg(p.mean + col + e) : 0.0f;
+        rstd[e] = in ? __ldg(p.rstd + col + e) : 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long long r = r0 + lane_row + c * rows;
+        float a = 0.0f, d = 0.0f;
+        if (r < r1 && in) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float dy = g[c].get(e), xh = (x[c].get(e) - mean[e]) * rstd[e];
+                v[0][e] += dy * w[c];
+                v[1][e] += dy * w[c] * xh;
+                a += dy * xh;
+                d += dy;
+            }
+        }
+        if (p.part) {
+            for (int o = q.lpr >> 1; o; o >>= 1) {
+                a += __shfl_xor_sync(~0u, a, o);
+                d += __shfl_xor_sync(~0u, d, o);
+            }
+            if (at == 0 && r < r1) {
+                p.part[strip * p.n + r] = a;
+                p.part[(strips + strip) * p.n + r] = d;
+            }
+        }
+    }
+    if (!p.dX) return;
+    strip_sum(v, q.lpr, s, sums);
+    cluster.sync();
+    for (int j = threadIdx.x; j < 2 * width; j += STRIP_THREADS) {
+        const int k = j / width, c = j - k * width;
+        float t = 0.0f;
+        for (int i = 0; i < ranks; ++i) t += cluster.map_shared_rank(&sums[0][0], i)[k * STRIP_MAX + c];
+        fin[k][c] = t / (float)p.n;
+    }
+    __syncthreads();
+    if (in) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long long r = r0 + lane_row + c * rows;
+            if (r < r1) {
+                float d[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float xh = (x[c].get(e) - mean[e]) * rstd[e];
+                    d[e] = rstd[e] * (g[c].get(e) * w[c] - fin[0][at + e] - xh * fin[1][at + e]);
+                }
+                store_pack<VEC>((T *)p.dX + r * p.lddx + col, d);
+            }
+        }
+    }
+    cluster.sync();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_long_bwd(const NormGradParams p, long long sv, long long si, long long gv, long long gi,
+                                                      long long dv, long long di)
+{
+    __shared__ float s[32];
+    for (long long v = blockIdx.x; v < p.vecs; v += gridDim.x) {
+        const T *x = (const T *)p.X + v * sv;
+        const float mean = p.mean[v], rstd = p.rstd[v];
+        float a = 0.0f, c = 0.0f;
+        for (long long i = threadIdx.x; i < p.n; i += blockDim.x) {
+            const float g = load_as(p.dY, p.dyt, v * gv + i * gi) * (p.w ? load_as(p.w, p.pt, i) : 1.0f);
+            a += g;
+            c += g * ((to_float(x[i * si]) - mean) * rstd);
+        }
+        a = block_sum(a, s) / (float)p.n;
+        c = block_sum(c, s) / (float)p.n;
+        for (long long i = threadIdx.x; i < p.n; i += blockDim.x) {
+            const float g = load_as(p.dY, p.dyt, v * gv + i * gi) * (p.w ? load_as(p.w, p.pt, i) : 1.0f);
+            const float xh = (to_float(x[i * si]) - mean) * rstd;
+            ((T *)p.dX)[v * dv + i * di] = from_float<T>(rstd * (g - a - xh * c));
+        }
+    }
+}
+
+// Partial weight and bias gradients of rows too long for norm_rows_bwd: a thread per feature, a block row per part.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_long_rows_wgrad(const NormGradParams p)
+{
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= p.n) return;
+    float a = 0.0f, c = 0.0f;
+    for (long long v = blockIdx.y; v < p.vecs; v += gridDim.y) {
+        const float dy = load_as(p.dY, p.dyt, v * p.lddy + i);
+        a += dy * ((to_float(((const T *)p.X)[v * p.ldx + i]) - p.mean[v]) * p.rstd[v]);
+        c += dy;
+    }
+    p.part[blockIdx.y * p.n + i] = a;
+    p.part[(gridDim.y + blockIdx.y) * p.n + i] = c;
+}
+
+// The same of columns too long for norm_cols_bwd: a block per feature, whose values lie side by side.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_long_cols_wgrad(const NormGradParams p)
+{
+    __shared__ float s[8];
+    for (long long i = blockIdx.x; i < p.n; i += gridDim.x) {
+        float a = 0.0f, c = 0.0f;
+        for (long long v = threadIdx.x; v < p.vecs; v += blockDim.x) {
+            const float dy = load_as(p.dY, p.dyt, i * p.lddy + v);
+            a += dy * ((to_float(((const T *)p.X)[i * p.ldx + v]) - p.mean[v]) * p.rstd[v]);
+            c += dy;
+        }
+        a = block_sum(a, s);
+        c = block_sum(c, s);
+        if (threadIdx.x == 0) {
+            p.part[i] = a;
+            p.part[p.n + i] = c;
+        }
+    }
+}
+
+template <typename T, typename G, int VEC>
+tcaspmm_status backward(const NormGradParams &p, int dim, long long *parts, cudaStream_t st)
+{
+    const int sms = sm_count();
+    if (dim == 1) {
+        const RowPlan r = plan_rows(p.n, VEC, BWD_MOST, 1024);
+        if (r.nch) {
+            // Blocks an SM holds, at most ROW_PARTS: their count is the number of partial gradients.
+            const int fit = !r.lanes ? std::min(ROW_PARTS, std::max(1, 512 / r.threads)) : r.nch * VEC > 8 ? 1 : r.nch * VEC > 4 ? 2 : ROW_PARTS;
+            const long long grid = std::min(ceil_div(p.vecs, r.lanes ? 256 / r.lanes : 1), (long long)fit * sms);
+            *parts = grid;
+            return with_chunks<BWD_MOST / VEC>(r.nch, [&](auto nch) {
+                constexpr int N = nch.value;
+                const size_t shared = r.lanes ? sizeof(float) * 2 * r.lanes * VEC * N : 0;
+                if (r.lanes)
+                    norm_rows_bwd<T, G, VEC, N, 256><<<(unsigned)grid, 256, shared, st>>>(p, r.lanes);
+                else if (r.threads <= 512)
+                    norm_rows_bwd<T, G, VEC, N, 512><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
+                else
+                    norm_rows_bwd<T, G, VEC, N, 1024><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
+                return launched("layer_norm_backward launch");
+            });
+        }
+    } else {
+        constexpr int MOST = VEC == 1 ? STRIP_ROWS_ONE : STRIP_ROWS_VEC;
+        const StripPlan s = plan_strips(p.n, p.vecs, VEC, MOST, sms);
+        if (s.ranks && s.strips * s.ranks <= INT_MAX) {
+            *parts = s.strips;
+            return with_chunks<MOST>(s.nch, [&](auto nch) {
+                return launch_cluster(norm_cols_bwd<T, G, VEC, nch.value>, s.strips * s.ranks, s.ranks, st, p, s.q);
+            });
+        }
+    }
+    if (p.dX)
+        norm_long_bwd<T><<<blocks_of(p.vecs), 1024, 0, st>>>(p, dim ? p.ldx : 1, dim ? 1 : p.ldx, dim ? p.lddy : 1, dim ? 1 : p.lddy,
+                                                             dim ? p.lddx : 1, dim ? 1 : p.lddx);
+    *parts = 1;
+    if (p.part && dim == 1) {
+        *parts = std::min<long long>(p.vecs, LONG_PARTS);
+        norm_long_rows_wgrad<T><<<dim3(blocks_of(ceil_div(p.n, 256)), (unsigned)*parts), 256, 0, st>>>(p);
+    } else if (p.part) {
+        norm_long_cols_wgrad<T><<<blocks_of(p.n), 256, 0, st>>>(p);
+    }
+    return launched("layer_norm_backward launch");
+}
+
+}  // namespace
+
+// dX and the partial weight gradients; *parts: how many there are.
+template <typename T>
+tcaspmm_status norm_backward(NormGradParams p, int dim, long long *parts, cudaStream_t st)
+{
+    const long long cols = dim == 1 ? p.n : p.vecs;
+    const int xt = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 1 : 2;
+    return with_type(p.dyt, [&](auto u) {
+        using G = decltype(u);
+        constexpr int VEC = 16 / (int)(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G));
+        p.pvec = aligned(p.w, 0, p.pt, VEC);
+        if (cols % VEC == 0 && aligned(p.X, p.ldx, xt, VEC) && aligned(p.dY, p.lddy, p.dyt, VEC) && aligned(p.dX, p.lddx, xt, VEC))
+            return backward<T, G, VEC>(p, dim, parts, st);
+        return backward<T, G, 1>(p, dim, parts, st);
+    });
+}
+
+}  // namespace tca
