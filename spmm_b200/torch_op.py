@@ -23,12 +23,12 @@ the same kernels; its backward gives dX (through A^T) and d(bias).
 
 are what trains around a fixed A: low-rank adapters beside the product, chosen per column
 of X, and layer norm of rows or columns (``torch.ops.tcaspmm.spmm_lora``, ``lora`` and
-``layer_norm`` also return what their backward passes read).  There is no CPU or
+``layer_norm``; the first also returns what its backward pass reads).  There is no CPU or
 PyTorch fallback: without the library or a CUDA device the ops raise.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import numpy as np
 import torch
@@ -207,136 +207,9 @@ spmm_fused.register_autograd(_backward_fused, setup_context=_setup_fused)
 
 
 # ------------------------------------------- layer norm and low-rank adapters
-def _needed(t: torch.Tensor, wanted: bool) -> Optional[torch.Tensor]:
-    return t if wanted else None
-
-
-@torch.library.custom_op("tcaspmm::layer_norm", mutates_args=())
-def _layer_norm(X: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float, dim: int,
-                out_dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return dense.layer_norm(X, weight, bias, eps, dim, out_dtype, stats=True)
-
-
-@_layer_norm.register_fake
-def _(X, weight, bias, eps, dim, out_dtype):
-    vecs = X.new_empty(X.shape[1 - dim % 2], dtype=torch.float32)
-    return torch.empty(X.shape, dtype=out_dtype, device=X.device), vecs, torch.empty_like(vecs)
-
-
-@torch.library.custom_op("tcaspmm::layer_norm_backward", mutates_args=())
-def _layer_norm_backward(dY: torch.Tensor, X: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
-                         weight: Optional[torch.Tensor], dim: int, needed: List[bool],
-                         param_dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dX, dweight, dbias); an empty tensor for what is not needed."""
-    got = dense.layer_norm_backward(dY, X, mean, rstd, weight, dim, need_input=needed[0], need_weight=needed[1],
-                                    need_bias=needed[2], param_dtype=param_dtype)
-    return tuple(X.new_empty(0) if t is None else t for t in got)
-
-
-@_layer_norm_backward.register_fake
-def _(dY, X, mean, rstd, weight, dim, needed, param_dtype):
-    p = torch.empty(X.shape[dim], dtype=param_dtype, device=X.device)
-    return tuple(t if n else X.new_empty(0)
-                 for t, n in zip((torch.empty(X.shape, dtype=X.dtype, device=X.device), p, torch.empty_like(p)), needed))
-
-
-def _setup_norm(ctx, inputs, output):
-    X, weight, bias, _, dim, _ = inputs
-    _, mean, rstd = output
-    ctx.mark_non_differentiable(mean, rstd)
-    ctx.set_materialize_grads(False)
-    ctx.save_for_backward(X, weight, mean, rstd)
-    ctx.dim = dim
-    p = weight if weight is not None else bias
-    ctx.param_dtype = p.dtype if p is not None else torch.float32
-
-
-def _backward_norm(ctx, dY, *_):
-    if dY is None:
-        return (None,) * 6
-    X, weight, mean, rstd = ctx.saved_tensors
-    needed = [bool(n) for n in ctx.needs_input_grad[:3]]
-    got = torch.ops.tcaspmm.layer_norm_backward(dY, X, mean, rstd, weight, ctx.dim, needed, ctx.param_dtype)
-    return (*(_needed(t, n) for t, n in zip(got, needed)), None, None, None)
-
-
-_layer_norm.register_autograd(_backward_norm, setup_context=_setup_norm)
-
-
-def layer_norm(X: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
-               eps: float = 1e-5, dim: int = 1, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """spmm_b200.layer_norm with gradients for X, weight and bias: the norm of each row (dim=1, a node's features) or
-    each column (dim=0, a token's features) of X, stored as out_dtype (default: X's type)."""
-    return torch.ops.tcaspmm.layer_norm(X, weight, bias, eps, dim, X.dtype if out_dtype is None else out_dtype)[0]
-
-
-def _lora_grads(ctx, dY, base, needed):
-    """(dX, ddown, dup) of the adapters from what the forward pass saved."""
-    X, down, up, index, scale, H = ctx.saved_tensors[-6:]
-    if dY.dtype not in (torch.float32, X.dtype):
-        dY = dY.float()
-    got = torch.ops.tcaspmm.lora_backward(dY, X, down, up, H, index, scale, base, needed)
-    return tuple(_needed(t, n) for t, n in zip(got, needed))
-
-
-def _refuse_scale(ctx, at: int) -> None:
-    if ctx.needs_input_grad[at]:
-        raise ValueError("the adapters' scale is a constant: it has no gradient")
-
-
-@torch.library.custom_op("tcaspmm::lora", mutates_args=())
-def _lora(X: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: Optional[torch.Tensor],
-          scale: Optional[torch.Tensor], base: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    return dense.lora(X, down, up, index, scale, base, hidden=True)
-
-
-@_lora.register_fake
-def _(X, down, up, index, scale, base):
-    shape = (up.shape[1], X.shape[1])
-    return (torch.empty(shape, dtype=torch.float32 if base is None else base.dtype, device=X.device),
-            torch.empty((down.shape[1], X.shape[1]), dtype=torch.float32, device=X.device))
-
-
-@torch.library.custom_op("tcaspmm::lora_backward", mutates_args=())
-def _lora_backward(dY: torch.Tensor, X: torch.Tensor, down: torch.Tensor, up: torch.Tensor, H: torch.Tensor,
-                   index: Optional[torch.Tensor], scale: Optional[torch.Tensor], base: Optional[torch.Tensor],
-                   needed: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dX (+ base), ddown, dup); an empty tensor for what is not needed."""
-    got = dense.lora_backward(dY, X, down, up, H, index, scale, base, need_input=needed[0], need_down=needed[1],
-                              need_up=needed[2])
-    return tuple(X.new_empty(0) if t is None else t for t in got)
-
-
-@_lora_backward.register_fake
-def _(dY, X, down, up, H, index, scale, base, needed):
-    return tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else X.new_empty(0)
-                 for t, n in zip((X, down, up), needed))
-
-
-def _setup_lora(ctx, inputs, output):
-    X, down, up, index, scale, base = inputs
-    ctx.mark_non_differentiable(output[1])
-    ctx.set_materialize_grads(False)
-    ctx.save_for_backward(X, down, up, index, scale, output[1])
-
-
-def _backward_lora(ctx, dY, *_):
-    _refuse_scale(ctx, 4)
-    if dY is None:
-        return (None,) * 6
-    needed = [bool(n) for n in ctx.needs_input_grad[:3]]
-    grads = _lora_grads(ctx, dY, None, needed) if any(needed) else (None, None, None)
-    return (*grads, None, None, dY if ctx.needs_input_grad[5] else None)
-
-
-_lora.register_autograd(_backward_lora, setup_context=_setup_lora)
-
-
-def lora(X: torch.Tensor, down: torch.Tensor, up: torch.Tensor, index: Optional[torch.Tensor] = None,
-         scale: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """spmm_b200.lora with gradients for X, down, up and base: base + scale[a] * up[a] @ (down[a] @ X[:, t]) for every
-    column t, a = index[t] (None = adapter 0, outside [0, L) = no adapter)."""
-    return torch.ops.tcaspmm.lora(X, down, up, index, scale, base)[0]
+dense._op("layer_norm")  # loads the operators
+layer_norm = dense.layer_norm
+lora = dense.lora
 
 
 @torch.library.custom_op("tcaspmm::spmm_lora", mutates_args=())
@@ -365,13 +238,20 @@ def _setup_spmm_lora(ctx, inputs, output):
 
 
 def _backward_spmm_lora(ctx, dY, *_):
-    _refuse_scale(ctx, 7)
+    if ctx.needs_input_grad[7]:
+        raise ValueError("the adapters' scale is a constant: it has no gradient")
     if dY is None:
         return (None,) * 8
     crow, col, val, X = ctx.saved_tensors[:4]
     needed = [bool(n) for n in ctx.needs_input_grad[3:6]]
     base = torch.ops.tcaspmm.spmm_t(crow, col, val, dY.to(X.dtype), X.shape[0]) if needed[0] else None
-    grads = _lora_grads(ctx, dY, base, needed) if any(needed) else (None, None, None)
+    down, up, index, scale, H = ctx.saved_tensors[4:]
+    if dY.dtype not in (torch.float32, X.dtype):
+        dY = dY.float()
+    grads = (None, None, None)
+    if any(needed):
+        grads = dense.lora_backward(dY, X, down, up, H, index, scale, base, need_input=needed[0], need_down=needed[1],
+                                    need_up=needed[2])
     return (None, None, None, *grads, None, None)
 
 

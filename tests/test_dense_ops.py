@@ -228,8 +228,15 @@ def test_norm_autograd_matches_differences(dim):
         ana = float((grads[k].double().cpu() * v).sum())
         # Central difference in 64 bits: h^2 times a third derivative of order 100; the gradient's fp32 rounding.
         assert abs(num - ana) <= 1e-5 * (1 + abs(num)) + 200 * U * float((grads[k].double().cpu() * v).abs().sum())
-    assert torch_op.layer_norm(X.detach(), w, b, dim=dim).requires_grad
-    assert not torch.ops.tcaspmm.layer_norm(X, w, b, 1e-5, dim, F32)[1].requires_grad
+    for k in range(3):  # one leaf at a time: the same gradient, and none for the others
+        one = [t.detach().requires_grad_(j == k) for j, t in enumerate(leaves)]
+        torch_op.layer_norm(*one, 1e-3, dim).backward(dY)
+        assert [t.grad is not None for t in one] == [j == k for j in range(3)] and torch.equal(one[k].grad, grads[k])
+    only_bias = torch_op.layer_norm(X.detach(), None, b, 1e-3, dim)
+    assert torch.equal(torch.autograd.grad(only_bias, b, dY)[0], grads[2])
+    with pytest.raises(RuntimeError):  # no second derivatives
+        dX, = torch.autograd.grad(torch_op.layer_norm(X, w, b, 1e-3, dim), X, dY, create_graph=True)
+        dX.sum().backward()
 
 
 # --------------------------------------------------------- low-rank adapters
@@ -477,7 +484,14 @@ def test_lora_autograd_matches_differences():
         num = (f(ts[0]) - f(ts[1])) / (2 * h)  # linear in each leaf: exact up to rounding
         ana = (grads[k].double().cpu() * v)
         assert abs(num - float(ana.sum())) <= 1e-9 + 1e-4 * float(ana.abs().sum())
-    with pytest.raises(Exception, match="scale"):
+    for k in range(4):
+        one = [t.detach().requires_grad_(j == k) for j, t in enumerate(leaves)]
+        for idx, sc in ((index, scale), (None, scale), (index, None), (None, None)):
+            Y = torch_op.lora(*one[:3], idx, sc, one[3])
+            g, = torch.autograd.grad(Y, one[k], dY)
+            if idx is not None and sc is not None:
+                assert torch.equal(g, grads[k])
+    with pytest.raises(ValueError, match="scale"):
         torch_op.lora(X, down, up, index, scale.clone().requires_grad_(True), base).sum().backward()
 
 
