@@ -1,93 +1,20 @@
-// Low-rank adapters of many requests beside a sparse product: C (M x N) gets, column by column, the two small factors of
-// the column's own adapter.  With a = index[t], D_a (R x K), U_a (M x R) and the scale s_a:
-//
-//   H[:, t] = s_a D_a X[:, t]        Y[:, t] = base[:, t] + U_a H[:, t]
-//   P[:, t] = s_a U_a^T dY[:, t]     dX[:, t] = base[:, t] + D_a^T P[:, t]
-//   dD_a = sum_t P[:, t] X[:, t]^T   dU_a = sum_t dY[:, t] H[:, t]^T     (over the columns of adapter a)
-//
-// A column whose index is not in [0, L) has no adapter: H = P = 0 there and Y = base.
-#include <algorithm>
-#include <climits>
-
-#include "dense.h"
+// The C entries of the low-rank adapters (kernels: lora.cuh).
+#include "lora.cuh"
 
 namespace tca {
+
+int sm_count();
+
+#define TCA_LORA(k)                                                                         \
+    tcaspmm_status lora_forward_##k(const ApplyParams &p, int sms, cudaStream_t st);        \
+    tcaspmm_status lora_input_grad_##k(const ApplyParams &p, bool in32, int sms, cudaStream_t st); \
+    tcaspmm_status lora_factor_grads_##k(const GradParams &w, int sms, cudaStream_t st);
+TCA_LORA(f32)
+TCA_LORA(f16)
+TCA_LORA(bf16)
+#undef TCA_LORA
+
 namespace {
-
-struct Columns {
-    const void *index;  // one per column, or NULL: adapter 0 for all
-    int wide;           // 64-bit indices
-    int L;
-    __device__ int of(long long t) const
-    {
-        if (!index) return L > 0 ? 0 : -1;
-        const long long a = wide ? __ldg((const long long *)index + t) : (long long)__ldg((const int *)index + t);
-        return a >= 0 && a < L ? (int)a : -1;
-    }
-};
-
-// S[r, t] = scale * sum_i F[a][r, i] In[i, t], element (r, i) of adapter a at a * R * n + r * fr + i * fi.
-template <typename T>
-__global__ void lora_shrink(const T *F, long long fr, long long fi, int R, long long n, const void *In, long long ldin, int intype,
-                            Columns c, const float *scale, float *S, long long N)
-{
-    const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int r = blockIdx.y;
-    if (t >= N) return;
-    const int a = c.of(t);
-    float v = 0.0f;
-    if (a >= 0) {
-        const T *f = F + (long long)a * R * n + r * fr;
-        for (long long i = 0; i < n; ++i) v += to_float(f[i * fi]) * load_as(In, intype, i * ldin + t);
-        if (scale) v *= scale[a];
-    }
-    S[r * N + t] = v;
-}
-
-// Out[j, t] = base[j, t] + sum_r F[a][j, r] S[r, t].
-template <typename T>
-__global__ void lora_expand(const T *F, long long fj, long long fr, int R, long long n, const float *S, Columns c, const void *base,
-                            long long ldbase, int basetype, void *Out, long long ldout, int outtype, long long N)
-{
-    const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (t >= N) return;
-    const int a = c.of(t);
-    for (long long j = blockIdx.y; j < n; j += gridDim.y) {
-        float v = 0.0f;
-        if (a >= 0) {
-            const T *f = F + (long long)a * R * n + j * fj;
-            for (int r = 0; r < R; ++r) v += to_float(f[r * fr]) * S[r * N + t];
-        }
-        store_as(Out, outtype, j * ldout + t, base ? load_as(base, basetype, j * ldbase + t) + v : v);
-    }
-}
-
-// G[a][j, r] = sum over the columns of adapter a of Z[j, t] S[r, t], stored at a * R * n + j * gj + r * gr.  A warp per element.
-template <typename T>
-__global__ void lora_grad(const void *Z, long long ldz, int ztype, const float *S, int R, long long n, Columns c, T *G, long long gj,
-                          long long gr, long long N)
-{
-    const long long total = (long long)c.L * n * R;
-    for (long long e = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; e < total;
-         e += ((long long)gridDim.x * blockDim.x) >> 5) {
-        const int a = (int)(e / (n * R));
-        const long long j = e / R % n;
-        const int r = (int)(e % R);
-        float v = 0.0f;
-        for (long long t = threadIdx.x & 31; t < N; t += 32)
-            if (c.of(t) == a) v += load_as(Z, ztype, j * ldz + t) * S[r * N + t];
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-        if ((threadIdx.x & 31) == 0) G[(long long)a * R * n + j * gj + r * gr] = from_float<T>(v);
-    }
-}
-
-tcaspmm_status launched(const char *what)
-{
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, what);
-}
-
-unsigned grid_y(long long n) { return (unsigned)std::min<long long>(std::max<long long>(n, 1), 65535); }
 
 constexpr int64_t MAX_RANK = 256;
 
@@ -108,21 +35,12 @@ tcaspmm_status check(const tcaspmm_adapters *ad, int64_t N, const char *who)
     return TCASPMM_OK;
 }
 
-// Out = base + F2 (scale F1 In): the forward pass with (D, U), dX with (U^T, D^T).
-template <typename T>
-void apply(const tcaspmm_adapters *ad, bool forward, const void *In, int64_t ldin, int intype, float *S, const void *base,
-           int64_t ldbase, int basetype, void *Out, int64_t ldout, int outtype, int64_t N, cudaStream_t st)
+int size_of(int type) { return type == 0 ? 4 : 2; }
+
+// Rows of an array start where `bytes`-byte accesses may.
+bool aligned(const void *p, int64_t ld, int type, int bytes)
 {
-    const Columns c{ad->index, ad->index_bytes == 8, (int)ad->count};
-    const long long R = ad->rank, M = ad->M, K = ad->K;
-    const dim3 b(128), gs((unsigned)((N + 127) / 128), (unsigned)R);
-    if (forward) {
-        lora_shrink<T><<<gs, b, 0, st>>>((const T *)ad->down, K, 1, (int)R, K, In, ldin, intype, c, ad->scale, S, N);
-        if (Out) lora_expand<T><<<dim3(gs.x, grid_y(M)), b, 0, st>>>((const T *)ad->up, R, 1, (int)R, M, S, c, base, ldbase, basetype, Out, ldout, outtype, N);
-    } else {
-        lora_shrink<T><<<gs, b, 0, st>>>((const T *)ad->up, 1, R, (int)R, M, In, ldin, intype, c, ad->scale, S, N);
-        if (Out) lora_expand<T><<<dim3(gs.x, grid_y(K)), b, 0, st>>>((const T *)ad->down, 1, K, (int)R, K, S, c, base, ldbase, basetype, Out, ldout, outtype, N);
-    }
+    return (uintptr_t)p % bytes == 0 && ld * size_of(type) % bytes == 0;
 }
 
 }  // namespace
@@ -141,12 +59,32 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
         return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld or NULL pointer",
                     (long long)ldx, (long long)ldbase, (long long)ldy);
     if (N == 0) return TCASPMM_OK;
-    if (!dH) return fail(TCASPMM_ERR_INVALID_ARG, "lora: NULL dH");
-    return with_type(type_code(ad->dt), [&](auto t) {
-        apply<decltype(t)>(ad, true, dX, ldx, type_code(ad->dt), dH, dBase, ldbase, type_code(y_dt), dY, ldy, type_code(y_dt), N,
-                           (cudaStream_t)stream);
-        return launched("lora launch");
-    });
+    const int ft = type_code(ad->dt), yt = type_code(y_dt);
+    ApplyParams p = {};
+    p.F1 = ad->down;
+    p.F2 = ad->up;
+    p.scale = ad->scale;
+    p.c = Columns{ad->index, ad->index_bytes == 8, (int)ad->count};
+    p.R = (int)ad->rank;
+    p.n1 = ad->K;
+    p.n2 = ad->M;
+    p.N = N;
+    p.In = dX;
+    p.ldin = ldx;
+    p.base = dBase;
+    p.ldbase = ldbase;
+    p.basetype = yt;
+    p.Out = dY;
+    p.ldout = ldy;
+    p.outtype = yt;
+    p.S = dH;
+    p.vec_in = aligned(dX, ldx, ft, 16);
+    p.vec_f1 = aligned(ad->down, ad->K, ft, 16);
+    p.pair_f2 = aligned(ad->up, ad->rank, ft, 4);
+    p.vec_base = aligned(dBase, ldbase, yt, 4 * size_of(yt));
+    p.vec_out = aligned(dY, ldy, yt, 4 * size_of(yt));
+    const auto run = ft == 0 ? lora_forward_f32 : ft == 1 ? lora_forward_f16 : lora_forward_bf16;
+    return run(p, sm_count(), (cudaStream_t)stream);
 }
 
 extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt,
@@ -158,6 +96,8 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
     const tcaspmm_status s = check(ad, N, "lora_backward");
     if (s != TCASPMM_OK) return s;
     if (!dtype_valid(dy_dt)) return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: unknown dtype %d", (int)dy_dt);
+    const int ft = type_code(ad->dt), gt = type_code(dy_dt);
+    if (gt != 0 && gt != ft) return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: dY must be fp32 or of the factors' type");
     if (!matrix_ok(dDY, ad->M, N, lddy) || (ddown && !matrix_ok(dX, ad->K, N, ldx)) || (dBase && ldbase < N) ||
         (dDX && lddx < N) || (dup && !dH && N > 0) || (!dP && N > 0 && (dDX || ddown)))
         return fail(TCASPMM_ERR_INVALID_ARG,
@@ -165,16 +105,39 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
                     (long long)lddy, (long long)ldx, (long long)ldbase, (long long)lddx);
     const cudaStream_t st = (cudaStream_t)stream;
     const Columns c{ad->index, ad->index_bytes == 8, (int)ad->count};
-    const long long R = ad->rank;
-    return with_type(type_code(ad->dt), [&](auto t) {
-        using T = decltype(t);
-        if ((dDX || ddown) && N > 0)
-            apply<T>(ad, false, dDY, lddy, type_code(dy_dt), dP, dBase, ldbase, 0, dDX, lddx, type_code(ad->dt), N, st);
-        const auto blocks = [&](long long n) { return (unsigned)std::min<long long>((c.L * n * R + 7) / 8, 1 << 20); };
-        if (ddown && c.L > 0 && ad->K > 0)
-            lora_grad<T><<<blocks(ad->K), 256, 0, st>>>(dX, ldx, type_code(ad->dt), dP, (int)R, ad->K, c, (T *)ddown, 1, ad->K, N);
-        if (dup && c.L > 0 && ad->M > 0)
-            lora_grad<T><<<blocks(ad->M), 256, 0, st>>>(dDY, lddy, type_code(dy_dt), dH, (int)R, ad->M, c, (T *)dup, R, 1, N);
-        return launched("lora_backward launch");
-    });
+    if ((dDX || ddown) && N > 0) {
+        ApplyParams p = {};
+        p.F1 = ad->up;
+        p.F2 = ad->down;
+        p.scale = ad->scale;
+        p.c = c;
+        p.R = (int)ad->rank;
+        p.n1 = ad->M;
+        p.n2 = ad->K;
+        p.N = N;
+        p.In = dDY;
+        p.ldin = lddy;
+        p.base = dBase;
+        p.ldbase = ldbase;
+        p.Out = dDX;
+        p.ldout = lddx;
+        p.outtype = ft;
+        p.S = dP;
+        p.vec_in = aligned(dDY, lddy, gt, 16);
+        p.vec_f1 = aligned(ad->up, ad->rank, ft, 16);
+        p.vec_base = aligned(dBase, ldbase, 0, 16);
+        p.vec_out = aligned(dDX, lddx, ft, 4 * size_of(ft));
+        const auto run = ft == 0 ? lora_input_grad_f32 : ft == 1 ? lora_input_grad_f16 : lora_input_grad_bf16;
+        const tcaspmm_status e = run(p, gt == 0, sm_count(), st);
+        if (e != TCASPMM_OK) return e;
+    }
+    GradParams w = {};
+    w.c = c;
+    w.R = (int)ad->rank;
+    w.N = N;
+    w.vec_s = N % 4 == 0 && (uintptr_t)dP % 16 == 0 && (uintptr_t)dH % 16 == 0;
+    w.p[0] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), dP, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
+    w.p[1] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), dH, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
+    const auto run = ft == 0 ? lora_factor_grads_f32 : ft == 1 ? lora_factor_grads_f16 : lora_factor_grads_bf16;
+    return run(w, sm_count(), st);
 }
