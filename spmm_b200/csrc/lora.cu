@@ -80,7 +80,7 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
     p.S = dH;
     p.vec_in = aligned(dX, ldx, ft, 16);
     p.vec_f1 = aligned(ad->down, ad->K, ft, 16);
-    p.pair_f2 = aligned(ad->up, ad->rank, ft, 4);
+    p.vec_f2 = aligned(ad->up, ad->rank, ft, 16);
     p.vec_base = aligned(dBase, ldbase, yt, 4 * size_of(yt));
     p.vec_out = aligned(dY, ldy, yt, 4 * size_of(yt));
     const auto run = ft == 0 ? lora_forward_f32 : ft == 1 ? lora_forward_f16 : lora_forward_bf16;
@@ -125,6 +125,7 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
         p.S = dP;
         p.vec_in = aligned(dDY, lddy, gt, 16);
         p.vec_f1 = aligned(ad->up, ad->rank, ft, 16);
+        p.vec_f2 = aligned(ad->down, ad->K, ft, 16);
         p.vec_base = aligned(dBase, ldbase, 0, 16);
         p.vec_out = aligned(dDX, lddx, ft, 4 * size_of(ft));
         const auto run = ft == 0 ? lora_input_grad_f32 : ft == 1 ? lora_input_grad_f16 : lora_input_grad_bf16;

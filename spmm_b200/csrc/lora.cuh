@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstring>
 #include <type_traits>
 
 #include <cooperative_groups.h>
@@ -50,7 +51,7 @@ struct ApplyParams {
     long long ldout;
     int outtype;
     float *S;  // R x N, or NULL
-    int vec_in, vec_f1, pair_f2, vec_base, vec_out;  // what alignment allows
+    int vec_in, vec_f1, vec_f2, vec_base, vec_out;  // what alignment allows
     long long per1, per2;  // rows of In and of Out for each block of a cluster
 };
 
@@ -72,7 +73,7 @@ struct GradParams {
     Columns c;
     int R;
     int vec_s;
-    long long N, per;  // columns, columns for each block of a cluster
+    long long N;
 };
 
 // ------------------------------------------------------------------ instructions
@@ -84,6 +85,11 @@ __device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)
 __device__ __forceinline__ void copy16(void *dst, const void *src, int valid)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
+}
+// 8 bytes, all of them or (valid 0) zeros.
+__device__ __forceinline__ void copy8(void *dst, const void *src, int valid)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -104,24 +110,24 @@ template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
 {
     if (std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // D (16 x 8) += A (16 x 8) B (8 x 8), TF32 operands.
 __device__ __forceinline__ void mma8(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ unsigned to_tf32(float x)
 {
     unsigned r;
-    asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
     return r;
 }
 
@@ -175,13 +181,14 @@ __device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SPLIT> (&a
 // (8 in fp32) in turn, each through a ring of its own in shared memory (In's rows and F1's slice by asynchronous copies, no
 // barrier in the loop), with all R x TN sums in the warp's registers.  The sums are joined over warps, then over blocks
 // through distributed shared memory, in a fixed order, so that S never crosses device memory on its way to the second
-// product.  Then each block multiplies its part of Out's rows: a warp takes 16 rows, F2 straight from L2, base read and Out
-// written 16 bytes a thread (columns are dealt to the matrix instruction so that a thread's results lie side by side).
-// With several adapters among a tile's columns the products run once for each, and a column keeps its own adapter's.
+// product.  Then each block multiplies its part of Out's rows: a warp takes 16 rows, F2 and base through rings again, Out
+// written 16 bytes a thread (columns are dealt to the matrix instruction so that a thread's results lie side by side); the
+// first of these copies start before the sums are joined.  With several adapters among a tile's columns the products run
+// once for each, and a column keeps its own adapter's.
 //
 // In 16 bits S is held in two parts (split16), so that an fp32 Out is as exact as fp32 sums of exact products; fp16 parts
 // are scaled by a power of two for each column, as S may exceed fp16's range.  The tensor cores' legacy form (mma.sync) is
-// enough: the kernel moves R / 8 or fewer products a byte and is bound by In, base and Out.
+// enough: the kernel does about R products for each byte of In, base and Out, and is bound by those.
 constexpr int APPLY_WARPS = 8;
 constexpr int APPLY_THREADS = APPLY_WARPS * 32;
 
@@ -191,41 +198,68 @@ struct ApplyShape {
     static constexpr bool SPLIT = sizeof(TF) == 4;
     static constexpr int KS = sizeof(TF) == 4 ? 8 : 16;  // rows of In a step
     static constexpr int RP = RT * 16;
-    // Row pitches in bytes, padded so that a matrix fragment's rows fall into different banks.
+    // Row pitches in bytes, padded so that a matrix fragment's rows fall into different banks (ranks above 128, whose ring
+    // would not fit, go without).
     static constexpr int IN_PITCH = TN * (int)sizeof(TI) + (sizeof(TI) == 4 ? 32 : 16);
     static constexpr int F_ROWS = TRANS ? KS : RP;
     static constexpr int F_COLS = TRANS ? RP : KS;
-    static constexpr int F_PITCH = F_COLS * (int)sizeof(TF) + (TRANS && sizeof(TF) == 4 ? 32 : 16);
+    static constexpr int F_PITCH = F_COLS * (int)sizeof(TF) + (!TRANS && RT > 8 ? 0 : TRANS && sizeof(TF) == 4 ? 32 : 16);
     static constexpr int STAGE = KS * IN_PITCH + F_ROWS * F_PITCH;
-    static constexpr int FIT = 100 * 1024 / (APPLY_WARPS * STAGE);
-    static constexpr int STAGES = FIT >= 6 ? 6 : FIT >= 3 ? FIT : 208 * 1024 / (APPLY_WARPS * STAGE) >= 3 ? 3 : 2;
+    // Second product: F2 in pieces of RC along r.
+    static constexpr int RC_MOST = sizeof(TF) == 4 ? 16 : 64;
+    static constexpr int RC = RP < RC_MOST ? RP : RC_MOST;
+    static constexpr int PIECES = RP / RC;
+    static constexpr int G_ROWS = TRANS ? RC : 16;
+    static constexpr int G_COLS = TRANS ? 16 : RC;
+    static constexpr int G_PITCH = G_COLS * (int)sizeof(TF) + (TRANS && sizeof(TF) == 4 ? 32 : 16);
+    static constexpr int STAGE2 = G_ROWS * G_PITCH + 16 * TN * 4;
     static constexpr int S_PITCH = TN + 8;  // floats
     static constexpr int S_BYTES = RP * S_PITCH * 4;
     static constexpr int H_PITCH = TN * 2 + 16;  // bytes
-    static constexpr int RING = APPLY_WARPS * STAGES * STAGE;
-    static constexpr int BYTES = RING > 4 * S_BYTES ? RING : 4 * S_BYTES;
+    // Two blocks an SM where a thread's sums leave the registers for it, else one.
+    static constexpr int BUDGET = (RT <= 4 ? 110 : 222) * 1024 - 2 * S_BYTES;
+    static constexpr int fit(int stage) { return BUDGET / (APPLY_WARPS * stage) >= 4 ? 4 : BUDGET / (APPLY_WARPS * stage); }
+    static constexpr int STAGES = fit(STAGE);
+    static constexpr int STAGES2 = fit(STAGE2);
+    static_assert(STAGES >= 2 && STAGES2 >= 2, "the rings do not fit");
+    static constexpr int most(int a, int b) { return a > b ? a : b; }
+    static constexpr int RING = most(most(APPLY_WARPS * STAGES * STAGE, APPLY_WARPS * STAGES2 * STAGE2), 4 * S_BYTES);
+    static constexpr int BYTES = RING + 2 * S_BYTES;
 };
 
+// Element `type` at p as fp32 in shared memory's copy of it.
+__device__ __forceinline__ float raw_as(const unsigned char *p, int type, int e)
+{
+    if (type == 0) return ((const float *)p)[e];
+    const unsigned short u = ((const unsigned short *)p)[e];
+    return type == 1 ? __half2float(__ushort_as_half(u)) : __bfloat162float(__ushort_as_bfloat16(u));
+}
+
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
-__global__ void __launch_bounds__(APPLY_THREADS) lora_apply(const ApplyParams p)
+__global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(const ApplyParams p)
 {
     using Q = ApplyShape<TF, TI, RT, TN, TRANS>;
     constexpr int NB = TN / 8, RP = Q::RP, KS = Q::KS;
+    constexpr bool HALF = std::is_same<TF, __half>::value;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int ids[TN], list[TN], count;
     __shared__ float colscale[TN];
+    __shared__ int colmax[TN];
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2;
     const long long t0 = (long long)(blockIdx.x / ranks) * TN;
 
-    for (int t = threadIdx.x; t < TN; t += APPLY_THREADS) ids[t] = t0 + t < p.N ? p.c.of(t0 + t) : -1;
+    for (int t = threadIdx.x; t < TN; t += APPLY_THREADS) {
+        ids[t] = t0 + t < p.N ? p.c.of(t0 + t) : -1;
+        colmax[t] = 0;
+    }
     __syncthreads();
     if (warp == 0) {  // the tile's adapters, in the order of their first columns
         int n = 0;
         for (int b = 0; b < TN; b += 32) {
             const int t = b + lane;
-            bool first = t < TN && ids[t] >= 0;
+            bool first = t < TN && ids[t] >= 0 && (t == 0 || ids[t] != ids[t - 1]);
             for (int s = 0; first && s < t; ++s) first = ids[s] != ids[t];
             const unsigned m = __ballot_sync(~0u, first);
             if (first) list[n + __popc(m & ((1u << lane) - 1))] = ids[t];
@@ -250,147 +284,163 @@ __global__ void __launch_bounds__(APPLY_THREADS) lora_apply(const ApplyParams p)
     const int items = mine * nd;
     unsigned char *ring = smem + warp * (Q::STAGES * Q::STAGE);
 
+    // A lane's 16-byte pieces of a step lie in rows first + k * (32 / CH) (CH pieces a row, a power of two), one column.
+    constexpr int IN_PER = 16 / (int)sizeof(TI), IN_CH = TN / IN_PER;
+    constexpr int F_PER = 16 / (int)sizeof(TF), F_CH = Q::F_COLS / F_PER;
+    const int in_row = lane / IN_CH, in_col = lane % IN_CH * IN_PER;
+    const long long in_left = p.N - t0 - in_col;
+    const int in_bytes = in_left <= 0 ? 0 : in_left >= IN_PER ? 16 : (int)in_left * (int)sizeof(TI);
+    const TI *const in_src = (const TI *)p.In + in_row * p.ldin + t0 + in_col;
+    const long long f_ld = TRANS ? p.R : p.n1;
+
     auto fill = [&](int slot, int step, int a) {
         unsigned char *in = ring + slot * Q::STAGE, *f = in + KS * Q::IN_PITCH;
         const long long i0 = i_begin + (long long)(warp + step * APPLY_WARPS) * KS;
-        const TI *src = (const TI *)p.In + i0 * p.ldin + t0;
+        const int rows = (int)min((long long)KS, i_end - i0);
         if (p.vec_in) {
-            constexpr int PER = 16 / (int)sizeof(TI), CH = TN / PER;
-            for (int k = lane; k < KS * CH; k += 32) {
-                const int r = k / CH, c = (k - r * CH) * PER;
-                const long long left = i0 + r < i_end ? p.N - t0 - c : 0;
-                const int valid = left <= 0 ? 0 : left >= PER ? 16 : (int)left * (int)sizeof(TI);
-                copy16(in + r * Q::IN_PITCH + c * sizeof(TI), valid ? src + r * p.ldin + c : (const TI *)p.In, valid);
+            const TI *src = in_src + i0 * p.ldin;
+            unsigned char *to = in + in_row * Q::IN_PITCH + in_col * (int)sizeof(TI);
+#pragma unroll
+            for (int k = 0; k < KS * IN_CH / 32; ++k) {
+                constexpr int RS = 32 / IN_CH;
+                const int valid = in_row + k * RS < rows ? in_bytes : 0;
+                copy16(to + k * RS * Q::IN_PITCH, valid ? src + k * RS * p.ldin : (const TI *)p.In, valid);
             }
         } else {
             for (int k = lane; k < KS * TN; k += 32) {
                 const int r = k / TN, c = k - r * TN;
                 TI v = from_float<TI>(0.0f);
-                if (i0 + r < i_end && t0 + c < p.N) v = src[r * p.ldin + c];
+                if (r < rows && t0 + c < p.N) v = ((const TI *)p.In)[(i0 + r) * p.ldin + t0 + c];
                 *(TI *)(in + r * Q::IN_PITCH + c * sizeof(TI)) = v;
             }
         }
-        const TF *F = (const TF *)p.F1 + (long long)a * p.R * p.n1;
-        const long long rows_left = i_end - i0;
+        const TF *F = (const TF *)p.F1 + (long long)a * p.R * p.n1 + (TRANS ? i0 * p.R : i0);
         if (p.vec_f1) {
-            constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER;
-            for (int k = lane; k < Q::F_ROWS * CH; k += 32) {
-                const int r = k / CH, c = (k - r * CH) * PER;
-                const long long left = TRANS ? (r < rows_left ? p.R - c : 0) : (r < p.R ? rows_left - c : 0);
-                const int valid = left <= 0 ? 0 : left >= PER ? 16 : (int)left * (int)sizeof(TF);
-                const TF *s = TRANS ? F + (i0 + r) * p.R + c : F + (long long)r * p.n1 + i0 + c;
-                copy16(f + r * Q::F_PITCH + c * sizeof(TF), valid ? s : (const TF *)p.F1, valid);
+            constexpr int COUNT = Q::F_ROWS * F_CH;
+#pragma unroll
+            for (int k = 0; k < (COUNT + 31) / 32; ++k) {
+                const int r = (lane + k * 32) / F_CH, c = (lane + k * 32) % F_CH * F_PER;
+                const int left = TRANS ? (r < rows ? p.R - c : 0) : (r < p.R ? rows - c : 0);
+                const int valid = left <= 0 ? 0 : left >= F_PER ? 16 : left * (int)sizeof(TF);
+                if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
+                    copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F1, valid);
             }
         } else {
             for (int k = lane; k < Q::F_ROWS * Q::F_COLS; k += 32) {
                 const int r = k / Q::F_COLS, c = k - r * Q::F_COLS;
                 TF v = from_float<TF>(0.0f);
-                if (TRANS ? (r < rows_left && c < p.R) : (r < p.R && c < rows_left))
-                    v = TRANS ? F[(i0 + r) * p.R + c] : F[(long long)r * p.n1 + i0 + c];
+                if (TRANS ? (r < rows && c < p.R) : (r < p.R && c < rows)) v = F[r * f_ld + c];
                 *(TF *)(f + r * Q::F_PITCH + c * sizeof(TF)) = v;
             }
         }
     };
 
-    int next_step = 0, next_d = 0, filled = 0;
-    auto fill_next = [&]() {
-        if (filled < items) {
-            fill(filled % Q::STAGES, next_step, list[next_d]);
-            if (++next_d == nd) {
-                next_d = 0;
-                ++next_step;
+    {
+        int next_step = 0, next_d = 0, filled = 0, slot = 0;
+        auto fill_next = [&]() {
+            if (filled < items) {
+                fill(slot, next_step, list[next_d]);
+                if (++next_d == nd) {
+                    next_d = 0;
+                    ++next_step;
+                }
+                ++filled;
+                if (++slot == Q::STAGES) slot = 0;
             }
-            ++filled;
-        }
-        copy_commit();
-    };
+            copy_commit();
+        };
+        for (int s = 0; s < Q::STAGES - 1; ++s) fill_next();
+        int d = 0, at = 0;
+        for (int it = 0; it < items; ++it) {
+            copy_wait<Q::STAGES - 2>();
+            __syncwarp();  // the copies of all lanes have landed, and the slot filled next has been read by all
+            fill_next();
+            const unsigned char *in = ring + at * Q::STAGE, *f = in + KS * Q::IN_PITCH;
+            if (++at == Q::STAGES) at = 0;
+            const int a = list[d];
+            if (++d == nd) d = 0;
+            // Which blocks of 8 columns hold columns of adapter a, and which others beside them.
+            unsigned some = ~0u, mixed = 0u;
+            if (nd > 1) {
+                some = 0u;
 #pragma unroll
-    for (int s = 0; s < Q::STAGES - 1; ++s) fill_next();
-    int d = 0;
-    for (int it = 0; it < items; ++it) {
-        copy_wait<Q::STAGES - 2>();
-        __syncwarp();
-        const unsigned char *in = ring + (it % Q::STAGES) * Q::STAGE, *f = in + KS * Q::IN_PITCH;
-        const int a = list[d];
-        // Which blocks of 8 columns hold columns of adapter a, and which others beside them.
-        unsigned some = ~0u, mixed = 0u;
-        if (nd > 1) {
-            some = 0u;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int o = ids[b * 8 + (lane & 7)];
-                if (__any_sync(~0u, o == a)) some |= 1u << b;
-                if (__any_sync(~0u, o != a && o >= 0)) mixed |= 1u << b;
+                for (int b = 0; b < NB; ++b) {
+                    const int o = ids[b * 8 + (lane & 7)];
+                    if (__any_sync(~0u, o == a)) some |= 1u << b;
+                    if (__any_sync(~0u, o != a && o >= 0)) mixed |= 1u << b;
+                }
             }
-        }
-        // acc += part, or in a mixed block only for adapter a's columns.
-        auto add = [&](auto &&product) {
+            // acc += part, or in a mixed block only for adapter a's columns.
+            auto add = [&](auto &&product) {
+                if (some == ~0u && !mixed) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (!(some >> b & 1)) continue;
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int m = 0; m < RT; ++m) {
-                    if (!(mixed >> b & 1)) {
-                        product(m, b, acc[m][b]);
-                    } else {
+                        for (int m = 0; m < RT; ++m) product(m, b, acc[m][b]);
+                    return;
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (!(some >> b & 1)) continue;
+                    const bool own[2] = {ids[b * 8 + 2 * q] == a, ids[b * 8 + 2 * q + 1] == a};
+#pragma unroll
+                    for (int m = 0; m < RT; ++m) {
                         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         product(m, b, part);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (ids[b * 8 + 2 * q + (e & 1)] == a) acc[m][b][e] += part[e];
+                            if (own[e & 1]) acc[m][b][e] += part[e];
                     }
                 }
-            }
-        };
-        if constexpr (Q::M16) {
-            unsigned A[RT][4], B[NB][2];
-#pragma unroll
-            for (int m = 0; m < RT; ++m)
-                load_matrices<TRANS>(A[m], TRANS ? f + ((lane & 7) + (lane >> 4) * 8) * Q::F_PITCH + (m * 16 + (lane >> 3 & 1) * 8) * 2
-                                                 : f + (m * 16 + (lane & 15)) * Q::F_PITCH + (lane >> 4) * 16);
-#pragma unroll
-            for (int b = 0; b < NB; b += 2) {
-                unsigned t[4];
-                load_matrices<true>(t, in + (lane & 15) * Q::IN_PITCH + (b + (lane >> 4)) * 16);
-                B[b][0] = t[0];
-                B[b][1] = t[1];
-                B[b + 1][0] = t[2];
-                B[b + 1][1] = t[3];
-            }
-            add([&](int m, int b, float (&to)[4]) { mma16<TF>(to, A[m], B[b][0], B[b][1]); });
-        } else {
-#pragma unroll
-            for (int k = 0; k < KS; k += 8) {
-                Operand<Q::SPLIT> A[RT][4];
+            };
+            if constexpr (Q::M16) {
+                unsigned A[RT][4], B[NB][2];
 #pragma unroll
                 for (int m = 0; m < RT; ++m)
+                    load_matrices<TRANS>(A[m], TRANS ? f + ((lane & 7) + (lane >> 4) * 8) * Q::F_PITCH + (m * 16 + (lane >> 3 & 1) * 8) * 2
+                                                     : f + (m * 16 + (lane & 15)) * Q::F_PITCH + (lane >> 4) * 16);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = m * 16 + g + (e & 1) * 8, i = k + q + (e >> 1) * 4;
-                        A[m][e].set(to_float(*(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF))));
-                    }
-                Operand<Q::SPLIT> B[2];
-                int have = -1;
-                add([&](int m, int b, float (&to)[4]) {
-                    if (have != b) {
+                for (int b = 0; b < NB; b += 2) {
+                    unsigned t[4];
+                    load_matrices<true>(t, in + (lane & 15) * Q::IN_PITCH + (b + (lane >> 4)) * 16);
+                    B[b][0] = t[0];
+                    B[b][1] = t[1];
+                    B[b + 1][0] = t[2];
+                    B[b + 1][1] = t[3];
+                }
+                add([&](int m, int b, float (&to)[4]) { mma16<TF>(to, A[m], B[b][0], B[b][1]); });
+            } else {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            B[e].set(to_float(*(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI))));
-                        have = b;
-                    }
-                    mma8_any<Q::SPLIT>(to, A[m], B[0], B[1]);
-                });
+                for (int k = 0; k < KS; k += 8) {
+                    Operand<Q::SPLIT> A[RT][4];
+#pragma unroll
+                    for (int m = 0; m < RT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = m * 16 + g + (e & 1) * 8, i = k + q + (e >> 1) * 4;
+                            A[m][e].set(to_float(*(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF))));
+                        }
+                    Operand<Q::SPLIT> B[2];
+                    int have = -1;
+                    add([&](int m, int b, float (&to)[4]) {
+                        if (have != b) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                B[e].set(to_float(*(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI))));
+                            have = b;
+                        }
+                        mma8_any<Q::SPLIT>(to, A[m], B[0], B[1]);
+                    });
+                }
             }
         }
-        if (++d == nd) d = 0;
-        __syncwarp();
-        fill_next();
+        copy_wait<0>();
     }
-    copy_wait<0>();
     __syncthreads();
 
     // ---- S joined over the warps: 4 to 7 leave theirs, 0 to 3 add them to their own, all threads add those four
     float *slot = (float *)smem;
+    float *part = (float *)(smem + Q::RING), *Hf = part + Q::S_BYTES / 4;
     constexpr int SLOT = Q::S_BYTES / 4, PITCH = Q::S_PITCH;
     auto frag = [&](float *s, bool add) {
 #pragma unroll
@@ -414,57 +464,183 @@ __global__ void __launch_bounds__(APPLY_THREADS) lora_apply(const ApplyParams p)
     if (warp < 4) frag(slot + warp * SLOT, true);
     __syncthreads();
     for (int i = threadIdx.x; i < RP * TN; i += APPLY_THREADS) {
-        float *s = slot + i / TN * PITCH + i % TN;
-        s[0] = (s[0] + s[SLOT]) + (s[2 * SLOT] + s[3 * SLOT]);
+        const int at = i / TN * PITCH + i % TN;
+        const float *s = slot + at;
+        part[at] = (s[0] + s[SLOT]) + (s[2 * SLOT] + s[3 * SLOT]);
     }
-    cluster.sync();
+    auto sync_all = [&]() {
+        if (ranks > 1)
+            cluster.sync();
+        else
+            __syncthreads();
+    };
+    sync_all();
+
+    // ---- the second product's first copies: rows j0 of base, F2's slices
+    const long long j_begin = min(p.n2, rank * p.per2), j_end = min(p.n2, j_begin + p.per2);
+    constexpr int PAIRS = TN / 16;
+    const int tiles = p.Out && j_end > j_begin + warp * 16 ? (int)((j_end - j_begin - warp * 16 + APPLY_WARPS * 16 - 1) / (APPLY_WARPS * 16)) : 0;
+    const int passes = nd > 1 ? nd : 1;  // over a tile of rows, one for each adapter
+    const int items2 = tiles * passes * Q::PIECES;
+    unsigned char *ring2 = smem + warp * (Q::STAGES2 * Q::STAGE2);
+    const int base_size = p.basetype == 0 ? 4 : 2;
+
+    const bool inner = t0 + TN <= p.N && p.vec_base;  // base's pieces are whole
+    const unsigned char *const base_row = (const unsigned char *)p.base + ((j_begin + warp * 16 + g) * p.ldbase + t0 + 4 * q) * base_size;
+    const long long g_ld = TRANS ? p.n2 : p.R;
+
+    // Piece `piece` of adapter d's F2 and, for a tile's first item, base: a thread copies what it will add to.
+    auto fill2 = [&](int slot, int tile, int d, int piece) {
+        unsigned char *f = ring2 + slot * Q::STAGE2, *old = f + Q::G_ROWS * Q::G_PITCH + lane * 16;
+        const long long j0 = j_begin + warp * 16 + (long long)tile * (APPLY_WARPS * 16);
+        const int rows = (int)min(16ll, j_end - j0);
+        if (nd > 0) {
+            const int r0 = piece * Q::RC;
+            const TF *F = (const TF *)p.F2 + (long long)list[d] * p.R * p.n2 + (TRANS ? r0 * p.n2 + j0 : j0 * p.R + r0);
+            constexpr int PER = 16 / (int)sizeof(TF), CH = Q::G_COLS / PER, COUNT = Q::G_ROWS * CH;
+            if (p.vec_f2 && rows == 16 && CH <= 32 && COUNT % 32 == 0) {  // a lane's pieces lie in one column
+                const int r = lane / CH, c = lane % CH * PER;
+                const int left = p.R - r0 - c, bytes = TRANS ? 16 : left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
+                const TF *src = F + r * g_ld + c;
+                unsigned char *to = f + r * Q::G_PITCH + c * (int)sizeof(TF);
+#pragma unroll
+                for (int k = 0; k < COUNT / 32; ++k) {
+                    const int valid = TRANS && r0 + r + k * (32 / CH) >= p.R ? 0 : bytes;
+                    copy16(to + k * (32 / CH) * Q::G_PITCH, valid ? src : (const TF *)p.F2, valid);
+                    src += (32 / CH) * g_ld;
+                }
+            } else if (p.vec_f2) {
+#pragma unroll
+                for (int k = 0; k < (COUNT + 31) / 32; ++k) {
+                    const int r = (lane + k * 32) / CH, c = (lane + k * 32) % CH * PER;
+                    const int left = TRANS ? (r0 + r < p.R ? rows - c : 0) : (r < rows ? p.R - r0 - c : 0);
+                    const int valid = left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
+                    if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
+                        copy16(f + r * Q::G_PITCH + c * (int)sizeof(TF), valid ? F + r * g_ld + c : (const TF *)p.F2, valid);
+                }
+            } else {
+                for (int k = lane; k < Q::G_ROWS * Q::G_COLS; k += 32) {
+                    const int r = k / Q::G_COLS, c = k - r * Q::G_COLS;
+                    TF v = from_float<TF>(0.0f);
+                    if (TRANS ? (r0 + r < p.R && c < rows) : (r < rows && r0 + c < p.R)) v = F[r * g_ld + c];
+                    *(TF *)(f + r * Q::G_PITCH + c * sizeof(TF)) = v;
+                }
+            }
+        }
+        if (!p.base || d > 0 || piece > 0) return;
+        const unsigned char *from = base_row + (long long)tile * (APPLY_WARPS * 16) * p.ldbase * base_size;
+        const long long down = 8 * p.ldbase * base_size;
+        if (inner) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int valid = g + h * 8 < rows ? 16 : 0;
+                const unsigned char *row = valid ? from + h * down : (const unsigned char *)p.base;
+#pragma unroll
+                for (int b = 0; b < PAIRS; ++b) {
+                    if (base_size == 4)
+                        copy16(old + (b * 2 + h) * 512, row + (valid ? b * 64 : 0), valid);
+                    else
+                        copy8(old + (b * 2 + h) * 512, row + (valid ? b * 32 : 0), valid >> 1);
+                }
+            }
+            return;
+        }
+        for (int i = 0; i < PAIRS * 2; ++i) {
+            const long long t = t0 + (i >> 1) * 16 + 4 * q;
+            const bool row = g + (i & 1) * 8 < rows, whole = p.vec_base && t + 3 < p.N;
+            const unsigned char *src = from + (i & 1) * down + (i >> 1) * 16 * base_size;
+            unsigned char *to = old + i * 512;
+            if (whole) {
+                if (base_size == 4)
+                    copy16(to, row ? src : (const unsigned char *)p.base, row ? 16 : 0);
+                else
+                    copy8(to, row ? src : (const unsigned char *)p.base, row ? 8 : 0);
+            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (row && t + e < p.N) {
+                        if (base_size == 4)
+                            ((float *)to)[e] = ((const float *)src)[e];
+                        else
+                            ((unsigned short *)to)[e] = ((const unsigned short *)src)[e];
+                    }
+            }
+        }
+    };
+    int filled2 = 0, slot2 = 0, next_tile = 0, next_pass = 0, next_piece = 0;
+    auto fill2_next = [&]() {
+        if (filled2 < items2) {
+            fill2(slot2, next_tile, next_pass, next_piece);
+            if (++next_piece == Q::PIECES) {
+                next_piece = 0;
+                if (++next_pass == passes) {
+                    next_pass = 0;
+                    ++next_tile;
+                }
+            }
+            ++filled2;
+            if (++slot2 == Q::STAGES2) slot2 = 0;
+        }
+        copy_commit();
+    };
+    for (int s = 0; s < Q::STAGES2 - 1; ++s) fill2_next();
 
     // ---- S joined over the blocks: each takes TN / ranks columns, scales them and gives them to all
-    float *Hf = slot + SLOT;
-    const int own = TN / ranks;
-    for (int cgroup = warp; cgroup * 4 < own; cgroup += APPLY_WARPS) {
-        const int c = rank * own + cgroup * 4 + q;
-        const bool in = cgroup * 4 + q < own;
+    const int own = TN / ranks;  // a power of two: a thread keeps one column
+    {
+        const int c = rank * own + (threadIdx.x & (own - 1)), a = ids[c];
+        const int r_first = threadIdx.x / own, r_step = APPLY_THREADS / own;
+        const float s = a < 0 ? 0.0f : p.scale ? __ldg(p.scale + a) : 1.0f;
+        const bool keep = p.S && t0 + c < p.N;
+        float *const S = p.S + t0 + c;
         float most = 0.0f;
-        const int a = in ? ids[c] : -1;
-        const float s = a >= 0 ? (p.scale ? __ldg(p.scale + a) : 1.0f) : 0.0f;
-        for (int r = g; r < RP; r += 8) {
+        for (int r = r_first; r < RP; r += r_step) {
             float v = 0.0f;
-            if (a >= 0) {
-                for (int k = 0; k < ranks; ++k) v += cluster.map_shared_rank(slot, k)[r * PITCH + c];
-                v *= s;
+            if (ranks == 1) {
+                v = part[r * PITCH + c];
+            } else {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = k < ranks ? cluster.map_shared_rank(part, k)[r * PITCH + c] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v += x[k];
             }
-            if (in && p.S && r < p.R && t0 + c < p.N) p.S[(long long)r * p.N + t0 + c] = v;
-            if (std::is_same<TF, __half>::value) {
-                if (in) Hf[r * PITCH + c] = v;
+            v = a >= 0 ? v * s : 0.0f;  // whatever a column without an adapter has gathered
+            if (keep && r < p.R) S[(long long)r * p.N] = v;
+            if (HALF || ranks == 1) {
+                Hf[r * PITCH + c] = v;
                 most = fmaxf(most, fabsf(v));
-            } else if (in) {
-                for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(Hf, k)[r * PITCH + c] = v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < ranks) cluster.map_shared_rank(Hf, k)[r * PITCH + c] = v;
             }
         }
-        if (std::is_same<TF, __half>::value) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, o));
+        if (HALF) {
+            atomicMax(&colmax[c], __float_as_int(most));  // the order does not matter
+            __syncthreads();
             // The column's largest value goes to [2^13, 2^14); zeros and infinities stay.
-            const int e = (__float_as_int(most) >> 23) - 127;
+            const int e = (colmax[c] >> 23) - 127;
             const int shift = e == -127 || e == 128 ? 0 : max(-100, min(100, e - 13));
-            const float down = __int_as_float((127 - shift) << 23), up = __int_as_float((127 + shift) << 23);
-            if (in) {
-                for (int r = g; r < RP; r += 8) {
-                    const float v = Hf[r * PITCH + c] * down;
-                    for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(Hf, k)[r * PITCH + c] = v;
-                }
-                if (g == 0)
-                    for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(colscale, k)[c] = up;
+            const float down = __int_as_float((127 - shift) << 23);
+            for (int r = r_first; r < RP; r += r_step) {
+                const float v = Hf[r * PITCH + c] * down;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < ranks) cluster.map_shared_rank(Hf, k)[r * PITCH + c] = v;
+            }
+            if (r_first == 0) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < ranks) cluster.map_shared_rank(colscale, k)[c] = __int_as_float((127 + shift) << 23);
             }
         }
     }
-    cluster.sync();
+    sync_all();
     if (!p.Out) return;
 
     // ---- S as the second product's operand.  Column c of a pair of 8-column blocks holds the tile's column
     // 4 (c % 8 / 2) + 2 (c / 8) + c % 2, so that a thread's results of the pair are four neighbours.
-    unsigned char *hi = (unsigned char *)(slot + 2 * SLOT), *lo = (unsigned char *)(slot + 3 * SLOT);
+    unsigned char *hi = (unsigned char *)part, *lo = hi + RP * Q::H_PITCH;
     if constexpr (sizeof(TF) == 2) {
         for (int i = threadIdx.x; i < RP * TN; i += APPLY_THREADS) {
             const int r = i / TN, c = i % TN, t = (c & ~15) + 4 * (c >> 1 & 3) + 2 * (c >> 3 & 1) + (c & 1);
@@ -477,179 +653,171 @@ __global__ void __launch_bounds__(APPLY_THREADS) lora_apply(const ApplyParams p)
     }
 
     // ---- Out: this block's rows
-    const long long j_begin = min(p.n2, rank * p.per2), j_end = min(p.n2, j_begin + p.per2);
-    constexpr int PAIRS = TN / 16;
-    constexpr int KT = sizeof(TF) == 2 ? RT : RT * 2;  // matrix instructions along r
-    for (long long j0 = j_begin + warp * 16; j0 < j_end; j0 += APPLY_WARPS * 16) {
-        float4 old[PAIRS][2];
+    float old[PAIRS][2][4] = {};  // rows g, g + 8; columns 16 pair + 4 q ...
+    float sum[PAIRS][2][4];       // [pair][block of the pair][e]: rows g, g + 8; columns 16 pair + 4 q + 2 block + (e & 1)
+    const int out_size = p.outtype == 0 ? 4 : 2;
+    unsigned char *const out_row = (unsigned char *)p.Out + ((j_begin + warp * 16 + g) * p.ldout + t0 + 4 * q) * out_size;
+    // A bit for each of a thread's columns (4 q + (k & 3) of pair k / 4): it exists, has an adapter, is written now.
+    unsigned exist = 0u, has = 0u;
 #pragma unroll
-        for (int b = 0; b < PAIRS; ++b)
+    for (int k = 0; k < PAIRS * 4; ++k) {
+        const int c = (k >> 2) * 16 + 4 * q + (k & 3);
+        if (t0 + c < p.N) exist |= 1u << k;
+        if (ids[c] >= 0) has |= 1u << k;
+    }
+    unsigned write = exist;
+    auto store = [&](auto type, unsigned char *to, int rows) {
+        using TO = std::conditional_t<type.value == 0, float, std::conditional_t<type.value == 1, __half, __nv_bfloat16>>;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const long long j = j0 + g + h * 8, t = t0 + b * 16 + 4 * q;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (p.base && j < j_end && t < p.N) {
-                    const long long at = j * p.ldbase + t;
-                    if (p.vec_base && t + 3 < p.N) {
-                        if (p.basetype == 0) {
-                            v = *(const float4 *)((const float *)p.base + at);
-                        } else {
-                            const uint2 w = *(const uint2 *)((const unsigned short *)p.base + at);
-                            const unsigned short u[4] = {(unsigned short)w.x, (unsigned short)(w.x >> 16), (unsigned short)w.y,
-                                                         (unsigned short)(w.y >> 16)};
-                            float x[4];
+        for (int h = 0; h < 2; ++h) {
+            if (g + h * 8 >= rows) continue;
+            TO *row = (TO *)to + h * 8 * p.ldout;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                x[e] = p.basetype == 1 ? __half2float(__ushort_as_half(u[e])) : __bfloat162float(__ushort_as_bfloat16(u[e]));
-                            v = make_float4(x[0], x[1], x[2], x[3]);
-                        }
-                    } else {
-                        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (t + e < p.N) {
-                                if (p.basetype == 0)
-                                    x[e] = ((const float *)p.base)[at + e];
-                                else if (p.basetype == 1)
-                                    x[e] = __half2float(__ushort_as_half(((const unsigned short *)p.base)[at + e]));
-                                else
-                                    x[e] = __bfloat162float(__ushort_as_bfloat16(((const unsigned short *)p.base)[at + e]));
-                            }
-                        v = make_float4(x[0], x[1], x[2], x[3]);
-                    }
-                }
-                old[b][h] = v;
-            }
-        unsigned A16[sizeof(TF) == 2 ? RT : 1][4];
-        Operand<true> A32[sizeof(TF) == 4 ? KT : 1][4];
-        auto load_f2 = [&](int a) {
-            const TF *F = (const TF *)p.F2 + (long long)a * p.R * p.n2;
-            if constexpr (sizeof(TF) == 2) {
-                const unsigned short *f = (const unsigned short *)F;
-#pragma unroll
-                for (int k = 0; k < RT; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const long long j = j0 + g + (e & 1) * 8;
-                        const int r = k * 16 + 2 * q + (e >> 1) * 8;
-                        unsigned v = 0u;
-                        if (j < j_end && r < p.R) {
-                            if (!TRANS && p.pair_f2) {
-                                v = __ldg((const unsigned *)(f + j * p.R + r));
-                            } else {
-                                v = __ldg(TRANS ? f + (long long)r * p.n2 + j : f + j * p.R + r);
-                                if (r + 1 < p.R) v |= (unsigned)__ldg(TRANS ? f + (long long)(r + 1) * p.n2 + j : f + j * p.R + r + 1) << 16;
-                            }
-                        }
-                        A16[k][e] = v;
-                    }
-            } else {
-#pragma unroll
-                for (int k = 0; k < KT; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const long long j = j0 + g + (e & 1) * 8;
-                        const int r = k * 8 + q + (e >> 1) * 4;
-                        float v = 0.0f;
-                        if (j < j_end && r < p.R) v = __ldg((const float *)F + (TRANS ? (long long)r * p.n2 + j : j * p.R + r));
-                        A32[k][e].set(v);
-                    }
-            }
-        };
-        if (nd == 1) load_f2(list[0]);
-#pragma unroll
-        for (int b = 0; b < PAIRS; ++b) {
-            int id[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) id[e] = ids[b * 16 + 4 * q + e];
-            float sum[2][4] = {};  // [block of the pair][e]: rows g, g + 8; columns 4q + 2 block + (e & 1)
-            for (int k = 0; k < nd; ++k) {
-                const int a = list[k];
-                if (nd > 1) {
-                    if (!__any_sync(~0u, id[0] == a || id[1] == a || id[2] == a || id[3] == a)) continue;
-                    load_f2(a);
-                }
-                float part[2][4] = {};
-                if constexpr (sizeof(TF) == 2) {
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        unsigned B[4];
-                        const int at = (r * 16 + (lane & 15)) * Q::H_PITCH + (b * 2 + (lane >> 4)) * 16;
-                        load_matrices<true>(B, lo + at);
-                        mma16<TF>(part[0], A16[r], B[0], B[1]);
-                        mma16<TF>(part[1], A16[r], B[2], B[3]);
-                        load_matrices<true>(B, hi + at);
-                        mma16<TF>(part[0], A16[r], B[0], B[1]);
-                        mma16<TF>(part[1], A16[r], B[2], B[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < KT; ++r)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int t = b * 16 + 4 * (g >> 1) + 2 * h + (g & 1);
-                            Operand<true> B[2];
-                            B[0].set(Hf[(r * 8 + q) * PITCH + t]);
-                            B[1].set(Hf[(r * 8 + q + 4) * PITCH + t]);
-                            mma8_any<true>(part[h], A32[r], B[0], B[1]);
-                        }
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (id[2 * h + (e & 1)] == a) sum[h][e] = part[h][e];
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const long long j = j0 + g + h * 8, t = t0 + b * 16 + 4 * q;
-                if (j >= j_end || t >= p.N) continue;
-                const float x[4] = {old[b][h].x, old[b][h].y, old[b][h].z, old[b][h].w};
+            for (int b = 0; b < PAIRS; ++b) {
                 float y[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float v = sum[e >> 1][2 * h + (e & 1)];
-                    if (std::is_same<TF, __half>::value) v *= colscale[b * 16 + 4 * q + e];
-                    y[e] = id[e] >= 0 ? x[e] + v : x[e];
+                    float v = sum[b][e >> 1][2 * h + (e & 1)];
+                    if (HALF) v *= colscale[b * 16 + 4 * q + e];
+                    y[e] = has >> (b * 4 + e) & 1 ? old[b][h][e] + v : old[b][h][e];
                 }
-                const long long at = j * p.ldout + t;
-                if (p.vec_out && t + 3 < p.N) {
-                    if (p.outtype == 0) {
-                        *(float4 *)((float *)p.Out + at) = make_float4(y[0], y[1], y[2], y[3]);
+                const unsigned w = write >> (b * 4) & 15u;
+                if (p.vec_out && w == 15u) {
+                    if constexpr (type.value == 0) {
+                        *(float4 *)(row + b * 16) = make_float4(y[0], y[1], y[2], y[3]);
                     } else {
-                        unsigned short u[4];
+                        TO u[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            u[e] = p.outtype == 1 ? __half_as_ushort(__float2half_rn(y[e])) : __bfloat16_as_ushort(__float2bfloat16_rn(y[e]));
-                        *(uint2 *)((unsigned short *)p.Out + at) =
-                            make_uint2(u[0] | (unsigned)u[1] << 16, u[2] | (unsigned)u[3] << 16);
+                        for (int e = 0; e < 4; ++e) u[e] = from_float<TO>(y[e]);
+                        uint2 bits;
+                        memcpy(&bits, u, sizeof bits);
+                        *(uint2 *)(row + b * 16) = bits;
                     }
-                } else {
+                } else if (w) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (t + e < p.N) store_as(p.Out, p.outtype, at + e, y[e]);
+                        if (w >> e & 1) row[b * 16 + e] = from_float<TO>(y[e]);
                 }
             }
         }
+    };
+    int tile = 0, pass = 0, piece = 0, at = 0;
+    for (int it = 0; it < items2; ++it) {
+        copy_wait<Q::STAGES2 - 2>();
+        __syncwarp();
+        fill2_next();
+        const unsigned char *f = ring2 + at * Q::STAGE2;
+        if (++at == Q::STAGES2) at = 0;
+        if (pass == 0 && piece == 0 && p.base) {
+            const unsigned char *mine = f + Q::G_ROWS * Q::G_PITCH + lane * 16;
+            if (p.basetype == 0) {
+#pragma unroll
+                for (int i = 0; i < PAIRS * 2; ++i) {
+                    const float4 v = *(const float4 *)(mine + i * 512);
+                    old[i >> 1][i & 1][0] = v.x;
+                    old[i >> 1][i & 1][1] = v.y;
+                    old[i >> 1][i & 1][2] = v.z;
+                    old[i >> 1][i & 1][3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PAIRS * 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) old[i >> 1][i & 1][e] = raw_as(mine + i * 512, p.basetype, e);
+            }
+        }
+        if (piece == 0) {
+#pragma unroll
+            for (int b = 0; b < PAIRS; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[b][h][e] = 0.0f;
+        }
+        if (nd > 0) {
+            if constexpr (sizeof(TF) == 2) {
+#pragma unroll
+                for (int k = 0; k < Q::RC / 16; ++k) {
+                    unsigned A[4];
+                    load_matrices<TRANS>(A, TRANS ? f + (k * 16 + (lane & 7) + (lane >> 4) * 8) * Q::G_PITCH + (lane >> 3 & 1) * 16
+                                                  : f + (lane & 15) * Q::G_PITCH + (k * 16 + (lane >> 4) * 8) * 2);
+                    const int row = (piece * Q::RC + k * 16 + (lane & 15)) * Q::H_PITCH + (lane >> 4) * 16;
+#pragma unroll
+                    for (int b = 0; b < PAIRS; ++b) {
+                        unsigned L[4], H[4];
+                        load_matrices<true>(L, lo + row + b * 32);
+                        load_matrices<true>(H, hi + row + b * 32);
+                        mma16<TF>(sum[b][0], A, L[0], L[1]);
+                        mma16<TF>(sum[b][1], A, L[2], L[3]);
+                        mma16<TF>(sum[b][0], A, H[0], H[1]);
+                        mma16<TF>(sum[b][1], A, H[2], H[3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < Q::RC; k += 8) {
+                    Operand<true> A[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = g + (e & 1) * 8, r = k + q + (e >> 1) * 4;
+                        A[e].set(*(const float *)(TRANS ? f + r * Q::G_PITCH + j * 4 : f + j * Q::G_PITCH + r * 4));
+                    }
+#pragma unroll
+                    for (int b = 0; b < PAIRS; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float *s = Hf + (piece * Q::RC + k + q) * PITCH + b * 16 + 4 * (g >> 1) + 2 * h + (g & 1);
+                            Operand<true> B[2];
+                            B[0].set(s[0]);
+                            B[1].set(s[4 * PITCH]);
+                            mma8_any<true>(sum[b][h], A, B[0], B[1]);
+                        }
+                }
+            }
+        }
+        if (++piece < Q::PIECES) continue;
+        piece = 0;
+        const int rows = (int)min(16ll, j_end - (j_begin + warp * 16 + (long long)tile * (APPLY_WARPS * 16)));
+        unsigned char *const to = out_row + (long long)tile * (APPLY_WARPS * 16) * p.ldout * out_size;
+        if (nd > 1) {  // columns of this pass's adapter are done; those without any are written in the first pass
+            write = 0u;
+#pragma unroll
+            for (int k = 0; k < PAIRS * 4; ++k) {
+                const int id = ids[(k >> 2) * 16 + 4 * q + (k & 3)];
+                if (id == list[pass] || (id < 0 && pass == 0)) write |= 1u << k;
+            }
+            write &= exist;
+        }
+        if (p.outtype == 0)
+            store(std::integral_constant<int, 0>{}, to, rows);
+        else if (p.outtype == 1)
+            store(std::integral_constant<int, 1>{}, to, rows);
+        else
+            store(std::integral_constant<int, 2>{}, to, rows);
+        if (++pass == passes) {
+            pass = 0;
+            ++tile;
+        }
     }
+    copy_wait<0>();
 }
 
 // ------------------------------------------------------------------ gradients of the factors
 //
-// A cluster of up to 8 blocks takes 128 rows j of Z and one adapter; its blocks share the columns.  A block goes over the
-// chunks of 32 columns that hold any of the adapter's, Z's and S's chunks through a ring in shared memory; a warp takes 16
-// rows and all R of S.  Columns of other adapters count as zeros in both operands (an infinity there meets a zero nowhere).
+// A cluster of up to 8 blocks takes 128 rows j of Z and one adapter; its blocks share the chunks of 32 columns that hold any
+// of the adapter's, in turn.  A block takes Z's and S's chunks through a ring in shared memory; a warp takes 16 rows and all
+// R of S.  Columns of other adapters count as zeros in both operands (an infinity there meets a zero nowhere).
 // The blocks' sums are joined through distributed shared memory in a fixed order.  Both products of a backward pass are one
 // launch.
 constexpr int GRAD_ROWS = 128;
 constexpr int GRAD_CHUNK = 32;
-constexpr int GRAD_SCAN = 64;  // chunks looked over at once
+constexpr int GRAD_SCAN = 128;  // chunks looked over at once
 
 template <int RT>
 struct GradShape {
     static constexpr int RP = RT * 16;
     static constexpr int PITCH = GRAD_CHUNK * 4 + 16;  // bytes of a chunk's row (16-bit rows use a part)
-    static constexpr int STAGE = (GRAD_ROWS + RP) * PITCH + GRAD_CHUNK * 4;
+    static constexpr int STAGE = (GRAD_ROWS + RP) * PITCH;
     static constexpr int STAGES = RT <= 4 ? 4 : 3;
     static constexpr int SUM_PITCH = RP + 4;  // floats
     static constexpr int SUM = GRAD_ROWS * SUM_PITCH * 4;
@@ -662,66 +830,90 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
 {
     using Q = GradShape<RT>;
     constexpr bool SPLIT = sizeof(TF) == 4;
-    __shared__ unsigned char flags[GRAD_SCAN];
+    __shared__ unsigned members[GRAD_SCAN];  // which columns of a chunk are the adapter's
     __shared__ unsigned char list[GRAD_SCAN];
-    __shared__ int count;
+    __shared__ int count, seen;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2;
     const cg::cluster_group cluster = cg::this_cluster();
-    const long long t_begin = min(w.N, cluster.block_rank() * w.per), t_end = min(w.N, t_begin + w.per);
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const long long t_end = w.N;
 
+    // A thread's 16-byte pieces of a chunk lie in rows first + k * (256 / CH), one column.
+    constexpr int PER = 16 / (int)sizeof(TZ), CH = GRAD_CHUNK / PER;
+    const int z_row = threadIdx.x / CH, z_col = threadIdx.x % CH * PER, s_row = threadIdx.x / 8, s_col = threadIdx.x % 8 * 4;
+    const TZ *const z_src = (const TZ *)p.Z + (j0 + z_row) * p.ldz + z_col;
+    const float *const s_src = p.S + (long long)s_row * w.N + s_col;
+    const int j_left = (int)min((long long)GRAD_ROWS, p.n - j0);
     auto fill = [&](int slot, long long t0) {
         unsigned char *z = smem + slot * Q::STAGE, *s = z + GRAD_ROWS * Q::PITCH;
-        int *ids = (int *)(s + Q::RP * Q::PITCH);
+        const int cols = (int)min((long long)GRAD_CHUNK, t_end - t0);
         if (p.vec) {
-            constexpr int PER = 16 / (int)sizeof(TZ), CH = GRAD_CHUNK / PER;
-            for (int k = threadIdx.x; k < GRAD_ROWS * CH; k += 256) {
-                const int r = k / CH, c = (k - r * CH) * PER;
-                const long long left = j0 + r < p.n ? t_end - t0 - c : 0;
-                const int valid = left <= 0 ? 0 : left >= PER ? 16 : (int)left * (int)sizeof(TZ);
-                copy16(z + r * Q::PITCH + c * sizeof(TZ), valid ? (const TZ *)p.Z + (j0 + r) * p.ldz + t0 + c : (const TZ *)p.Z, valid);
+            const int left = cols - z_col, bytes = left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TZ);
+#pragma unroll
+            for (int k = 0; k < GRAD_ROWS * CH / 256; ++k) {
+                constexpr int RS = 256 / CH;
+                const int valid = z_row + k * RS < j_left ? bytes : 0;
+                copy16(z + (z_row + k * RS) * Q::PITCH + z_col * (int)sizeof(TZ), valid ? z_src + t0 + k * RS * p.ldz : (const TZ *)p.Z, valid);
             }
         } else {
             for (int k = threadIdx.x; k < GRAD_ROWS * GRAD_CHUNK; k += 256) {
                 const int r = k / GRAD_CHUNK, c = k % GRAD_CHUNK;
                 TZ v = from_float<TZ>(0.0f);
-                if (j0 + r < p.n && t0 + c < t_end) v = ((const TZ *)p.Z)[(j0 + r) * p.ldz + t0 + c];
+                if (r < j_left && c < cols) v = ((const TZ *)p.Z)[(j0 + r) * p.ldz + t0 + c];
                 *(TZ *)(z + r * Q::PITCH + c * sizeof(TZ)) = v;
             }
         }
         if (w.vec_s) {
-            constexpr int CH = GRAD_CHUNK / 4;
-            for (int k = threadIdx.x; k < Q::RP * CH; k += 256) {
-                const int r = k / CH, c = (k - r * CH) * 4;
-                const long long left = r < w.R ? t_end - t0 - c : 0;
-                const int valid = left <= 0 ? 0 : left >= 4 ? 16 : (int)left * 4;
-                copy16(s + r * Q::PITCH + c * 4, valid ? p.S + (long long)r * w.N + t0 + c : p.S, valid);
+            const int left = cols - s_col, bytes = left <= 0 ? 0 : left >= 4 ? 16 : left * 4;
+#pragma unroll
+            for (int k = 0; k < (Q::RP * 8 + 255) / 256; ++k) {
+                const int valid = s_row + k * 32 < w.R ? bytes : 0;
+                if (Q::RP >= 32 || s_row < Q::RP)
+                    copy16(s + (s_row + k * 32) * Q::PITCH + s_col * 4, valid ? s_src + t0 + k * 32 * w.N : p.S, valid);
             }
         } else {
             for (int k = threadIdx.x; k < Q::RP * GRAD_CHUNK; k += 256) {
                 const int r = k / GRAD_CHUNK, c = k % GRAD_CHUNK;
-                *(float *)(s + r * Q::PITCH + c * 4) = r < w.R && t0 + c < t_end ? p.S[(long long)r * w.N + t0 + c] : 0.0f;
+                *(float *)(s + r * Q::PITCH + c * 4) = r < w.R && c < cols ? p.S[(long long)r * w.N + t0 + c] : 0.0f;
             }
         }
-        if (threadIdx.x < GRAD_CHUNK) ids[threadIdx.x] = t0 + threadIdx.x < t_end ? w.c.of(t0 + threadIdx.x) : a;
     };
 
-    for (long long scan = t_begin; scan < t_end; scan += GRAD_SCAN * GRAD_CHUNK) {
+    if (threadIdx.x == 0) seen = 0;
+    for (long long scan = 0; scan < t_end; scan += GRAD_SCAN * GRAD_CHUNK) {
         __syncthreads();
-        for (int k = warp; k < GRAD_SCAN; k += 8) {
-            const long long t = scan + k * GRAD_CHUNK + lane;
-            const int id = t < t_end ? w.c.of(t) : -1;
-            const bool any = __any_sync(~0u, id == a), other = __any_sync(~0u, t < t_end && id != a);
-            if (lane == 0) flags[k] = any ? (other ? 2 : 1) : 0;
+        int id[GRAD_SCAN / 8];
+#pragma unroll
+        for (int k = 0; k < GRAD_SCAN / 8; ++k) {
+            const long long t = scan + (warp + k * 8) * GRAD_CHUNK + lane;
+            id[k] = t < t_end ? w.c.of(t) : -2;
+        }
+#pragma unroll
+        for (int k = 0; k < GRAD_SCAN / 8; ++k) {
+            // Columns past the end are read as zeros: they may count as the adapter's.
+            const bool any = __any_sync(~0u, id[k] == a);
+            const unsigned m = __ballot_sync(~0u, id[k] == a || id[k] == -2);
+            if (lane == 0) members[warp + k * 8] = any ? m : 0u;
         }
         __syncthreads();
         if (warp == 0) {
-            int n = 0;
+            int n = 0, all = seen;
+#pragma unroll
             for (int k = lane; k < GRAD_SCAN; k += 32) {
-                const unsigned m = __ballot_sync(~0u, flags[k] != 0);
-                if (flags[k]) list[n + __popc(m & ((1u << lane) - 1))] = (unsigned char)k;
-                n += __popc(m);
+                const bool any = members[k] != 0u;
+                const unsigned m = __ballot_sync(~0u, any), before = m & ((1u << lane) - 1);
+                // Every ranks-th chunk of the adapter's, over all scans, is this block's.
+                const bool own = any && (all + __popc(before)) % ranks == rank;
+                const unsigned o = __ballot_sync(~0u, own);
+                if (own) list[n + __popc(o & ((1u << lane) - 1))] = (unsigned char)k;
+                n += __popc(o);
+                all += __popc(m);
             }
-            if (lane == 0) count = n;
+            __syncwarp();
+            if (lane == 0) {
+                count = n;
+                seen = all;
+            }
         }
         __syncthreads();
         const int chunks = count;
@@ -737,12 +929,11 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
             fill_at(i + Q::STAGES - 1);
             const unsigned char *z = smem + (i % Q::STAGES) * Q::STAGE + warp * 16 * Q::PITCH;
             const unsigned char *s = smem + (i % Q::STAGES) * Q::STAGE + GRAD_ROWS * Q::PITCH;
-            const int *ids = (const int *)(s + Q::RP * Q::PITCH);
-            const bool mixed = flags[list[i]] == 2;
+            const unsigned member = members[list[i]];
 #pragma unroll
             for (int k = 0; k < GRAD_CHUNK; k += 8) {
                 Operand<SPLIT> A[4];
-                const bool in[2] = {!mixed || ids[k + q] == a, !mixed || ids[k + q + 4] == a};
+                const bool in[2] = {(member >> (k + q) & 1) != 0, (member >> (k + q + 4) & 1) != 0};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = to_float(*(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ)));
@@ -844,8 +1035,8 @@ tcaspmm_status with_rank(int R, F &&f)
     return f(std::integral_constant<int, 16>{});
 }
 
-// Columns of a tile: a warp's sums (RT x TN / 8 x 4 registers a thread) take at most 128 registers.
-constexpr int tile_columns(int rt) { return rt <= 4 ? 64 : rt == 8 ? 32 : 16; }
+// Columns of a tile: a warp's sums (RT x TN / 8 x 4 registers a thread) leave room for two blocks an SM, up to rank 64.
+constexpr int tile_columns(int rt) { return rt <= 2 ? 64 : rt <= 8 ? 32 : 16; }
 
 template <typename TF, typename TI, bool TRANS>
 tcaspmm_status apply(ApplyParams p, int sms, cudaStream_t st)
@@ -854,8 +1045,10 @@ tcaspmm_status apply(ApplyParams p, int sms, cudaStream_t st)
         constexpr int RT = rt.value, TN = tile_columns(RT);
         using Q = ApplyShape<TF, TI, RT, TN, TRANS>;
         const long long tiles = ceil_div(p.N, TN);
-        int ranks = 1;  // idle SMs take a share, while a warp has a step to do
-        while (ranks < 8 && tiles * ranks < 2 * sms && std::max(p.n1, p.n2) > (long long)ranks * APPLY_WARPS * 16) ranks *= 2;
+        // Idle SMs take a share, while a warp has a step to do.
+        int ranks = 1;
+        while (ranks < 8 && tiles * ranks * 2 <= sms * (RT <= 4 ? 2 : 1) && std::max(p.n1, p.n2) > (long long)ranks * APPLY_WARPS * 16)
+            ranks *= 2;
         p.per1 = ceil_div(ceil_div(p.n1, ranks), Q::KS) * Q::KS;
         p.per2 = ceil_div(ceil_div(p.n2, ranks), 16) * 16;
         if (tiles * ranks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many columns");
@@ -874,7 +1067,6 @@ tcaspmm_status grads(GradParams w, int sms, cudaStream_t st)
         if (tiles == 0 || w.c.L == 0) return TCASPMM_OK;
         int ranks = 1;
         while (ranks < 8 && tiles * ranks < 2 * sms && w.N > (long long)ranks * 2 * GRAD_CHUNK) ranks *= 2;
-        w.per = ceil_div(ceil_div(w.N, ranks), GRAD_CHUNK) * GRAD_CHUNK;
         if (tiles * ranks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora_backward: too many rows");
         return launch_cluster("lora_backward launch", lora_grad<TF, RT>, dim3((unsigned)(tiles * ranks), (unsigned)std::min(w.c.L, 65535)),
                               256, ranks, GradShape<RT>::BYTES, st, w);
