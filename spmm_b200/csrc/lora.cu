@@ -48,8 +48,13 @@ bool aligned(const void *p, int64_t ld, int type, int bytes)
 
 using namespace tca;
 
+extern "C" size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t N, tcaspmm_dtype dt)
+{
+    return rank < 1 || N < 1 || !dtype_valid(dt) ? 0 : Hidden::bytes(rank, N, type_code(dt));
+}
+
 extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *dX, int64_t ldx, int64_t N, const void *dBase,
-                                       int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, float *dH, void *stream)
+                                       int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, void *hidden, void *stream)
 {
     clear_error();
     const tcaspmm_status s = check(ad, N, "lora");
@@ -59,6 +64,7 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
         return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld or NULL pointer",
                     (long long)ldx, (long long)ldbase, (long long)ldy);
     if (N == 0) return TCASPMM_OK;
+    if (!hidden || (uintptr_t)hidden % 16) return fail(TCASPMM_ERR_INVALID_ARG, "lora: hidden must be a 16-byte aligned device pointer");
     const int ft = type_code(ad->dt), yt = type_code(y_dt);
     ApplyParams p = {};
     p.F1 = ad->down;
@@ -77,7 +83,7 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
     p.Out = dY;
     p.ldout = ldy;
     p.outtype = yt;
-    p.S = dH;
+    p.hidden = hidden;
     p.vec_in = aligned(dX, ldx, ft, 16);
     p.vec_f1 = aligned(ad->down, ad->K, ft, 16);
     p.vec_f2 = aligned(ad->up, ad->rank, ft, 16);
@@ -88,8 +94,8 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
 }
 
 extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt,
-                                                const void *dX, int64_t ldx, int64_t N, const float *dH, const float *dBase,
-                                                int64_t ldbase, void *dDX, int64_t lddx, void *ddown, void *dup, float *dP,
+                                                const void *dX, int64_t ldx, int64_t N, const void *hidden, const float *dBase,
+                                                int64_t ldbase, void *dDX, int64_t lddx, void *ddown, void *dup, void *scratch,
                                                 void *stream)
 {
     clear_error();
@@ -99,10 +105,12 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
     const int ft = type_code(ad->dt), gt = type_code(dy_dt);
     if (gt != 0 && gt != ft) return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: dY must be fp32 or of the factors' type");
     if (!matrix_ok(dDY, ad->M, N, lddy) || (ddown && !matrix_ok(dX, ad->K, N, ldx)) || (dBase && ldbase < N) ||
-        (dDX && lddx < N) || (dup && !dH && N > 0) || (!dP && N > 0 && (dDX || ddown)))
+        (dDX && lddx < N))
         return fail(TCASPMM_ERR_INVALID_ARG,
                     "lora_backward: bad leading dimension lddy=%lld ldx=%lld ldbase=%lld lddx=%lld or NULL pointer",
                     (long long)lddy, (long long)ldx, (long long)ldbase, (long long)lddx);
+    if (N > 0 && ((dup && !hidden) || ((dDX || ddown) && !scratch) || (uintptr_t)hidden % 16 || (uintptr_t)scratch % 16))
+        return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: hidden and scratch must be 16-byte aligned device pointers");
     const cudaStream_t st = (cudaStream_t)stream;
     const Columns c{ad->index, ad->index_bytes == 8, (int)ad->count};
     if ((dDX || ddown) && N > 0) {
@@ -122,7 +130,7 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
         p.Out = dDX;
         p.ldout = lddx;
         p.outtype = ft;
-        p.S = dP;
+        p.hidden = scratch;
         p.vec_in = aligned(dDY, lddy, gt, 16);
         p.vec_f1 = aligned(ad->up, ad->rank, ft, 16);
         p.vec_f2 = aligned(ad->down, ad->K, ft, 16);
@@ -136,9 +144,8 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
     w.c = c;
     w.R = (int)ad->rank;
     w.N = N;
-    w.vec_s = N % 4 == 0 && (uintptr_t)dP % 16 == 0 && (uintptr_t)dH % 16 == 0;
-    w.p[0] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), dP, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
-    w.p[1] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), dH, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
+    w.p[0] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), (const float *)scratch, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
+    w.p[1] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), (const float *)hidden, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
     const auto run = ft == 0 ? lora_factor_grads_f32 : ft == 1 ? lora_factor_grads_f16 : lora_factor_grads_bf16;
     return run(w, sm_count(), st);
 }

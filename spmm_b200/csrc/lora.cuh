@@ -9,6 +9,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstring>
 #include <type_traits>
@@ -50,9 +51,30 @@ struct ApplyParams {
     void *Out;  // or NULL
     long long ldout;
     int outtype;
-    float *S;  // R x N, or NULL
+    void *hidden;  // S (Hidden)
     int vec_in, vec_f1, vec_f2, vec_base, vec_out;  // what alignment allows
-    long long per1, per2;  // rows of In and of Out for each block of a cluster
+    long long per1;  // rows of In for each block of a cluster
+};
+
+// S in device memory between the kernels, rows of `pitch` columns (64 or a multiple, so that every row is aligned): fp32 for
+// the gradients and for fp32 factors, and for 16-bit factors two parts of their type whose sum it is (split16).  fp16 parts
+// are scaled: a column's, times its colscale, is S.  The parts' columns are dealt out within each 16 (place) so that the
+// second product's matrix instructions give a thread four neighbours.  Columns past N hold nothing that counts.
+struct Hidden {
+    long long pitch, rows;
+    unsigned char *p;
+    __host__ __device__ static long long pitch_of(long long N) { return (N + 63) / 64 * 64; }
+    __host__ static size_t bytes(long long R, long long N, int type)
+    {
+        return (size_t)pitch_of(N) * (R * (type == 0 ? 4 : 8) + (type == 1 ? 4 : 0));
+    }
+    __host__ __device__ Hidden(void *at, long long R, long long N) : pitch(pitch_of(N)), rows(R), p((unsigned char *)at) {}
+    // Where column c of the parts lies: c = 4 i + 2 b + e of each 16 is column 2 i + e of block b of 8.
+    __host__ __device__ static int place(int c) { return (c & ~15) + 8 * (c >> 1 & 1) + 2 * (c >> 2 & 3) + (c & 1); }
+    __host__ __device__ float *s() const { return (float *)p; }
+    template <typename T> __device__ T *hi() const { return (T *)(p + pitch * rows * 4); }
+    template <typename T> __device__ T *lo() const { return (T *)(p + pitch * rows * 6); }
+    __device__ float *colscale() const { return (float *)(p + pitch * rows * 8); }
 };
 
 // One of the two products of a backward pass: G[a][j, r] = sum over the columns of adapter a of Z[j, t] S[r, t].
@@ -61,7 +83,7 @@ struct GradProblem {
     long long ldz;
     int z32;  // Z is fp32 (else the factors' type)
     int vec;
-    const float *S;
+    const float *S;  // rows of Hidden's pitch
     long long n;
     void *G;  // or NULL: left out
     long long gj, gr;  // strides of G's elements (j, r) within an adapter
@@ -72,7 +94,6 @@ struct GradParams {
     GradProblem p[2];
     Columns c;
     int R;
-    int vec_s;
     long long N;
 };
 
@@ -85,11 +106,6 @@ __device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)
 __device__ __forceinline__ void copy16(void *dst, const void *src, int valid)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
-}
-// 8 bytes, all of them or (valid 0) zeros.
-__device__ __forceinline__ void copy8(void *dst, const void *src, int valid)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -175,25 +191,65 @@ __device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SPLIT> (&a
     mma8(d, hi, b0.v, b1.v);
 }
 
-// ------------------------------------------------------------------ Out = base + F2 (scale F1 In)
+// A 16-bit element of type code 1 (fp16) or 2 (bf16).
+__device__ __forceinline__ float as_float(unsigned bits, int type)
+{
+    return type == 1 ? __half2float(__ushort_as_half((unsigned short)bits)) : __bfloat162float(__ushort_as_bfloat16((unsigned short)bits));
+}
+
+template <typename T>
+__device__ __forceinline__ void store_four(T *p, const float (&y)[4])
+{
+    if constexpr (sizeof(T) == 4) {
+        *(float4 *)p = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+        T u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = from_float<T>(y[e]);
+        uint2 bits;
+        memcpy(&bits, u, sizeof bits);
+        *(uint2 *)p = bits;
+    }
+}
+
+// ------------------------------------------------------------------ S = scale F1 In
 //
-// A cluster of up to 8 blocks takes TN columns.  First each block multiplies its part of In's rows: its 8 warps take 16 rows
-// (8 in fp32) in turn, each through a ring of its own in shared memory (In's rows and F1's slice by asynchronous copies, no
-// barrier in the loop), with all R x TN sums in the warp's registers.  The sums are joined over warps, then over blocks
-// through distributed shared memory, in a fixed order, so that S never crosses device memory on its way to the second
-// product.  Then each block multiplies its part of Out's rows: a warp takes 16 rows, F2 and base through rings again, Out
-// written 16 bytes a thread (columns are dealt to the matrix instruction so that a thread's results lie side by side); the
-// first of these copies start before the sums are joined.  With several adapters among a tile's columns the products run
-// once for each, and a column keeps its own adapter's.
-//
-// In 16 bits S is held in two parts (split16), so that an fp32 Out is as exact as fp32 sums of exact products; fp16 parts
-// are scaled by a power of two for each column, as S may exceed fp16's range.  The tensor cores' legacy form (mma.sync) is
-// enough: the kernel does about R products for each byte of In, base and Out, and is bound by those.
-constexpr int APPLY_WARPS = 8;
-constexpr int APPLY_THREADS = APPLY_WARPS * 32;
+// A cluster of up to 8 blocks takes TN columns, each block a part of In's rows: its 8 warps take 16 rows (8 in fp32) in turn,
+// each through a ring of its own in shared memory (In's rows and F1's slice by asynchronous copies, no barrier in the loop),
+// with all R x TN sums in the warp's registers.  The sums are joined over warps, then over blocks through distributed shared
+// memory, in a fixed order.  With several adapters among a tile's columns the product runs once for each, and a column keeps
+// its own adapter's.  It does R products for each element of In, so the tensor cores' legacy form (mma.sync, 8 cycles an
+// instruction for each quarter of an SM) is enough: in 16 bits it keeps up with memory to rank 128.
+constexpr int WARPS = 8;
+constexpr int THREADS = WARPS * 32;
+
+// Of a tile's columns: their adapters (-1: none, or past the end), and those that occur, by their first columns.
+template <int TN>
+struct TileColumns {
+    int ids[TN], list[TN], count;
+    __device__ __forceinline__ void load(const Columns &c, long long t0, long long N)
+    {
+        for (int t = threadIdx.x; t < TN; t += THREADS) ids[t] = t0 + t < N ? c.of(t0 + t) : -1;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            const int lane = threadIdx.x;
+            int n = 0;
+            for (int b = 0; b < TN; b += 32) {
+                const int t = b + lane;
+                bool first = t < TN && ids[t] >= 0 && (t == 0 || ids[t] != ids[t - 1]);
+                for (int s = 0; first && s < t; ++s) first = ids[s] != ids[t];
+                const unsigned m = __ballot_sync(~0u, first);
+                if (first) list[n + __popc(m & ((1u << lane) - 1))] = ids[t];
+                n += __popc(m);
+            }
+            if (lane == 0) count = n;
+        }
+        __syncthreads();
+    }
+};
 
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
-struct ApplyShape {
+struct ShrinkShape {
     static constexpr bool M16 = sizeof(TF) == 2 && sizeof(TI) == 2;  // 16-bit matrix instructions (else TF32)
     static constexpr bool SPLIT = sizeof(TF) == 4;
     static constexpr int KS = sizeof(TF) == 4 ? 8 : 16;  // rows of In a step
@@ -205,72 +261,37 @@ struct ApplyShape {
     static constexpr int F_COLS = TRANS ? RP : KS;
     static constexpr int F_PITCH = F_COLS * (int)sizeof(TF) + (!TRANS && RT > 8 ? 0 : TRANS && sizeof(TF) == 4 ? 32 : 16);
     static constexpr int STAGE = KS * IN_PITCH + F_ROWS * F_PITCH;
-    // Second product: F2 in pieces of RC along r.
-    static constexpr int RC_MOST = sizeof(TF) == 4 ? 16 : 64;
-    static constexpr int RC = RP < RC_MOST ? RP : RC_MOST;
-    static constexpr int PIECES = RP / RC;
-    static constexpr int G_ROWS = TRANS ? RC : 16;
-    static constexpr int G_COLS = TRANS ? 16 : RC;
-    static constexpr int G_PITCH = G_COLS * (int)sizeof(TF) + (TRANS && sizeof(TF) == 4 ? 32 : 16);
-    static constexpr int STAGE2 = G_ROWS * G_PITCH + 16 * TN * 4;
     static constexpr int S_PITCH = TN + 8;  // floats
     static constexpr int S_BYTES = RP * S_PITCH * 4;
-    static constexpr int H_PITCH = TN * 2 + 16;  // bytes
     // Two blocks an SM where a thread's sums leave the registers for it, else one.
-    static constexpr int BUDGET = (RT <= 4 ? 110 : 222) * 1024 - 2 * S_BYTES;
-    static constexpr int fit(int stage) { return BUDGET / (APPLY_WARPS * stage) >= 4 ? 4 : BUDGET / (APPLY_WARPS * stage); }
-    static constexpr int STAGES = fit(STAGE);
-    static constexpr int STAGES2 = fit(STAGE2);
-    static_assert(STAGES >= 2 && STAGES2 >= 2, "the rings do not fit");
-    static constexpr int most(int a, int b) { return a > b ? a : b; }
-    static constexpr int RING = most(most(APPLY_WARPS * STAGES * STAGE, APPLY_WARPS * STAGES2 * STAGE2), 4 * S_BYTES);
-    static constexpr int BYTES = RING + 2 * S_BYTES;
+    static constexpr int BUDGET = (RT <= 4 ? 110 : 222) * 1024;
+    static constexpr int FIT = BUDGET / (WARPS * STAGE);
+    static constexpr int STAGES = FIT >= 4 ? 4 : FIT;
+    static_assert(STAGES >= 2, "the ring does not fit");
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int BYTES = RING > 4 * S_BYTES ? RING : 4 * S_BYTES;  // the ring, then four warps' sums
 };
 
-// Element `type` at p as fp32 in shared memory's copy of it.
-__device__ __forceinline__ float raw_as(const unsigned char *p, int type, int e)
-{
-    if (type == 0) return ((const float *)p)[e];
-    const unsigned short u = ((const unsigned short *)p)[e];
-    return type == 1 ? __half2float(__ushort_as_half(u)) : __bfloat162float(__ushort_as_bfloat16(u));
-}
-
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
-__global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(const ApplyParams p)
+__global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_shrink(const ApplyParams p)
 {
-    using Q = ApplyShape<TF, TI, RT, TN, TRANS>;
+    using Q = ShrinkShape<TF, TI, RT, TN, TRANS>;
     constexpr int NB = TN / 8, RP = Q::RP, KS = Q::KS;
     constexpr bool HALF = std::is_same<TF, __half>::value;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int ids[TN], list[TN], count;
-    __shared__ float colscale[TN];
+    __shared__ TileColumns<TN> tile;
     __shared__ int colmax[TN];
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2;
     const long long t0 = (long long)(blockIdx.x / ranks) * TN;
+    cudaTriggerProgrammaticLaunchCompletion();  // the next kernel may start: it waits for this one before it reads S
+    if (threadIdx.x < TN) colmax[threadIdx.x] = 0;
+    tile.load(p.c, t0, p.N);
+    const int *const ids = tile.ids, *const list = tile.list;
+    const int nd = tile.count;
 
-    for (int t = threadIdx.x; t < TN; t += APPLY_THREADS) {
-        ids[t] = t0 + t < p.N ? p.c.of(t0 + t) : -1;
-        colmax[t] = 0;
-    }
-    __syncthreads();
-    if (warp == 0) {  // the tile's adapters, in the order of their first columns
-        int n = 0;
-        for (int b = 0; b < TN; b += 32) {
-            const int t = b + lane;
-            bool first = t < TN && ids[t] >= 0 && (t == 0 || ids[t] != ids[t - 1]);
-            for (int s = 0; first && s < t; ++s) first = ids[s] != ids[t];
-            const unsigned m = __ballot_sync(~0u, first);
-            if (first) list[n + __popc(m & ((1u << lane) - 1))] = ids[t];
-            n += __popc(m);
-        }
-        if (lane == 0) count = n;
-    }
-    __syncthreads();
-    const int nd = count;
-
-    // ---- S: this block's rows of In
+    // ---- this block's rows of In
     float acc[RT][NB][4];
 #pragma unroll
     for (int m = 0; m < RT; ++m)
@@ -280,7 +301,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
             for (int e = 0; e < 4; ++e) acc[m][b][e] = 0.0f;
     const long long i_begin = min(p.n1, rank * p.per1), i_end = min(p.n1, i_begin + p.per1);
     const int steps = (int)((i_end - i_begin + KS - 1) / KS);
-    const int mine = steps > warp ? (steps - warp + APPLY_WARPS - 1) / APPLY_WARPS : 0;
+    const int mine = steps > warp ? (steps - warp + WARPS - 1) / WARPS : 0;
     const int items = mine * nd;
     unsigned char *ring = smem + warp * (Q::STAGES * Q::STAGE);
 
@@ -295,7 +316,7 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
 
     auto fill = [&](int slot, int step, int a) {
         unsigned char *in = ring + slot * Q::STAGE, *f = in + KS * Q::IN_PITCH;
-        const long long i0 = i_begin + (long long)(warp + step * APPLY_WARPS) * KS;
+        const long long i0 = i_begin + (long long)(warp + step * WARPS) * KS;
         const int rows = (int)min((long long)KS, i_end - i0);
         if (p.vec_in) {
             const TI *src = in_src + i0 * p.ldin;
@@ -438,9 +459,8 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
     }
     __syncthreads();
 
-    // ---- S joined over the warps: 4 to 7 leave theirs, 0 to 3 add them to their own, all threads add those four
+    // ---- S joined over the warps: 4 to 7 leave theirs, 0 to 3 add them to their own
     float *slot = (float *)smem;
-    float *part = (float *)(smem + Q::RING), *Hf = part + Q::S_BYTES / 4;
     constexpr int SLOT = Q::S_BYTES / 4, PITCH = Q::S_PITCH;
     auto frag = [&](float *s, bool add) {
 #pragma unroll
@@ -463,10 +483,9 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
     __syncthreads();
     if (warp < 4) frag(slot + warp * SLOT, true);
     __syncthreads();
-    for (int i = threadIdx.x; i < RP * TN; i += APPLY_THREADS) {
-        const int at = i / TN * PITCH + i % TN;
-        const float *s = slot + at;
-        part[at] = (s[0] + s[SLOT]) + (s[2 * SLOT] + s[3 * SLOT]);
+    for (int i = threadIdx.x; i < RP * TN; i += THREADS) {
+        float *s = slot + i / TN * PITCH + i % TN;
+        s[0] = (s[0] + s[SLOT]) + (s[2 * SLOT] + s[3 * SLOT]);
     }
     auto sync_all = [&]() {
         if (ranks > 1)
@@ -476,188 +495,166 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
     };
     sync_all();
 
-    // ---- the second product's first copies: rows j0 of base, F2's slices
-    const long long j_begin = min(p.n2, rank * p.per2), j_end = min(p.n2, j_begin + p.per2);
-    constexpr int PAIRS = TN / 16;
-    const int tiles = p.Out && j_end > j_begin + warp * 16 ? (int)((j_end - j_begin - warp * 16 + APPLY_WARPS * 16 - 1) / (APPLY_WARPS * 16)) : 0;
-    const int passes = nd > 1 ? nd : 1;  // over a tile of rows, one for each adapter
-    const int items2 = tiles * passes * Q::PIECES;
-    unsigned char *ring2 = smem + warp * (Q::STAGES2 * Q::STAGE2);
-    const int base_size = p.basetype == 0 ? 4 : 2;
-
-    const bool inner = t0 + TN <= p.N && p.vec_base;  // base's pieces are whole
-    const unsigned char *const base_row = (const unsigned char *)p.base + ((j_begin + warp * 16 + g) * p.ldbase + t0 + 4 * q) * base_size;
-    const long long g_ld = TRANS ? p.n2 : p.R;
-
-    // Piece `piece` of adapter d's F2 and, for a tile's first item, base: a thread copies what it will add to.
-    auto fill2 = [&](int slot, int tile, int d, int piece) {
-        unsigned char *f = ring2 + slot * Q::STAGE2, *old = f + Q::G_ROWS * Q::G_PITCH + lane * 16;
-        const long long j0 = j_begin + warp * 16 + (long long)tile * (APPLY_WARPS * 16);
-        const int rows = (int)min(16ll, j_end - j0);
-        if (nd > 0) {
-            const int r0 = piece * Q::RC;
-            const TF *F = (const TF *)p.F2 + (long long)list[d] * p.R * p.n2 + (TRANS ? r0 * p.n2 + j0 : j0 * p.R + r0);
-            constexpr int PER = 16 / (int)sizeof(TF), CH = Q::G_COLS / PER, COUNT = Q::G_ROWS * CH;
-            if (p.vec_f2 && rows == 16 && CH <= 32 && COUNT % 32 == 0) {  // a lane's pieces lie in one column
-                const int r = lane / CH, c = lane % CH * PER;
-                const int left = p.R - r0 - c, bytes = TRANS ? 16 : left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
-                const TF *src = F + r * g_ld + c;
-                unsigned char *to = f + r * Q::G_PITCH + c * (int)sizeof(TF);
+    // ---- S joined over the blocks: each takes TN / ranks columns (a power of two: a thread keeps one)
+    const int own = TN / ranks;
+    const int c = rank * own + (threadIdx.x & (own - 1)), a = ids[c];
+    const int r_first = threadIdx.x / own, r_step = THREADS / own;
+    const float scale = a < 0 ? 0.0f : p.scale ? __ldg(p.scale + a) : 1.0f;
+    const Hidden h(p.hidden, p.R, p.N);
+    const int place = Hidden::place(c);
+    const bool keep = t0 + c < h.pitch;
+    float most = 0.0f;
+    for (int r = r_first; r < p.R; r += r_step) {
+        float v = 0.0f;
+        if (ranks == 1) {
+            v = slot[r * PITCH + c];
+        } else {
+            float x[8];
 #pragma unroll
-                for (int k = 0; k < COUNT / 32; ++k) {
-                    const int valid = TRANS && r0 + r + k * (32 / CH) >= p.R ? 0 : bytes;
-                    copy16(to + k * (32 / CH) * Q::G_PITCH, valid ? src : (const TF *)p.F2, valid);
-                    src += (32 / CH) * g_ld;
-                }
-            } else if (p.vec_f2) {
+            for (int k = 0; k < 8; ++k) x[k] = k < ranks ? cluster.map_shared_rank(slot, k)[r * PITCH + c] : 0.0f;
 #pragma unroll
-                for (int k = 0; k < (COUNT + 31) / 32; ++k) {
-                    const int r = (lane + k * 32) / CH, c = (lane + k * 32) % CH * PER;
-                    const int left = TRANS ? (r0 + r < p.R ? rows - c : 0) : (r < rows ? p.R - r0 - c : 0);
-                    const int valid = left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
-                    if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
-                        copy16(f + r * Q::G_PITCH + c * (int)sizeof(TF), valid ? F + r * g_ld + c : (const TF *)p.F2, valid);
-                }
-            } else {
-                for (int k = lane; k < Q::G_ROWS * Q::G_COLS; k += 32) {
-                    const int r = k / Q::G_COLS, c = k - r * Q::G_COLS;
-                    TF v = from_float<TF>(0.0f);
-                    if (TRANS ? (r0 + r < p.R && c < rows) : (r < rows && r0 + c < p.R)) v = F[r * g_ld + c];
-                    *(TF *)(f + r * Q::G_PITCH + c * sizeof(TF)) = v;
-                }
-            }
+            for (int k = 0; k < 8; ++k) v += x[k];
         }
-        if (!p.base || d > 0 || piece > 0) return;
-        const unsigned char *from = base_row + (long long)tile * (APPLY_WARPS * 16) * p.ldbase * base_size;
-        const long long down = 8 * p.ldbase * base_size;
-        if (inner) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int valid = g + h * 8 < rows ? 16 : 0;
-                const unsigned char *row = valid ? from + h * down : (const unsigned char *)p.base;
-#pragma unroll
-                for (int b = 0; b < PAIRS; ++b) {
-                    if (base_size == 4)
-                        copy16(old + (b * 2 + h) * 512, row + (valid ? b * 64 : 0), valid);
-                    else
-                        copy8(old + (b * 2 + h) * 512, row + (valid ? b * 32 : 0), valid >> 1);
-                }
-            }
-            return;
-        }
-        for (int i = 0; i < PAIRS * 2; ++i) {
-            const long long t = t0 + (i >> 1) * 16 + 4 * q;
-            const bool row = g + (i & 1) * 8 < rows, whole = p.vec_base && t + 3 < p.N;
-            const unsigned char *src = from + (i & 1) * down + (i >> 1) * 16 * base_size;
-            unsigned char *to = old + i * 512;
-            if (whole) {
-                if (base_size == 4)
-                    copy16(to, row ? src : (const unsigned char *)p.base, row ? 16 : 0);
-                else
-                    copy8(to, row ? src : (const unsigned char *)p.base, row ? 8 : 0);
-            } else {
-                for (int e = 0; e < 4; ++e)
-                    if (row && t + e < p.N) {
-                        if (base_size == 4)
-                            ((float *)to)[e] = ((const float *)src)[e];
-                        else
-                            ((unsigned short *)to)[e] = ((const unsigned short *)src)[e];
-                    }
-            }
-        }
-    };
-    int filled2 = 0, slot2 = 0, next_tile = 0, next_pass = 0, next_piece = 0;
-    auto fill2_next = [&]() {
-        if (filled2 < items2) {
-            fill2(slot2, next_tile, next_pass, next_piece);
-            if (++next_piece == Q::PIECES) {
-                next_piece = 0;
-                if (++next_pass == passes) {
-                    next_pass = 0;
-                    ++next_tile;
-                }
-            }
-            ++filled2;
-            if (++slot2 == Q::STAGES2) slot2 = 0;
-        }
-        copy_commit();
-    };
-    for (int s = 0; s < Q::STAGES2 - 1; ++s) fill2_next();
-
-    // ---- S joined over the blocks: each takes TN / ranks columns, scales them and gives them to all
-    const int own = TN / ranks;  // a power of two: a thread keeps one column
-    {
-        const int c = rank * own + (threadIdx.x & (own - 1)), a = ids[c];
-        const int r_first = threadIdx.x / own, r_step = APPLY_THREADS / own;
-        const float s = a < 0 ? 0.0f : p.scale ? __ldg(p.scale + a) : 1.0f;
-        const bool keep = p.S && t0 + c < p.N;
-        float *const S = p.S + t0 + c;
-        float most = 0.0f;
-        for (int r = r_first; r < RP; r += r_step) {
-            float v = 0.0f;
-            if (ranks == 1) {
-                v = part[r * PITCH + c];
-            } else {
-                float x[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = k < ranks ? cluster.map_shared_rank(part, k)[r * PITCH + c] : 0.0f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v += x[k];
-            }
-            v = a >= 0 ? v * s : 0.0f;  // whatever a column without an adapter has gathered
-            if (keep && r < p.R) S[(long long)r * p.N] = v;
-            if (HALF || ranks == 1) {
-                Hf[r * PITCH + c] = v;
-                most = fmaxf(most, fabsf(v));
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k < ranks) cluster.map_shared_rank(Hf, k)[r * PITCH + c] = v;
-            }
-        }
+        v = a >= 0 ? v * scale : 0.0f;  // whatever a column without an adapter has gathered
+        if (keep) h.s()[r * h.pitch + t0 + c] = v;
         if (HALF) {
-            atomicMax(&colmax[c], __float_as_int(most));  // the order does not matter
-            __syncthreads();
-            // The column's largest value goes to [2^13, 2^14); zeros and infinities stay.
-            const int e = (colmax[c] >> 23) - 127;
-            const int shift = e == -127 || e == 128 ? 0 : max(-100, min(100, e - 13));
-            const float down = __int_as_float((127 - shift) << 23);
-            for (int r = r_first; r < RP; r += r_step) {
-                const float v = Hf[r * PITCH + c] * down;
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k < ranks) cluster.map_shared_rank(Hf, k)[r * PITCH + c] = v;
-            }
-            if (r_first == 0) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k < ranks) cluster.map_shared_rank(colscale, k)[c] = __int_as_float((127 + shift) << 23);
-            }
+            slot[SLOT + r * PITCH + c] = v;
+            most = fmaxf(most, fabsf(v));
+        } else if (sizeof(TF) == 2 && keep) {
+            TF hi, lo;
+            split16<TF>(v, hi, lo);
+            h.hi<TF>()[r * h.pitch + t0 + place] = hi;
+            h.lo<TF>()[r * h.pitch + t0 + place] = lo;
         }
     }
-    sync_all();
-    if (!p.Out) return;
-
-    // ---- S as the second product's operand.  Column c of a pair of 8-column blocks holds the tile's column
-    // 4 (c % 8 / 2) + 2 (c / 8) + c % 2, so that a thread's results of the pair are four neighbours.
-    unsigned char *hi = (unsigned char *)part, *lo = hi + RP * Q::H_PITCH;
-    if constexpr (sizeof(TF) == 2) {
-        for (int i = threadIdx.x; i < RP * TN; i += APPLY_THREADS) {
-            const int r = i / TN, c = i % TN, t = (c & ~15) + 4 * (c >> 1 & 3) + 2 * (c >> 3 & 1) + (c & 1);
-            TF h, l;
-            split16<TF>(Hf[r * PITCH + t], h, l);
-            *(TF *)(hi + r * Q::H_PITCH + c * 2) = h;
-            *(TF *)(lo + r * Q::H_PITCH + c * 2) = l;
-        }
+    if (HALF) {
+        atomicMax(&colmax[c], __float_as_int(most));  // the order does not matter
         __syncthreads();
+        // The column's largest value goes to [2^13, 2^14); zeros and infinities stay.
+        const int e = (colmax[c] >> 23) - 127;
+        const int shift = e == -127 || e == 128 ? 0 : max(-100, min(100, e - 13));
+        const float down = __int_as_float((127 - shift) << 23);
+        if (keep) {
+            for (int r = r_first; r < p.R; r += r_step) {
+                TF hi, lo;
+                split16<TF>(slot[SLOT + r * PITCH + c] * down, hi, lo);
+                h.hi<TF>()[r * h.pitch + t0 + place] = hi;
+                h.lo<TF>()[r * h.pitch + t0 + place] = lo;
+            }
+            if (r_first == 0) h.colscale()[t0 + c] = __int_as_float((127 + shift) << 23);
+        }
     }
+    if (ranks > 1) cluster.sync();  // the others have read this block's sums
+}
 
-    // ---- Out: this block's rows
-    float old[PAIRS][2][4] = {};  // rows g, g + 8; columns 16 pair + 4 q ...
-    float sum[PAIRS][2][4];       // [pair][block of the pair][e]: rows g, g + 8; columns 16 pair + 4 q + 2 block + (e & 1)
-    const int out_size = p.outtype == 0 ? 4 : 2;
-    unsigned char *const out_row = (unsigned char *)p.Out + ((j_begin + warp * 16 + g) * p.ldout + t0 + 4 * q) * out_size;
-    // A bit for each of a thread's columns (4 q + (k & 3) of pair k / 4): it exists, has an adapter, is written now.
+// ------------------------------------------------------------------ Out = base + F2 S
+//
+// A block takes 128 rows of Out and 64 columns, a warp 16 rows.  base is read into registers and F2's slice copied to shared
+// memory before the block waits for the kernel that makes S (programmatic dependent launch), so that the start of this
+// kernel hides behind the end of that one.  Columns are dealt to the matrix instruction so that a thread's results of two
+// blocks of 8 lie side by side: base and Out move 16 bytes a thread.  In 16 bits both parts of S are multiplied, so that an
+// fp32 Out is as exact as fp32 sums of exact products.  With several adapters among the columns the product runs once for
+// each, for the pairs of blocks that have any of its columns.  Bound by base and Out: R / 8 products a byte.
+constexpr int EXP_COLS = 64;
+constexpr int EXP_ROWS = WARPS * 16;
+constexpr int EXP_PAIRS = EXP_COLS / 16;
+
+template <typename TF, int RC, bool TRANS>  // RC: r's a piece
+struct ExpandShape {
+    static constexpr int F_ROWS = TRANS ? RC : 16;
+    static constexpr int F_COLS = TRANS ? 16 : RC;
+    static constexpr int F_PITCH = F_COLS * (int)sizeof(TF) + (TRANS && sizeof(TF) == 4 ? 32 : 16);
+    static constexpr int F_BYTES = F_ROWS * F_PITCH;
+    static constexpr int S_PITCH = EXP_COLS * (int)sizeof(TF) + (sizeof(TF) == 4 ? 32 : 16);
+    static constexpr int S_BYTES = RC * S_PITCH;  // one part
+    static constexpr int BYTES = WARPS * F_BYTES + S_BYTES * (sizeof(TF) == 2 ? 2 : 1);
+};
+
+template <typename TF, int RC, bool TRANS>
+__global__ void __launch_bounds__(THREADS, 2) lora_expand(const ApplyParams p)
+{
+    using Q = ExpandShape<TF, RC, TRANS>;
+    constexpr bool HALF = std::is_same<TF, __half>::value;
+    constexpr int PAIRS = EXP_PAIRS;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ TileColumns<EXP_COLS> tile;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2;
+    const unsigned across = (unsigned)((p.N + EXP_COLS - 1) / EXP_COLS);  // neighbouring blocks share rows
+    const long long t0 = (long long)(blockIdx.x % across) * EXP_COLS, j0 = (long long)(blockIdx.x / across) * EXP_ROWS + warp * 16;
+    const int rows = (int)max(0ll, min(16ll, p.n2 - j0));
+    unsigned char *const f = smem + warp * Q::F_BYTES, *const sh = smem + WARPS * Q::F_BYTES, *const sl = sh + Q::S_BYTES;
+
+    float old[PAIRS][2][4];  // rows g, g + 8; columns 16 pair + 4 q ...
+    const int base_size = p.basetype == 0 ? 4 : 2;
+    const unsigned char *const base = (const unsigned char *)p.base + ((j0 + g) * p.ldbase + t0 + 4 * q) * base_size;
+    const bool inner = t0 + EXP_COLS <= p.N && p.vec_base;
+#pragma unroll
+    for (int b = 0; b < PAIRS; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool in = p.base && g + h * 8 < rows;
+            const unsigned char *at = base + (h * 8 * p.ldbase + b * 16) * base_size;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (in && inner) {
+                if (base_size == 4) {
+                    v = *(const float4 *)at;
+                } else {
+                    const uint2 u = *(const uint2 *)at;
+                    v = make_float4(as_float(u.x & 0xffffu, p.basetype), as_float(u.x >> 16, p.basetype), as_float(u.y & 0xffffu, p.basetype),
+                                    as_float(u.y >> 16, p.basetype));
+                }
+            } else if (in) {
+                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (t0 + b * 16 + 4 * q + e < p.N)
+                        x[e] = base_size == 4 ? ((const float *)at)[e] : as_float(((const unsigned short *)at)[e], p.basetype);
+                v = make_float4(x[0], x[1], x[2], x[3]);
+            }
+            old[b][h][0] = v.x;
+            old[b][h][1] = v.y;
+            old[b][h][2] = v.z;
+            old[b][h][3] = v.w;
+        }
+
+    const long long f_ld = TRANS ? p.n2 : p.R;
+    auto fill_f = [&](int a, int r0) {  // the warp's rows of adapter a's F2, RC from r0 on
+        const TF *F = (const TF *)p.F2 + (long long)a * p.R * p.n2 + (TRANS ? r0 * p.n2 + j0 : j0 * p.R + r0);
+        constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, COUNT = Q::F_ROWS * CH;
+        if (p.vec_f2) {
+#pragma unroll
+            for (int k = 0; k < (COUNT + 31) / 32; ++k) {
+                const int r = (lane + k * 32) / CH, c = (lane + k * 32) % CH * PER;
+                const int left = TRANS ? (r0 + r < p.R ? rows - c : 0) : (r < rows ? p.R - r0 - c : 0);
+                const int valid = left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
+                if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
+                    copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F2, valid);
+            }
+        } else {
+            for (int k = lane; k < Q::F_ROWS * Q::F_COLS; k += 32) {
+                const int r = k / Q::F_COLS, c = k - r * Q::F_COLS;
+                TF v = from_float<TF>(0.0f);
+                if (TRANS ? (r0 + r < p.R && c < rows) : (r < rows && r0 + c < p.R)) v = F[r * f_ld + c];
+                *(TF *)(f + r * Q::F_PITCH + c * sizeof(TF)) = v;
+            }
+        }
+    };
+    const Hidden hid(p.hidden, p.R, p.N);
+    auto fill_s = [&](int r0) {  // the block's columns of S, rows r0 .. r0 + RC - 1
+        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER, PARTS = sizeof(TF) == 2 ? 2 : 1;
+        for (int k = threadIdx.x; k < PARTS * RC * CH; k += THREADS) {
+            const int part = k / (RC * CH), r = k % (RC * CH) / CH, c = k % CH * PER;
+            const TF *src = sizeof(TF) == 4 ? (const TF *)hid.s() : part ? hid.template lo<TF>() : hid.template hi<TF>();
+            const int valid = r0 + r < p.R ? 16 : 0;
+            copy16((part ? sl : sh) + r * Q::S_PITCH + c * (int)sizeof(TF), valid ? src + (r0 + r) * hid.pitch + t0 + c : src, valid);
+        }
+    };
+
+    tile.load(p.c, t0, p.N);
+    const int *const ids = tile.ids, *const list = tile.list;
+    const int nd = tile.count, pieces = (p.R + RC - 1) / RC;
+    if (nd > 0) fill_f(list[0], 0);
+    // A bit for each of a thread's columns (4 q + (k & 3) of pair k / 4): it exists, has an adapter.
     unsigned exist = 0u, has = 0u;
 #pragma unroll
     for (int k = 0; k < PAIRS * 4; ++k) {
@@ -665,34 +662,40 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
         if (t0 + c < p.N) exist |= 1u << k;
         if (ids[c] >= 0) has |= 1u << k;
     }
-    unsigned write = exist;
-    auto store = [&](auto type, unsigned char *to, int rows) {
+    cudaGridDependencySynchronize();
+    float colscale[PAIRS][4];
+    if (HALF) {
+#pragma unroll
+        for (int b = 0; b < PAIRS; ++b) {
+            const float4 v = nd > 0 ? *(const float4 *)(hid.colscale() + t0 + b * 16 + 4 * q) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            colscale[b][0] = v.x;
+            colscale[b][1] = v.y;
+            colscale[b][2] = v.z;
+            colscale[b][3] = v.w;
+        }
+    }
+
+    const int out_size = p.outtype == 0 ? 4 : 2;
+    unsigned char *const out = (unsigned char *)p.Out + ((j0 + g) * p.ldout + t0 + 4 * q) * out_size;
+    float sum[PAIRS][2][4];  // [pair][block of the pair][e]: rows g, g + 8; columns 16 pair + 4 q + 2 block + (e & 1)
+    auto store = [&](auto type, unsigned write) {
         using TO = std::conditional_t<type.value == 0, float, std::conditional_t<type.value == 1, __half, __nv_bfloat16>>;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (g + h * 8 >= rows) continue;
-            TO *row = (TO *)to + h * 8 * p.ldout;
+            TO *row = (TO *)out + h * 8 * p.ldout;
 #pragma unroll
             for (int b = 0; b < PAIRS; ++b) {
                 float y[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float v = sum[b][e >> 1][2 * h + (e & 1)];
-                    if (HALF) v *= colscale[b * 16 + 4 * q + e];
+                    if (HALF) v *= colscale[b][e];
                     y[e] = has >> (b * 4 + e) & 1 ? old[b][h][e] + v : old[b][h][e];
                 }
                 const unsigned w = write >> (b * 4) & 15u;
                 if (p.vec_out && w == 15u) {
-                    if constexpr (type.value == 0) {
-                        *(float4 *)(row + b * 16) = make_float4(y[0], y[1], y[2], y[3]);
-                    } else {
-                        TO u[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) u[e] = from_float<TO>(y[e]);
-                        uint2 bits;
-                        memcpy(&bits, u, sizeof bits);
-                        *(uint2 *)(row + b * 16) = bits;
-                    }
+                    store_four(row + b * 16, y);
                 } else if (w) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -701,52 +704,56 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
             }
         }
     };
-    int tile = 0, pass = 0, piece = 0, at = 0;
-    for (int it = 0; it < items2; ++it) {
-        copy_wait<Q::STAGES2 - 2>();
-        __syncwarp();
-        fill2_next();
-        const unsigned char *f = ring2 + at * Q::STAGE2;
-        if (++at == Q::STAGES2) at = 0;
-        if (pass == 0 && piece == 0 && p.base) {
-            const unsigned char *mine = f + Q::G_ROWS * Q::G_PITCH + lane * 16;
-            if (p.basetype == 0) {
+
+    for (int pass = 0; pass < max(nd, 1); ++pass) {
+        const int a = nd > 0 ? list[pass] : -1;
+        unsigned some = ~0u, write = exist;  // pairs with columns of adapter a; columns that this pass writes
+        if (nd > 1) {
+            some = write = 0u;
 #pragma unroll
-                for (int i = 0; i < PAIRS * 2; ++i) {
-                    const float4 v = *(const float4 *)(mine + i * 512);
-                    old[i >> 1][i & 1][0] = v.x;
-                    old[i >> 1][i & 1][1] = v.y;
-                    old[i >> 1][i & 1][2] = v.z;
-                    old[i >> 1][i & 1][3] = v.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < PAIRS * 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) old[i >> 1][i & 1][e] = raw_as(mine + i * 512, p.basetype, e);
+            for (int k = 0; k < PAIRS * 4; ++k) {
+                const int id = ids[(k >> 2) * 16 + 4 * q + (k & 3)];
+                // Those without an adapter are written in the first pass.
+                if (id == a || (id < 0 && pass == 0)) write |= 1u << k;
+                if (id == a) some |= 1u << (k >> 2);
             }
+            write &= exist;
+            some = __reduce_or_sync(~0u, some);
         }
-        if (piece == 0) {
 #pragma unroll
-            for (int b = 0; b < PAIRS; ++b)
+        for (int b = 0; b < PAIRS; ++b)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[b][h][e] = 0.0f;
-        }
-        if (nd > 0) {
+                for (int e = 0; e < 4; ++e) sum[b][h][e] = 0.0f;
+        for (int piece = 0; piece < (nd > 0 ? pieces : 0); ++piece) {
+            if (pass > 0 || piece > 0) {
+                __syncwarp();
+                fill_f(a, piece * RC);
+            }
+            if (pieces > 1 || pass == 0) {
+                if (pass > 0 || piece > 0) __syncthreads();  // the last piece has been read by all
+                fill_s(piece * RC);
+            }
+            copy_commit();
+            copy_wait<0>();
+            if (pieces > 1 || pass == 0)
+                __syncthreads();
+            else
+                __syncwarp();
             if constexpr (sizeof(TF) == 2) {
 #pragma unroll
-                for (int k = 0; k < Q::RC / 16; ++k) {
+                for (int k = 0; k < RC / 16; ++k) {
                     unsigned A[4];
-                    load_matrices<TRANS>(A, TRANS ? f + (k * 16 + (lane & 7) + (lane >> 4) * 8) * Q::G_PITCH + (lane >> 3 & 1) * 16
-                                                  : f + (lane & 15) * Q::G_PITCH + (k * 16 + (lane >> 4) * 8) * 2);
-                    const int row = (piece * Q::RC + k * 16 + (lane & 15)) * Q::H_PITCH + (lane >> 4) * 16;
+                    load_matrices<TRANS>(A, TRANS ? f + (k * 16 + (lane & 7) + (lane >> 4) * 8) * Q::F_PITCH + (lane >> 3 & 1) * 16
+                                                  : f + (lane & 15) * Q::F_PITCH + (k * 16 + (lane >> 4) * 8) * 2);
+                    const int row = (k * 16 + (lane & 15)) * Q::S_PITCH + (lane >> 4) * 16;
 #pragma unroll
                     for (int b = 0; b < PAIRS; ++b) {
+                        if (!(some >> b & 1)) continue;
                         unsigned L[4], H[4];
-                        load_matrices<true>(L, lo + row + b * 32);
-                        load_matrices<true>(H, hi + row + b * 32);
+                        load_matrices<true>(L, sl + row + b * 32);
+                        load_matrices<true>(H, sh + row + b * 32);
                         mma16<TF>(sum[b][0], A, L[0], L[1]);
                         mma16<TF>(sum[b][1], A, L[2], L[3]);
                         mma16<TF>(sum[b][0], A, H[0], H[1]);
@@ -755,51 +762,33 @@ __global__ void __launch_bounds__(APPLY_THREADS, RT <= 4 ? 2 : 1) lora_apply(con
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < Q::RC; k += 8) {
+                for (int k = 0; k < RC; k += 8) {
                     Operand<true> A[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int j = g + (e & 1) * 8, r = k + q + (e >> 1) * 4;
-                        A[e].set(*(const float *)(TRANS ? f + r * Q::G_PITCH + j * 4 : f + j * Q::G_PITCH + r * 4));
+                        A[e].set(*(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4));
                     }
 #pragma unroll
                     for (int b = 0; b < PAIRS; ++b)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float *s = Hf + (piece * Q::RC + k + q) * PITCH + b * 16 + 4 * (g >> 1) + 2 * h + (g & 1);
+                            const unsigned char *s = sh + (k + q) * Q::S_PITCH + (b * 16 + 4 * (g >> 1) + 2 * h + (g & 1)) * 4;
                             Operand<true> B[2];
-                            B[0].set(s[0]);
-                            B[1].set(s[4 * PITCH]);
+                            B[0].set(*(const float *)s);
+                            B[1].set(*(const float *)(s + 4 * Q::S_PITCH));
                             mma8_any<true>(sum[b][h], A, B[0], B[1]);
                         }
                 }
             }
         }
-        if (++piece < Q::PIECES) continue;
-        piece = 0;
-        const int rows = (int)min(16ll, j_end - (j_begin + warp * 16 + (long long)tile * (APPLY_WARPS * 16)));
-        unsigned char *const to = out_row + (long long)tile * (APPLY_WARPS * 16) * p.ldout * out_size;
-        if (nd > 1) {  // columns of this pass's adapter are done; those without any are written in the first pass
-            write = 0u;
-#pragma unroll
-            for (int k = 0; k < PAIRS * 4; ++k) {
-                const int id = ids[(k >> 2) * 16 + 4 * q + (k & 3)];
-                if (id == list[pass] || (id < 0 && pass == 0)) write |= 1u << k;
-            }
-            write &= exist;
-        }
         if (p.outtype == 0)
-            store(std::integral_constant<int, 0>{}, to, rows);
+            store(std::integral_constant<int, 0>{}, write);
         else if (p.outtype == 1)
-            store(std::integral_constant<int, 1>{}, to, rows);
+            store(std::integral_constant<int, 1>{}, write);
         else
-            store(std::integral_constant<int, 2>{}, to, rows);
-        if (++pass == passes) {
-            pass = 0;
-            ++tile;
-        }
+            store(std::integral_constant<int, 2>{}, write);
     }
-    copy_wait<0>();
 }
 
 // ------------------------------------------------------------------ gradients of the factors
@@ -842,7 +831,8 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
     constexpr int PER = 16 / (int)sizeof(TZ), CH = GRAD_CHUNK / PER;
     const int z_row = threadIdx.x / CH, z_col = threadIdx.x % CH * PER, s_row = threadIdx.x / 8, s_col = threadIdx.x % 8 * 4;
     const TZ *const z_src = (const TZ *)p.Z + (j0 + z_row) * p.ldz + z_col;
-    const float *const s_src = p.S + (long long)s_row * w.N + s_col;
+    const long long s_ld = Hidden::pitch_of(w.N);
+    const float *const s_src = p.S + s_row * s_ld + s_col;
     const int j_left = (int)min((long long)GRAD_ROWS, p.n - j0);
     auto fill = [&](int slot, long long t0) {
         unsigned char *z = smem + slot * Q::STAGE, *s = z + GRAD_ROWS * Q::PITCH;
@@ -863,19 +853,12 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                 *(TZ *)(z + r * Q::PITCH + c * sizeof(TZ)) = v;
             }
         }
-        if (w.vec_s) {
-            const int left = cols - s_col, bytes = left <= 0 ? 0 : left >= 4 ? 16 : left * 4;
+        const int left = cols - s_col, bytes = left <= 0 ? 0 : left >= 4 ? 16 : left * 4;
 #pragma unroll
-            for (int k = 0; k < (Q::RP * 8 + 255) / 256; ++k) {
-                const int valid = s_row + k * 32 < w.R ? bytes : 0;
-                if (Q::RP >= 32 || s_row < Q::RP)
-                    copy16(s + (s_row + k * 32) * Q::PITCH + s_col * 4, valid ? s_src + t0 + k * 32 * w.N : p.S, valid);
-            }
-        } else {
-            for (int k = threadIdx.x; k < Q::RP * GRAD_CHUNK; k += 256) {
-                const int r = k / GRAD_CHUNK, c = k % GRAD_CHUNK;
-                *(float *)(s + r * Q::PITCH + c * 4) = r < w.R && c < cols ? p.S[(long long)r * w.N + t0 + c] : 0.0f;
-            }
+        for (int k = 0; k < (Q::RP * 8 + 255) / 256; ++k) {
+            const int valid = s_row + k * 32 < w.R ? bytes : 0;
+            if (Q::RP >= 32 || s_row < Q::RP)
+                copy16(s + (s_row + k * 32) * Q::PITCH + s_col * 4, valid ? s_src + t0 + k * 32 * s_ld : p.S, valid);
         }
     };
 
@@ -999,27 +982,39 @@ __global__ void __launch_bounds__(256) lora_grad(const GradParams w)
 }
 
 // ------------------------------------------------------------------ launches
+// A launch in clusters of `ranks` blocks (0: none), or one that may start before the kernel ahead of it has ended.
 template <typename... Args>
-tcaspmm_status launch_cluster(const char *what, void (*kernel)(Args...), dim3 grid, int threads, int ranks, int shared, cudaStream_t st,
-                              Args... args)
+tcaspmm_status launch(const char *what, void (*kernel)(Args...), dim3 grid, int ranks, bool early, int shared, cudaStream_t st, Args... args)
 {
-    if (shared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-        if (e != cudaSuccess) return cuda_fail(e, what);
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    if (ranks) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)ranks;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    } else {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = early;
+    }
     cfg.attrs = at;
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, what);
+}
+
+// Allows a kernel `shared` bytes of dynamic shared memory on the current device; `done` is the kernel's, a bit a device.
+inline tcaspmm_status allow_shared(const char *what, const void *kernel, int shared, std::atomic<unsigned long long> &done)
+{
+    int dev = 0;
+    if (shared <= 48 * 1024 || (cudaGetDevice(&dev) == cudaSuccess && dev < 64 && (done.load() >> dev & 1))) return TCASPMM_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e != cudaSuccess) return cuda_fail(e, what);
+    if (dev < 64) done.fetch_or(1ull << dev);
+    return TCASPMM_OK;
 }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -1035,26 +1030,55 @@ tcaspmm_status with_rank(int R, F &&f)
     return f(std::integral_constant<int, 16>{});
 }
 
-// Columns of a tile: a warp's sums (RT x TN / 8 x 4 registers a thread) leave room for two blocks an SM, up to rank 64.
+// Columns of a tile of the first product: a warp's sums (RT x TN / 8 x 4 registers a thread) leave room for two blocks an SM
+// up to rank 64.
 constexpr int tile_columns(int rt) { return rt <= 2 ? 64 : rt <= 8 ? 32 : 16; }
 
 template <typename TF, typename TI, bool TRANS>
-tcaspmm_status apply(ApplyParams p, int sms, cudaStream_t st)
+tcaspmm_status shrink(ApplyParams p, int sms, cudaStream_t st)
 {
     return with_rank(p.R, [&](auto rt) {
         constexpr int RT = rt.value, TN = tile_columns(RT);
-        using Q = ApplyShape<TF, TI, RT, TN, TRANS>;
+        using Q = ShrinkShape<TF, TI, RT, TN, TRANS>;
+        const auto kernel = lora_shrink<TF, TI, RT, TN, TRANS>;
         const long long tiles = ceil_div(p.N, TN);
         // Idle SMs take a share, while a warp has a step to do.
         int ranks = 1;
-        while (ranks < 8 && tiles * ranks * 2 <= sms * (RT <= 4 ? 2 : 1) && std::max(p.n1, p.n2) > (long long)ranks * APPLY_WARPS * 16)
-            ranks *= 2;
+        while (ranks < 8 && tiles * ranks < 2 * sms && p.n1 > (long long)ranks * WARPS * Q::KS) ranks *= 2;
         p.per1 = ceil_div(ceil_div(p.n1, ranks), Q::KS) * Q::KS;
-        p.per2 = ceil_div(ceil_div(p.n2, ranks), 16) * 16;
         if (tiles * ranks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many columns");
-        return launch_cluster("lora launch", lora_apply<TF, TI, RT, TN, TRANS>, dim3((unsigned)(tiles * ranks)), APPLY_THREADS, ranks,
-                              Q::BYTES, st, p);
+        static std::atomic<unsigned long long> done{0};
+        const tcaspmm_status s = allow_shared("lora launch", (const void *)kernel, Q::BYTES, done);
+        return s != TCASPMM_OK ? s : launch("lora launch", kernel, dim3((unsigned)(tiles * ranks)), ranks, false, Q::BYTES, st, p);
     });
+}
+
+template <typename TF, bool TRANS, int RC>
+tcaspmm_status expand_pieces(const ApplyParams &p, cudaStream_t st)
+{
+    using Q = ExpandShape<TF, RC, TRANS>;
+    const auto kernel = lora_expand<TF, RC, TRANS>;
+    const long long blocks = ceil_div(p.N, EXP_COLS) * ceil_div(p.n2, EXP_ROWS);
+    if (blocks == 0) return TCASPMM_OK;
+    if (blocks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many elements");
+    static std::atomic<unsigned long long> done{0};
+    const tcaspmm_status s = allow_shared("lora launch", (const void *)kernel, Q::BYTES, done);
+    return s != TCASPMM_OK ? s : launch("lora launch", kernel, dim3((unsigned)blocks), 0, true, Q::BYTES, st, p);
+}
+
+template <typename TF, bool TRANS>
+tcaspmm_status expand(const ApplyParams &p, cudaStream_t st)
+{
+    if (p.R <= 16) return expand_pieces<TF, TRANS, 16>(p, st);
+    if (p.R <= 32 || sizeof(TF) == 4) return expand_pieces<TF, TRANS, 32>(p, st);
+    return expand_pieces<TF, TRANS, sizeof(TF) == 4 ? 32 : 64>(p, st);
+}
+
+template <typename TF, typename TI, bool TRANS>
+tcaspmm_status apply(const ApplyParams &p, int sms, cudaStream_t st)
+{
+    const tcaspmm_status s = shrink<TF, TI, TRANS>(p, sms, st);
+    return s != TCASPMM_OK || !p.Out ? s : expand<TF, TRANS>(p, st);
 }
 
 template <typename TF>
@@ -1062,14 +1086,18 @@ tcaspmm_status grads(GradParams w, int sms, cudaStream_t st)
 {
     return with_rank(w.R, [&](auto rt) {
         constexpr int RT = rt.value;
+        const auto kernel = lora_grad<TF, RT>;
         for (GradProblem &p : w.p) p.tiles = p.G ? (int)ceil_div(p.n, GRAD_ROWS) : 0;
         const long long tiles = (long long)w.p[0].tiles + w.p[1].tiles;
         if (tiles == 0 || w.c.L == 0) return TCASPMM_OK;
         int ranks = 1;
         while (ranks < 8 && tiles * ranks < 2 * sms && w.N > (long long)ranks * 2 * GRAD_CHUNK) ranks *= 2;
         if (tiles * ranks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora_backward: too many rows");
-        return launch_cluster("lora_backward launch", lora_grad<TF, RT>, dim3((unsigned)(tiles * ranks), (unsigned)std::min(w.c.L, 65535)),
-                              256, ranks, GradShape<RT>::BYTES, st, w);
+        static std::atomic<unsigned long long> done{0};
+        const tcaspmm_status s = allow_shared("lora_backward launch", (const void *)kernel, GradShape<RT>::BYTES, done);
+        return s != TCASPMM_OK ? s
+                               : launch("lora_backward launch", kernel, dim3((unsigned)(tiles * ranks), (unsigned)std::min(w.c.L, 65535)),
+                                        ranks, false, GradShape<RT>::BYTES, st, w);
     });
 }
 

@@ -281,6 +281,13 @@ struct Adapters {
     }
 };
 
+int64_t hidden_bytes(const Tensor &x, int64_t R, int64_t N) { return (int64_t)tcaspmm_lora_hidden_bytes(R, N, code(x.scalar_type())); }
+
+Tensor hidden_buffer(const Tensor &x, int64_t R, int64_t N)
+{
+    return at::empty({hidden_bytes(x, R, N)}, x.options().dtype(at::kByte));
+}
+
 Tensor lora_call(const Tensor &x, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
                  const MaybeTensor &base_, const Tensor *out, Tensor *H)
 {
@@ -305,8 +312,8 @@ Tensor lora_call(const Tensor &x, const Tensor &down, const Tensor &up, const Ma
     if (out) check_with(x, *out, "out");
     const c10::cuda::CUDAGuard guard(x.device());
     if (!out) Y = Matrix(at::empty({a.M, a.N}, x.options().dtype(type)), "out");
-    *H = at::empty({a.R, a.N}, x.options().dtype(at::kFloat));
-    check(tcaspmm_lora(a.args(), a.X.ptr(), a.X.ld, a.N, base.ptr(), base.ld, Y.ptr(), Y.ld, code(type), H->data_ptr<float>(),
+    *H = hidden_buffer(x, a.R, a.N);
+    check(tcaspmm_lora(a.args(), a.X.ptr(), a.X.ld, a.N, base.ptr(), base.ld, Y.ptr(), Y.ld, code(type), H->data_ptr(),
                        at::cuda::getCurrentCUDAStream().stream()));
     return Y.t;
 }
@@ -344,8 +351,8 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
     check_shape(dy, "dY", {a.M, a.N});
     TORCH_CHECK_VALUE(dy.scalar_type() == at::kFloat || dy.scalar_type() == x.scalar_type(), "dY must be float32 or X's type ",
                       x.scalar_type(), ", not ", dy.scalar_type());
-    check_shape(H, "H", {a.R, a.N});
-    TORCH_CHECK_VALUE(H.scalar_type() == at::kFloat && H.is_contiguous(), "H must be the contiguous float32 tensor that lora returned");
+    TORCH_CHECK_VALUE(H.scalar_type() == at::kByte && H.dim() == 1 && H.is_contiguous() && H.numel() == hidden_bytes(x, a.R, a.N),
+                      "H must be the tensor that lora returned with hidden");
     const Tensor b = given(base_);
     Matrix base;
     if (b.defined()) {
@@ -363,10 +370,10 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
     Tensor dD = at::empty(need_down ? a.down.sizes() : at::IntArrayRef{0}, x.options());
     Tensor dU = at::empty(need_up ? a.up.sizes() : at::IntArrayRef{0}, x.options());
     Tensor P;
-    if (need_input || need_down) P = at::empty({a.R, a.N}, x.options().dtype(at::kFloat));
-    check(tcaspmm_lora_backward(a.args(), dY.ptr(), dY.ld, code(dy.scalar_type()), a.X.ptr(), a.X.ld, a.N, H.data_ptr<float>(),
+    if (need_input || need_down) P = hidden_buffer(x, a.R, a.N);
+    check(tcaspmm_lora_backward(a.args(), dY.ptr(), dY.ld, code(dy.scalar_type()), a.X.ptr(), a.X.ld, a.N, H.data_ptr(),
                                 (const float *)base.ptr(), base.ld, need_input ? dX.data_ptr() : nullptr, a.N,
-                                need_down ? dD.data_ptr() : nullptr, need_up ? dU.data_ptr() : nullptr, (float *)ptr(P),
+                                need_down ? dD.data_ptr() : nullptr, need_up ? dU.data_ptr() : nullptr, ptr(P),
                                 at::cuda::getCurrentCUDAStream().stream()));
     return {dX, dD, dU};
 }

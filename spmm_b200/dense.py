@@ -27,6 +27,7 @@ _sig("tcaspmm_layer_norm", [_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, C.
 _sig("tcaspmm_layer_norm_backward_workspace", [_i64, _i64, C.c_int], C.c_size_t)
 _sig("tcaspmm_layer_norm_backward", [_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, _vp, C.c_int, _vp, _i64, _vp, _vp,
                                      _i64, _i64, C.c_int, _vp, C.c_size_t, _vp])
+_sig("tcaspmm_lora_hidden_bytes", [_i64, _i64, C.c_int], C.c_size_t)
 _sig("tcaspmm_lora", [C.POINTER(_Adapters), _vp, _i64, _i64, _vp, _i64, _vp, _i64, C.c_int, _vp, _vp])
 _sig("tcaspmm_lora_backward", [C.POINTER(_Adapters), _vp, _i64, C.c_int, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
                                _vp, _vp, _vp])
@@ -51,7 +52,12 @@ def _op(name: str):
 def _register_shapes() -> None:
     import torch
 
+    from . import as_dtype, lib
+
     fake = torch.library.register_fake
+
+    def hidden(X, down):
+        return X.new_empty(lib.tcaspmm_lora_hidden_bytes(down.shape[1], X.shape[1], int(as_dtype(X.dtype))), dtype=torch.uint8)
 
     @fake("tcaspmm::layer_norm")
     def _(X, weight, bias, eps, dim, out_dtype):
@@ -74,12 +80,11 @@ def _register_shapes() -> None:
 
     @fake("tcaspmm::lora_hidden")
     def _(X, down, up, index, scale, base):
-        return (X.new_empty((up.shape[1], X.shape[1]), dtype=torch.float32 if base is None else base.dtype),
-                X.new_empty((down.shape[1], X.shape[1]), dtype=torch.float32))
+        return X.new_empty((up.shape[1], X.shape[1]), dtype=torch.float32 if base is None else base.dtype), hidden(X, down)
 
     @fake("tcaspmm::lora_into")
     def _(X, down, up, index, scale, base, out):
-        return X.new_empty((down.shape[1], X.shape[1]), dtype=torch.float32)
+        return hidden(X, down)
 
     @fake("tcaspmm::lora_backward")
     def _(dY, X, down, up, H, index, scale, base, need_input, need_down, need_up):
@@ -119,8 +124,8 @@ def lora(X, down, up, index=None, scale=None, base=None, *, out=None, hidden: bo
     X: K x N; down: L x R x K and up: L x M x R, in X's type, R <= 256; index: int32 or int64, one per column, None =
     adapter 0 for all, a value outside [0, L) = no adapter (the column of base as it is); scale: float32, one per
     adapter, None = 1.  Differentiable in X, down, up and base.  out: a tensor to write, base itself included.  With
-    hidden, returns (Y, H) with the R x N float32 H = scale * down @ X as lora_backward takes it.  (No autograd with
-    out or hidden.)"""
+    hidden, returns (Y, H) with scale * down @ X as lora_backward takes it (an opaque buffer).  (No autograd with out or
+    hidden.)"""
     if out is not None:
         H = _op("lora_into")(X, down, up, index, scale, base, out)
         return (out, H) if hidden else out
