@@ -394,20 +394,23 @@ typedef struct tcaspmm_adapters {
     int index_bytes;
 } tcaspmm_adapters;
 
-/* Bytes of the buffer in which tcaspmm_lora keeps scale * down * X for the backward
- * pass (opaque; device memory, 16-byte aligned): both calls take one. */
-size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t N, tcaspmm_dtype dt);
+/* Bytes of the buffer tcaspmm_lora works in (device memory, 16-byte aligned).
+ * With keep it leaves scale * down * X there for the backward pass (opaque);
+ * without, the buffer is scratch, and 0 bytes where none is needed. */
+size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t K, int64_t N, tcaspmm_dtype dt, int keep);
 /* Y[:, t] = base[:, t] + scale[a] * up[a] * (down[a] * X[:, t]), a = index[t];
  * Y = base where column t has no adapter.  X is K x N in dt; base (M x N, or NULL
  * = 0: usually the C of an execute call) and Y are in y_dt, and Y may be base
- * itself (same ld).  hidden: tcaspmm_lora_hidden_bytes(rank, N, dt) bytes. */
+ * itself (same ld).  hidden: tcaspmm_lora_hidden_bytes(rank, K, N, dt, keep)
+ * bytes. */
 tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *dX, int64_t ldx, int64_t N, const void *dBase,
-                            int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, void *hidden, void *stream);
+                            int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, void *hidden, int keep,
+                            void *stream);
 /* Gradients from dY (dy_dt: fp32 or dt): dX = base + scale * down^T (up^T dY) in
  * dt, with dBase an fp32 K x N matrix (usually A^T dY) or NULL; ddown and dup in
  * dt, zeros for adapters without columns.  Any of the three may be NULL.  hidden
- * is what the forward pass left (for dup); scratch is another buffer of its size
- * (for dX and ddown). */
+ * is what the forward pass left with keep (for dup); scratch is another buffer of
+ * that size (for dX and ddown). */
 tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt,
                                      const void *dX, int64_t ldx, int64_t N, const void *hidden, const float *dBase,
                                      int64_t ldbase, void *dDX, int64_t lddx, void *ddown, void *dup, void *scratch,

@@ -1,6 +1,8 @@
 // Shared by the dense operators around a sparse product (norm.cu, lora.cu): element access by type, argument checks.
 #pragma once
 
+#include <cstring>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -38,6 +40,26 @@ __device__ __forceinline__ void store_as(void *p, int type, long long i, float v
     else
         ((__nv_bfloat16 *)p)[i] = __float2bfloat16_rn(v);
 }
+
+template <int BYTES> struct Bits;
+template <> struct Bits<2> { using type = unsigned short; };
+template <> struct Bits<4> { using type = unsigned; };
+template <> struct Bits<8> { using type = uint2; };
+template <> struct Bits<16> { using type = uint4; };
+
+// VEC elements of type T as they lie in memory (at most 16 bytes).
+template <typename T, int VEC>
+struct Pack {
+    typename Bits<sizeof(T) * VEC>::type bits;
+    __device__ void load(const T *p) { bits = __ldg(reinterpret_cast<const decltype(bits) *>(p)); }
+    __device__ void zero() { bits = {}; }
+    __device__ float get(int i) const
+    {
+        T v[VEC];
+        memcpy(v, &bits, sizeof bits);
+        return to_float(v[i]);
+    }
+};
 
 // Type code of the kernels; TF32 is fp32 storage.
 inline int type_code(tcaspmm_dtype dt) { return dt == TCASPMM_F16 ? 1 : dt == TCASPMM_BF16 ? 2 : 0; }

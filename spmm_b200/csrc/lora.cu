@@ -6,7 +6,7 @@ namespace tca {
 int sm_count();
 
 #define TCA_LORA(k)                                                                         \
-    tcaspmm_status lora_forward_##k(const ApplyParams &p, int sms, cudaStream_t st);        \
+    tcaspmm_status lora_forward_##k(const ApplyParams &p, bool tokens, int sms, cudaStream_t st); \
     tcaspmm_status lora_input_grad_##k(const ApplyParams &p, bool in32, int sms, cudaStream_t st); \
     tcaspmm_status lora_factor_grads_##k(const GradParams &w, int sms, cudaStream_t st);
 TCA_LORA(f32)
@@ -48,13 +48,14 @@ bool aligned(const void *p, int64_t ld, int type, int bytes)
 
 using namespace tca;
 
-extern "C" size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t N, tcaspmm_dtype dt)
+extern "C" size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t K, int64_t N, tcaspmm_dtype dt, int keep)
 {
-    return rank < 1 || N < 1 || !dtype_valid(dt) ? 0 : Hidden::bytes(rank, N, type_code(dt));
+    if (rank < 1 || N < 1 || !dtype_valid(dt) || (!keep && by_token(K, N))) return 0;
+    return Hidden::bytes(rank, N, type_code(dt));
 }
 
 extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *dX, int64_t ldx, int64_t N, const void *dBase,
-                                       int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, void *hidden, void *stream)
+                                       int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, void *hidden, int keep, void *stream)
 {
     clear_error();
     const tcaspmm_status s = check(ad, N, "lora");
@@ -64,7 +65,8 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
         return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld or NULL pointer",
                     (long long)ldx, (long long)ldbase, (long long)ldy);
     if (N == 0) return TCASPMM_OK;
-    if (!hidden || (uintptr_t)hidden % 16) return fail(TCASPMM_ERR_INVALID_ARG, "lora: hidden must be a 16-byte aligned device pointer");
+    const bool tokens = !keep && by_token(ad->K, N);
+    if (!tokens && (!hidden || (uintptr_t)hidden % 16)) return fail(TCASPMM_ERR_INVALID_ARG, "lora: hidden must be a 16-byte aligned device pointer");
     const int ft = type_code(ad->dt), yt = type_code(y_dt);
     ApplyParams p = {};
     p.F1 = ad->down;
@@ -90,7 +92,7 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
     p.vec_base = aligned(dBase, ldbase, yt, 4 * size_of(yt));
     p.vec_out = aligned(dY, ldy, yt, 4 * size_of(yt));
     const auto run = ft == 0 ? lora_forward_f32 : ft == 1 ? lora_forward_f16 : lora_forward_bf16;
-    return run(p, sm_count(), (cudaStream_t)stream);
+    return run(p, tokens, sm_count(), (cudaStream_t)stream);
 }
 
 extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt,

@@ -54,6 +54,7 @@ struct ApplyParams {
     void *hidden;  // S (Hidden)
     int vec_in, vec_f1, vec_f2, vec_base, vec_out;  // what alignment allows
     long long per1;  // rows of In for each block of a cluster
+    int chunks;      // of EXP_ROWS rows of Out for each block
 };
 
 // S in device memory between the kernels, rows of `pitch` columns (64 or a multiple, so that every row is aligned): fp32 for
@@ -106,6 +107,11 @@ __device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)
 __device__ __forceinline__ void copy16(void *dst, const void *src, int valid)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
+}
+// 8 bytes, all of them or (valid 0) zeros.
+__device__ __forceinline__ void copy8(void *dst, const void *src, int valid)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -226,7 +232,8 @@ constexpr int THREADS = WARPS * 32;
 // Of a tile's columns: their adapters (-1: none, or past the end), and those that occur, by their first columns.
 template <int TN>
 struct TileColumns {
-    int ids[TN], list[TN], count;
+    __align__(16) int ids[TN];
+    int list[TN], count;
     __device__ __forceinline__ void load(const Columns &c, long long t0, long long N)
     {
         for (int t = threadIdx.x; t < TN; t += THREADS) ids[t] = t0 + t < N ? c.of(t0 + t) : -1;
@@ -549,83 +556,82 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_shrink(const Ap
 
 // ------------------------------------------------------------------ Out = base + F2 S
 //
-// A block takes 128 rows of Out and 64 columns, a warp 16 rows.  base is read into registers and F2's slice copied to shared
-// memory before the block waits for the kernel that makes S (programmatic dependent launch), so that the start of this
-// kernel hides behind the end of that one.  Columns are dealt to the matrix instruction so that a thread's results of two
-// blocks of 8 lie side by side: base and Out move 16 bytes a thread.  In 16 bits both parts of S are multiplied, so that an
-// fp32 Out is as exact as fp32 sums of exact products.  With several adapters among the columns the product runs once for
-// each, for the pairs of blocks that have any of its columns.  Bound by base and Out: R / 8 products a byte.
+// A block takes 64 columns and up to 8 chunks of 128 rows of Out, a warp 16 rows of a chunk.  S's columns stay in shared
+// memory; F2's slices and base come a chunk ahead (asynchronous copies), the first of them before the block waits for the
+// kernel that makes S (programmatic dependent launch), so that the start of this kernel hides behind the end of that
+// one.  Columns are dealt to the matrix instruction so that a thread's results of two blocks of 8 lie side by side: base and
+// Out move 16 bytes a thread.  In 16 bits both parts of S are multiplied, so that an fp32 Out is as exact as fp32 sums of
+// exact products.  With several adapters among the columns the product runs once for each, for the pairs of blocks that have
+// any of its columns.  Bound by base and Out: R / 8 products a byte.
 constexpr int EXP_COLS = 64;
 constexpr int EXP_ROWS = WARPS * 16;
 constexpr int EXP_PAIRS = EXP_COLS / 16;
 
-template <typename TF, int RC, bool TRANS>  // RC: r's a piece
+template <typename TF, int RT, bool TRANS>
 struct ExpandShape {
-    static constexpr int F_ROWS = TRANS ? RC : 16;
-    static constexpr int F_COLS = TRANS ? 16 : RC;
-    static constexpr int F_PITCH = F_COLS * (int)sizeof(TF) + (TRANS && sizeof(TF) == 4 ? 32 : 16);
+    static constexpr int RP = RT * 16;
+    static constexpr int F_ROWS = TRANS ? RP : 16;
+    static constexpr int F_COLS = TRANS ? 16 : RP;
+    static constexpr int F_PITCH = F_COLS * (int)sizeof(TF) + (!TRANS || sizeof(TF) == 2 ? 16 : RT > 8 ? 0 : 32);
     static constexpr int F_BYTES = F_ROWS * F_PITCH;
     static constexpr int S_PITCH = EXP_COLS * (int)sizeof(TF) + (sizeof(TF) == 4 ? 32 : 16);
-    static constexpr int S_BYTES = RC * S_PITCH;  // one part
-    static constexpr int BYTES = WARPS * F_BYTES + S_BYTES * (sizeof(TF) == 2 ? 2 : 1);
+    static constexpr int S_BYTES = RP * S_PITCH;  // one part
+    static constexpr int S_ALL = S_BYTES * (sizeof(TF) == 2 ? 2 : 1);
+    static constexpr int BASE_BYTES = EXP_PAIRS * 2 * 16;  // a thread's part of a chunk of base
+    // Two blocks an SM; above rank 128 one, without base in shared memory.
+    static constexpr bool BASE = RT <= 8;
+    static constexpr int FIXED = S_ALL + (BASE ? BASE_BYTES * THREADS : 0);
+    static constexpr int BUFFERS = FIXED + 2 * WARPS * F_BYTES <= (BASE ? 110 : 222) * 1024 ? 2 : 1;
+    static constexpr int BYTES = FIXED + BUFFERS * WARPS * F_BYTES;
+    static_assert(BYTES <= 222 * 1024, "F2's slices do not fit");
 };
 
-template <typename TF, int RC, bool TRANS>
-__global__ void __launch_bounds__(THREADS, 2) lora_expand(const ApplyParams p)
+template <typename TF, int RT, bool TRANS>
+__global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const ApplyParams p)
 {
-    using Q = ExpandShape<TF, RC, TRANS>;
+    using Q = ExpandShape<TF, RT, TRANS>;
     constexpr bool HALF = std::is_same<TF, __half>::value;
-    constexpr int PAIRS = EXP_PAIRS;
+    constexpr int PAIRS = EXP_PAIRS, RP = Q::RP;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ TileColumns<EXP_COLS> tile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, g = lane >> 2;
     const unsigned across = (unsigned)((p.N + EXP_COLS - 1) / EXP_COLS);  // neighbouring blocks share rows
-    const long long t0 = (long long)(blockIdx.x % across) * EXP_COLS, j0 = (long long)(blockIdx.x / across) * EXP_ROWS + warp * 16;
-    const int rows = (int)max(0ll, min(16ll, p.n2 - j0));
-    unsigned char *const f = smem + warp * Q::F_BYTES, *const sh = smem + WARPS * Q::F_BYTES, *const sl = sh + Q::S_BYTES;
+    const long long t0 = (long long)(blockIdx.x % across) * EXP_COLS;
+    const long long j_first = (long long)(blockIdx.x / across) * p.chunks * EXP_ROWS + warp * 16;
+    const int chunks = (int)max(0ll, min((long long)p.chunks, (p.n2 - j_first + EXP_ROWS - 1) / EXP_ROWS));  // this warp's
+    const int last_rows = chunks > 0 ? (int)min(16ll, p.n2 - j_first - (long long)(chunks - 1) * EXP_ROWS) : 0;
+    unsigned char *const sh = smem, *const sl = smem + Q::S_BYTES, *const f0 = smem + Q::S_ALL + warp * (Q::BUFFERS * Q::F_BYTES);
+    unsigned char *const ahead_base = smem + Q::S_ALL + WARPS * Q::BUFFERS * Q::F_BYTES + threadIdx.x * 16;  // pieces THREADS * 16 apart
+    __shared__ __align__(16) float colscale[EXP_COLS];
 
-    float old[PAIRS][2][4];  // rows g, g + 8; columns 16 pair + 4 q ...
     const int base_size = p.basetype == 0 ? 4 : 2;
-    const unsigned char *const base = (const unsigned char *)p.base + ((j0 + g) * p.ldbase + t0 + 4 * q) * base_size;
-    const bool inner = t0 + EXP_COLS <= p.N && p.vec_base;
-#pragma unroll
-    for (int b = 0; b < PAIRS; ++b)
+    const unsigned char *base = (const unsigned char *)p.base + ((j_first + g) * p.ldbase + t0 + 4 * q) * base_size;
+    const bool fetch = Q::BASE && p.base && t0 + EXP_COLS <= p.N && p.vec_base;  // base comes by asynchronous copies
+    const long long base_step = (long long)EXP_ROWS * p.ldbase * base_size, base_down = 8 * p.ldbase * base_size;
+    auto fetch_base = [&](const unsigned char *at, int rows) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const bool in = p.base && g + h * 8 < rows;
-            const unsigned char *at = base + (h * 8 * p.ldbase + b * 16) * base_size;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (in && inner) {
-                if (base_size == 4) {
-                    v = *(const float4 *)at;
-                } else {
-                    const uint2 u = *(const uint2 *)at;
-                    v = make_float4(as_float(u.x & 0xffffu, p.basetype), as_float(u.x >> 16, p.basetype), as_float(u.y & 0xffffu, p.basetype),
-                                    as_float(u.y >> 16, p.basetype));
-                }
-            } else if (in) {
-                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int valid = g + h * 8 < rows ? 16 : 0;
+            const unsigned char *row = valid ? at + (h ? base_down : 0) : (const unsigned char *)p.base;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (t0 + b * 16 + 4 * q + e < p.N)
-                        x[e] = base_size == 4 ? ((const float *)at)[e] : as_float(((const unsigned short *)at)[e], p.basetype);
-                v = make_float4(x[0], x[1], x[2], x[3]);
+            for (int b = 0; b < PAIRS; ++b) {
+                if (base_size == 4)
+                    copy16(ahead_base + (b * 2 + h) * (THREADS * 16), row + (valid ? b * 64 : 0), valid);
+                else
+                    copy8(ahead_base + (b * 2 + h) * (THREADS * 16), row + (valid ? b * 32 : 0), valid >> 1);
             }
-            old[b][h][0] = v.x;
-            old[b][h][1] = v.y;
-            old[b][h][2] = v.z;
-            old[b][h][3] = v.w;
         }
-
+    };
     const long long f_ld = TRANS ? p.n2 : p.R;
-    auto fill_f = [&](int a, int r0) {  // the warp's rows of adapter a's F2, RC from r0 on
-        const TF *F = (const TF *)p.F2 + (long long)a * p.R * p.n2 + (TRANS ? r0 * p.n2 + j0 : j0 * p.R + r0);
+    auto fill_f = [&](unsigned char *f, int a, int chunk, int rows) {  // the warp's rows of adapter a's F2
+        const long long j0 = j_first + (long long)chunk * EXP_ROWS;
+        const TF *F = (const TF *)p.F2 + (long long)a * p.R * p.n2 + (TRANS ? j0 : j0 * p.R);
         constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, COUNT = Q::F_ROWS * CH;
         if (p.vec_f2) {
 #pragma unroll
             for (int k = 0; k < (COUNT + 31) / 32; ++k) {
                 const int r = (lane + k * 32) / CH, c = (lane + k * 32) % CH * PER;
-                const int left = TRANS ? (r0 + r < p.R ? rows - c : 0) : (r < rows ? p.R - r0 - c : 0);
+                const int left = TRANS ? (r < p.R ? rows - c : 0) : (r < rows ? p.R - c : 0);
                 const int valid = left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
                 if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
                     copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F2, valid);
@@ -634,51 +640,103 @@ __global__ void __launch_bounds__(THREADS, 2) lora_expand(const ApplyParams p)
             for (int k = lane; k < Q::F_ROWS * Q::F_COLS; k += 32) {
                 const int r = k / Q::F_COLS, c = k - r * Q::F_COLS;
                 TF v = from_float<TF>(0.0f);
-                if (TRANS ? (r0 + r < p.R && c < rows) : (r < rows && r0 + c < p.R)) v = F[r * f_ld + c];
+                if (TRANS ? (r < p.R && c < rows) : (r < rows && c < p.R)) v = F[r * f_ld + c];
                 *(TF *)(f + r * Q::F_PITCH + c * sizeof(TF)) = v;
             }
         }
     };
-    const Hidden hid(p.hidden, p.R, p.N);
-    auto fill_s = [&](int r0) {  // the block's columns of S, rows r0 .. r0 + RC - 1
-        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER, PARTS = sizeof(TF) == 2 ? 2 : 1;
-        for (int k = threadIdx.x; k < PARTS * RC * CH; k += THREADS) {
-            const int part = k / (RC * CH), r = k % (RC * CH) / CH, c = k % CH * PER;
-            const TF *src = sizeof(TF) == 4 ? (const TF *)hid.s() : part ? hid.template lo<TF>() : hid.template hi<TF>();
-            const int valid = r0 + r < p.R ? 16 : 0;
-            copy16((part ? sl : sh) + r * Q::S_PITCH + c * (int)sizeof(TF), valid ? src + (r0 + r) * hid.pitch + t0 + c : src, valid);
-        }
-    };
+    auto rows_of = [&](int chunk) { return chunk >= chunks ? 0 : chunk == chunks - 1 ? last_rows : 16; };
 
+    if (fetch) fetch_base(base, rows_of(0));
     tile.load(p.c, t0, p.N);
     const int *const ids = tile.ids, *const list = tile.list;
-    const int nd = tile.count, pieces = (p.R + RC - 1) / RC;
-    if (nd > 0) fill_f(list[0], 0);
+    const int nd = tile.count;
+    if (nd > 0 && chunks > 0) fill_f(f0, list[0], 0, rows_of(0));
     // A bit for each of a thread's columns (4 q + (k & 3) of pair k / 4): it exists, has an adapter.
     unsigned exist = 0u, has = 0u;
 #pragma unroll
-    for (int k = 0; k < PAIRS * 4; ++k) {
-        const int c = (k >> 2) * 16 + 4 * q + (k & 3);
-        if (t0 + c < p.N) exist |= 1u << k;
-        if (ids[c] >= 0) has |= 1u << k;
-    }
-    cudaGridDependencySynchronize();
-    float colscale[PAIRS][4];
-    if (HALF) {
+    for (int b = 0; b < PAIRS; ++b) {
+        const int4 id = *(const int4 *)(ids + b * 16 + 4 * q);
+        has |= ((id.x >= 0) | (id.y >= 0) << 1 | (id.z >= 0) << 2 | (id.w >= 0) << 3) << (b * 4);
 #pragma unroll
-        for (int b = 0; b < PAIRS; ++b) {
-            const float4 v = nd > 0 ? *(const float4 *)(hid.colscale() + t0 + b * 16 + 4 * q) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-            colscale[b][0] = v.x;
-            colscale[b][1] = v.y;
-            colscale[b][2] = v.z;
-            colscale[b][3] = v.w;
-        }
+        for (int e = 0; e < 4; ++e) exist |= (unsigned)(t0 + b * 16 + 4 * q + e < p.N) << (b * 4 + e);
     }
+    // The usual tile, without masks: one adapter for all of its columns.
+    const bool plain = __all_sync(~0u, has == 0xffffu) && nd == 1 && p.vec_out;
+    cudaGridDependencySynchronize();
+    const Hidden hid(p.hidden, p.R, p.N);
+    if (nd > 0) {  // S's columns
+        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER, PARTS = sizeof(TF) == 2 ? 2 : 1;
+        const TF *src[2] = {sizeof(TF) == 4 ? (const TF *)hid.s() : hid.template hi<TF>(), hid.template lo<TF>()};
+        const int c = threadIdx.x % CH * PER, r = threadIdx.x / CH;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int k = 0; k < (RP * CH + THREADS - 1) / THREADS; ++k) {
+                const int row = r + k * (THREADS / CH), valid = row < p.R ? 16 : 0;
+                if (RP * CH % THREADS == 0 || row < RP)
+                    copy16((part ? sl : sh) + row * Q::S_PITCH + c * (int)sizeof(TF), valid ? src[part] + row * hid.pitch + t0 + c : src[part], valid);
+            }
+    }
+    copy_commit();
+    if (HALF && threadIdx.x < EXP_COLS) colscale[threadIdx.x] = nd > 0 ? hid.colscale()[t0 + threadIdx.x] : 1.0f;
+    copy_wait<0>();
+    __syncthreads();
 
-    const int out_size = p.outtype == 0 ? 4 : 2;
-    unsigned char *const out = (unsigned char *)p.Out + ((j0 + g) * p.ldout + t0 + 4 * q) * out_size;
     float sum[PAIRS][2][4];  // [pair][block of the pair][e]: rows g, g + 8; columns 16 pair + 4 q + 2 block + (e & 1)
-    auto store = [&](auto type, unsigned write) {
+    auto multiply = [&](const unsigned char *f, unsigned some) {
+#pragma unroll
+        for (int b = 0; b < PAIRS; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[b][h][e] = 0.0f;
+        if constexpr (sizeof(TF) == 2) {
+#pragma unroll(RT <= 4 ? RT : 2)
+            for (int k = 0; k < RT; ++k) {
+                unsigned A[4];
+                load_matrices<TRANS>(A, TRANS ? f + (k * 16 + (lane & 7) + (lane >> 4) * 8) * Q::F_PITCH + (lane >> 3 & 1) * 16
+                                              : f + (lane & 15) * Q::F_PITCH + (k * 16 + (lane >> 4) * 8) * 2);
+                const int row = (k * 16 + (lane & 15)) * Q::S_PITCH + (lane >> 4) * 16;
+#pragma unroll
+                for (int b = 0; b < PAIRS; ++b) {
+                    if (!(some >> b & 1)) continue;
+                    unsigned L[4], H[4];
+                    load_matrices<true>(L, sl + row + b * 32);
+                    load_matrices<true>(H, sh + row + b * 32);
+                    mma16<TF>(sum[b][0], A, L[0], L[1]);
+                    mma16<TF>(sum[b][1], A, L[2], L[3]);
+                    mma16<TF>(sum[b][0], A, H[0], H[1]);
+                    mma16<TF>(sum[b][1], A, H[2], H[3]);
+                }
+            }
+        } else {
+#pragma unroll 2
+            for (int k = 0; k < RP; k += 8) {
+                Operand<true> A[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = g + (e & 1) * 8, r = k + q + (e >> 1) * 4;
+                    A[e].set(*(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4));
+                }
+#pragma unroll
+                for (int b = 0; b < PAIRS; ++b) {
+                    if (!(some >> b & 1)) continue;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned char *s = sh + (k + q) * Q::S_PITCH + (b * 16 + 4 * (g >> 1) + 2 * h + (g & 1)) * 4;
+                        Operand<true> B[2];
+                        B[0].set(*(const float *)s);
+                        B[1].set(*(const float *)(s + 4 * Q::S_PITCH));
+                        mma8_any<true>(sum[b][h], A, B[0], B[1]);
+                    }
+                }
+            }
+        }
+    };
+    const int out_size = p.outtype == 0 ? 4 : 2;
+    unsigned char *out = (unsigned char *)p.Out + ((j_first + g) * p.ldout + t0 + 4 * q) * out_size;
+    auto store = [&](auto type, const float (&old)[PAIRS][2][4], unsigned write, int rows) {
         using TO = std::conditional_t<type.value == 0, float, std::conditional_t<type.value == 1, __half, __nv_bfloat16>>;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -686,13 +744,22 @@ __global__ void __launch_bounds__(THREADS, 2) lora_expand(const ApplyParams p)
             TO *row = (TO *)out + h * 8 * p.ldout;
 #pragma unroll
             for (int b = 0; b < PAIRS; ++b) {
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = sum[b][e >> 1][2 * h + (e & 1)];
-                    if (HALF) v *= colscale[b][e];
-                    y[e] = has >> (b * 4 + e) & 1 ? old[b][h][e] + v : old[b][h][e];
+                float y[4] = {sum[b][0][2 * h], sum[b][0][2 * h + 1], sum[b][1][2 * h], sum[b][1][2 * h + 1]};
+                if (HALF) {
+                    const float4 c = *(const float4 *)(colscale + b * 16 + 4 * q);
+                    y[0] *= c.x;
+                    y[1] *= c.y;
+                    y[2] *= c.z;
+                    y[3] *= c.w;
                 }
+                if (plain) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] += old[b][h][e];
+                    store_four(row + b * 16, y);
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = has >> (b * 4 + e) & 1 ? old[b][h][e] + y[e] : old[b][h][e];
                 const unsigned w = write >> (b * 4) & 15u;
                 if (p.vec_out && w == 15u) {
                     store_four(row + b * 16, y);
@@ -705,90 +772,191 @@ __global__ void __launch_bounds__(THREADS, 2) lora_expand(const ApplyParams p)
         }
     };
 
-    for (int pass = 0; pass < max(nd, 1); ++pass) {
-        const int a = nd > 0 ? list[pass] : -1;
-        unsigned some = ~0u, write = exist;  // pairs with columns of adapter a; columns that this pass writes
-        if (nd > 1) {
-            some = write = 0u;
-#pragma unroll
-            for (int k = 0; k < PAIRS * 4; ++k) {
-                const int id = ids[(k >> 2) * 16 + 4 * q + (k & 3)];
-                // Those without an adapter are written in the first pass.
-                if (id == a || (id < 0 && pass == 0)) write |= 1u << k;
-                if (id == a) some |= 1u << (k >> 2);
-            }
-            write &= exist;
-            some = __reduce_or_sync(~0u, some);
-        }
+    const long long out_step = (long long)EXP_ROWS * p.ldout * out_size;
+    for (int chunk = 0; chunk < chunks; ++chunk, out += out_step, base += base_step) {
+        const int rows = rows_of(chunk);
+        copy_wait<0>();
+        __syncwarp();
+        float old[PAIRS][2][4];  // rows g, g + 8; columns 16 pair + 4 q ...
 #pragma unroll
         for (int b = 0; b < PAIRS; ++b)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const unsigned char *at = ahead_base + (b * 2 + h) * (THREADS * 16);
+                if (fetch && base_size == 4) {
+                    v = *(const float4 *)at;
+                } else if (fetch) {
+                    const uint2 u = *(const uint2 *)at;
+                    v = make_float4(as_float(u.x & 0xffffu, p.basetype), as_float(u.x >> 16, p.basetype), as_float(u.y & 0xffffu, p.basetype),
+                                    as_float(u.y >> 16, p.basetype));
+                } else if (p.base && g + h * 8 < rows) {
+                    const unsigned char *from = base + (h ? base_down : 0);
+                    const auto element = [&](int e) {
+                        return t0 + b * 16 + 4 * q + e >= p.N ? 0.0f
+                               : base_size == 4               ? ((const float *)from)[b * 16 + e]
+                                                              : as_float(((const unsigned short *)from)[b * 16 + e], p.basetype);
+                    };
+                    v = make_float4(element(0), element(1), element(2), element(3));
+                }
+                old[b][h][0] = v.x;
+                old[b][h][1] = v.y;
+                old[b][h][2] = v.z;
+                old[b][h][3] = v.w;
+            }
+        // With one adapter and two buffers, F2's slice for the next chunk is fetched now; else each when it is needed.
+        const bool more = chunk + 1 < chunks, ahead = Q::BUFFERS == 2 && nd == 1;
+        unsigned char *const f = Q::BUFFERS == 2 ? f0 + (chunk & 1) * Q::F_BYTES : f0;
+        if (more && fetch) fetch_base(base + base_step, rows_of(chunk + 1));
+        if (more && ahead) fill_f(f0 + (chunk + 1 & 1) * Q::F_BYTES, list[0], chunk + 1, rows_of(chunk + 1));
+        copy_commit();
+        for (int pass = 0; pass < max(nd, 1); ++pass) {
+            unsigned some = 0u, write = exist;  // pairs with columns of this pass's adapter; columns that it writes
+            if (nd == 1) {
+                some = ~0u;
+            } else if (nd > 1) {
+                const int a = list[pass];
+                unsigned mine = 0u;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[b][h][e] = 0.0f;
-        for (int piece = 0; piece < (nd > 0 ? pieces : 0); ++piece) {
-            if (pass > 0 || piece > 0) {
-                __syncwarp();
-                fill_f(a, piece * RC);
+                for (int b = 0; b < PAIRS; ++b) {
+                    const int4 id = *(const int4 *)(ids + b * 16 + 4 * q);
+                    const unsigned m = (id.x == a) | (id.y == a) << 1 | (id.z == a) << 2 | (id.w == a) << 3;
+                    mine |= m << (b * 4);
+                    some |= (unsigned)(m != 0u) << b;
+                }
+                some = __reduce_or_sync(~0u, some);
+                write = exist & (pass == 0 ? mine | ~has : mine);  // those without an adapter in the first pass
             }
-            if (pieces > 1 || pass == 0) {
-                if (pass > 0 || piece > 0) __syncthreads();  // the last piece has been read by all
-                fill_s(piece * RC);
+            if (nd > 0) {
+                if (!ahead && (pass > 0 || chunk > 0)) {
+                    __syncwarp();
+                    fill_f(f, list[pass], chunk, rows);
+                    copy_commit();
+                    copy_wait<0>();
+                    __syncwarp();
+                }
+                multiply(f, some);
             }
-            copy_commit();
-            copy_wait<0>();
-            if (pieces > 1 || pass == 0)
-                __syncthreads();
+            if (p.outtype == 0)
+                store(std::integral_constant<int, 0>{}, old, write, rows);
+            else if (p.outtype == 1)
+                store(std::integral_constant<int, 1>{}, old, write, rows);
             else
-                __syncwarp();
-            if constexpr (sizeof(TF) == 2) {
+                store(std::integral_constant<int, 2>{}, old, write, rows);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ few columns
+//
+// A cluster of 8 blocks for one column, where a matrix instruction's 8 columns would mostly stand empty: each block takes an
+// eighth of D's columns (a lane 16 bytes of a row), the blocks add their R sums through distributed shared memory, and each
+// takes an eighth of U's rows, whose first loads start before the sums are joined.  fp32 sums throughout.  A call is bound
+// by its latency, many columns by the reads of their factors from L2.
+constexpr int TOKEN_RANKS = 8;
+
+// Element i of base (which may be Out: no read-only loads).
+__device__ __forceinline__ float load_base(const ApplyParams &p, long long i)
+{
+    return p.basetype == 0 ? ((const float *)p.base)[i] : as_float(((const unsigned short *)p.base)[i], p.basetype);
+}
+
+template <typename T, int VEC1, int VEC2>
+__global__ void __launch_bounds__(THREADS) lora_token(const ApplyParams p)
+{
+    constexpr int AHEAD = 4;  // rows of U in flight a thread
+    extern __shared__ __align__(16) float xs[];  // the block's part of the column
+    __shared__ float part[256], H[256 + 8];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long t = blockIdx.x / TOKEN_RANKS;
+    const int a = p.c.of(t);
+    const long long per2 = (p.n2 + TOKEN_RANKS - 1) / TOKEN_RANKS;
+    const long long m0 = min(p.n2, rank * per2), m1 = min(p.n2, m0 + per2);
+    if (a < 0) {  // the same in all blocks of the cluster
+        for (long long m = m0 + threadIdx.x; m < m1; m += THREADS)
+            store_as(p.Out, p.outtype, m * p.ldout + t, p.base ? load_base(p, m * p.ldbase + t) : 0.0f);
+        return;
+    }
+    // U: lanes2 threads a row; their rows' first loads.
+    const T *const U = (const T *)p.F2 + (long long)a * p.R * p.n2;
+    const int pieces2 = (p.R + VEC2 - 1) / VEC2;
+    int lanes2 = 1;
+    while (lanes2 < 32 && lanes2 < pieces2) lanes2 *= 2;
+    const int l2 = threadIdx.x & (lanes2 - 1), per_pass = THREADS / lanes2;
+    long long m = m0 + threadIdx.x / lanes2;
+    Pack<T, VEC2> u[AHEAD];
+    float old[AHEAD];
+    auto load_u = [&](long long first) {
 #pragma unroll
-                for (int k = 0; k < RC / 16; ++k) {
-                    unsigned A[4];
-                    load_matrices<TRANS>(A, TRANS ? f + (k * 16 + (lane & 7) + (lane >> 4) * 8) * Q::F_PITCH + (lane >> 3 & 1) * 16
-                                                  : f + (lane & 15) * Q::F_PITCH + (k * 16 + (lane >> 4) * 8) * 2);
-                    const int row = (k * 16 + (lane & 15)) * Q::S_PITCH + (lane >> 4) * 16;
-#pragma unroll
-                    for (int b = 0; b < PAIRS; ++b) {
-                        if (!(some >> b & 1)) continue;
-                        unsigned L[4], H[4];
-                        load_matrices<true>(L, sl + row + b * 32);
-                        load_matrices<true>(H, sh + row + b * 32);
-                        mma16<TF>(sum[b][0], A, L[0], L[1]);
-                        mma16<TF>(sum[b][1], A, L[2], L[3]);
-                        mma16<TF>(sum[b][0], A, H[0], H[1]);
-                        mma16<TF>(sum[b][1], A, H[2], H[3]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < RC; k += 8) {
-                    Operand<true> A[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = g + (e & 1) * 8, r = k + q + (e >> 1) * 4;
-                        A[e].set(*(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4));
-                    }
-#pragma unroll
-                    for (int b = 0; b < PAIRS; ++b)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const unsigned char *s = sh + (k + q) * Q::S_PITCH + (b * 16 + 4 * (g >> 1) + 2 * h + (g & 1)) * 4;
-                            Operand<true> B[2];
-                            B[0].set(*(const float *)s);
-                            B[1].set(*(const float *)(s + 4 * Q::S_PITCH));
-                            mma8_any<true>(sum[b][h], A, B[0], B[1]);
-                        }
-                }
+        for (int k = 0; k < AHEAD; ++k) {
+            const long long row = first + (long long)k * per_pass;
+            u[k].zero();
+            old[k] = 0.0f;
+            if (row < m1) {
+                if (l2 < pieces2) u[k].load(U + row * p.R + l2 * VEC2);
+                if (l2 == 0 && p.base) old[k] = load_base(p, row * p.ldbase + t);
             }
         }
-        if (p.outtype == 0)
-            store(std::integral_constant<int, 0>{}, write);
-        else if (p.outtype == 1)
-            store(std::integral_constant<int, 1>{}, write);
-        else
-            store(std::integral_constant<int, 2>{}, write);
+    };
+    load_u(m);
+
+    const long long k0 = min(p.n1, rank * p.per1), len = min(p.n1, k0 + p.per1) - k0;
+    for (long long i = threadIdx.x; i < len; i += THREADS) xs[i] = to_float(((const T *)p.In)[(k0 + i) * p.ldin + t]);
+    for (int r = p.R + (int)threadIdx.x; r < 256 + 8; r += THREADS) H[r] = 0.0f;
+    __syncthreads();
+    // D: lanes1 threads a row.
+    const T *const D = (const T *)p.F1 + (long long)a * p.R * p.n1 + k0;
+    int lanes1 = 1;
+    while (lanes1 < 32 && lanes1 * VEC1 < len) lanes1 *= 2;
+    const int l1 = lane & (lanes1 - 1), sub = lane / lanes1, rows1 = 32 / lanes1;
+#pragma unroll 4
+    for (int r0 = warp * rows1; r0 < p.R; r0 += WARPS * rows1) {
+        const int r = r0 + sub;
+        float v = 0.0f;
+        if (r < p.R) {
+#pragma unroll 2
+            for (long long i = l1 * VEC1; i < len; i += lanes1 * VEC1) {
+                Pack<T, VEC1> d;
+                d.load(D + r * p.n1 + i);
+#pragma unroll
+                for (int e = 0; e < VEC1; ++e) v += d.get(e) * xs[i + e];
+            }
+        }
+        for (int o = lanes1 >> 1; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+        if (l1 == 0 && r < p.R) part[r] = v;
     }
+    cluster.sync();
+    if (threadIdx.x < p.R) {
+        float x[TOKEN_RANKS], v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < TOKEN_RANKS; ++k) x[k] = cluster.map_shared_rank(part, k)[threadIdx.x];
+#pragma unroll
+        for (int k = 0; k < TOKEN_RANKS; ++k) v += x[k];
+        H[threadIdx.x] = p.scale ? v * __ldg(p.scale + a) : v;
+    }
+    cluster.barrier_arrive();
+    __syncthreads();
+    for (; m - (int)threadIdx.x / lanes2 < m1; m += (long long)AHEAD * per_pass) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const long long row = m + (long long)k * per_pass;
+            float v = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC2; ++e) v += u[k].get(e) * H[min(l2, pieces2 - 1) * VEC2 + e];
+            if (l2 >= pieces2) v = 0.0f;
+            for (int c = l2 + lanes2; c < pieces2 && row < m1; c += lanes2) {
+                Pack<T, VEC2> w;
+                w.load(U + row * p.R + c * VEC2);
+#pragma unroll
+                for (int e = 0; e < VEC2; ++e) v += w.get(e) * H[c * VEC2 + e];
+            }
+            for (int o = lanes2 >> 1; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+            if (l2 == 0 && row < m1) store_as(p.Out, p.outtype, row * p.ldout + t, old[k] + v);
+        }
+        load_u(m + (long long)AHEAD * per_pass);
+    }
+    cluster.barrier_wait();  // the others have read this block's sums
 }
 
 // ------------------------------------------------------------------ gradients of the factors
@@ -1053,32 +1221,47 @@ tcaspmm_status shrink(ApplyParams p, int sms, cudaStream_t st)
     });
 }
 
-template <typename TF, bool TRANS, int RC>
-tcaspmm_status expand_pieces(const ApplyParams &p, cudaStream_t st)
+template <typename TF, bool TRANS>
+tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
 {
-    using Q = ExpandShape<TF, RC, TRANS>;
-    const auto kernel = lora_expand<TF, RC, TRANS>;
-    const long long blocks = ceil_div(p.N, EXP_COLS) * ceil_div(p.n2, EXP_ROWS);
-    if (blocks == 0) return TCASPMM_OK;
-    if (blocks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many elements");
-    static std::atomic<unsigned long long> done{0};
-    const tcaspmm_status s = allow_shared("lora launch", (const void *)kernel, Q::BYTES, done);
-    return s != TCASPMM_OK ? s : launch("lora launch", kernel, dim3((unsigned)blocks), 0, true, Q::BYTES, st, p);
+    return with_rank(p.R, [&](auto rt) {
+        constexpr int RT = rt.value;
+        using Q = ExpandShape<TF, RT, TRANS>;
+        const auto kernel = lora_expand<TF, RT, TRANS>;
+        const long long across = ceil_div(p.N, EXP_COLS), chunks = ceil_div(p.n2, EXP_ROWS);
+        if (chunks == 0) return TCASPMM_OK;
+        // As many chunks a block as leave every SM four blocks.
+        p.chunks = (int)std::max<long long>(1, std::min<long long>(8, across * chunks / (4 * sms)));
+        const long long blocks = across * ceil_div(chunks, p.chunks);
+        if (blocks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many elements");
+        static std::atomic<unsigned long long> done{0};
+        const tcaspmm_status s = allow_shared("lora launch", (const void *)kernel, Q::BYTES, done);
+        return s != TCASPMM_OK ? s : launch("lora launch", kernel, dim3((unsigned)blocks), 0, true, Q::BYTES, st, p);
+    });
 }
 
-template <typename TF, bool TRANS>
-tcaspmm_status expand(const ApplyParams &p, cudaStream_t st)
+// Where the forward pass takes column by column: up to this many, when a column's part fits in shared memory.
+constexpr int TOKEN_MOST = 64;
+inline bool by_token(long long K, long long N) { return N <= TOKEN_MOST && K <= 8ll * 8192; }
+
+template <typename TF>
+tcaspmm_status token(ApplyParams p, cudaStream_t st)
 {
-    if (p.R <= 16) return expand_pieces<TF, TRANS, 16>(p, st);
-    if (p.R <= 32 || sizeof(TF) == 4) return expand_pieces<TF, TRANS, 32>(p, st);
-    return expand_pieces<TF, TRANS, sizeof(TF) == 4 ? 32 : 64>(p, st);
+    constexpr int VEC = 16 / (int)sizeof(TF);
+    p.per1 = ceil_div(ceil_div(p.n1, TOKEN_RANKS), VEC) * VEC;
+    const int shared = (int)std::max<long long>(p.per1, 1) * 4;
+    const dim3 grid((unsigned)(p.N * TOKEN_RANKS));
+    if (p.vec_f1 && p.vec_f2) return launch("lora launch", lora_token<TF, VEC, VEC>, grid, TOKEN_RANKS, false, shared, st, p);
+    if (p.vec_f1) return launch("lora launch", lora_token<TF, VEC, 1>, grid, TOKEN_RANKS, false, shared, st, p);
+    if (p.vec_f2) return launch("lora launch", lora_token<TF, 1, VEC>, grid, TOKEN_RANKS, false, shared, st, p);
+    return launch("lora launch", lora_token<TF, 1, 1>, grid, TOKEN_RANKS, false, shared, st, p);
 }
 
 template <typename TF, typename TI, bool TRANS>
 tcaspmm_status apply(const ApplyParams &p, int sms, cudaStream_t st)
 {
     const tcaspmm_status s = shrink<TF, TI, TRANS>(p, sms, st);
-    return s != TCASPMM_OK || !p.Out ? s : expand<TF, TRANS>(p, st);
+    return s != TCASPMM_OK || !p.Out ? s : expand<TF, TRANS>(p, sms, st);
 }
 
 template <typename TF>

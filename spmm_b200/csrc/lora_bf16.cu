@@ -3,7 +3,10 @@
 
 namespace tca {
 
-tcaspmm_status lora_forward_bf16(const ApplyParams &p, int sms, cudaStream_t st) { return apply<__nv_bfloat16, __nv_bfloat16, false>(p, sms, st); }
+tcaspmm_status lora_forward_bf16(const ApplyParams &p, bool tokens, int sms, cudaStream_t st)
+{
+    return tokens ? token<__nv_bfloat16>(p, st) : apply<__nv_bfloat16, __nv_bfloat16, false>(p, sms, st);
+}
 
 tcaspmm_status lora_input_grad_bf16(const ApplyParams &p, bool in32, int sms, cudaStream_t st)
 {

@@ -3,7 +3,10 @@
 
 namespace tca {
 
-tcaspmm_status lora_forward_f16(const ApplyParams &p, int sms, cudaStream_t st) { return apply<__half, __half, false>(p, sms, st); }
+tcaspmm_status lora_forward_f16(const ApplyParams &p, bool tokens, int sms, cudaStream_t st)
+{
+    return tokens ? token<__half>(p, st) : apply<__half, __half, false>(p, sms, st);
+}
 
 tcaspmm_status lora_input_grad_f16(const ApplyParams &p, bool in32, int sms, cudaStream_t st)
 {

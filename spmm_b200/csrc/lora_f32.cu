@@ -3,7 +3,10 @@
 
 namespace tca {
 
-tcaspmm_status lora_forward_f32(const ApplyParams &p, int sms, cudaStream_t st) { return apply<float, float, false>(p, sms, st); }
+tcaspmm_status lora_forward_f32(const ApplyParams &p, bool tokens, int sms, cudaStream_t st)
+{
+    return tokens ? token<float>(p, st) : apply<float, float, false>(p, sms, st);
+}
 
 tcaspmm_status lora_input_grad_f32(const ApplyParams &p, bool in32, int sms, cudaStream_t st)
 {

@@ -62,27 +62,6 @@ struct NormGradParams {
 
 namespace {
 
-// ------------------------------------------------------------------ vectors of elements
-template <int BYTES> struct Bits;
-template <> struct Bits<2> { using type = unsigned short; };
-template <> struct Bits<4> { using type = unsigned; };
-template <> struct Bits<8> { using type = uint2; };
-template <> struct Bits<16> { using type = uint4; };
-
-// VEC elements of type T as they lie in memory (at most 16 bytes).
-template <typename T, int VEC>
-struct Pack {
-    typename Bits<sizeof(T) * VEC>::type bits;
-    __device__ void load(const T *p) { bits = __ldg(reinterpret_cast<const decltype(bits) *>(p)); }
-    __device__ void zero() { bits = {}; }
-    __device__ float get(int i) const
-    {
-        T v[VEC];
-        memcpy(v, &bits, sizeof bits);
-        return to_float(v[i]);
-    }
-};
-
 template <int VEC, typename T>
 __device__ __forceinline__ void store_pack(T *p, const float (&v)[VEC])
 {

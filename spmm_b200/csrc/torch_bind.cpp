@@ -281,13 +281,18 @@ struct Adapters {
     }
 };
 
-int64_t hidden_bytes(const Tensor &x, int64_t R, int64_t N) { return (int64_t)tcaspmm_lora_hidden_bytes(R, N, code(x.scalar_type())); }
-
-Tensor hidden_buffer(const Tensor &x, int64_t R, int64_t N)
+int64_t hidden_bytes(const Tensor &x, int64_t R, bool keep)
 {
-    return at::empty({hidden_bytes(x, R, N)}, x.options().dtype(at::kByte));
+    return (int64_t)tcaspmm_lora_hidden_bytes(R, x.size(0), x.size(1), code(x.scalar_type()), keep);
 }
 
+Tensor hidden_buffer(const Tensor &x, int64_t R, bool keep)
+{
+    const int64_t size = hidden_bytes(x, R, keep);
+    return size || keep ? at::empty({size}, x.options().dtype(at::kByte)) : Tensor();
+}
+
+// H: where the caller wants what the backward pass reads, or null.
 Tensor lora_call(const Tensor &x, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
                  const MaybeTensor &base_, const Tensor *out, Tensor *H)
 {
@@ -312,17 +317,17 @@ Tensor lora_call(const Tensor &x, const Tensor &down, const Tensor &up, const Ma
     if (out) check_with(x, *out, "out");
     const c10::cuda::CUDAGuard guard(x.device());
     if (!out) Y = Matrix(at::empty({a.M, a.N}, x.options().dtype(type)), "out");
-    *H = hidden_buffer(x, a.R, a.N);
-    check(tcaspmm_lora(a.args(), a.X.ptr(), a.X.ld, a.N, base.ptr(), base.ld, Y.ptr(), Y.ld, code(type), H->data_ptr(),
-                       at::cuda::getCurrentCUDAStream().stream()));
+    const Tensor hidden = hidden_buffer(x, a.R, H != nullptr);
+    check(tcaspmm_lora(a.args(), a.X.ptr(), a.X.ld, a.N, base.ptr(), base.ld, Y.ptr(), Y.ld, code(type), ptr(hidden),
+                       H != nullptr, at::cuda::getCurrentCUDAStream().stream()));
+    if (H) *H = hidden;
     return Y.t;
 }
 
 Tensor lora(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
             const MaybeTensor &base)
 {
-    Tensor H;
-    return lora_call(X, down, up, index, scale, base, nullptr, &H);
+    return lora_call(X, down, up, index, scale, base, nullptr, nullptr);
 }
 
 std::tuple<Tensor, Tensor> lora_hidden(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index,
@@ -351,7 +356,7 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
     check_shape(dy, "dY", {a.M, a.N});
     TORCH_CHECK_VALUE(dy.scalar_type() == at::kFloat || dy.scalar_type() == x.scalar_type(), "dY must be float32 or X's type ",
                       x.scalar_type(), ", not ", dy.scalar_type());
-    TORCH_CHECK_VALUE(H.scalar_type() == at::kByte && H.dim() == 1 && H.is_contiguous() && H.numel() == hidden_bytes(x, a.R, a.N),
+    TORCH_CHECK_VALUE(H.scalar_type() == at::kByte && H.dim() == 1 && H.is_contiguous() && H.numel() == hidden_bytes(x, a.R, true),
                       "H must be the tensor that lora returned with hidden");
     const Tensor b = given(base_);
     Matrix base;
@@ -370,7 +375,7 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
     Tensor dD = at::empty(need_down ? a.down.sizes() : at::IntArrayRef{0}, x.options());
     Tensor dU = at::empty(need_up ? a.up.sizes() : at::IntArrayRef{0}, x.options());
     Tensor P;
-    if (need_input || need_down) P = hidden_buffer(x, a.R, a.N);
+    if (need_input || need_down) P = hidden_buffer(x, a.R, true);
     check(tcaspmm_lora_backward(a.args(), dY.ptr(), dY.ld, code(dy.scalar_type()), a.X.ptr(), a.X.ld, a.N, H.data_ptr(),
                                 (const float *)base.ptr(), base.ld, need_input ? dX.data_ptr() : nullptr, a.N,
                                 need_down ? dD.data_ptr() : nullptr, need_up ? dU.data_ptr() : nullptr, ptr(P),

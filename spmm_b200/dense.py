@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 
-from . import LIB_DIR, _sig
+from . import LIB_DIR, _sig, as_dtype, lib
 
 TORCH_PATH = os.path.join(LIB_DIR, "libtcaspmm_torch.so")
 _vp, _i64 = C.c_void_p, C.c_int64
@@ -27,12 +27,17 @@ _sig("tcaspmm_layer_norm", [_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, C.
 _sig("tcaspmm_layer_norm_backward_workspace", [_i64, _i64, C.c_int], C.c_size_t)
 _sig("tcaspmm_layer_norm_backward", [_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, _vp, C.c_int, _vp, _i64, _vp, _vp,
                                      _i64, _i64, C.c_int, _vp, C.c_size_t, _vp])
-_sig("tcaspmm_lora_hidden_bytes", [_i64, _i64, C.c_int], C.c_size_t)
-_sig("tcaspmm_lora", [C.POINTER(_Adapters), _vp, _i64, _i64, _vp, _i64, _vp, _i64, C.c_int, _vp, _vp])
+_sig("tcaspmm_lora_hidden_bytes", [_i64, _i64, _i64, C.c_int, C.c_int], C.c_size_t)
+_sig("tcaspmm_lora", [C.POINTER(_Adapters), _vp, _i64, _i64, _vp, _i64, _vp, _i64, C.c_int, _vp, C.c_int, _vp])
 _sig("tcaspmm_lora_backward", [C.POINTER(_Adapters), _vp, _i64, C.c_int, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
                                _vp, _vp, _vp])
 
 _OPS: dict = {}
+
+
+def hidden_bytes(rank: int, K: int, N: int, dt) -> int:
+    """Size of the buffer that lora returns with hidden."""
+    return lib.tcaspmm_lora_hidden_bytes(rank, K, N, int(as_dtype(dt)), 1)
 
 
 def _op(name: str):
@@ -52,12 +57,10 @@ def _op(name: str):
 def _register_shapes() -> None:
     import torch
 
-    from . import as_dtype, lib
-
     fake = torch.library.register_fake
 
     def hidden(X, down):
-        return X.new_empty(lib.tcaspmm_lora_hidden_bytes(down.shape[1], X.shape[1], int(as_dtype(X.dtype))), dtype=torch.uint8)
+        return X.new_empty(hidden_bytes(down.shape[1], X.shape[0], X.shape[1], X.dtype), dtype=torch.uint8)
 
     @fake("tcaspmm::layer_norm")
     def _(X, weight, bias, eps, dim, out_dtype):

@@ -33,7 +33,7 @@ from typing import Dict, Optional, Tuple
 import numpy as np
 import torch
 
-from . import CSR, Epilogue, Plan, as_dtype, dense, lib
+from . import CSR, Epilogue, Plan, as_dtype, dense
 
 
 class _Entry:
@@ -226,7 +226,7 @@ def _spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torc
 
 @_spmm_lora.register_fake
 def _(crow, col, val, X, down, up, index, scale):
-    size = lib.tcaspmm_lora_hidden_bytes(down.shape[1], X.shape[1], int(as_dtype(X.dtype)))
+    size = dense.hidden_bytes(down.shape[1], X.shape[0], X.shape[1], X.dtype)
     return X.new_empty((crow.shape[0] - 1, X.shape[1]), dtype=torch.float32), X.new_empty(size, dtype=torch.uint8)
 
 
