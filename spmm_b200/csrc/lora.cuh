@@ -270,17 +270,18 @@ struct ShrinkShape {
     static constexpr int STAGE = KS * IN_PITCH + F_ROWS * F_PITCH;
     static constexpr int S_PITCH = TN + 8;  // floats
     static constexpr int S_BYTES = RP * S_PITCH * 4;
-    // Two blocks an SM where a thread's sums leave the registers for it, else one.
-    static constexpr int BUDGET = (RT <= 4 ? 110 : 222) * 1024;
+    // Two blocks an SM where a thread's sums leave the registers for it, else one with a deeper ring.
+    static constexpr int BLOCKS = RT * TN <= 128 ? 2 : 1;
+    static constexpr int BUDGET = (BLOCKS == 2 ? 110 : 222) * 1024;
     static constexpr int FIT = BUDGET / (WARPS * STAGE);
-    static constexpr int STAGES = FIT >= 4 ? 4 : FIT;
+    static constexpr int STAGES = FIT >= 5 ? 5 : FIT;
     static_assert(STAGES >= 2, "the ring does not fit");
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int BYTES = RING > 4 * S_BYTES ? RING : 4 * S_BYTES;  // the ring, then four warps' sums
 };
 
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
-__global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_shrink(const ApplyParams p)
+__global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(const ApplyParams p)
 {
     using Q = ShrinkShape<TF, TI, RT, TN, TRANS>;
     constexpr int NB = TN / 8, RP = Q::RP, KS = Q::KS;
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_shrink(const Ap
     const long long in_left = p.N - t0 - in_col;
     const int in_bytes = in_left <= 0 ? 0 : in_left >= IN_PER ? 16 : (int)in_left * (int)sizeof(TI);
     const TI *const in_src = (const TI *)p.In + in_row * p.ldin + t0 + in_col;
+    const bool in_whole = t0 + TN <= p.N, f_whole = p.R == RP;
     const long long f_ld = TRANS ? p.R : p.n1;
 
     auto fill = [&](int slot, int step, int a) {
@@ -328,11 +330,16 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_shrink(const Ap
         if (p.vec_in) {
             const TI *src = in_src + i0 * p.ldin;
             unsigned char *to = in + in_row * Q::IN_PITCH + in_col * (int)sizeof(TI);
+            constexpr int RS = 32 / IN_CH;
+            if (rows == KS && in_whole) {
 #pragma unroll
-            for (int k = 0; k < KS * IN_CH / 32; ++k) {
-                constexpr int RS = 32 / IN_CH;
-                const int valid = in_row + k * RS < rows ? in_bytes : 0;
-                copy16(to + k * RS * Q::IN_PITCH, valid ? src + k * RS * p.ldin : (const TI *)p.In, valid);
+                for (int k = 0; k < KS * IN_CH / 32; ++k) copy16(to + k * RS * Q::IN_PITCH, src + k * RS * p.ldin, 16);
+            } else {
+#pragma unroll
+                for (int k = 0; k < KS * IN_CH / 32; ++k) {
+                    const int valid = in_row + k * RS < rows ? in_bytes : 0;
+                    copy16(to + k * RS * Q::IN_PITCH, valid ? src + k * RS * p.ldin : (const TI *)p.In, valid);
+                }
             }
         } else {
             for (int k = lane; k < KS * TN; k += 32) {
@@ -345,13 +352,20 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_shrink(const Ap
         const TF *F = (const TF *)p.F1 + (long long)a * p.R * p.n1 + (TRANS ? i0 * p.R : i0);
         if (p.vec_f1) {
             constexpr int COUNT = Q::F_ROWS * F_CH;
+            if (rows == KS && f_whole && COUNT % 32 == 0 && (F_CH <= 32 && 32 % F_CH == 0)) {
+                const TF *src = F + lane / F_CH * f_ld + lane % F_CH * F_PER;
+                unsigned char *to = f + lane / F_CH * Q::F_PITCH + lane % F_CH * 16;
 #pragma unroll
-            for (int k = 0; k < (COUNT + 31) / 32; ++k) {
-                const int r = (lane + k * 32) / F_CH, c = (lane + k * 32) % F_CH * F_PER;
-                const int left = TRANS ? (r < rows ? p.R - c : 0) : (r < p.R ? rows - c : 0);
-                const int valid = left <= 0 ? 0 : left >= F_PER ? 16 : left * (int)sizeof(TF);
-                if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
-                    copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F1, valid);
+                for (int k = 0; k < COUNT / 32; ++k) copy16(to + k * (32 / F_CH) * Q::F_PITCH, src + k * (32 / F_CH) * f_ld, 16);
+            } else {
+#pragma unroll
+                for (int k = 0; k < (COUNT + 31) / 32; ++k) {
+                    const int r = (lane + k * 32) / F_CH, c = (lane + k * 32) % F_CH * F_PER;
+                    const int left = TRANS ? (r < rows ? p.R - c : 0) : (r < p.R ? rows - c : 0);
+                    const int valid = left <= 0 ? 0 : left >= F_PER ? 16 : left * (int)sizeof(TF);
+                    if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
+                        copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F1, valid);
+                }
             }
         } else {
             for (int k = lane; k < Q::F_ROWS * Q::F_COLS; k += 32) {
@@ -661,8 +675,8 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
 #pragma unroll
         for (int e = 0; e < 4; ++e) exist |= (unsigned)(t0 + b * 16 + 4 * q + e < p.N) << (b * 4 + e);
     }
-    // The usual tile, without masks: one adapter for all of its columns.
-    const bool plain = __all_sync(~0u, has == 0xffffu) && nd == 1 && p.vec_out;
+    // The usual tile, without masks: one adapter for all of its columns, everything aligned.
+    const bool plain = __all_sync(~0u, has == 0xffffu) && nd == 1 && p.vec_out && p.vec_f2 && (fetch || !p.base) && Q::BUFFERS == 2;
     cudaGridDependencySynchronize();
     const Hidden hid(p.hidden, p.R, p.N);
     if (nd > 0) {  // S's columns
@@ -684,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
     __syncthreads();
 
     float sum[PAIRS][2][4];  // [pair][block of the pair][e]: rows g, g + 8; columns 16 pair + 4 q + 2 block + (e & 1)
-    auto multiply = [&](const unsigned char *f, unsigned some) {
+    auto multiply = [&](const unsigned char *f, auto all, unsigned some) {  // all: every pair, whatever `some` says
 #pragma unroll
         for (int b = 0; b < PAIRS; ++b)
 #pragma unroll
@@ -700,7 +714,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                 const int row = (k * 16 + (lane & 15)) * Q::S_PITCH + (lane >> 4) * 16;
 #pragma unroll
                 for (int b = 0; b < PAIRS; ++b) {
-                    if (!(some >> b & 1)) continue;
+                    if (!all.value && !(some >> b & 1)) continue;
                     unsigned L[4], H[4];
                     load_matrices<true>(L, sl + row + b * 32);
                     load_matrices<true>(H, sh + row + b * 32);
@@ -721,7 +735,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                 }
 #pragma unroll
                 for (int b = 0; b < PAIRS; ++b) {
-                    if (!(some >> b & 1)) continue;
+                    if (!all.value && !(some >> b & 1)) continue;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const unsigned char *s = sh + (k + q) * Q::S_PITCH + (b * 16 + 4 * (g >> 1) + 2 * h + (g & 1)) * 4;
@@ -752,12 +766,6 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                     y[2] *= c.z;
                     y[3] *= c.w;
                 }
-                if (plain) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] += old[b][h][e];
-                    store_four(row + b * 16, y);
-                    continue;
-                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] = has >> (b * 4 + e) & 1 ? old[b][h][e] + y[e] : old[b][h][e];
                 const unsigned w = write >> (b * 4) & 15u;
@@ -773,7 +781,112 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
     };
 
     const long long out_step = (long long)EXP_ROWS * p.ldout * out_size;
-    for (int chunk = 0; chunk < chunks; ++chunk, out += out_step, base += base_step) {
+    int chunk = 0;
+    if (plain) {
+        // Whole chunks of a usual tile: a lane's pieces of F2's slice lie CH pieces apart in one column (or row), all
+        // addresses advance by constants, and the next chunk's copies are under way while this one is multiplied.
+        constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, COUNT = Q::F_ROWS * CH;
+        constexpr int ROWS = CH >= 32 ? 1 : 32 / CH;  // rows from a lane's piece to its next
+        const int f_row = lane / CH, f_col = lane % CH * PER;
+        const TF *f_src = (const TF *)p.F2 + (long long)list[0] * p.R * p.n2 + (TRANS ? j_first : j_first * p.R) + f_row * f_ld + f_col;
+        const long long f_step = TRANS ? EXP_ROWS : (long long)EXP_ROWS * p.R;
+        const bool simple = CH <= 32 && COUNT % 32 == 0 && (TRANS ? true : f_col + PER <= p.R || f_col >= p.R);
+        auto fetch_f = [&](unsigned char *f, const TF *src) {
+            unsigned char *to = f + f_row * Q::F_PITCH + f_col * (int)sizeof(TF);
+#pragma unroll
+            for (int k = 0; k < COUNT / 32; ++k) {
+                const bool in = TRANS ? f_row + k * ROWS < p.R : f_col < p.R;
+                copy16(to + k * ROWS * Q::F_PITCH, in ? src + k * ROWS * f_ld : (const TF *)p.F2, in ? 16 : 0);
+            }
+        };
+        auto run = [&](auto base_type, auto out_type) {  // base_type -1: none
+            using TO = std::conditional_t<out_type.value == 0, float, std::conditional_t<out_type.value == 1, __half, __nv_bfloat16>>;
+            constexpr bool B32 = base_type.value == 0, B16 = base_type.value > 0;
+            for (; chunk < chunks && rows_of(chunk) == 16; ++chunk, out += out_step, base += base_step) {
+                copy_wait<0>();
+                __syncwarp();
+                float4 old[B32 ? PAIRS * 2 : 1];
+                uint2 old16[B16 ? PAIRS * 2 : 1];
+                if (B32) {
+#pragma unroll
+                    for (int i = 0; i < PAIRS * 2; ++i) old[i] = *(const float4 *)(ahead_base + i * (THREADS * 16));
+                }
+                if (B16) {
+#pragma unroll
+                    for (int i = 0; i < PAIRS * 2; ++i) old16[i] = *(const uint2 *)(ahead_base + i * (THREADS * 16));
+                }
+                if (chunk + 1 < chunks) {
+                    if (rows_of(chunk + 1) == 16 && simple) {
+                        if (B32 || B16) {
+                            const unsigned char *at = base + base_step;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int b = 0; b < PAIRS; ++b) {
+                                    const unsigned char *src = at + (h ? base_down : 0) + b * (B32 ? 64 : 32);
+                                    if (B32)
+                                        copy16(ahead_base + (b * 2 + h) * (THREADS * 16), src, 16);
+                                    else
+                                        copy8(ahead_base + (b * 2 + h) * (THREADS * 16), src, 8);
+                                }
+                        }
+                        f_src += f_step;
+                        fetch_f(f0 + (chunk + 1 & 1) * Q::F_BYTES, f_src);
+                    } else {
+                        if (B32 || B16) fetch_base(base + base_step, rows_of(chunk + 1));
+                        f_src += f_step;
+                        fill_f(f0 + (chunk + 1 & 1) * Q::F_BYTES, list[0], chunk + 1, rows_of(chunk + 1));
+                    }
+                }
+                copy_commit();
+                multiply(f0 + (chunk & 1) * Q::F_BYTES, std::true_type{}, 0u);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    TO *row = (TO *)out + h * 8 * p.ldout;
+#pragma unroll
+                    for (int b = 0; b < PAIRS; ++b) {
+                        float y[4] = {sum[b][0][2 * h], sum[b][0][2 * h + 1], sum[b][1][2 * h], sum[b][1][2 * h + 1]};
+                        if (HALF) {
+                            const float4 c = *(const float4 *)(colscale + b * 16 + 4 * q);
+                            y[0] *= c.x;
+                            y[1] *= c.y;
+                            y[2] *= c.z;
+                            y[3] *= c.w;
+                        }
+                        if (B32) {
+                            y[0] += old[b * 2 + h].x;
+                            y[1] += old[b * 2 + h].y;
+                            y[2] += old[b * 2 + h].z;
+                            y[3] += old[b * 2 + h].w;
+                        }
+                        if (B16) {
+                            y[0] += as_float(old16[b * 2 + h].x & 0xffffu, base_type.value);
+                            y[1] += as_float(old16[b * 2 + h].x >> 16, base_type.value);
+                            y[2] += as_float(old16[b * 2 + h].y & 0xffffu, base_type.value);
+                            y[3] += as_float(old16[b * 2 + h].y >> 16, base_type.value);
+                        }
+                        store_four(row + b * 16, y);
+                    }
+                }
+            }
+        };
+        // base has Out's type, or is fp32 beside a 16-bit Out, or there is none.
+        const auto with_base = [&](auto out_type) {
+            if (!p.base)
+                run(std::integral_constant<int, -1>{}, out_type);
+            else if (p.basetype == 0)
+                run(std::integral_constant<int, 0>{}, out_type);
+            else
+                run(out_type, out_type);
+        };
+        if (p.outtype == 0)
+            with_base(std::integral_constant<int, 0>{});
+        else if (p.outtype == 1)
+            with_base(std::integral_constant<int, 1>{});
+        else
+            with_base(std::integral_constant<int, 2>{});
+    }
+    for (; chunk < chunks; ++chunk, out += out_step, base += base_step) {
         const int rows = rows_of(chunk);
         copy_wait<0>();
         __syncwarp();
@@ -835,7 +948,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                     copy_wait<0>();
                     __syncwarp();
                 }
-                multiply(f, some);
+                multiply(f, std::false_type{}, some);
             }
             if (p.outtype == 0)
                 store(std::integral_constant<int, 0>{}, old, write, rows);
@@ -1198,9 +1311,8 @@ tcaspmm_status with_rank(int R, F &&f)
     return f(std::integral_constant<int, 16>{});
 }
 
-// Columns of a tile of the first product: a warp's sums (RT x TN / 8 x 4 registers a thread) leave room for two blocks an SM
-// up to rank 64.
-constexpr int tile_columns(int rt) { return rt <= 2 ? 64 : rt <= 8 ? 32 : 16; }
+// Columns of a tile of the first product: a warp's sums (RT x TN / 8 x 4 registers a thread) take at most 128 registers.
+constexpr int tile_columns(int rt) { return rt <= 4 ? 64 : rt == 8 ? 32 : 16; }
 
 template <typename TF, typename TI, bool TRANS>
 tcaspmm_status shrink(ApplyParams p, int sms, cudaStream_t st)
@@ -1210,9 +1322,9 @@ tcaspmm_status shrink(ApplyParams p, int sms, cudaStream_t st)
         using Q = ShrinkShape<TF, TI, RT, TN, TRANS>;
         const auto kernel = lora_shrink<TF, TI, RT, TN, TRANS>;
         const long long tiles = ceil_div(p.N, TN);
-        // Idle SMs take a share, while a warp has a step to do.
+        // Idle SMs take a share, while a warp has a step to do: at most one wave of blocks.
         int ranks = 1;
-        while (ranks < 8 && tiles * ranks < 2 * sms && p.n1 > (long long)ranks * WARPS * Q::KS) ranks *= 2;
+        while (ranks < 8 && tiles * ranks * 2 <= Q::BLOCKS * sms && p.n1 > (long long)ranks * WARPS * Q::KS) ranks *= 2;
         p.per1 = ceil_div(ceil_div(p.n1, ranks), Q::KS) * Q::KS;
         if (tiles * ranks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many columns");
         static std::atomic<unsigned long long> done{0};
@@ -1230,8 +1342,8 @@ tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
         const auto kernel = lora_expand<TF, RT, TRANS>;
         const long long across = ceil_div(p.N, EXP_COLS), chunks = ceil_div(p.n2, EXP_ROWS);
         if (chunks == 0) return TCASPMM_OK;
-        // As many chunks a block as leave every SM four blocks.
-        p.chunks = (int)std::max<long long>(1, std::min<long long>(8, across * chunks / (4 * sms)));
+        // As many chunks a block as leave every SM eight blocks (those with several adapters take longer).
+        p.chunks = (int)std::max<long long>(1, std::min<long long>(8, across * chunks / (8 * sms)));
         const long long blocks = across * ceil_div(chunks, p.chunks);
         if (blocks > INT_MAX) return fail(TCASPMM_ERR_UNSUPPORTED, "lora: too many elements");
         static std::atomic<unsigned long long> done{0};
