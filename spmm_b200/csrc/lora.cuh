@@ -33,6 +33,29 @@ struct Columns {
         const long long a = wide ? __ldg((const long long *)index + t) : (long long)__ldg((const int *)index + t);
         return a >= 0 && a < L ? (int)a : -1;
     }
+    // Those of columns t, t + step, ... below `end` (-2 past it), all loads in flight at once.
+    template <int COUNT>
+    __device__ __forceinline__ void of(long long t, long long step, long long end, int (&a)[COUNT]) const
+    {
+        if (index && wide) {
+            long long raw[COUNT];
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) raw[k] = t + k * step < end ? __ldg((const long long *)index + t + k * step) : -1;
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) a[k] = raw[k] >= 0 && raw[k] < L ? (int)raw[k] : -1;
+        } else if (index) {
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) a[k] = t + k * step < end ? __ldg((const int *)index + t + k * step) : -1;
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) a[k] = a[k] < L ? max(a[k], -1) : -1;
+        } else {
+#pragma unroll
+            for (int k = 0; k < COUNT; ++k) a[k] = L > 0 ? 0 : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < COUNT; ++k)
+            if (t + k * step >= end) a[k] = -2;
+    }
 };
 
 // Out = base + F2 S, S = scale F1 In, column by column with the column's adapter.  Forward: F1 = D (stored [r][i]), F2 = U
@@ -179,10 +202,18 @@ template <bool SPLIT> struct Operand;
 template <> struct Operand<false> {
     unsigned v;
     __device__ __forceinline__ void set(float x) { v = to_tf32(x); }
+    template <typename T> __device__ __forceinline__ void of(T x)
+    {
+        if (sizeof(T) == 2)
+            v = __float_as_uint(to_float(x));
+        else
+            set(to_float(x));
+    }
 };
 template <> struct Operand<true> {
     unsigned v, lo;
     __device__ __forceinline__ void set(float x) { split_tf32(x, v, lo); }
+    template <typename T> __device__ __forceinline__ void of(T x) { set(to_float(x)); }
 };
 
 template <bool SPLIT>
@@ -234,9 +265,14 @@ template <int TN>
 struct TileColumns {
     __align__(16) int ids[TN];
     int list[TN], count;
-    __device__ __forceinline__ void load(const Columns &c, long long t0, long long N)
+    // `meanwhile` runs while the indices are on their way.
+    template <typename F>
+    __device__ __forceinline__ void load(const Columns &c, long long t0, long long N, F &&meanwhile)
     {
-        for (int t = threadIdx.x; t < TN; t += THREADS) ids[t] = t0 + t < N ? c.of(t0 + t) : -1;
+        const long long mine = t0 + threadIdx.x;
+        const int id = threadIdx.x < TN && mine < N ? c.of(mine) : -1;
+        meanwhile();
+        if (threadIdx.x < TN) ids[threadIdx.x] = id;
         __syncthreads();
         if (threadIdx.x < 32) {
             const int lane = threadIdx.x;
@@ -295,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
     const long long t0 = (long long)(blockIdx.x / ranks) * TN;
     cudaTriggerProgrammaticLaunchCompletion();  // the next kernel may start: it waits for this one before it reads S
     if (threadIdx.x < TN) colmax[threadIdx.x] = 0;
-    tile.load(p.c, t0, p.N);
+    tile.load(p.c, t0, p.N, [] {});
     const int *const ids = tile.ids, *const list = tile.list;
     const int nd = tile.count;
 
@@ -323,11 +359,13 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
     const bool in_whole = t0 + TN <= p.N, f_whole = p.R == RP;
     const long long f_ld = TRANS ? p.R : p.n1;
 
-    auto fill = [&](int slot, int step, int a) {
+    auto fill = [&](int slot, int step, int a, bool with_in) {
         unsigned char *in = ring + slot * Q::STAGE, *f = in + KS * Q::IN_PITCH;
         const long long i0 = i_begin + (long long)(warp + step * WARPS) * KS;
         const int rows = (int)min((long long)KS, i_end - i0);
-        if (p.vec_in) {
+        if (!with_in) {
+            // The step's rows are still in registers.
+        } else if (p.vec_in) {
             const TI *src = in_src + i0 * p.ldin;
             unsigned char *to = in + in_row * Q::IN_PITCH + in_col * (int)sizeof(TI);
             constexpr int RS = 32 / IN_CH;
@@ -381,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
         int next_step = 0, next_d = 0, filled = 0, slot = 0;
         auto fill_next = [&]() {
             if (filled < items) {
-                fill(slot, next_step, list[next_d]);
+                fill(slot, next_step, list[next_d], !Q::M16 || next_d == 0);
                 if (++next_d == nd) {
                     next_d = 0;
                     ++next_step;
@@ -393,6 +431,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
         };
         for (int s = 0; s < Q::STAGES - 1; ++s) fill_next();
         int d = 0, at = 0;
+        unsigned B[Q::M16 ? NB : 1][2];
         for (int it = 0; it < items; ++it) {
             copy_wait<Q::STAGES - 2>();
             __syncwarp();  // the copies of all lanes have landed, and the slot filled next has been read by all
@@ -400,6 +439,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
             const unsigned char *in = ring + at * Q::STAGE, *f = in + KS * Q::IN_PITCH;
             if (++at == Q::STAGES) at = 0;
             const int a = list[d];
+            const bool first = d == 0;
             if (++d == nd) d = 0;
             // Which blocks of 8 columns hold columns of adapter a, and which others beside them.
             unsigned some = ~0u, mixed = 0u;
@@ -436,19 +476,21 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
                 }
             };
             if constexpr (Q::M16) {
-                unsigned A[RT][4], B[NB][2];
+                unsigned A[RT][4];
 #pragma unroll
                 for (int m = 0; m < RT; ++m)
                     load_matrices<TRANS>(A[m], TRANS ? f + ((lane & 7) + (lane >> 4) * 8) * Q::F_PITCH + (m * 16 + (lane >> 3 & 1) * 8) * 2
                                                      : f + (m * 16 + (lane & 15)) * Q::F_PITCH + (lane >> 4) * 16);
+                if (first) {  // the step's rows stay in registers for its other adapters
 #pragma unroll
-                for (int b = 0; b < NB; b += 2) {
-                    unsigned t[4];
-                    load_matrices<true>(t, in + (lane & 15) * Q::IN_PITCH + (b + (lane >> 4)) * 16);
-                    B[b][0] = t[0];
-                    B[b][1] = t[1];
-                    B[b + 1][0] = t[2];
-                    B[b + 1][1] = t[3];
+                    for (int b = 0; b < NB; b += 2) {
+                        unsigned t[4];
+                        load_matrices<true>(t, in + (lane & 15) * Q::IN_PITCH + (b + (lane >> 4)) * 16);
+                        B[b][0] = t[0];
+                        B[b][1] = t[1];
+                        B[b + 1][0] = t[2];
+                        B[b + 1][1] = t[3];
+                    }
                 }
                 add([&](int m, int b, float (&to)[4]) { mma16<TF>(to, A[m], B[b][0], B[b][1]); });
             } else {
@@ -460,18 +502,18 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = m * 16 + g + (e & 1) * 8, i = k + q + (e >> 1) * 4;
-                            A[m][e].set(to_float(*(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF))));
+                            A[m][e].of(*(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF)));
                         }
-                    Operand<Q::SPLIT> B[2];
+                    Operand<Q::SPLIT> B8[2];
                     int have = -1;
                     add([&](int m, int b, float (&to)[4]) {
                         if (have != b) {
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
-                                B[e].set(to_float(*(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI))));
+                                B8[e].of(*(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI)));
                             have = b;
                         }
-                        mma8_any<Q::SPLIT>(to, A[m], B[0], B[1]);
+                        mma8_any<Q::SPLIT>(to, A[m], B8[0], B8[1]);
                     });
                 }
             }
@@ -661,8 +703,9 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
     };
     auto rows_of = [&](int chunk) { return chunk >= chunks ? 0 : chunk == chunks - 1 ? last_rows : 16; };
 
-    if (fetch) fetch_base(base, rows_of(0));
-    tile.load(p.c, t0, p.N);
+    tile.load(p.c, t0, p.N, [&] {
+        if (fetch) fetch_base(base, rows_of(0));
+    });
     const int *const ids = tile.ids, *const list = tile.list;
     const int nd = tile.count;
     if (nd > 0 && chunks > 0) fill_f(f0, list[0], 0, rows_of(0));
@@ -886,7 +929,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
         else
             with_base(std::integral_constant<int, 2>{});
     }
-    for (; chunk < chunks; ++chunk, out += out_step, base += base_step) {
+    for (int turn = chunk; chunk < chunks; ++chunk, out += out_step, base += base_step) {
         const int rows = rows_of(chunk);
         copy_wait<0>();
         __syncwarp();
@@ -917,11 +960,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                 old[b][h][2] = v.z;
                 old[b][h][3] = v.w;
             }
-        // With one adapter and two buffers, F2's slice for the next chunk is fetched now; else each when it is needed.
-        const bool more = chunk + 1 < chunks, ahead = Q::BUFFERS == 2 && nd == 1;
-        unsigned char *const f = Q::BUFFERS == 2 ? f0 + (chunk & 1) * Q::F_BYTES : f0;
-        if (more && fetch) fetch_base(base + base_step, rows_of(chunk + 1));
-        if (more && ahead) fill_f(f0 + (chunk + 1 & 1) * Q::F_BYTES, list[0], chunk + 1, rows_of(chunk + 1));
+        if (chunk + 1 < chunks && fetch) fetch_base(base + base_step, rows_of(chunk + 1));
         copy_commit();
         for (int pass = 0; pass < max(nd, 1); ++pass) {
             unsigned some = 0u, write = exist;  // pairs with columns of this pass's adapter; columns that it writes
@@ -941,14 +980,20 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                 write = exist & (pass == 0 ? mine | ~has : mine);  // those without an adapter in the first pass
             }
             if (nd > 0) {
-                if (!ahead && (pass > 0 || chunk > 0)) {
-                    __syncwarp();
-                    fill_f(f, list[pass], chunk, rows);
-                    copy_commit();
+                // F2's slices alternate between two buffers: the next pass's (or chunk's) is fetched during this one.
+                const bool more = pass + 1 < nd || chunk + 1 < chunks;
+                const int next_pass = pass + 1 < nd ? pass + 1 : 0, next_chunk = pass + 1 < nd ? chunk : chunk + 1;
+                if (pass > 0) {
                     copy_wait<0>();
                     __syncwarp();
                 }
-                multiply(f, std::false_type{}, some);
+                if (Q::BUFFERS == 2 && more) fill_f(f0 + (turn + 1 & 1) * Q::F_BYTES, list[next_pass], next_chunk, rows_of(next_chunk));
+                copy_commit();
+                multiply(Q::BUFFERS == 2 ? f0 + (turn & 1) * Q::F_BYTES : f0, std::false_type{}, some);
+                __syncwarp();
+                if (Q::BUFFERS == 1 && more) fill_f(f0, list[next_pass], next_chunk, rows_of(next_chunk));
+                copy_commit();
+                ++turn;
             }
             if (p.outtype == 0)
                 store(std::integral_constant<int, 0>{}, old, write, rows);
@@ -1147,11 +1192,7 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
     for (long long scan = 0; scan < t_end; scan += GRAD_SCAN * GRAD_CHUNK) {
         __syncthreads();
         int id[GRAD_SCAN / 8];
-#pragma unroll
-        for (int k = 0; k < GRAD_SCAN / 8; ++k) {
-            const long long t = scan + (warp + k * 8) * GRAD_CHUNK + lane;
-            id[k] = t < t_end ? w.c.of(t) : -2;
-        }
+        w.c.of(scan + warp * GRAD_CHUNK + lane, 8 * GRAD_CHUNK, t_end, id);
 #pragma unroll
         for (int k = 0; k < GRAD_SCAN / 8; ++k) {
             // Columns past the end are read as zeros: they may count as the adapter's.
@@ -1200,8 +1241,8 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                 const bool in[2] = {(member >> (k + q) & 1) != 0, (member >> (k + q + 4) & 1) != 0};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float v = to_float(*(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ)));
-                    A[e].set(in[e >> 1] ? v : 0.0f);
+                    const TZ v = *(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ));
+                    A[e].of(in[e >> 1] ? v : from_float<TZ>(0.0f));
                 }
 #pragma unroll
                 for (int b = 0; b < RT * 2; ++b) {
@@ -1254,8 +1295,11 @@ __global__ void __launch_bounds__(256) lora_grad(const GradParams w)
             // Neighbouring threads write neighbouring elements.
             const int r = p.gr == 1 ? i % w.R : i / own, j = rank * own + (p.gr == 1 ? i / w.R : i % own);
             if (j0 + j >= p.n) continue;
-            float v = 0.0f;
-            for (int k = 0; k < ranks; ++k) v += cluster.map_shared_rank(sum, k)[j * Q::SUM_PITCH + r];
+            float x[8], v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = k < ranks ? cluster.map_shared_rank(sum, k)[j * Q::SUM_PITCH + r] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += x[k];
             G[(j0 + j) * p.gj + r * p.gr] = from_float<TF>(v);
         }
         cluster.sync();
