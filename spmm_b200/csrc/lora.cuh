@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
 // ------------------------------------------------------------------ Out = base + F2 S
 //
 // A block takes 64 columns and up to 8 chunks of 128 rows of Out, a warp 16 rows of a chunk.  S's columns stay in shared
-// memory; F2's slices and base come a chunk ahead (asynchronous copies), the first of them before the block waits for the
+// memory; F2's slices come a chunk ahead and base two (asynchronous copies), the first of them before the block waits for the
 // kernel that makes S (programmatic dependent launch), so that the start of this kernel hides behind the end of that
 // one.  Columns are dealt to the matrix instruction so that a thread's results of two blocks of 8 lie side by side: base and
 // Out move 16 bytes a thread.  In 16 bits both parts of S are multiplied, so that an fp32 Out is as exact as fp32 sums of
@@ -633,17 +633,20 @@ struct ExpandShape {
     static constexpr int S_PITCH = EXP_COLS * (int)sizeof(TF) + (sizeof(TF) == 4 ? 32 : 16);
     static constexpr int S_BYTES = RP * S_PITCH;  // one part
     static constexpr int S_ALL = S_BYTES * (sizeof(TF) == 2 ? 2 : 1);
-    static constexpr int BASE_BYTES = EXP_PAIRS * 2 * 16;  // a thread's part of a chunk of base
-    // Two blocks an SM; above rank 128 one, without base in shared memory.
-    static constexpr bool BASE = RT <= 8;
-    static constexpr int FIXED = S_ALL + (BASE ? BASE_BYTES * THREADS : 0);
-    static constexpr int BUFFERS = FIXED + 2 * WARPS * F_BYTES <= (BASE ? 110 : 222) * 1024 ? 2 : 1;
-    static constexpr int BYTES = FIXED + BUFFERS * WARPS * F_BYTES;
-    static_assert(BYTES <= 222 * 1024, "F2's slices do not fit");
+    // Two blocks an SM up to rank 64, else one; two chunks of base ahead, or as many as fit; F2's slices in two buffers where
+    // they fit.
+    static constexpr int BLOCKS = RT <= 4 ? 2 : 1;
+    static constexpr int ROOM = BLOCKS == 2 ? 112 * 1024 : 222 * 1024;
+    static constexpr int SLOT = EXP_PAIRS * 2 * 16 * THREADS;
+    static constexpr int LEAST = S_ALL + WARPS * F_BYTES;
+    static constexpr int SLOTS = LEAST + 2 * SLOT <= ROOM ? 2 : LEAST + SLOT <= ROOM ? 1 : 0;
+    static constexpr int BUFFERS = LEAST + SLOTS * SLOT + WARPS * F_BYTES <= ROOM ? 2 : 1;
+    static constexpr int BYTES = S_ALL + SLOTS * SLOT + BUFFERS * WARPS * F_BYTES;
+    static_assert(BYTES <= ROOM, "F2's slices do not fit");
 };
 
 template <typename TF, int RT, bool TRANS>
-__global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const ApplyParams p)
+__global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const ApplyParams p)
 {
     using Q = ExpandShape<TF, RT, TRANS>;
     constexpr bool HALF = std::is_same<TF, __half>::value;
@@ -657,14 +660,15 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
     const int chunks = (int)max(0ll, min((long long)p.chunks, (p.n2 - j_first + EXP_ROWS - 1) / EXP_ROWS));  // this warp's
     const int last_rows = chunks > 0 ? (int)min(16ll, p.n2 - j_first - (long long)(chunks - 1) * EXP_ROWS) : 0;
     unsigned char *const sh = smem, *const sl = smem + Q::S_BYTES, *const f0 = smem + Q::S_ALL + warp * (Q::BUFFERS * Q::F_BYTES);
-    unsigned char *const ahead_base = smem + Q::S_ALL + WARPS * Q::BUFFERS * Q::F_BYTES + threadIdx.x * 16;  // pieces THREADS * 16 apart
+    unsigned char *const slots = smem + Q::S_ALL + WARPS * Q::BUFFERS * Q::F_BYTES + threadIdx.x * 16;  // pieces THREADS * 16 apart
     __shared__ __align__(16) float colscale[EXP_COLS];
 
     const int base_size = p.basetype == 0 ? 4 : 2;
     const unsigned char *base = (const unsigned char *)p.base + ((j_first + g) * p.ldbase + t0 + 4 * q) * base_size;
-    const bool fetch = Q::BASE && p.base && t0 + EXP_COLS <= p.N && p.vec_base;  // base comes by asynchronous copies
+    const bool fetch = Q::SLOTS > 0 && p.base && t0 + EXP_COLS <= p.N && p.vec_base;  // base comes by asynchronous copies
     const long long base_step = (long long)EXP_ROWS * p.ldbase * base_size, base_down = 8 * p.ldbase * base_size;
-    auto fetch_base = [&](const unsigned char *at, int rows) {
+    auto fetch_base = [&](int chunk, const unsigned char *at, int rows) {  // a chunk's part of base, into its slot
+        unsigned char *const slot = slots + (Q::SLOTS == 2 ? (chunk & 1) * Q::SLOT : 0);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int valid = g + h * 8 < rows ? 16 : 0;
@@ -672,9 +676,9 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
 #pragma unroll
             for (int b = 0; b < PAIRS; ++b) {
                 if (base_size == 4)
-                    copy16(ahead_base + (b * 2 + h) * (THREADS * 16), row + (valid ? b * 64 : 0), valid);
+                    copy16(slot + (b * 2 + h) * (THREADS * 16), row + (valid ? b * 64 : 0), valid);
                 else
-                    copy8(ahead_base + (b * 2 + h) * (THREADS * 16), row + (valid ? b * 32 : 0), valid >> 1);
+                    copy8(slot + (b * 2 + h) * (THREADS * 16), row + (valid ? b * 32 : 0), valid >> 1);
             }
         }
     };
@@ -703,8 +707,25 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
     };
     auto rows_of = [&](int chunk) { return chunk >= chunks ? 0 : chunk == chunks - 1 ? last_rows : 16; };
 
-    tile.load(p.c, t0, p.N, [&] {
-        if (fetch) fetch_base(base, rows_of(0));
+    const Hidden hid(p.hidden, p.R, p.N);
+    tile.load(p.c, t0, p.N, [&] {  // while the indices are on their way: base, and S's columns
+        if (fetch) {
+            fetch_base(0, base, rows_of(0));
+            if (Q::SLOTS == 2 && chunks > 1) fetch_base(1, base + base_step, rows_of(1));
+        }
+        cudaGridDependencySynchronize();
+        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER, PARTS = sizeof(TF) == 2 ? 2 : 1;
+        const TF *src[2] = {sizeof(TF) == 4 ? (const TF *)hid.s() : hid.template hi<TF>(), hid.template lo<TF>()};
+        const int c = threadIdx.x % CH * PER, r = threadIdx.x / CH;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int k = 0; k < (RP * CH + THREADS - 1) / THREADS; ++k) {
+                const int row = r + k * (THREADS / CH), valid = row < p.R ? 16 : 0;
+                if (RP * CH % THREADS == 0 || row < RP)
+                    copy16((part ? sl : sh) + row * Q::S_PITCH + c * (int)sizeof(TF), valid ? src[part] + row * hid.pitch + t0 + c : src[part], valid);
+            }
+        if (HALF && threadIdx.x < EXP_COLS) colscale[threadIdx.x] = hid.colscale()[t0 + threadIdx.x];
     });
     const int *const ids = tile.ids, *const list = tile.list;
     const int nd = tile.count;
@@ -719,24 +740,8 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
         for (int e = 0; e < 4; ++e) exist |= (unsigned)(t0 + b * 16 + 4 * q + e < p.N) << (b * 4 + e);
     }
     // The usual tile, without masks: one adapter for all of its columns, everything aligned.
-    const bool plain = __all_sync(~0u, has == 0xffffu) && nd == 1 && p.vec_out && p.vec_f2 && (fetch || !p.base) && Q::BUFFERS == 2;
-    cudaGridDependencySynchronize();
-    const Hidden hid(p.hidden, p.R, p.N);
-    if (nd > 0) {  // S's columns
-        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER, PARTS = sizeof(TF) == 2 ? 2 : 1;
-        const TF *src[2] = {sizeof(TF) == 4 ? (const TF *)hid.s() : hid.template hi<TF>(), hid.template lo<TF>()};
-        const int c = threadIdx.x % CH * PER, r = threadIdx.x / CH;
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-            for (int k = 0; k < (RP * CH + THREADS - 1) / THREADS; ++k) {
-                const int row = r + k * (THREADS / CH), valid = row < p.R ? 16 : 0;
-                if (RP * CH % THREADS == 0 || row < RP)
-                    copy16((part ? sl : sh) + row * Q::S_PITCH + c * (int)sizeof(TF), valid ? src[part] + row * hid.pitch + t0 + c : src[part], valid);
-            }
-    }
+    const bool plain = __all_sync(~0u, has == 0xffffu) && nd == 1 && p.vec_out && p.vec_f2 && (fetch || !p.base);
     copy_commit();
-    if (HALF && threadIdx.x < EXP_COLS) colscale[threadIdx.x] = nd > 0 ? hid.colscale()[t0 + threadIdx.x] : 1.0f;
     copy_wait<0>();
     __syncthreads();
 
@@ -793,7 +798,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
     };
     const int out_size = p.outtype == 0 ? 4 : 2;
     unsigned char *out = (unsigned char *)p.Out + ((j_first + g) * p.ldout + t0 + 4 * q) * out_size;
-    auto store = [&](auto type, const float (&old)[PAIRS][2][4], unsigned write, int rows) {
+    auto store = [&](auto type, const float (&y)[PAIRS][2][4], int rows) {
         using TO = std::conditional_t<type.value == 0, float, std::conditional_t<type.value == 1, __half, __nv_bfloat16>>;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -801,23 +806,13 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
             TO *row = (TO *)out + h * 8 * p.ldout;
 #pragma unroll
             for (int b = 0; b < PAIRS; ++b) {
-                float y[4] = {sum[b][0][2 * h], sum[b][0][2 * h + 1], sum[b][1][2 * h], sum[b][1][2 * h + 1]};
-                if (HALF) {
-                    const float4 c = *(const float4 *)(colscale + b * 16 + 4 * q);
-                    y[0] *= c.x;
-                    y[1] *= c.y;
-                    y[2] *= c.z;
-                    y[3] *= c.w;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = has >> (b * 4 + e) & 1 ? old[b][h][e] + y[e] : old[b][h][e];
-                const unsigned w = write >> (b * 4) & 15u;
+                const unsigned w = exist >> (b * 4) & 15u;
                 if (p.vec_out && w == 15u) {
-                    store_four(row + b * 16, y);
+                    store_four(row + b * 16, y[b][h]);
                 } else if (w) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (w >> e & 1) row[b * 16 + e] = from_float<TO>(y[e]);
+                        if (w >> e & 1) row[b * 16 + e] = from_float<TO>(y[b][h][e]);
                 }
             }
         }
@@ -845,44 +840,58 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
         auto run = [&](auto base_type, auto out_type) {  // base_type -1: none
             using TO = std::conditional_t<out_type.value == 0, float, std::conditional_t<out_type.value == 1, __half, __nv_bfloat16>>;
             constexpr bool B32 = base_type.value == 0, B16 = base_type.value > 0;
+            // F2's slice of the next chunk, then base of the one after it: in groups of their own, so that the wait for the
+            // first leaves the second under way.
+            auto fetch_next = [&]() {
+                if (chunk + 1 < chunks) {
+                    f_src += f_step;
+                    unsigned char *const f = f0 + (Q::BUFFERS == 2 ? (chunk + 1 & 1) * Q::F_BYTES : 0);
+                    if (rows_of(chunk + 1) == 16 && simple)
+                        fetch_f(f, f_src);
+                    else
+                        fill_f(f, list[0], chunk + 1, rows_of(chunk + 1));
+                }
+                copy_commit();
+                if ((B32 || B16) && chunk + Q::SLOTS < chunks) {
+                    const unsigned char *at = base + Q::SLOTS * base_step;
+                    if (rows_of(chunk + Q::SLOTS) == 16) {
+                        unsigned char *const slot = slots + (Q::SLOTS == 2 ? (chunk & 1) * Q::SLOT : 0);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int b = 0; b < PAIRS; ++b) {
+                                const unsigned char *src = at + (h ? base_down : 0) + b * (B32 ? 64 : 32);
+                                if (B32)
+                                    copy16(slot + (b * 2 + h) * (THREADS * 16), src, 16);
+                                else
+                                    copy8(slot + (b * 2 + h) * (THREADS * 16), src, 8);
+                            }
+                    } else {
+                        fetch_base(chunk + Q::SLOTS, at, rows_of(chunk + Q::SLOTS));
+                    }
+                }
+                copy_commit();
+            };
             for (; chunk < chunks && rows_of(chunk) == 16; ++chunk, out += out_step, base += base_step) {
-                copy_wait<0>();
+                copy_wait<Q::SLOTS == 2 ? 1 : 0>();
                 __syncwarp();
+                const unsigned char *const slot = slots + (Q::SLOTS == 2 ? (chunk & 1) * Q::SLOT : 0);
                 float4 old[B32 ? PAIRS * 2 : 1];
                 uint2 old16[B16 ? PAIRS * 2 : 1];
                 if (B32) {
 #pragma unroll
-                    for (int i = 0; i < PAIRS * 2; ++i) old[i] = *(const float4 *)(ahead_base + i * (THREADS * 16));
+                    for (int i = 0; i < PAIRS * 2; ++i) old[i] = *(const float4 *)(slot + i * (THREADS * 16));
                 }
                 if (B16) {
 #pragma unroll
-                    for (int i = 0; i < PAIRS * 2; ++i) old16[i] = *(const uint2 *)(ahead_base + i * (THREADS * 16));
+                    for (int i = 0; i < PAIRS * 2; ++i) old16[i] = *(const uint2 *)(slot + i * (THREADS * 16));
                 }
-                if (chunk + 1 < chunks) {
-                    if (rows_of(chunk + 1) == 16 && simple) {
-                        if (B32 || B16) {
-                            const unsigned char *at = base + base_step;
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int b = 0; b < PAIRS; ++b) {
-                                    const unsigned char *src = at + (h ? base_down : 0) + b * (B32 ? 64 : 32);
-                                    if (B32)
-                                        copy16(ahead_base + (b * 2 + h) * (THREADS * 16), src, 16);
-                                    else
-                                        copy8(ahead_base + (b * 2 + h) * (THREADS * 16), src, 8);
-                                }
-                        }
-                        f_src += f_step;
-                        fetch_f(f0 + (chunk + 1 & 1) * Q::F_BYTES, f_src);
-                    } else {
-                        if (B32 || B16) fetch_base(base + base_step, rows_of(chunk + 1));
-                        f_src += f_step;
-                        fill_f(f0 + (chunk + 1 & 1) * Q::F_BYTES, list[0], chunk + 1, rows_of(chunk + 1));
-                    }
+                if (Q::BUFFERS == 2) fetch_next();
+                multiply(f0 + (Q::BUFFERS == 2 ? (chunk & 1) * Q::F_BYTES : 0), std::true_type{}, 0u);
+                if (Q::BUFFERS == 1) {
+                    __syncwarp();
+                    fetch_next();
                 }
-                copy_commit();
-                multiply(f0 + (chunk & 1) * Q::F_BYTES, std::true_type{}, 0u);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     TO *row = (TO *)out + h * 8 * p.ldout;
@@ -939,7 +948,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const unsigned char *at = ahead_base + (b * 2 + h) * (THREADS * 16);
+                const unsigned char *at = slots + (Q::SLOTS == 2 ? (chunk & 1) * Q::SLOT : 0) + (b * 2 + h) * (THREADS * 16);
                 if (fetch && base_size == 4) {
                     v = *(const float4 *)at;
                 } else if (fetch) {
@@ -960,48 +969,52 @@ __global__ void __launch_bounds__(THREADS, RT <= 8 ? 2 : 1) lora_expand(const Ap
                 old[b][h][2] = v.z;
                 old[b][h][3] = v.w;
             }
-        if (chunk + 1 < chunks && fetch) fetch_base(base + base_step, rows_of(chunk + 1));
+        if (chunk + Q::SLOTS < chunks && fetch) fetch_base(chunk + Q::SLOTS, base + Q::SLOTS * base_step, rows_of(chunk + Q::SLOTS));
         copy_commit();
-        for (int pass = 0; pass < max(nd, 1); ++pass) {
-            unsigned some = 0u, write = exist;  // pairs with columns of this pass's adapter; columns that it writes
-            if (nd == 1) {
-                some = ~0u;
-            } else if (nd > 1) {
-                const int a = list[pass];
-                unsigned mine = 0u;
+        for (int pass = 0; pass < nd; ++pass) {
+            // The thread's columns of this pass's adapter; pairs of blocks with any.
+            const int a = list[pass];
+            unsigned mine = 0u, some = 0u;
 #pragma unroll
-                for (int b = 0; b < PAIRS; ++b) {
-                    const int4 id = *(const int4 *)(ids + b * 16 + 4 * q);
-                    const unsigned m = (id.x == a) | (id.y == a) << 1 | (id.z == a) << 2 | (id.w == a) << 3;
-                    mine |= m << (b * 4);
-                    some |= (unsigned)(m != 0u) << b;
-                }
-                some = __reduce_or_sync(~0u, some);
-                write = exist & (pass == 0 ? mine | ~has : mine);  // those without an adapter in the first pass
+            for (int b = 0; b < PAIRS; ++b) {
+                const int4 id = *(const int4 *)(ids + b * 16 + 4 * q);
+                const unsigned m = (id.x == a) | (id.y == a) << 1 | (id.z == a) << 2 | (id.w == a) << 3;
+                mine |= m << (b * 4);
+                some |= (unsigned)(m != 0u) << b;
             }
-            if (nd > 0) {
-                // F2's slices alternate between two buffers: the next pass's (or chunk's) is fetched during this one.
-                const bool more = pass + 1 < nd || chunk + 1 < chunks;
-                const int next_pass = pass + 1 < nd ? pass + 1 : 0, next_chunk = pass + 1 < nd ? chunk : chunk + 1;
-                if (pass > 0) {
-                    copy_wait<0>();
-                    __syncwarp();
-                }
-                if (Q::BUFFERS == 2 && more) fill_f(f0 + (turn + 1 & 1) * Q::F_BYTES, list[next_pass], next_chunk, rows_of(next_chunk));
-                copy_commit();
-                multiply(Q::BUFFERS == 2 ? f0 + (turn & 1) * Q::F_BYTES : f0, std::false_type{}, some);
+            some = __reduce_or_sync(~0u, some);
+            // F2's slices alternate between two buffers: the next pass's (or chunk's) is fetched during this one.
+            const bool more = pass + 1 < nd || chunk + 1 < chunks;
+            const int next_pass = pass + 1 < nd ? pass + 1 : 0, next_chunk = pass + 1 < nd ? chunk : chunk + 1;
+            if (pass > 0) {
+                copy_wait<0>();
                 __syncwarp();
-                if (Q::BUFFERS == 1 && more) fill_f(f0, list[next_pass], next_chunk, rows_of(next_chunk));
-                copy_commit();
-                ++turn;
             }
-            if (p.outtype == 0)
-                store(std::integral_constant<int, 0>{}, old, write, rows);
-            else if (p.outtype == 1)
-                store(std::integral_constant<int, 1>{}, old, write, rows);
-            else
-                store(std::integral_constant<int, 2>{}, old, write, rows);
+            if (Q::BUFFERS == 2 && more) fill_f(f0 + (turn + 1 & 1) * Q::F_BYTES, list[next_pass], next_chunk, rows_of(next_chunk));
+            copy_commit();
+            multiply(Q::BUFFERS == 2 ? f0 + (turn & 1) * Q::F_BYTES : f0, std::false_type{}, some);
+            __syncwarp();
+            if (Q::BUFFERS == 1 && more) fill_f(f0, list[next_pass], next_chunk, rows_of(next_chunk));
+            copy_commit();
+            ++turn;
+#pragma unroll
+            for (int b = 0; b < PAIRS; ++b) {
+                float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                if (HALF) c = *(const float4 *)(colscale + b * 16 + 4 * q);
+                const float by[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (mine >> (b * 4 + e) & 1) old[b][h][e] += sum[b][e >> 1][2 * h + (e & 1)] * by[e];
+            }
         }
+        if (p.outtype == 0)
+            store(std::integral_constant<int, 0>{}, old, rows);
+        else if (p.outtype == 1)
+            store(std::integral_constant<int, 1>{}, old, rows);
+        else
+            store(std::integral_constant<int, 2>{}, old, rows);
     }
 }
 
