@@ -24,70 +24,84 @@ int sm_count()
 
 namespace {
 
-// A row's elements are dealt to its threads VEC at a time, NCH times; a thread's elements are the same in every row.
-template <typename T, int VEC, int NCH, bool BLOCK>
+// A row's elements are dealt to its threads VEC at a time, NCH times; a thread's elements are the same in every row.  Short rows
+// go ROWS at a time, so that enough bytes are on their way; the next rows are fetched before the present ones are summed.
+template <typename T, int VEC, int NCH, int ROWS, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_rows_fwd(const NormParams p, int lanes)
 {
     constexpr bool KEEP = VEC * NCH <= 8;  // weights stay in registers
-    __shared__ float s[2][1][32];
+    __shared__ float s[2][ROWS][32];
+    const int n = (int)p.n;
     const int tpr = BLOCK ? (int)blockDim.x : lanes;
     const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
-    const int per = BLOCK ? 1 : (int)blockDim.x / lanes;
-    const long long first = (long long)blockIdx.x * per + (BLOCK ? 0 : (int)threadIdx.x / lanes);
-    const long long step = (long long)gridDim.x * per;
-    const float inv = 1.0f / (float)p.n;
+    const int per = BLOCK ? 1 : (int)blockDim.x / lanes;  // rows side by side in a block
+    const long long first = (long long)blockIdx.x * per * ROWS + (BLOCK ? 0 : (int)threadIdx.x / lanes);
+    const long long step = (long long)gridDim.x * per * ROWS;
+    const float inv = 1.0f / (float)n;
     float w[KEEP ? VEC * NCH : 1], b[KEEP ? VEC * NCH : 1];
     if (KEEP) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const long long i = ((long long)c * tpr + t) * VEC;
-            if (i < p.n) {
+            const int i = (c * tpr + t) * VEC;
+            if (i < n) {
                 load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, w + c * VEC);
                 load_params<VEC>(p.b, p.pt, p.pvec, i, 0.0f, b + c * VEC);
             }
         }
     }
-    Pack<T, VEC> x[NCH], next[NCH];
-    auto fetch = [&](long long row, Pack<T, VEC> (&to)[NCH]) {
+    Pack<T, VEC> x[ROWS][NCH], next[ROWS][NCH];
+    auto fetch = [&](long long row, Pack<T, VEC> (&to)[ROWS][NCH]) {  // rows row, row + per, ...
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const long long i = ((long long)c * tpr + t) * VEC;
-            if (row < p.vecs && i < p.n)
-                to[c].load((const T *)p.X + row * p.ldx + i);
-            else
-                to[c].zero();
+        for (int r = 0; r < ROWS; ++r) {
+            const bool in = row + r * per < p.vecs;
+            const T *src = (const T *)p.X + (row + r * per) * p.ldx + t * VEC;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                if (in && (c * tpr + t) * VEC < n)
+                    to[r][c].load(src + c * tpr * VEC);
+                else
+                    to[r][c].zero();
+            }
         }
     };
     fetch(first, x);
     // Every thread of a warp (block) takes the same number of turns: rows past the end are read as zeros and not written.
-    const long long turns = (p.vecs - (long long)blockIdx.x * per + step - 1) / step;
-    for (long long k = 0; k < turns; ++k) {
-        const long long row = first + k * step;
+    for (long long start = (long long)blockIdx.x * per * ROWS, row = first; start < p.vecs; start += step, row += step) {
         fetch(row + step, next);
-        float a[1] = {0.0f};
+        float mean[ROWS], sq[ROWS];
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+        for (int r = 0; r < ROWS; ++r) {
+            mean[r] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) a[0] += x[c].get(e);
-        row_sum<BLOCK>(a, lanes, s[0]);
-        const float mean = a[0] * inv;
-        a[0] = 0.0f;
+            for (int c = 0; c < NCH; ++c)
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
-            if (((long long)c * tpr + t) * VEC < p.n) {
+                for (int e = 0; e < VEC; ++e) mean[r] += x[r][c].get(e);
+        }
+        row_sum<BLOCK>(mean, lanes, s[0]);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float d = x[c].get(e) - mean;
-                    a[0] += d * d;
+        for (int r = 0; r < ROWS; ++r) {
+            mean[r] *= inv;
+            sq[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+                if ((c * tpr + t) * VEC < n) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float d = x[r][c].get(e) - mean[r];
+                        sq[r] += d * d;
+                    }
                 }
-            }
-        row_sum<BLOCK>(a, lanes, s[1]);
-        const float rstd = 1.0f / sqrtf(a[0] * inv + p.eps);
-        if (row < p.vecs) {
+        }
+        row_sum<BLOCK>(sq, lanes, s[1]);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long at = row + r * per;
+            if (at >= p.vecs) continue;
+            const float rstd = 1.0f / sqrtf(sq[r] * inv + p.eps);
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                const long long i = ((long long)c * tpr + t) * VEC;
-                if (i < p.n) {
+                const int i = (c * tpr + t) * VEC;
+                if (i < n) {
                     float y[VEC], ww[VEC], bb[VEC];
                     if (!KEEP) {
                         load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
@@ -95,110 +109,129 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_rows_fwd(const NormPa
                     }
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
-                        y[e] = (x[c].get(e) - mean) * rstd * (KEEP ? w[c * VEC + e] : ww[e]) + (KEEP ? b[c * VEC + e] : bb[e]);
-                    store_vec<VEC>(p.Y, p.yt, row * p.ldy + i, y);
+                        y[e] = (x[r][c].get(e) - mean[r]) * rstd * (KEEP ? w[c * VEC + e] : ww[e]) + (KEEP ? b[c * VEC + e] : bb[e]);
+                    store_vec<VEC>(p.Y, p.yt, at * p.ldy + i, y);
                 }
             }
             if (t == 0 && p.mean) {
-                p.mean[row] = mean;
-                p.rstd[row] = rstd;
+                p.mean[at] = mean[r];
+                p.rstd[at] = rstd;
             }
         }
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) x[c] = next[c];
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) x[r][c] = next[r][c];
     }
 }
 
-template <typename T, int VEC, int NCH>
-__global__ void __launch_bounds__(STRIP_THREADS) norm_cols_fwd(const NormParams p, const Strip q)
+template <typename T>
+__global__ void __launch_bounds__(STRIP_THREADS) norm_cols_fwd(const NormParams p, const Strip q, int vec)
 {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float s[1][STRIP_WARPS][STRIP_MAX];
     __shared__ float sums[2][STRIP_MAX];  // this block's sum of x, then of squared differences from its own mean
-    __shared__ float fin[2][STRIP_MAX];   // the strip's mean and rstd
+    __shared__ __align__(16) float fin[2][STRIP_MAX];  // the strip's mean and rstd
+    T *const tile = (T *)smem;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int width = q.lpr * VEC, at = (threadIdx.x & (q.lpr - 1)) * VEC;
-    const long long col = (long long)(blockIdx.x / ranks) * width + at;
-    const long long r0 = min(p.n, rank * q.per_block), r1 = min(p.n, r0 + q.per_block);
-    const int lane_row = threadIdx.x >> q.shift, rows = STRIP_THREADS >> q.shift;
-    Pack<T, VEC> x[NCH];
+    const long long c0 = (long long)(blockIdx.x / ranks) * width;
+    const long long r0 = min(p.n, (long long)rank * q.per_block);
+    const int rows = (int)(min(p.n, r0 + q.per_block) - r0);
+    const int row = threadIdx.x >> q.shift, step = STRIP_THREADS >> q.shift;
+    load_strip<T, VEC>(tile, (const T *)p.X, p.ldx, r0, rows, c0, p.vecs, width, q, vec);
+    copy_async_wait();
+    __syncthreads();
     float v[1][VEC] = {};
+#pragma unroll 4
+    for (int r = row; r < rows; r += step) {
+        float x[VEC];
+        load_shared<T, VEC>(tile + r * width + at, x);
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const long long r = r0 + lane_row + c * rows;
-        if (r < r1 && col < p.vecs)
-            x[c].load((const T *)p.X + r * p.ldx + col);
-        else
-            x[c].zero();
+        for (int e = 0; e < VEC; ++e) v[0][e] += x[e];
     }
-#pragma unroll
-    for (int c = 0; c < NCH; ++c)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[0][e] += x[c].get(e);
     strip_sum(v, q.lpr, s, sums);
-    const float inv = r1 > r0 ? 1.0f / (float)(r1 - r0) : 0.0f;
+    const float inv = rows > 0 ? 1.0f / (float)rows : 0.0f;
     float m[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         m[e] = sums[0][at + e] * inv;
         v[0][e] = 0.0f;
     }
+#pragma unroll 4
+    for (int r = row; r < rows; r += step) {
+        float x[VEC];
+        load_shared<T, VEC>(tile + r * width + at, x);
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
-        if (r0 + lane_row + c * rows < r1) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float d = x[c].get(e) - m[e];
-                v[0][e] += d * d;
-            }
+        for (int e = 0; e < VEC; ++e) {
+            const float d = x[e] - m[e];
+            v[0][e] += d * d;
         }
+    }
     strip_sum(v, q.lpr, s, sums + 1);
-    cluster.sync();
+    if (ranks > 1) cluster.sync();
     // Blocks' sums joined: sum (x - mean)^2 = sum over blocks of its own about its mean + rows (its mean - mean)^2.
     if ((int)threadIdx.x < width) {
         const int j = threadIdx.x;
-        float total = 0.0f, sq = 0.0f;
-        for (int k = 0; k < ranks; ++k) total += cluster.map_shared_rank(&sums[0][0], k)[j];
+        float part[8], own[8], total = 0.0f, sq = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float *o = cluster.map_shared_rank(&sums[0][0], k < ranks ? k : 0);
+            part[k] = k < ranks ? o[j] : 0.0f;
+            own[k] = k < ranks ? o[STRIP_MAX + j] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) total += part[k];
         const float mean = total / (float)p.n;
-        for (int k = 0; k < ranks; ++k) {
-            const float *o = cluster.map_shared_rank(&sums[0][0], k);
-            const long long cnt = min(p.n, (k + 1) * q.per_block) - min(p.n, k * q.per_block);
-            if (cnt > 0) {
-                const float d = o[j] * (1.0f / (float)cnt) - mean;
-                sq += o[STRIP_MAX + j] + (float)cnt * d * d;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const long long count = k < ranks ? min(p.n, (long long)(k + 1) * q.per_block) - min(p.n, (long long)k * q.per_block) : 0;
+            if (count > 0) {
+                const float d = part[k] * (1.0f / (float)count) - mean;
+                sq += own[k] + (float)count * d * d;
             }
         }
         fin[0][j] = mean;
         fin[1][j] = 1.0f / sqrtf(sq / (float)p.n + p.eps);
+        if (p.mean && rank == 0 && c0 + j < p.vecs) {
+            p.mean[c0 + j] = mean;
+            p.rstd[c0 + j] = fin[1][j];
+        }
     }
     __syncthreads();
-    float mean[VEC], rstd[VEC];
+    if (ranks > 1) cluster.barrier_arrive();  // this block has read the others' sums
+    if (vec) {
+        float mean[VEC], rstd[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        mean[e] = fin[0][at + e];
-        rstd[e] = fin[1][at + e];
-    }
-    if (col < p.vecs) {
+        for (int e = 0; e < VEC; ++e) {
+            mean[e] = fin[0][at + e];
+            rstd[e] = fin[1][at + e];
+        }
+        if (c0 + at < p.vecs) {
+#pragma unroll 4
+            for (int r = row; r < rows; r += step) {
+                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f, b = p.b ? load_as(p.b, p.pt, r0 + r) : 0.0f;
+                float x[VEC];
+                load_shared<T, VEC>(tile + r * width + at, x);
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const long long r = r0 + lane_row + c * rows;
-            if (r < r1) {
-                const float w = p.w ? load_as(p.w, p.pt, r) : 1.0f, b = p.b ? load_as(p.b, p.pt, r) : 0.0f;
-                float y[VEC];
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) y[e] = (x[c].get(e) - mean[e]) * rstd[e] * w + b;
-                store_vec<VEC>(p.Y, p.yt, r * p.ldy + col, y);
+                for (int e = 0; e < VEC; ++e) x[e] = (x[e] - mean[e]) * rstd[e] * w + b;
+                store_vec<VEC>(p.Y, p.yt, (r0 + r) * p.ldy + c0 + at, x);
             }
         }
-        if (p.mean && rank == 0 && lane_row == 0) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                p.mean[col + e] = mean[e];
-                p.rstd[col + e] = rstd[e];
+    } else {
+        const int c = threadIdx.x & (width - 1);
+        const float mean = fin[0][c], rstd = fin[1][c];
+        if (c0 + c < p.vecs) {
+#pragma unroll 4
+            for (int r = threadIdx.x / width; r < rows; r += STRIP_THREADS / width) {
+                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f, b = p.b ? load_as(p.b, p.pt, r0 + r) : 0.0f;
+                store_as(p.Y, p.yt, (r0 + r) * p.ldy + c0 + c, (to_float(tile[r * width + c]) - mean) * rstd * w + b);
             }
         }
     }
-    cluster.sync();  // a block's sums are read by the others until here
+    if (ranks > 1) cluster.barrier_wait();
 }
 
 // One block per vector, read three times: for vectors too long for the registers of a block (rows) or a cluster (columns).
@@ -256,25 +289,23 @@ tcaspmm_status forward(const NormParams &p, int dim, cudaStream_t st)
     if (dim == 1) {
         const RowPlan r = plan_rows(p.n, VEC, FWD_MOST, 1024);
         if (r.nch) {
-            const long long per = r.lanes ? 256 / r.lanes : 1;
-            // Blocks an SM holds: at most 64 registers a thread up to 8 elements (2048 threads at 1), 128 above.
-            const long long fit = !r.lanes ? std::max(1, 1024 / r.threads) : r.nch * VEC > 8 ? 2 : r.nch * VEC > 4 ? 4 : 8;
-            const unsigned grid = blocks_of(std::min(ceil_div(p.vecs, per), fit * sm_count()));
+            // Blocks an SM holds: at most 64 registers a thread up to 8 elements, 128 above.
+            const long long fit = !r.lanes ? std::max(1, 1024 / r.threads) : r.nch * VEC > 8 ? 2 : 4;
             return with_chunks<FWD_MOST / VEC>(r.nch, [&](auto nch) {
+                constexpr int N = nch.value, ROWS = N * VEC * (int)sizeof(T) <= 16 ? 4 : N * VEC * (int)sizeof(T) <= 32 ? 2 : 1;
+                const long long per = r.lanes ? 256 / r.lanes * ROWS : 1;
+                const unsigned grid = blocks_of(std::min(ceil_div(p.vecs, per), fit * sm_count()));
                 if (r.lanes)
-                    norm_rows_fwd<T, VEC, nch.value, false><<<grid, 256, 0, st>>>(p, r.lanes);
+                    norm_rows_fwd<T, VEC, N, ROWS, false><<<grid, 256, 0, st>>>(p, r.lanes);
                 else
-                    norm_rows_fwd<T, VEC, nch.value, true><<<grid, r.threads, 0, st>>>(p, 32);
+                    norm_rows_fwd<T, VEC, N, 1, true><<<grid, r.threads, 0, st>>>(p, 32);
                 return launched("layer_norm launch");
             });
         }
     } else {
-        constexpr int MOST = VEC == 1 ? STRIP_ROWS_ONE : STRIP_ROWS_VEC;
-        const StripPlan s = plan_strips(p.n, p.vecs, VEC, MOST, sm_count());
-        if (s.ranks && s.strips * s.ranks <= INT_MAX)
-            return with_chunks<MOST>(s.nch, [&](auto nch) {
-                return launch_cluster(norm_cols_fwd<T, VEC, nch.value>, s.strips * s.ranks, s.ranks, st, p, s.q);
-            });
+        const StripPlan q = plan_strips(p.n, p.vecs, 16 / (int)sizeof(T), sizeof(T), sizeof(T), 128, sm_count());
+        static std::atomic<unsigned long long> done{0};
+        if (q.ranks && q.strips * q.ranks <= INT_MAX) return launch_cluster(norm_cols_fwd<T>, q, done, st, p, q.q, (int)(VEC > 1));
     }
     norm_long_fwd<T><<<blocks_of(p.vecs), 1024, 0, st>>>(p, dim ? p.ldx : 1, dim ? 1 : p.ldx, dim ? p.ldy : 1, dim ? 1 : p.ldy);
     return launched("layer_norm launch");
@@ -318,10 +349,10 @@ extern "C" size_t tcaspmm_layer_norm_backward_workspace(int64_t rows, int64_t co
 {
     if (rows <= 0 || cols <= 0) return 0;
     const long long n = dim == 1 ? cols : rows, vecs = dim == 1 ? rows : cols;
-    // Rows: ROW_PARTS blocks an SM, or LONG_PARTS.  Columns: a strip for every 32 columns up to 4096 rows; longer ones have
-    // strips of at least 131072 / rows columns rounded down to a power of two (plan_strips, elements one by one or by vectors).
-    long long width = 32;
-    while (width > 1 && width * n > 131072) width /= 2;
+    // Rows: ROW_PARTS blocks an SM, or LONG_PARTS.  Columns: a strip for every 16 columns; of columns that 8 blocks' shared
+    // memory holds only in narrower strips (199 KB each, at most 8 bytes an element), for every 8, 4, ...
+    long long width = 16;
+    while (width > 4 && width * n * 8 > 8 * 199 * 1024) width /= 2;
     const long long parts = dim == 1 ? std::max<long long>((long long)ROW_PARTS * sm_count(), LONG_PARTS) : ceil_div(vecs, width);
     return (size_t)(2 * std::min(parts, std::max<long long>(vecs, 1)) * n) * sizeof(float);
 }

@@ -6,16 +6,17 @@
 //   mean = sum x / n    rstd = 1 / sqrt(sum (x - mean)^2 / n + eps)    xh = (x - mean) rstd    y = w xh + b
 //   g = w dy            dx = rstd (g - mean(g) - xh mean(g xh))        dw = sum dy xh          db = sum dy
 //
-// Every pass is bound by memory: the vector is read once, held in registers as it came, and summed twice there (the mean
+// Every pass is bound by memory: the vector is read once, held as it came (registers, or shared memory), and summed twice there (the mean
 // first, then the squared differences from it, so that a large mean costs no precision).  Rows: a part of a warp, a warp or a
 // block per row, whichever leaves a thread at most 16 elements.  Columns: a cluster of up to 8
-// blocks shares a strip of 32-64 columns, each block holds a part of the strip's rows, and the blocks exchange their sums
+// blocks shares a strip of 16-64 columns, each block holds a part of the strip's rows, and the blocks exchange their sums
 // through distributed shared memory, so that reads stay coalesced along the rows.  The weight's gradient is summed by each
 // thread over the vectors it meets (its features stay the same), by block through shared memory, and over the blocks by a
 // second kernel, in a fixed order.
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstring>
 #include <type_traits>
@@ -75,6 +76,17 @@ __device__ __forceinline__ void store_pack(T *p, const float (&v)[VEC])
         memcpy(&bits, t, sizeof bits);
         *reinterpret_cast<decltype(bits) *>(p + k) = bits;
     }
+}
+
+// VEC elements in shared memory.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_shared(const T *p, float *v)
+{
+    typename Bits<sizeof(T) * VEC>::type bits = *reinterpret_cast<const decltype(bits) *>(p);
+    T t[VEC];
+    memcpy(t, &bits, sizeof bits);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = to_float(t[e]);
 }
 
 template <int VEC>
@@ -149,9 +161,61 @@ __device__ __forceinline__ void row_sum(float (&v)[COUNT], int lanes, float (*s)
 }
 
 // ------------------------------------------------------------------ columns
-constexpr int STRIP_THREADS = 512;
+//
+// A cluster's block holds its part of a strip's rows in shared memory (asynchronous copies where the rows' alignment allows
+// them, 16 bytes a thread), so that several blocks an SM load, sum and write at the same time.
+constexpr int STRIP_THREADS = 256;
 constexpr int STRIP_WARPS = STRIP_THREADS / 32;
 constexpr int STRIP_MAX = 64;  // columns of a strip at most
+
+struct Strip {
+    int lpr, shift;  // threads along a row of the strip (a power of two), its logarithm
+    int per_block;   // rows of a block
+};
+
+__device__ __forceinline__ void copy_async(void *dst, const void *src, int bytes)  // 8 or 16
+{
+    const unsigned to = (unsigned)__cvta_generic_to_shared(dst);
+    if (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory"); }
+
+// Rows r0 .. r0 + rows - 1 of the strip of `width` columns (a power of two) from column c0 on, into `tile` ([row][width]); columns
+// past `cols` as zeros.  Every thread's copies have landed when it returns; the block's, after a barrier.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_strip(T *tile, const T *X, long long ld, long long r0, int rows, long long c0, long long cols, int width,
+                                           const Strip &q, bool vec)
+{
+    if (vec) {
+        const int c = (threadIdx.x & (q.lpr - 1)) * VEC;
+        const T *src = X + (r0 + (threadIdx.x >> q.shift)) * ld + c0 + c;
+        const long long step = (long long)(STRIP_THREADS >> q.shift) * ld;
+        if (c0 + c < cols) {
+            for (int r = threadIdx.x >> q.shift; r < rows; r += STRIP_THREADS >> q.shift, src += step)
+                copy_async(tile + r * width + c, src, VEC * (int)sizeof(T));
+        } else {
+            for (int r = threadIdx.x >> q.shift; r < rows; r += STRIP_THREADS >> q.shift)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) tile[r * width + c + e] = from_float<T>(0.0f);
+        }
+    } else {
+        // Element by element: a column for each thread along a row, eight rows in flight.
+        const int c = threadIdx.x & (width - 1), per = STRIP_THREADS / width;
+        const bool in = c0 + c < cols;
+        const T *src = X + c0 + c;
+        for (int r = threadIdx.x / width; r < rows; r += 8 * per) {
+            T v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = in && r + k * per < rows ? src[(r0 + r + k * per) * ld] : from_float<T>(0.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (r + k * per < rows) tile[(r + k * per) * width + c] = v[k];
+        }
+    }
+}
 
 // Sums over the block's rows of COUNT values for each of a thread's VEC columns, into `out`, one per column of the strip.
 // Threads of a warp whose numbers agree modulo `lpr` hold the same columns.
@@ -184,11 +248,6 @@ __device__ __forceinline__ void strip_sum(float (&v)[COUNT][VEC], int lpr, float
     }
     __syncthreads();
 }
-
-struct Strip {
-    int lpr, shift;       // threads along a row of the strip (a power of two), its logarithm
-    long long per_block;  // rows of a block
-};
 
 // ------------------------------------------------------------------ vectors of any length
 // Sum over the block's threads, the same in all of them.  `s` holds a float per warp.
@@ -246,43 +305,53 @@ RowPlan plan_rows(long long n, int vec, int most, int threads_most)
     return {nch, 0, (int)(ceil_div(ceil_div(chunks, nch), 32) * 32)};
 }
 
-// How columns are dealt to clusters: strips of lpr x vec columns, `ranks` blocks a strip, nch rows a thread.  ranks 0: too long.
+// How columns are dealt to clusters: strips of lpr x vec columns, `ranks` blocks a strip.  ranks 0: too long.
 struct StripPlan {
-    int nch, ranks;
+    int ranks;
     Strip q;
     long long strips;
+    int shared;
 };
 
-StripPlan plan_strips(long long n, long long vecs, int vec, int most, int sms)
+// Strips `bytes` wide (of the widest of the arrays, `size` bytes an element; `row` bytes an element over all arrays), narrower for
+// fewer columns, and for columns that 8 blocks cannot hold in MOST bytes each.
+StripPlan plan_strips(long long n, long long vecs, int vec, int size, int row, int bytes, int sms)
 {
-    // The widest strip of up to 64 columns (32 without vectors) whose rows fit in 8 blocks, narrower for fewer columns.
-    int lpr = vec == 1 ? 32 : STRIP_MAX / vec;
+    constexpr long long GOOD = 66 * 1024, MOST = 199 * 1024;  // three blocks an SM, one
+    int lpr = bytes / size / vec;
     while (lpr > 1 && (lpr / 2) * vec >= vecs) lpr /= 2;
-    while (lpr > 1 && n > 8ll * most * (STRIP_THREADS / lpr)) lpr /= 2;
-    const int rows = STRIP_THREADS / lpr;
-    if (n > 8ll * most * rows) return {};
+    const auto per_row = [&] { return (long long)lpr * vec * row; };
+    while (lpr > 1 && n * per_row() > 8 * MOST) lpr /= 2;
+    if (n * per_row() > 8 * MOST) return {};
     const long long strips = ceil_div(vecs, (long long)lpr * vec);
     int ranks = 1;
-    while (n > (long long)ranks * most * rows) ranks *= 2;
-    while (ranks < 8 && strips * ranks < sms && n > (long long)ranks * rows) ranks *= 2;  // idle SMs take a share
+    while (ranks < 8 && ceil_div(n, ranks) * per_row() > GOOD) ranks *= 2;
+    while (ranks < 8 && strips * ranks < sms && n > (long long)ranks * (STRIP_THREADS / lpr)) ranks *= 2;  // idle SMs take a share
     const long long per = ceil_div(n, ranks);
-    int nch = 1;
-    while ((long long)nch * rows < per) nch *= 2;
+    if (per * per_row() > MOST) return {};
     int shift = 0;
     while ((1 << shift) < lpr) ++shift;
-    return {nch, ranks, {lpr, shift, per}, strips};
+    return {ranks, {lpr, shift, (int)per}, strips, (int)(per * per_row()) + 16};  // the second array begins at 16 bytes
 }
 
 template <typename... Args>
-tcaspmm_status launch_cluster(void (*kernel)(Args...), long long blocks, int ranks, cudaStream_t st, Args... args)
+tcaspmm_status launch_cluster(void (*kernel)(Args...), const StripPlan &s, std::atomic<unsigned long long> &done, cudaStream_t st, Args... args)
 {
+    int dev = 0;
+    // More than the usual shared memory, allowed once a device.
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !(done.load() >> dev & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e != cudaSuccess) return cuda_fail(e, "layer_norm launch");
+        if (dev < 64) done.fetch_or(1ull << dev);
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = dim3((unsigned)(s.strips * s.ranks));
     cfg.blockDim = dim3(STRIP_THREADS);
+    cfg.dynamicSmemBytes = (size_t)s.shared;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ranks;
+    at[0].val.clusterDim.x = (unsigned)s.ranks;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
@@ -310,8 +379,6 @@ tcaspmm_status with_chunks(int nch, F &&f)
 
 constexpr int FWD_MOST = 16;       // elements of a row a thread holds, forward
 constexpr int BWD_MOST = 16;       // backward, where the sums of both gradients sit beside them
-constexpr int STRIP_ROWS_VEC = 8;  // vectors of a column strip a thread holds
-constexpr int STRIP_ROWS_ONE = 32; // elements, where rows do not allow vectors
 
 // Parts the weight gradient's sums come in: blocks of the backward kernel over rows, strips over columns.
 constexpr int ROW_PARTS = 4;

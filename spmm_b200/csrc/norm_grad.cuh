@@ -18,14 +18,15 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
     const int per = BLOCK ? 1 : (int)blockDim.x / lanes;
     const long long first = (long long)blockIdx.x * per + (BLOCK ? 0 : (int)threadIdx.x / lanes);
     const long long step = (long long)gridDim.x * per;
-    const float inv = 1.0f / (float)p.n;
+    const int n = (int)p.n;
+    const float inv = 1.0f / (float)n;
     float w[KEEP ? VEC * NCH : 1], dw[VEC * NCH], db[VEC * NCH];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const long long i = ((long long)c * tpr + t) * VEC;
+        const int i = (c * tpr + t) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dw[c * VEC + e] = db[c * VEC + e] = 0.0f;
-        if (KEEP && i < p.n) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, w + c * VEC);
+        if (KEEP && i < n) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, w + c * VEC);
     }
     Pack<T, VEC> x[NCH], nx[NCH];
     Pack<G, VEC> g[NCH], ng[NCH];
@@ -36,8 +37,8 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
         r = in ? __ldg(p.rstd + row) : 0.0f;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const long long i = ((long long)c * tpr + t) * VEC;
-            if (in && i < p.n) {
+            const int i = (c * tpr + t) * VEC;
+            if (in && i < n) {
                 tx[c].load((const T *)p.X + row * p.ldx + i);
                 tg[c].load((const G *)p.dY + row * p.lddy + i);
             } else {
@@ -55,8 +56,8 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
         const bool in = row < p.vecs;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const long long i = ((long long)c * tpr + t) * VEC;
-            if (in && i < p.n) {
+            const int i = (c * tpr + t) * VEC;
+            if (in && i < n) {
                 float ww[VEC];
                 if (!KEEP) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
 #pragma unroll
@@ -76,8 +77,8 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
             if (in) {
 #pragma unroll
                 for (int c = 0; c < NCH; ++c) {
-                    const long long i = ((long long)c * tpr + t) * VEC;
-                    if (i < p.n) {
+                    const int i = (c * tpr + t) * VEC;
+                    if (i < n) {
                         float d[VEC], ww[VEC];
                         if (!KEEP) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
 #pragma unroll
@@ -105,8 +106,8 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const long long i = ((long long)c * tpr + t) * VEC + e;
-                if (i < p.n) {
+                const int i = (c * tpr + t) * VEC + e;
+                if (i < n) {
                     pw[i] = dw[c * VEC + e];
                     pb[i] = db[c * VEC + e];
                 }
@@ -136,61 +137,62 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
             }
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < p.n; i += blockDim.x) {
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
             pw[i] = sum[i];
             pb[i] = sum[width + i];
         }
     }
 }
 
-template <typename T, typename G, int VEC, int NCH>
-__global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradParams p, const Strip q)
+template <typename T, typename G>
+__global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradParams p, const Strip q, int vec)
 {
+    constexpr int VEC = 16 / (int)(sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G));
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float s[2][STRIP_WARPS][STRIP_MAX];
     __shared__ float sums[2][STRIP_MAX];
     __shared__ float fin[2][STRIP_MAX];
+    __shared__ float stat[2][STRIP_MAX];  // the columns' mean and rstd
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int width = q.lpr * VEC, at = (threadIdx.x & (q.lpr - 1)) * VEC;
-    const long long strip = blockIdx.x / ranks, strips = gridDim.x / ranks;
-    const long long col = strip * width + at;
-    const bool in = col < p.vecs;
-    const long long r0 = min(p.n, rank * q.per_block), r1 = min(p.n, r0 + q.per_block);
-    const int lane_row = threadIdx.x >> q.shift, rows = STRIP_THREADS >> q.shift;
-    Pack<T, VEC> x[NCH];
-    Pack<G, VEC> g[NCH];
-    float w[NCH];
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const long long r = r0 + lane_row + c * rows;
-        w[c] = 1.0f;
-        if (r < r1 && in) {
-            x[c].load((const T *)p.X + r * p.ldx + col);
-            g[c].load((const G *)p.dY + r * p.lddy + col);
-            if (p.w) w[c] = load_as(p.w, p.pt, r);
-        } else {
-            x[c].zero();
-            g[c].zero();
-        }
+    const long long strip = blockIdx.x / ranks, strips = gridDim.x / ranks, c0 = strip * width;
+    const long long r0 = min(p.n, (long long)rank * q.per_block);
+    const int rows = (int)(min(p.n, r0 + q.per_block) - r0);
+    const int row = threadIdx.x >> q.shift, step = STRIP_THREADS >> q.shift;
+    T *const xs = (T *)smem;
+    G *const gs = (G *)(smem + ((size_t)q.per_block * width * sizeof(T) + 15) / 16 * 16);  // its vectors' alignment
+    load_strip<T, VEC>(xs, (const T *)p.X, p.ldx, r0, rows, c0, p.vecs, width, q, vec);
+    load_strip<G, VEC>(gs, (const G *)p.dY, p.lddy, r0, rows, c0, p.vecs, width, q, vec);
+    if ((int)threadIdx.x < width) {
+        const bool in = c0 + threadIdx.x < p.vecs;
+        stat[0][threadIdx.x] = in ? __ldg(p.mean + c0 + threadIdx.x) : 0.0f;
+        stat[1][threadIdx.x] = in ? __ldg(p.rstd + c0 + threadIdx.x) : 0.0f;
     }
+    copy_async_wait();
+    __syncthreads();
     float mean[VEC], rstd[VEC], v[2][VEC] = {};
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        mean[e] = in ? __ldg(p.mean + col + e) : 0.0f;
-        rstd[e] = in ? __ldg(p.rstd + col + e) : 0.0f;
+        mean[e] = stat[0][at + e];
+        rstd[e] = stat[1][at + e];
     }
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const long long r = r0 + lane_row + c * rows;
+    // Columns past the end hold zeros in both arrays and in mean and rstd: they add nothing.
+    for (int first = 0; first < rows; first += step) {  // the same number of turns for all threads of a warp
+        const int r = first + row;
         float a = 0.0f, d = 0.0f;
-        if (r < r1 && in) {
+        if (r < rows) {
+            const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
+            float x[VEC], g[VEC];
+            load_shared<T, VEC>(xs + r * width + at, x);
+            load_shared<G, VEC>(gs + r * width + at, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float dy = g[c].get(e), xh = (x[c].get(e) - mean[e]) * rstd[e];
-                v[0][e] += dy * w[c];
-                v[1][e] += dy * w[c] * xh;
-                a += dy * xh;
-                d += dy;
+                const float xh = (x[e] - mean[e]) * rstd[e];
+                v[0][e] += g[e] * w;
+                v[1][e] += g[e] * w * xh;
+                a += g[e] * xh;
+                d += g[e];
             }
         }
         if (p.part) {
@@ -198,38 +200,58 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradPar
                 a += __shfl_xor_sync(~0u, a, o);
                 d += __shfl_xor_sync(~0u, d, o);
             }
-            if (at == 0 && r < r1) {
-                p.part[strip * p.n + r] = a;
-                p.part[(strips + strip) * p.n + r] = d;
+            if (at == 0 && r < rows) {
+                p.part[strip * p.n + r0 + r] = a;
+                p.part[(strips + strip) * p.n + r0 + r] = d;
             }
         }
     }
     if (!p.dX) return;
     strip_sum(v, q.lpr, s, sums);
-    cluster.sync();
+    if (ranks > 1) cluster.sync();
     for (int j = threadIdx.x; j < 2 * width; j += STRIP_THREADS) {
         const int k = j / width, c = j - k * width;
-        float t = 0.0f;
-        for (int i = 0; i < ranks; ++i) t += cluster.map_shared_rank(&sums[0][0], i)[k * STRIP_MAX + c];
+        float part[8], t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[i] = i < ranks ? cluster.map_shared_rank(&sums[0][0], i)[k * STRIP_MAX + c] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += part[i];
         fin[k][c] = t / (float)p.n;
     }
     __syncthreads();
-    if (in) {
+    if (ranks > 1) cluster.barrier_arrive();  // this block has read the others' sums
+    if (vec) {
+        if (c0 + at < p.vecs) {
+            float c1[VEC], c2[VEC];
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const long long r = r0 + lane_row + c * rows;
-            if (r < r1) {
-                float d[VEC];
+            for (int e = 0; e < VEC; ++e) {
+                c1[e] = fin[0][at + e];
+                c2[e] = fin[1][at + e];
+            }
+#pragma unroll 2
+            for (int r = row; r < rows; r += step) {
+                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
+                float x[VEC], g[VEC];
+                load_shared<T, VEC>(xs + r * width + at, x);
+                load_shared<G, VEC>(gs + r * width + at, g);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float xh = (x[c].get(e) - mean[e]) * rstd[e];
-                    d[e] = rstd[e] * (g[c].get(e) * w[c] - fin[0][at + e] - xh * fin[1][at + e]);
-                }
-                store_pack<VEC>((T *)p.dX + r * p.lddx + col, d);
+                for (int e = 0; e < VEC; ++e) x[e] = rstd[e] * (g[e] * w - c1[e] - (x[e] - mean[e]) * rstd[e] * c2[e]);
+                store_pack<VEC>((T *)p.dX + (r0 + r) * p.lddx + c0 + at, x);
+            }
+        }
+    } else {
+        const int c = threadIdx.x & (width - 1);
+        if (c0 + c < p.vecs) {
+            const float m = stat[0][c], rs = stat[1][c], c1 = fin[0][c], c2 = fin[1][c];
+#pragma unroll 4
+            for (int r = threadIdx.x / width; r < rows; r += STRIP_THREADS / width) {
+                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
+                ((T *)p.dX)[(r0 + r) * p.lddx + c0 + c] =
+                    from_float<T>(rs * (to_float(gs[r * width + c]) * w - c1 - (to_float(xs[r * width + c]) - m) * rs * c2));
             }
         }
     }
-    cluster.sync();
+    if (ranks > 1) cluster.barrier_wait();
 }
 
 template <typename T>
@@ -317,13 +339,12 @@ tcaspmm_status backward(const NormGradParams &p, int dim, long long *parts, cuda
             });
         }
     } else {
-        constexpr int MOST = VEC == 1 ? STRIP_ROWS_ONE : STRIP_ROWS_VEC;
-        const StripPlan s = plan_strips(p.n, p.vecs, VEC, MOST, sms);
-        if (s.ranks && s.strips * s.ranks <= INT_MAX) {
-            *parts = s.strips;
-            return with_chunks<MOST>(s.nch, [&](auto nch) {
-                return launch_cluster(norm_cols_bwd<T, G, VEC, nch.value>, s.strips * s.ranks, s.ranks, st, p, s.q);
-            });
+        constexpr int WIDE = sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G);
+        const StripPlan q = plan_strips(p.n, p.vecs, 16 / WIDE, WIDE, sizeof(T) + sizeof(G), 64, sms);
+        static std::atomic<unsigned long long> done{0};
+        if (q.ranks && q.strips * q.ranks <= INT_MAX) {
+            *parts = q.strips;
+            return launch_cluster(norm_cols_bwd<T, G>, q, done, st, p, q.q, (int)(VEC > 1));
         }
     }
     if (p.dX)
