@@ -93,31 +93,35 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_rows_fwd(const NormPa
                 }
         }
         row_sum<BLOCK>(sq, lanes, s[1]);
+        by_type(p.yt, [&](auto type) {
+            using TO = decltype(type);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            const long long at = row + r * per;
-            if (at >= p.vecs) continue;
-            const float rstd = 1.0f / sqrtf(sq[r] * inv + p.eps);
+            for (int r = 0; r < ROWS; ++r) {
+                const long long at = row + r * per;
+                if (at >= p.vecs) continue;
+                const float rstd = 1.0f / sqrtf(sq[r] * inv + p.eps);
+                TO *const out = (TO *)p.Y + at * p.ldy + t * VEC;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                const int i = (c * tpr + t) * VEC;
-                if (i < n) {
-                    float y[VEC], ww[VEC], bb[VEC];
-                    if (!KEEP) {
-                        load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
-                        load_params<VEC>(p.b, p.pt, p.pvec, i, 0.0f, bb);
+                for (int c = 0; c < NCH; ++c) {
+                    const int i = (c * tpr + t) * VEC;
+                    if (i < n) {
+                        float y[VEC], ww[VEC], bb[VEC];
+                        if (!KEEP) {
+                            load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
+                            load_params<VEC>(p.b, p.pt, p.pvec, i, 0.0f, bb);
+                        }
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            y[e] = fmaf((x[r][c].get(e) - mean[r]) * rstd, KEEP ? w[c * VEC + e] : ww[e], KEEP ? b[c * VEC + e] : bb[e]);
+                        store_pack<VEC>(out + c * tpr * VEC, y);
                     }
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        y[e] = (x[r][c].get(e) - mean[r]) * rstd * (KEEP ? w[c * VEC + e] : ww[e]) + (KEEP ? b[c * VEC + e] : bb[e]);
-                    store_vec<VEC>(p.Y, p.yt, at * p.ldy + i, y);
+                }
+                if (t == 0 && p.mean) {
+                    p.mean[at] = mean[r];
+                    p.rstd[at] = rstd;
                 }
             }
-            if (t == 0 && p.mean) {
-                p.mean[at] = mean[r];
-                p.rstd[at] = rstd;
-            }
-        }
+        });
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
 #pragma unroll
@@ -134,6 +138,7 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_fwd(const NormParams 
     __shared__ float sums[2][STRIP_MAX];  // this block's sum of x, then of squared differences from its own mean
     __shared__ __align__(16) float fin[2][STRIP_MAX];  // the strip's mean and rstd
     T *const tile = (T *)smem;
+    float2 *const wb = (float2 *)(smem + ((size_t)q.per_block * (q.lpr * VEC) * sizeof(T) + 15) / 16 * 16);  // the rows' weight and bias
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int width = q.lpr * VEC, at = (threadIdx.x & (q.lpr - 1)) * VEC;
@@ -142,6 +147,8 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_fwd(const NormParams 
     const int rows = (int)(min(p.n, r0 + q.per_block) - r0);
     const int row = threadIdx.x >> q.shift, step = STRIP_THREADS >> q.shift;
     load_strip<T, VEC>(tile, (const T *)p.X, p.ldx, r0, rows, c0, p.vecs, width, q, vec);
+    for (int r = threadIdx.x; r < rows; r += STRIP_THREADS)
+        wb[r] = make_float2(p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f, p.b ? load_as(p.b, p.pt, r0 + r) : 0.0f);
     copy_async_wait();
     __syncthreads();
     float v[1][VEC] = {};
@@ -202,35 +209,40 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_fwd(const NormParams 
     }
     __syncthreads();
     if (ranks > 1) cluster.barrier_arrive();  // this block has read the others' sums
-    if (vec) {
-        float mean[VEC], rstd[VEC];
+    by_type(p.yt, [&](auto type) {
+        using TO = decltype(type);
+        if (vec) {
+            float mean[VEC], rstd[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            mean[e] = fin[0][at + e];
-            rstd[e] = fin[1][at + e];
-        }
-        if (c0 + at < p.vecs) {
+            for (int e = 0; e < VEC; ++e) {
+                mean[e] = fin[0][at + e];
+                rstd[e] = fin[1][at + e];
+            }
+            if (c0 + at >= p.vecs) return;
+            TO *out = (TO *)p.Y + (r0 + row) * p.ldy + c0 + at;
+            const long long down = step * p.ldy;
 #pragma unroll 4
-            for (int r = row; r < rows; r += step) {
-                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f, b = p.b ? load_as(p.b, p.pt, r0 + r) : 0.0f;
+            for (int r = row; r < rows; r += step, out += down) {
+                const float2 k = wb[r];
                 float x[VEC];
                 load_shared<T, VEC>(tile + r * width + at, x);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) x[e] = (x[e] - mean[e]) * rstd[e] * w + b;
-                store_vec<VEC>(p.Y, p.yt, (r0 + r) * p.ldy + c0 + at, x);
+                for (int e = 0; e < VEC; ++e) x[e] = fmaf((x[e] - mean[e]) * rstd[e], k.x, k.y);
+                store_pack<VEC>(out, x);
             }
-        }
-    } else {
-        const int c = threadIdx.x & (width - 1);
-        const float mean = fin[0][c], rstd = fin[1][c];
-        if (c0 + c < p.vecs) {
+        } else {
+            const int c = threadIdx.x & (width - 1), per = STRIP_THREADS / width;
+            const float mean = fin[0][c], rstd = fin[1][c];
+            if (c0 + c >= p.vecs) return;
+            TO *out = (TO *)p.Y + (r0 + threadIdx.x / width) * p.ldy + c0 + c;
+            const long long down = per * p.ldy;
 #pragma unroll 4
-            for (int r = threadIdx.x / width; r < rows; r += STRIP_THREADS / width) {
-                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f, b = p.b ? load_as(p.b, p.pt, r0 + r) : 0.0f;
-                store_as(p.Y, p.yt, (r0 + r) * p.ldy + c0 + c, (to_float(tile[r * width + c]) - mean) * rstd * w + b);
+            for (int r = threadIdx.x / width; r < rows; r += per, out += down) {
+                const float2 k = wb[r];
+                *out = from_float<TO>(fmaf((to_float(tile[r * width + c]) - mean) * rstd, k.x, k.y));
             }
         }
-    }
+    });
     if (ranks > 1) cluster.barrier_wait();
 }
 
@@ -289,21 +301,26 @@ tcaspmm_status forward(const NormParams &p, int dim, cudaStream_t st)
     if (dim == 1) {
         const RowPlan r = plan_rows(p.n, VEC, FWD_MOST, 1024);
         if (r.nch) {
-            // Blocks an SM holds: at most 64 registers a thread up to 8 elements, 128 above.
-            const long long fit = !r.lanes ? std::max(1, 1024 / r.threads) : r.nch * VEC > 8 ? 2 : 4;
             return with_chunks<FWD_MOST / VEC>(r.nch, [&](auto nch) {
                 constexpr int N = nch.value, ROWS = N * VEC * (int)sizeof(T) <= 16 ? 4 : N * VEC * (int)sizeof(T) <= 32 ? 2 : 1;
-                const long long per = r.lanes ? 256 / r.lanes * ROWS : 1;
-                const unsigned grid = blocks_of(std::min(ceil_div(p.vecs, per), fit * sm_count()));
-                if (r.lanes)
-                    norm_rows_fwd<T, VEC, N, ROWS, false><<<grid, 256, 0, st>>>(p, r.lanes);
-                else
-                    norm_rows_fwd<T, VEC, N, 1, true><<<grid, r.threads, 0, st>>>(p, 32);
+                // One wave of blocks, each with its share of the rows; of the shortest rows, whose weights are few, blocks of
+                // four turns (2^20 x 128 fp32: 162 us, in one wave 203 us; 2^19 x 256 fp16 the other way, 105 and 125 us).
+                if (r.lanes) {
+                    static std::atomic<int> known{0};
+                    const auto kernel = norm_rows_fwd<T, VEC, N, ROWS, false>;
+                    const long long wave = (long long)resident((const void *)kernel, 256, 0, known) * sm_count();
+                    const long long turns = ceil_div(p.vecs, 256 / r.lanes * ROWS);
+                    const long long blocks = std::min(turns, N * VEC <= 4 ? std::max(wave, ceil_div(turns, 4)) : wave);
+                    kernel<<<blocks_of(blocks), 256, 0, st>>>(p, r.lanes);
+                } else {
+                    const long long fit = (long long)std::max(1, 1024 / r.threads) * sm_count();
+                    norm_rows_fwd<T, VEC, N, 1, true><<<blocks_of(std::min(p.vecs, fit)), r.threads, 0, st>>>(p, 32);
+                }
                 return launched("layer_norm launch");
             });
         }
     } else {
-        const StripPlan q = plan_strips(p.n, p.vecs, 16 / (int)sizeof(T), sizeof(T), sizeof(T), 128, sm_count());
+        const StripPlan q = plan_strips(p.n, p.vecs, 16 / (int)sizeof(T), sizeof(T), sizeof(T), 8, 128, sm_count());
         static std::atomic<unsigned long long> done{0};
         if (q.ranks && q.strips * q.ranks <= INT_MAX) return launch_cluster(norm_cols_fwd<T>, q, done, st, p, q.q, (int)(VEC > 1));
     }
@@ -352,7 +369,7 @@ extern "C" size_t tcaspmm_layer_norm_backward_workspace(int64_t rows, int64_t co
     // Rows: ROW_PARTS blocks an SM, or LONG_PARTS.  Columns: a strip for every 16 columns; of columns that 8 blocks' shared
     // memory holds only in narrower strips (199 KB each, at most 8 bytes an element), for every 8, 4, ...
     long long width = 16;
-    while (width > 4 && width * n * 8 > 8 * 199 * 1024) width /= 2;
+    while (width > 4 && (width * 8 + 4) * n > 8 * 199 * 1024) width /= 2;
     const long long parts = dim == 1 ? std::max<long long>((long long)ROW_PARTS * sm_count(), LONG_PARTS) : ceil_div(vecs, width);
     return (size_t)(2 * std::min(parts, std::max<long long>(vecs, 1)) * n) * sizeof(float);
 }

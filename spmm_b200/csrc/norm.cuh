@@ -70,8 +70,21 @@ __device__ __forceinline__ void store_pack(T *p, const float (&v)[VEC])
 #pragma unroll
     for (int k = 0; k < VEC; k += PER) {
         T t[PER];
+        if constexpr (sizeof(T) == 2 && PER % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) t[i] = from_float<T>(v[k + i]);
+            for (int i = 0; i < PER; i += 2) {  // two at a time: one conversion instruction
+                if constexpr (std::is_same<T, __half>::value) {
+                    const __half2 two = __floats2half2_rn(v[k + i], v[k + i + 1]);
+                    memcpy(t + i, &two, 4);
+                } else {
+                    const __nv_bfloat162 two = __floats2bfloat162_rn(v[k + i], v[k + i + 1]);
+                    memcpy(t + i, &two, 4);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) t[i] = from_float<T>(v[k + i]);
+        }
         typename Bits<sizeof(T) * PER>::type bits;
         memcpy(&bits, t, sizeof bits);
         *reinterpret_cast<decltype(bits) *>(p + k) = bits;
@@ -89,15 +102,16 @@ __device__ __forceinline__ void load_shared(const T *p, float *v)
     for (int e = 0; e < VEC; ++e) v[e] = to_float(t[e]);
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_vec(void *p, int type, long long i, const float (&v)[VEC])
+// Calls f with a value of the type of code `type`: the same branch for every thread.
+template <typename F>
+__device__ __forceinline__ void by_type(int type, F &&f)
 {
     if (type == 0)
-        store_pack<VEC>((float *)p + i, v);
+        f(float{});
     else if (type == 1)
-        store_pack<VEC>((__half *)p + i, v);
+        f(__half{});
     else
-        store_pack<VEC>((__nv_bfloat16 *)p + i, v);
+        f(__nv_bfloat16{});
 }
 
 template <typename T, int VEC>
@@ -313,14 +327,14 @@ struct StripPlan {
     int shared;
 };
 
-// Strips `bytes` wide (of the widest of the arrays, `size` bytes an element; `row` bytes an element over all arrays), narrower for
-// fewer columns, and for columns that 8 blocks cannot hold in MOST bytes each.
-StripPlan plan_strips(long long n, long long vecs, int vec, int size, int row, int bytes, int sms)
+// Strips `bytes` wide (of the widest of the arrays, `size` bytes an element; `row` bytes an element over all arrays and `more`
+// a row), narrower for fewer columns, and for columns that 8 blocks cannot hold in MOST bytes each.
+StripPlan plan_strips(long long n, long long vecs, int vec, int size, int row, int more, int bytes, int sms)
 {
     constexpr long long GOOD = 66 * 1024, MOST = 199 * 1024;  // three blocks an SM, one
     int lpr = bytes / size / vec;
     while (lpr > 1 && (lpr / 2) * vec >= vecs) lpr /= 2;
-    const auto per_row = [&] { return (long long)lpr * vec * row; };
+    const auto per_row = [&] { return (long long)lpr * vec * row + more; };
     while (lpr > 1 && n * per_row() > 8 * MOST) lpr /= 2;
     if (n * per_row() > 8 * MOST) return {};
     const long long strips = ceil_div(vecs, (long long)lpr * vec);
@@ -331,7 +345,7 @@ StripPlan plan_strips(long long n, long long vecs, int vec, int size, int row, i
     if (per * per_row() > MOST) return {};
     int shift = 0;
     while ((1 << shift) < lpr) ++shift;
-    return {ranks, {lpr, shift, (int)per}, strips, (int)(per * per_row()) + 16};  // the second array begins at 16 bytes
+    return {ranks, {lpr, shift, (int)per}, strips, (int)(per * per_row()) + 32};  // the second array begins at 16 bytes
 }
 
 template <typename... Args>
@@ -357,6 +371,17 @@ tcaspmm_status launch_cluster(void (*kernel)(Args...), const StripPlan &s, std::
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, "layer_norm launch");
+}
+
+// Blocks of `threads` threads an SM holds of a kernel (asked once: `known` is the kernel's).
+inline int resident(const void *kernel, int threads, int shared, std::atomic<int> &known)
+{
+    int n = known.load();
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, shared) != cudaSuccess || n < 1) n = 1;
+        known.store(n);
+    }
+    return n;
 }
 
 // Calls f with the compile-time chunk count.

@@ -62,18 +62,17 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
                 if (!KEEP) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float dy = g[c].get(e), xh = (x[c].get(e) - mean) * rstd;
-                    const float v = dy * (KEEP ? w[c * VEC + e] : ww[e]);
-                    a[0] += v;
-                    a[1] += v * xh;
-                    dw[c * VEC + e] += dy * xh;
+                    const float dy = g[c].get(e), gx = dy * ((x[c].get(e) - mean) * rstd), we = KEEP ? w[c * VEC + e] : ww[e];
+                    a[0] = fmaf(dy, we, a[0]);
+                    a[1] = fmaf(gx, we, a[1]);
+                    dw[c * VEC + e] += gx;
                     db[c * VEC + e] += dy;
                 }
             }
         }
         if (p.dX) {
             row_sum<BLOCK>(a, lanes, s[k & 1]);
-            const float c1 = a[0] * inv, c2 = a[1] * inv;
+            const float c1 = a[0] * inv, k2 = rstd * (a[1] * inv);  // dx = rstd (g w - c1 - (x - mean) k2)
             if (in) {
 #pragma unroll
                 for (int c = 0; c < NCH; ++c) {
@@ -82,10 +81,8 @@ __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p,
                         float d[VEC], ww[VEC];
                         if (!KEEP) load_params<VEC>(p.w, p.pt, p.pvec, i, 1.0f, ww);
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) {
-                            const float xh = (x[c].get(e) - mean) * rstd;
-                            d[e] = rstd * (g[c].get(e) * (KEEP ? w[c * VEC + e] : ww[e]) - c1 - xh * c2);
-                        }
+                        for (int e = 0; e < VEC; ++e)
+                            d[e] = rstd * fmaf(g[c].get(e), KEEP ? w[c * VEC + e] : ww[e], -fmaf(x[c].get(e) - mean, k2, c1));
                         store_pack<VEC>((T *)p.dX + row * p.lddx + i, d);
                     }
                 }
@@ -162,8 +159,10 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradPar
     const int row = threadIdx.x >> q.shift, step = STRIP_THREADS >> q.shift;
     T *const xs = (T *)smem;
     G *const gs = (G *)(smem + ((size_t)q.per_block * width * sizeof(T) + 15) / 16 * 16);  // its vectors' alignment
+    float *const ws = (float *)((unsigned char *)gs + ((size_t)q.per_block * width * sizeof(G) + 15) / 16 * 16);  // the rows' weight
     load_strip<T, VEC>(xs, (const T *)p.X, p.ldx, r0, rows, c0, p.vecs, width, q, vec);
     load_strip<G, VEC>(gs, (const G *)p.dY, p.lddy, r0, rows, c0, p.vecs, width, q, vec);
+    for (int r = threadIdx.x; r < rows; r += STRIP_THREADS) ws[r] = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
     if ((int)threadIdx.x < width) {
         const bool in = c0 + threadIdx.x < p.vecs;
         stat[0][threadIdx.x] = in ? __ldg(p.mean + c0 + threadIdx.x) : 0.0f;
@@ -178,20 +177,21 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradPar
         rstd[e] = stat[1][at + e];
     }
     // Columns past the end hold zeros in both arrays and in mean and rstd: they add nothing.
+#pragma unroll 2
     for (int first = 0; first < rows; first += step) {  // the same number of turns for all threads of a warp
         const int r = first + row;
         float a = 0.0f, d = 0.0f;
         if (r < rows) {
-            const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
+            const float w = ws[r];
             float x[VEC], g[VEC];
             load_shared<T, VEC>(xs + r * width + at, x);
             load_shared<G, VEC>(gs + r * width + at, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float xh = (x[e] - mean[e]) * rstd[e];
-                v[0][e] += g[e] * w;
-                v[1][e] += g[e] * w * xh;
-                a += g[e] * xh;
+                const float gx = g[e] * ((x[e] - mean[e]) * rstd[e]);
+                v[0][e] = fmaf(g[e], w, v[0][e]);
+                v[1][e] = fmaf(gx, w, v[1][e]);
+                a += gx;
                 d += g[e];
             }
         }
@@ -222,33 +222,35 @@ __global__ void __launch_bounds__(STRIP_THREADS) norm_cols_bwd(const NormGradPar
     if (ranks > 1) cluster.barrier_arrive();  // this block has read the others' sums
     if (vec) {
         if (c0 + at < p.vecs) {
-            float c1[VEC], c2[VEC];
+            // dx = rstd (g w - c1 - xh c2),  xh c2 = (x - mean) k2,  k2 = rstd c2
+            float k1[VEC], k2[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                c1[e] = fin[0][at + e];
-                c2[e] = fin[1][at + e];
+                k1[e] = fin[0][at + e];
+                k2[e] = rstd[e] * fin[1][at + e];
             }
+            T *out = (T *)p.dX + (r0 + row) * p.lddx + c0 + at;
+            const long long down = step * p.lddx;
 #pragma unroll 2
-            for (int r = row; r < rows; r += step) {
-                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
+            for (int r = row; r < rows; r += step, out += down) {
+                const float w = ws[r];
                 float x[VEC], g[VEC];
                 load_shared<T, VEC>(xs + r * width + at, x);
                 load_shared<G, VEC>(gs + r * width + at, g);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) x[e] = rstd[e] * (g[e] * w - c1[e] - (x[e] - mean[e]) * rstd[e] * c2[e]);
-                store_pack<VEC>((T *)p.dX + (r0 + r) * p.lddx + c0 + at, x);
+                for (int e = 0; e < VEC; ++e) x[e] = rstd[e] * fmaf(g[e], w, -fmaf(x[e] - mean[e], k2[e], k1[e]));
+                store_pack<VEC>(out, x);
             }
         }
     } else {
-        const int c = threadIdx.x & (width - 1);
+        const int c = threadIdx.x & (width - 1), per = STRIP_THREADS / width;
         if (c0 + c < p.vecs) {
-            const float m = stat[0][c], rs = stat[1][c], c1 = fin[0][c], c2 = fin[1][c];
+            const float m = stat[0][c], rs = stat[1][c], k1 = fin[0][c], k2 = rs * fin[1][c];
+            T *out = (T *)p.dX + (r0 + threadIdx.x / width) * p.lddx + c0 + c;
+            const long long down = per * p.lddx;
 #pragma unroll 4
-            for (int r = threadIdx.x / width; r < rows; r += STRIP_THREADS / width) {
-                const float w = p.w ? load_as(p.w, p.pt, r0 + r) : 1.0f;
-                ((T *)p.dX)[(r0 + r) * p.lddx + c0 + c] =
-                    from_float<T>(rs * (to_float(gs[r * width + c]) * w - c1 - (to_float(xs[r * width + c]) - m) * rs * c2));
-            }
+            for (int r = threadIdx.x / width; r < rows; r += per, out += down)
+                *out = from_float<T>(rs * fmaf(to_float(gs[r * width + c]), ws[r], -fmaf(to_float(xs[r * width + c]) - m, k2, k1)));
         }
     }
     if (ranks > 1) cluster.barrier_wait();
@@ -340,7 +342,7 @@ tcaspmm_status backward(const NormGradParams &p, int dim, long long *parts, cuda
         }
     } else {
         constexpr int WIDE = sizeof(T) > sizeof(G) ? sizeof(T) : sizeof(G);
-        const StripPlan q = plan_strips(p.n, p.vecs, 16 / WIDE, WIDE, sizeof(T) + sizeof(G), 64, sms);
+        const StripPlan q = plan_strips(p.n, p.vecs, 16 / WIDE, WIDE, sizeof(T) + sizeof(G), 4, 64, sms);
         static std::atomic<unsigned long long> done{0};
         if (q.ranks && q.strips * q.ranks <= INT_MAX) {
             *parts = q.strips;
