@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cstring>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,11 +54,24 @@ struct Pack {
     typename Bits<sizeof(T) * VEC>::type bits;
     __device__ void load(const T *p) { bits = __ldg(reinterpret_cast<const decltype(bits) *>(p)); }
     __device__ void zero() { bits = {}; }
+    // Element i as fp32 (i a constant of an unrolled loop).
     __device__ float get(int i) const
     {
-        T v[VEC];
-        memcpy(v, &bits, sizeof bits);
-        return to_float(v[i]);
+        if constexpr (sizeof(T) == 4) {
+            float v[VEC];
+            memcpy(v, &bits, sizeof bits);
+            return v[i];
+        } else if constexpr (VEC == 1) {
+            T v;
+            memcpy(&v, &bits, sizeof v);
+            return to_float(v);
+        } else {
+            unsigned w[VEC / 2];
+            memcpy(w, &bits, sizeof bits);
+            const unsigned two = w[i >> 1];
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? two & 0xffff0000u : two << 16);
+            return __half2float(__ushort_as_half((unsigned short)(i & 1 ? two >> 16 : two)));
+        }
     }
 };
 

@@ -26,15 +26,17 @@ namespace {
 
 // A row's elements are dealt to its threads VEC at a time, NCH times; a thread's elements are the same in every row.  Short rows
 // go ROWS at a time, so that enough bytes are on their way; the next rows are fetched before the present ones are summed.
-template <typename T, int VEC, int NCH, int ROWS, bool BLOCK>
+// LANES: threads a row, where they are a whole warp; 0: `lanes` of one, or (BLOCK) the block.
+template <typename T, int VEC, int NCH, int ROWS, int LANES, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_rows_fwd(const NormParams p, int lanes)
 {
     constexpr bool KEEP = VEC * NCH <= 8;  // weights stay in registers
     __shared__ float s[2][ROWS][32];
     const int n = (int)p.n;
+    if (LANES) lanes = LANES;
     const int tpr = BLOCK ? (int)blockDim.x : lanes;
     const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
-    const int per = BLOCK ? 1 : (int)blockDim.x / lanes;  // rows side by side in a block
+    const int per = BLOCK ? 1 : 256 / lanes;  // rows side by side in a block
     const long long first = (long long)blockIdx.x * per * ROWS + (BLOCK ? 0 : (int)threadIdx.x / lanes);
     const long long step = (long long)gridDim.x * per * ROWS;
     const float inv = 1.0f / (float)n;
@@ -306,15 +308,16 @@ tcaspmm_status forward(const NormParams &p, int dim, cudaStream_t st)
                 // One wave of blocks, each with its share of the rows; of the shortest rows, whose weights are few, blocks of
                 // four turns (2^20 x 128 fp32: 162 us, in one wave 203 us; 2^19 x 256 fp16 the other way, 105 and 125 us).
                 if (r.lanes) {
-                    static std::atomic<int> known{0};
-                    const auto kernel = norm_rows_fwd<T, VEC, N, ROWS, false>;
-                    const long long wave = (long long)resident((const void *)kernel, 256, 0, known) * sm_count();
+                    static std::atomic<int> known[2];
+                    const bool whole = r.lanes == 32;
+                    const auto kernel = whole ? norm_rows_fwd<T, VEC, N, ROWS, 32, false> : norm_rows_fwd<T, VEC, N, ROWS, 0, false>;
+                    const long long wave = (long long)resident((const void *)kernel, 256, 0, known[whole]) * sm_count();
                     const long long turns = ceil_div(p.vecs, 256 / r.lanes * ROWS);
                     const long long blocks = std::min(turns, N * VEC <= 4 ? std::max(wave, ceil_div(turns, 4)) : wave);
                     kernel<<<blocks_of(blocks), 256, 0, st>>>(p, r.lanes);
                 } else {
                     const long long fit = (long long)std::max(1, 1024 / r.threads) * sm_count();
-                    norm_rows_fwd<T, VEC, N, 1, true><<<blocks_of(std::min(p.vecs, fit)), r.threads, 0, st>>>(p, 32);
+                    norm_rows_fwd<T, VEC, N, 1, 0, true><<<blocks_of(std::min(p.vecs, fit)), r.threads, 0, st>>>(p, 32);
                 }
                 return launched("layer_norm launch");
             });

@@ -95,11 +95,10 @@ __device__ __forceinline__ void store_pack(T *p, const float (&v)[VEC])
 template <typename T, int VEC>
 __device__ __forceinline__ void load_shared(const T *p, float *v)
 {
-    typename Bits<sizeof(T) * VEC>::type bits = *reinterpret_cast<const decltype(bits) *>(p);
-    T t[VEC];
-    memcpy(t, &bits, sizeof bits);
+    Pack<T, VEC> t;
+    t.bits = *reinterpret_cast<const decltype(t.bits) *>(p);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = to_float(t[e]);
+    for (int e = 0; e < VEC; ++e) v[e] = t.get(e);
 }
 
 // Calls f with a value of the type of code `type`: the same branch for every thread.

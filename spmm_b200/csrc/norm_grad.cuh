@@ -6,16 +6,17 @@
 namespace tca {
 namespace {
 
-template <typename T, typename G, int VEC, int NCH, int THREADS>
+template <typename T, typename G, int VEC, int NCH, int LANES, int THREADS>  // LANES as in norm_rows_fwd
 __global__ void __launch_bounds__(THREADS) norm_rows_bwd(const NormGradParams p, int lanes)
 {
     constexpr bool BLOCK = THREADS != 256;
     constexpr bool KEEP = VEC * NCH <= 8 || THREADS == 512;
     __shared__ float s[2][2][32];
     extern __shared__ float sum[];  // !BLOCK: a block's partial gradients, added warp by warp
+    if (LANES) lanes = LANES;
     const int tpr = BLOCK ? (int)blockDim.x : lanes;
     const int t = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1));
-    const int per = BLOCK ? 1 : (int)blockDim.x / lanes;
+    const int per = BLOCK ? 1 : 256 / lanes;
     const long long first = (long long)blockIdx.x * per + (BLOCK ? 0 : (int)threadIdx.x / lanes);
     const long long step = (long long)gridDim.x * per;
     const int n = (int)p.n;
@@ -331,12 +332,14 @@ tcaspmm_status backward(const NormGradParams &p, int dim, long long *parts, cuda
             return with_chunks<BWD_MOST / VEC>(r.nch, [&](auto nch) {
                 constexpr int N = nch.value;
                 const size_t shared = r.lanes ? sizeof(float) * 2 * r.lanes * VEC * N : 0;
-                if (r.lanes)
-                    norm_rows_bwd<T, G, VEC, N, 256><<<(unsigned)grid, 256, shared, st>>>(p, r.lanes);
+                if (r.lanes == 32)
+                    norm_rows_bwd<T, G, VEC, N, 32, 256><<<(unsigned)grid, 256, shared, st>>>(p, 32);
+                else if (r.lanes)
+                    norm_rows_bwd<T, G, VEC, N, 0, 256><<<(unsigned)grid, 256, shared, st>>>(p, r.lanes);
                 else if (r.threads <= 512)
-                    norm_rows_bwd<T, G, VEC, N, 512><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
+                    norm_rows_bwd<T, G, VEC, N, 0, 512><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
                 else
-                    norm_rows_bwd<T, G, VEC, N, 1024><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
+                    norm_rows_bwd<T, G, VEC, N, 0, 1024><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
                 return launched("layer_norm_backward launch");
             });
         }
