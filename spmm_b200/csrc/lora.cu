@@ -8,7 +8,7 @@ int sm_count();
 #define TCA_LORA(k)                                                                         \
     tcaspmm_status lora_forward_##k(const ApplyParams &p, bool tokens, int sms, cudaStream_t st); \
     tcaspmm_status lora_input_grad_##k(const ApplyParams &p, bool in32, int sms, cudaStream_t st); \
-    tcaspmm_status lora_factor_grads_##k(const GradParams &w, int sms, cudaStream_t st);
+    tcaspmm_status lora_factor_grads_##k(const GradParams &w, bool early, int sms, cudaStream_t st);
 TCA_LORA(f32)
 TCA_LORA(f16)
 TCA_LORA(bf16)
@@ -146,8 +146,9 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
     w.c = c;
     w.R = (int)ad->rank;
     w.N = N;
-    w.p[0] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), (const float *)scratch, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
-    w.p[1] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), (const float *)hidden, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
+    // The first needs nothing of this call; the second what dX's first kernel has made.
+    w.p[0] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), (const float *)hidden, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
+    w.p[1] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), (const float *)scratch, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
     const auto run = ft == 0 ? lora_factor_grads_f32 : ft == 1 ? lora_factor_grads_f16 : lora_factor_grads_bf16;
-    return run(w, sm_count(), st);
+    return run(w, (dDX || ddown) && N > 0, sm_count(), st);  // early only behind kernels of this call
 }

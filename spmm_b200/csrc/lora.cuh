@@ -81,8 +81,8 @@ struct ApplyParams {
 };
 
 // S in device memory between the kernels, rows of `pitch` columns (64 or a multiple, so that every row is aligned): fp32 for
-// the gradients and for fp32 factors, and for 16-bit factors two parts of their type whose sum it is (split16).  fp16 parts
-// are scaled: a column's, times its colscale, is S.  The parts' columns are dealt out within each 16 (place) so that the
+// the gradients and for fp32 factors, and for 16-bit factors parts of their type whose sum it is: two of fp16 (22 bits; they
+// are scaled: a column's, times its colscale, is S), three of bf16 (24 bits).  The parts' columns are dealt out within each 16 (place) so that the
 // second product's matrix instructions give a thread four neighbours.  Columns past N hold nothing that counts.
 struct Hidden {
     long long pitch, rows;
@@ -90,14 +90,13 @@ struct Hidden {
     __host__ __device__ static long long pitch_of(long long N) { return (N + 63) / 64 * 64; }
     __host__ static size_t bytes(long long R, long long N, int type)
     {
-        return (size_t)pitch_of(N) * (R * (type == 0 ? 4 : 8) + (type == 1 ? 4 : 0));
+        return (size_t)pitch_of(N) * (R * (type == 0 ? 4 : type == 1 ? 8 : 10) + (type == 1 ? 4 : 0));
     }
     __host__ __device__ Hidden(void *at, long long R, long long N) : pitch(pitch_of(N)), rows(R), p((unsigned char *)at) {}
     // Where column c of the parts lies: c = 4 i + 2 b + e of each 16 is column 2 i + e of block b of 8.
     __host__ __device__ static int place(int c) { return (c & ~15) + 8 * (c >> 1 & 1) + 2 * (c >> 2 & 3) + (c & 1); }
     __host__ __device__ float *s() const { return (float *)p; }
-    template <typename T> __device__ T *hi() const { return (T *)(p + pitch * rows * 4); }
-    template <typename T> __device__ T *lo() const { return (T *)(p + pitch * rows * 6); }
+    template <typename T> __device__ T *part(int i) const { return (T *)(p + pitch * rows * (4 + 2 * i)); }  // the largest first
     __device__ float *colscale() const { return (float *)(p + pitch * rows * 8); }
 };
 
@@ -185,46 +184,51 @@ __device__ __forceinline__ void split_tf32(float x, unsigned &hi, unsigned &lo)
     lo = special ? 0u : __float_as_uint(x - __uint_as_float(hi));
 }
 
-// x = hi + lo up to 2^-17 |x| (bf16) or 2^-22 (fp16, in its range): two values of type T.  Kept below the type's largest
-// value, hi is finite, and an infinity or NaN comes back whole from lo.
+// x as a sum of PARTS values of type T, each the nearest to what the ones before leave: 24 bits of x in three bf16 parts, 22 in
+// two fp16 ones.  Kept below the type's largest value, the first ones are finite, and an infinity or NaN comes back whole from
+// the last.
+template <typename T> constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
 template <typename T>
-__device__ __forceinline__ void split16(float x, T &hi, T &lo)
+__device__ __forceinline__ void split16(float x, T (&part)[PARTS<T>])
 {
     constexpr float MOST = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
-    hi = from_float<T>(fminf(fmaxf(x, -MOST), MOST));
-    lo = from_float<T>(x - to_float(hi));
+#pragma unroll
+    for (int i = 0; i < PARTS<T>; ++i) {
+        part[i] = from_float<T>(i + 1 < PARTS<T> ? fminf(fmaxf(x, -MOST), MOST) : x);
+        x -= to_float(part[i]);
+    }
 }
 
-// Operands of a product as TF32: factors of 16 bits are exact in it; an fp32 operand beside them is rounded (2^-11, a quarter
-// of a bf16 result's half step); two fp32 operands are split and multiplied three times (the product of both low parts, 2^-21,
-// is left out), which keeps fp32's precision.
+// Operands of a product as TF32.  16-bit values are exact in it.  An fp32 one is rounded (2^-11) beside bf16 factors, whose
+// results have an eighth of its bits; beside fp16 and fp32 factors it is split in two, and of two split ones the product of
+// both low parts (2^-21) is left out, which keeps fp32's precision.
 template <bool SPLIT> struct Operand;
 template <> struct Operand<false> {
     unsigned v;
-    __device__ __forceinline__ void set(float x) { v = to_tf32(x); }
     template <typename T> __device__ __forceinline__ void of(T x)
     {
-        if (sizeof(T) == 2)
+        if constexpr (sizeof(T) == 2)
             v = __float_as_uint(to_float(x));
         else
-            set(to_float(x));
+            v = to_tf32(x);
     }
 };
 template <> struct Operand<true> {
     unsigned v, lo;
-    __device__ __forceinline__ void set(float x) { split_tf32(x, v, lo); }
-    template <typename T> __device__ __forceinline__ void of(T x) { set(to_float(x)); }
+    __device__ __forceinline__ void of(float x) { split_tf32(x, v, lo); }
 };
+// Whether an operand of type T is split beside factors of type TF.
+template <typename TF, typename T> constexpr bool IS_SPLIT = sizeof(T) == 4 && !std::is_same<TF, __nv_bfloat16>::value;
 
-template <bool SPLIT>
-__device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SPLIT> (&a)[4], const Operand<SPLIT> &b0, const Operand<SPLIT> &b1)
+template <bool SA, bool SB>
+__device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SA> (&a)[4], const Operand<SB> &b0, const Operand<SB> &b1)
 {
     const unsigned hi[4] = {a[0].v, a[1].v, a[2].v, a[3].v};
-    if constexpr (SPLIT) {
+    if constexpr (SA) {
         const unsigned lo[4] = {a[0].lo, a[1].lo, a[2].lo, a[3].lo};
         mma8(d, lo, b0.v, b1.v);
-        mma8(d, hi, b0.lo, b1.lo);
     }
+    if constexpr (SB) mma8(d, hi, b0.lo, b1.lo);
     mma8(d, hi, b0.v, b1.v);
 }
 
@@ -294,7 +298,7 @@ struct TileColumns {
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
 struct ShrinkShape {
     static constexpr bool M16 = sizeof(TF) == 2 && sizeof(TI) == 2;  // 16-bit matrix instructions (else TF32)
-    static constexpr bool SPLIT = sizeof(TF) == 4;
+    static constexpr bool SA = IS_SPLIT<TF, TF>, SB = IS_SPLIT<TF, TI>;
     static constexpr int KS = sizeof(TF) == 4 ? 8 : 16;  // rows of In a step
     static constexpr int RP = RT * 16;
     // Row pitches in bytes, padded so that a matrix fragment's rows fall into different banks (ranks above 128, whose ring
@@ -458,7 +462,17 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int m = 0; m < RT; ++m) product(m, b, acc[m][b]);
+                        for (int m = 0; m < RT; ++m) {
+                            if constexpr (sizeof(TF) == 4) {
+                                // The tensor cores cut their sums instead of rounding them: in fp32 long sums are kept outside.
+                                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                product(m, b, part);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[m][b][e] += part[e];
+                            } else {
+                                product(m, b, acc[m][b]);
+                            }
+                        }
                     return;
                 }
 #pragma unroll
@@ -496,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
             } else {
 #pragma unroll
                 for (int k = 0; k < KS; k += 8) {
-                    Operand<Q::SPLIT> A[RT][4];
+                    Operand<Q::SA> A[RT][4];
 #pragma unroll
                     for (int m = 0; m < RT; ++m)
 #pragma unroll
@@ -504,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
                             const int r = m * 16 + g + (e & 1) * 8, i = k + q + (e >> 1) * 4;
                             A[m][e].of(*(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF)));
                         }
-                    Operand<Q::SPLIT> B8[2];
+                    Operand<Q::SB> B8[2];
                     int have = -1;
                     add([&](int m, int b, float (&to)[4]) {
                         if (have != b) {
@@ -513,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
                                 B8[e].of(*(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI)));
                             have = b;
                         }
-                        mma8_any<Q::SPLIT>(to, A[m], B8[0], B8[1]);
+                        mma8_any(to, A[m], B8[0], B8[1]);
                     });
                 }
             }
@@ -584,10 +598,10 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
             slot[SLOT + r * PITCH + c] = v;
             most = fmaxf(most, fabsf(v));
         } else if (sizeof(TF) == 2 && keep) {
-            TF hi, lo;
-            split16<TF>(v, hi, lo);
-            h.hi<TF>()[r * h.pitch + t0 + place] = hi;
-            h.lo<TF>()[r * h.pitch + t0 + place] = lo;
+            TF part[PARTS<TF>];
+            split16<TF>(v, part);
+#pragma unroll
+            for (int i = 0; i < PARTS<TF>; ++i) h.part<TF>(i)[r * h.pitch + t0 + place] = part[i];
         }
     }
     if (HALF) {
@@ -599,10 +613,10 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
         const float down = __int_as_float((127 - shift) << 23);
         if (keep) {
             for (int r = r_first; r < p.R; r += r_step) {
-                TF hi, lo;
-                split16<TF>(slot[SLOT + r * PITCH + c] * down, hi, lo);
-                h.hi<TF>()[r * h.pitch + t0 + place] = hi;
-                h.lo<TF>()[r * h.pitch + t0 + place] = lo;
+                TF part[PARTS<TF>];
+                split16<TF>(slot[SLOT + r * PITCH + c] * down, part);
+#pragma unroll
+                for (int i = 0; i < PARTS<TF>; ++i) h.part<TF>(i)[r * h.pitch + t0 + place] = part[i];
             }
             if (r_first == 0) h.colscale()[t0 + c] = __int_as_float((127 + shift) << 23);
         }
@@ -616,14 +630,14 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
 // memory; F2's slices come a chunk ahead and base two (asynchronous copies), the first of them before the block waits for the
 // kernel that makes S (programmatic dependent launch), so that the start of this kernel hides behind the end of that
 // one.  Columns are dealt to the matrix instruction so that a thread's results of two blocks of 8 lie side by side: base and
-// Out move 16 bytes a thread.  In 16 bits both parts of S are multiplied, so that an fp32 Out is as exact as fp32 sums of
-// exact products.  With several adapters among the columns the product runs once for each, for the pairs of blocks that have
+// Out move 16 bytes a thread.  In 16 bits S's parts are multiplied one by one (a 16-bit Out needs two), so that an fp32
+// Out is as exact as fp32 sums of exact products.  With several adapters among the columns the product runs once for each, for the pairs of blocks that have
 // any of its columns.  Bound by base and Out: R / 8 products a byte.
 constexpr int EXP_COLS = 64;
 constexpr int EXP_ROWS = WARPS * 16;
 constexpr int EXP_PAIRS = EXP_COLS / 16;
 
-template <typename TF, int RT, bool TRANS>
+template <typename TF, int RT, bool TRANS, int COUNT>  // COUNT: S's parts that are multiplied
 struct ExpandShape {
     static constexpr int RP = RT * 16;
     static constexpr int F_ROWS = TRANS ? RP : 16;
@@ -632,7 +646,7 @@ struct ExpandShape {
     static constexpr int F_BYTES = F_ROWS * F_PITCH;
     static constexpr int S_PITCH = EXP_COLS * (int)sizeof(TF) + (sizeof(TF) == 4 ? 32 : 16);
     static constexpr int S_BYTES = RP * S_PITCH;  // one part
-    static constexpr int S_ALL = S_BYTES * (sizeof(TF) == 2 ? 2 : 1);
+    static constexpr int S_ALL = S_BYTES * COUNT;
     // Two blocks an SM up to rank 64, else one; two chunks of base ahead, or as many as fit; F2's slices in two buffers where
     // they fit.
     static constexpr int BLOCKS = RT <= 4 ? 2 : 1;
@@ -645,10 +659,10 @@ struct ExpandShape {
     static_assert(BYTES <= ROOM, "F2's slices do not fit");
 };
 
-template <typename TF, int RT, bool TRANS>
+template <typename TF, int RT, bool TRANS, int COUNT>
 __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const ApplyParams p)
 {
-    using Q = ExpandShape<TF, RT, TRANS>;
+    using Q = ExpandShape<TF, RT, TRANS, COUNT>;
     constexpr bool HALF = std::is_same<TF, __half>::value;
     constexpr int PAIRS = EXP_PAIRS, RP = Q::RP;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -659,7 +673,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
     const long long j_first = (long long)(blockIdx.x / across) * p.chunks * EXP_ROWS + warp * 16;
     const int chunks = (int)max(0ll, min((long long)p.chunks, (p.n2 - j_first + EXP_ROWS - 1) / EXP_ROWS));  // this warp's
     const int last_rows = chunks > 0 ? (int)min(16ll, p.n2 - j_first - (long long)(chunks - 1) * EXP_ROWS) : 0;
-    unsigned char *const sh = smem, *const sl = smem + Q::S_BYTES, *const f0 = smem + Q::S_ALL + warp * (Q::BUFFERS * Q::F_BYTES);
+    unsigned char *const sh = smem, *const f0 = smem + Q::S_ALL + warp * (Q::BUFFERS * Q::F_BYTES);
     unsigned char *const slots = smem + Q::S_ALL + WARPS * Q::BUFFERS * Q::F_BYTES + threadIdx.x * 16;  // pieces THREADS * 16 apart
     __shared__ __align__(16) float colscale[EXP_COLS];
 
@@ -686,14 +700,14 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
     auto fill_f = [&](unsigned char *f, int a, int chunk, int rows) {  // the warp's rows of adapter a's F2
         const long long j0 = j_first + (long long)chunk * EXP_ROWS;
         const TF *F = (const TF *)p.F2 + (long long)a * p.R * p.n2 + (TRANS ? j0 : j0 * p.R);
-        constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, COUNT = Q::F_ROWS * CH;
+        constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, PIECES = Q::F_ROWS * CH;
         if (p.vec_f2) {
 #pragma unroll
-            for (int k = 0; k < (COUNT + 31) / 32; ++k) {
+            for (int k = 0; k < (PIECES + 31) / 32; ++k) {
                 const int r = (lane + k * 32) / CH, c = (lane + k * 32) % CH * PER;
                 const int left = TRANS ? (r < p.R ? rows - c : 0) : (r < rows ? p.R - c : 0);
                 const int valid = left <= 0 ? 0 : left >= PER ? 16 : left * (int)sizeof(TF);
-                if (COUNT % 32 == 0 || lane + k * 32 < COUNT)
+                if (PIECES % 32 == 0 || lane + k * 32 < PIECES)
                     copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F2, valid);
             }
         } else {
@@ -714,17 +728,19 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
             if (Q::SLOTS == 2 && chunks > 1) fetch_base(1, base + base_step, rows_of(1));
         }
         cudaGridDependencySynchronize();
-        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER, PARTS = sizeof(TF) == 2 ? 2 : 1;
-        const TF *src[2] = {sizeof(TF) == 4 ? (const TF *)hid.s() : hid.template hi<TF>(), hid.template lo<TF>()};
+        cudaTriggerProgrammaticLaunchCompletion();
+        constexpr int PER = 16 / (int)sizeof(TF), CH = EXP_COLS / PER;
         const int c = threadIdx.x % CH * PER, r = threadIdx.x / CH;
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+        for (int part = 0; part < COUNT; ++part) {
+            const TF *const src = sizeof(TF) == 4 ? (const TF *)hid.s() : hid.template part<TF>(part);
 #pragma unroll
             for (int k = 0; k < (RP * CH + THREADS - 1) / THREADS; ++k) {
                 const int row = r + k * (THREADS / CH), valid = row < p.R ? 16 : 0;
                 if (RP * CH % THREADS == 0 || row < RP)
-                    copy16((part ? sl : sh) + row * Q::S_PITCH + c * (int)sizeof(TF), valid ? src[part] + row * hid.pitch + t0 + c : src[part], valid);
+                    copy16(sh + part * Q::S_BYTES + row * Q::S_PITCH + c * (int)sizeof(TF), valid ? src + row * hid.pitch + t0 + c : src, valid);
             }
+        }
         if (HALF && threadIdx.x < EXP_COLS) colscale[threadIdx.x] = hid.colscale()[t0 + threadIdx.x];
     });
     const int *const ids = tile.ids, *const list = tile.list;
@@ -763,13 +779,13 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
 #pragma unroll
                 for (int b = 0; b < PAIRS; ++b) {
                     if (!all.value && !(some >> b & 1)) continue;
-                    unsigned L[4], H[4];
-                    load_matrices<true>(L, sl + row + b * 32);
-                    load_matrices<true>(H, sh + row + b * 32);
-                    mma16<TF>(sum[b][0], A, L[0], L[1]);
-                    mma16<TF>(sum[b][1], A, L[2], L[3]);
-                    mma16<TF>(sum[b][0], A, H[0], H[1]);
-                    mma16<TF>(sum[b][1], A, H[2], H[3]);
+#pragma unroll
+                    for (int part = COUNT - 1; part >= 0; --part) {
+                        unsigned B[4];
+                        load_matrices<true>(B, sh + part * Q::S_BYTES + row + b * 32);
+                        mma16<TF>(sum[b][0], A, B[0], B[1]);
+                        mma16<TF>(sum[b][1], A, B[2], B[3]);
+                    }
                 }
             }
         } else {
@@ -779,7 +795,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int j = g + (e & 1) * 8, r = k + q + (e >> 1) * 4;
-                    A[e].set(*(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4));
+                    A[e].of(*(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4));
                 }
 #pragma unroll
                 for (int b = 0; b < PAIRS; ++b) {
@@ -788,9 +804,9 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
                     for (int h = 0; h < 2; ++h) {
                         const unsigned char *s = sh + (k + q) * Q::S_PITCH + (b * 16 + 4 * (g >> 1) + 2 * h + (g & 1)) * 4;
                         Operand<true> B[2];
-                        B[0].set(*(const float *)s);
-                        B[1].set(*(const float *)(s + 4 * Q::S_PITCH));
-                        mma8_any<true>(sum[b][h], A, B[0], B[1]);
+                        B[0].of(*(const float *)s);
+                        B[1].of(*(const float *)(s + 4 * Q::S_PITCH));
+                        mma8_any(sum[b][h], A, B[0], B[1]);
                     }
                 }
             }
@@ -823,16 +839,16 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
     if (plain) {
         // Whole chunks of a usual tile: a lane's pieces of F2's slice lie CH pieces apart in one column (or row), all
         // addresses advance by constants, and the next chunk's copies are under way while this one is multiplied.
-        constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, COUNT = Q::F_ROWS * CH;
+        constexpr int PER = 16 / (int)sizeof(TF), CH = Q::F_COLS / PER, PIECES = Q::F_ROWS * CH;
         constexpr int ROWS = CH >= 32 ? 1 : 32 / CH;  // rows from a lane's piece to its next
         const int f_row = lane / CH, f_col = lane % CH * PER;
         const TF *f_src = (const TF *)p.F2 + (long long)list[0] * p.R * p.n2 + (TRANS ? j_first : j_first * p.R) + f_row * f_ld + f_col;
         const long long f_step = TRANS ? EXP_ROWS : (long long)EXP_ROWS * p.R;
-        const bool simple = CH <= 32 && COUNT % 32 == 0 && (TRANS ? true : f_col + PER <= p.R || f_col >= p.R);
+        const bool simple = CH <= 32 && PIECES % 32 == 0 && (TRANS ? true : f_col + PER <= p.R || f_col >= p.R);
         auto fetch_f = [&](unsigned char *f, const TF *src) {
             unsigned char *to = f + f_row * Q::F_PITCH + f_col * (int)sizeof(TF);
 #pragma unroll
-            for (int k = 0; k < COUNT / 32; ++k) {
+            for (int k = 0; k < PIECES / 32; ++k) {
                 const bool in = TRANS ? f_row + k * ROWS < p.R : f_col < p.R;
                 copy16(to + k * ROWS * Q::F_PITCH, in ? src + k * ROWS * f_ld : (const TF *)p.F2, in ? 16 : 0);
             }
@@ -1136,7 +1152,7 @@ __global__ void __launch_bounds__(THREADS) lora_token(const ApplyParams p)
 // of the adapter's, in turn.  A block takes Z's and S's chunks through a ring in shared memory; a warp takes 16 rows and all
 // R of S.  Columns of other adapters count as zeros in both operands (an infinity there meets a zero nowhere).
 // The blocks' sums are joined through distributed shared memory in a fixed order.  Both products of a backward pass are one
-// launch.
+// launch, dU first: it may start while dX is still being made.
 constexpr int GRAD_ROWS = 128;
 constexpr int GRAD_CHUNK = 32;
 constexpr int GRAD_SCAN = 128;  // chunks looked over at once
@@ -1157,7 +1173,7 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                                            float (&acc)[RT * 2][4])
 {
     using Q = GradShape<RT>;
-    constexpr bool SPLIT = sizeof(TF) == 4;
+    constexpr bool SA = IS_SPLIT<TF, TZ>, SB = IS_SPLIT<TF, float>;
     __shared__ unsigned members[GRAD_SCAN];  // which columns of a chunk are the adapter's
     __shared__ unsigned char list[GRAD_SCAN];
     __shared__ int count, seen;
@@ -1248,26 +1264,39 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
             const unsigned char *z = smem + (i % Q::STAGES) * Q::STAGE + warp * 16 * Q::PITCH;
             const unsigned char *s = smem + (i % Q::STAGES) * Q::STAGE + GRAD_ROWS * Q::PITCH;
             const unsigned member = members[list[i]];
+            const auto multiply = [&](auto mixed) {
 #pragma unroll
-            for (int k = 0; k < GRAD_CHUNK; k += 8) {
-                Operand<SPLIT> A[4];
-                const bool in[2] = {(member >> (k + q) & 1) != 0, (member >> (k + q + 4) & 1) != 0};
+                for (int k = 0; k < GRAD_CHUNK; k += 8) {
+                    Operand<SA> A[4];
+                    const bool in[2] = {!mixed.value || (member >> (k + q) & 1), !mixed.value || (member >> (k + q + 4) & 1)};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const TZ v = *(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ));
-                    A[e].of(in[e >> 1] ? v : from_float<TZ>(0.0f));
-                }
-#pragma unroll
-                for (int b = 0; b < RT * 2; ++b) {
-                    Operand<SPLIT> B[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float v = *(const float *)(s + (b * 8 + g) * Q::PITCH + (k + q + e * 4) * 4);
-                        B[e].set(in[e] ? v : 0.0f);
+                    for (int e = 0; e < 4; ++e) {
+                        const TZ v = *(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ));
+                        A[e].of(in[e >> 1] ? v : from_float<TZ>(0.0f));
                     }
-                    mma8_any<SPLIT>(acc[b], A, B[0], B[1]);
+#pragma unroll
+                    for (int b = 0; b < RT * 2; ++b) {
+                        Operand<SB> B[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float v = *(const float *)(s + (b * 8 + g) * Q::PITCH + (k + q + e * 4) * 4);
+                            B[e].of(in[e] ? v : 0.0f);
+                        }
+                        if constexpr (sizeof(TF) == 4) {  // long sums are kept outside the tensor cores, which cut them
+                            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma8_any(part, A, B[0], B[1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[b][e] += part[e];
+                        } else {
+                            mma8_any(acc[b], A, B[0], B[1]);
+                        }
+                    }
                 }
-            }
+            };
+            if (member == ~0u)
+                multiply(std::false_type{});
+            else
+                multiply(std::true_type{});
         }
         copy_wait<0>();
     }
@@ -1285,6 +1314,9 @@ __global__ void __launch_bounds__(256) lora_grad(const GradParams w)
     const bool second = tile >= w.p[0].tiles;
     const GradProblem p = second ? w.p[1] : w.p[0];
     const long long j0 = (long long)(second ? tile - w.p[0].tiles : tile) * GRAD_ROWS;
+    // The first product's S was there before the kernel ahead of this one; the second's was made just before that one, and
+    // nothing may come after this kernel while one ahead of it still runs.
+    if (second) cudaGridDependencySynchronize();
     for (int a = blockIdx.y; a < w.c.L; a += gridDim.y) {
         float acc[RT * 2][4];
 #pragma unroll
@@ -1302,25 +1334,31 @@ __global__ void __launch_bounds__(256) lora_grad(const GradParams w)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[(warp * 16 + g + (e >> 1) * 8) * Q::SUM_PITCH + b * 8 + 2 * q + (e & 1)] = acc[b][e];
         cluster.sync();
+        // Each block joins its share of the rows, in place (nobody else reads them), and writes them out.
         const int own = GRAD_ROWS / ranks;
+        for (int i = threadIdx.x; i < own * Q::RP; i += 256) {
+            const int at = (rank * own + i / Q::RP) * Q::SUM_PITCH + i % Q::RP;
+            float x[8], v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = k < ranks ? cluster.map_shared_rank(sum, k)[at] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += x[k];
+            sum[at] = v;
+        }
+        __syncthreads();
         TF *G = (TF *)p.G + (long long)a * p.n * w.R;
         for (int i = threadIdx.x; i < own * w.R; i += 256) {
             // Neighbouring threads write neighbouring elements.
             const int r = p.gr == 1 ? i % w.R : i / own, j = rank * own + (p.gr == 1 ? i / w.R : i % own);
-            if (j0 + j >= p.n) continue;
-            float x[8], v = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = k < ranks ? cluster.map_shared_rank(sum, k)[j * Q::SUM_PITCH + r] : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v += x[k];
-            G[(j0 + j) * p.gj + r * p.gr] = from_float<TF>(v);
+            if (j0 + j < p.n) G[(j0 + j) * p.gj + r * p.gr] = from_float<TF>(sum[j * Q::SUM_PITCH + r]);
         }
         cluster.sync();
     }
+    if (!second) cudaGridDependencySynchronize();
 }
 
 // ------------------------------------------------------------------ launches
-// A launch in clusters of `ranks` blocks (0: none), or one that may start before the kernel ahead of it has ended.
+// A launch in clusters of `ranks` blocks (0: none) that may (`early`) start before the kernel ahead of it has ended.
 template <typename... Args>
 tcaspmm_status launch(const char *what, void (*kernel)(Args...), dim3 grid, int ranks, bool early, int shared, cudaStream_t st, Args... args)
 {
@@ -1329,17 +1367,19 @@ tcaspmm_status launch(const char *what, void (*kernel)(Args...), dim3 grid, int 
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     if (ranks) {
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = (unsigned)ranks;
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    } else {
-        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[0].val.programmaticStreamSerializationAllowed = early;
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = (unsigned)ranks;
+        at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (early) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
     }
     cfg.attrs = at;
-    cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e == cudaSuccess ? TCASPMM_OK : cuda_fail(e, what);
 }
@@ -1390,13 +1430,13 @@ tcaspmm_status shrink(ApplyParams p, int sms, cudaStream_t st)
     });
 }
 
-template <typename TF, bool TRANS>
-tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
+template <typename TF, bool TRANS, int COUNT>
+tcaspmm_status expand_parts(ApplyParams p, int sms, cudaStream_t st)
 {
     return with_rank(p.R, [&](auto rt) {
         constexpr int RT = rt.value;
-        using Q = ExpandShape<TF, RT, TRANS>;
-        const auto kernel = lora_expand<TF, RT, TRANS>;
+        using Q = ExpandShape<TF, RT, TRANS, COUNT>;
+        const auto kernel = lora_expand<TF, RT, TRANS, COUNT>;
         const long long across = ceil_div(p.N, EXP_COLS), chunks = ceil_div(p.n2, EXP_ROWS);
         if (chunks == 0) return TCASPMM_OK;
         // As many chunks a block as leave every SM eight blocks (those with several adapters take longer).
@@ -1407,6 +1447,14 @@ tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
         const tcaspmm_status s = allow_shared("lora launch", (const void *)kernel, Q::BYTES, done);
         return s != TCASPMM_OK ? s : launch("lora launch", kernel, dim3((unsigned)blocks), 0, true, Q::BYTES, st, p);
     });
+}
+
+template <typename TF, bool TRANS>
+tcaspmm_status expand(const ApplyParams &p, int sms, cudaStream_t st)
+{
+    if constexpr (std::is_same<TF, __nv_bfloat16>::value && !TRANS)
+        if (p.outtype == 0) return expand_parts<TF, TRANS, 3>(p, sms, st);
+    return expand_parts<TF, TRANS, sizeof(TF) == 2 ? 2 : 1>(p, sms, st);
 }
 
 // Where the forward pass takes column by column: up to this many, when a column's part fits in shared memory.
@@ -1434,7 +1482,7 @@ tcaspmm_status apply(const ApplyParams &p, int sms, cudaStream_t st)
 }
 
 template <typename TF>
-tcaspmm_status grads(GradParams w, int sms, cudaStream_t st)
+tcaspmm_status grads(GradParams w, bool early, int sms, cudaStream_t st)
 {
     return with_rank(w.R, [&](auto rt) {
         constexpr int RT = rt.value;
@@ -1449,7 +1497,7 @@ tcaspmm_status grads(GradParams w, int sms, cudaStream_t st)
         const tcaspmm_status s = allow_shared("lora_backward launch", (const void *)kernel, GradShape<RT>::BYTES, done);
         return s != TCASPMM_OK ? s
                                : launch("lora_backward launch", kernel, dim3((unsigned)(tiles * ranks), (unsigned)std::min(w.c.L, 65535)),
-                                        ranks, false, GradShape<RT>::BYTES, st, w);
+                                        ranks, early, GradShape<RT>::BYTES, st, w);
     });
 }
 

@@ -13,6 +13,9 @@ tcaspmm_status lora_input_grad_bf16(const ApplyParams &p, bool in32, int sms, cu
     return in32 ? apply<__nv_bfloat16, float, true>(p, sms, st) : apply<__nv_bfloat16, __nv_bfloat16, true>(p, sms, st);
 }
 
-tcaspmm_status lora_factor_grads_bf16(const GradParams &w, int sms, cudaStream_t st) { return grads<__nv_bfloat16>(w, sms, st); }
+tcaspmm_status lora_factor_grads_bf16(const GradParams &w, bool early, int sms, cudaStream_t st)
+{
+    return grads<__nv_bfloat16>(w, early, sms, st);
+}
 
 }  // namespace tca

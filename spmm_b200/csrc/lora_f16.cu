@@ -13,6 +13,9 @@ tcaspmm_status lora_input_grad_f16(const ApplyParams &p, bool in32, int sms, cud
     return in32 ? apply<__half, float, true>(p, sms, st) : apply<__half, __half, true>(p, sms, st);
 }
 
-tcaspmm_status lora_factor_grads_f16(const GradParams &w, int sms, cudaStream_t st) { return grads<__half>(w, sms, st); }
+tcaspmm_status lora_factor_grads_f16(const GradParams &w, bool early, int sms, cudaStream_t st)
+{
+    return grads<__half>(w, early, sms, st);
+}
 
 }  // namespace tca

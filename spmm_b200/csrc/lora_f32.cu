@@ -13,6 +13,9 @@ tcaspmm_status lora_input_grad_f32(const ApplyParams &p, bool in32, int sms, cud
     return in32 ? apply<float, float, true>(p, sms, st) : apply<float, float, true>(p, sms, st);
 }
 
-tcaspmm_status lora_factor_grads_f32(const GradParams &w, int sms, cudaStream_t st) { return grads<float>(w, sms, st); }
+tcaspmm_status lora_factor_grads_f32(const GradParams &w, bool early, int sms, cudaStream_t st)
+{
+    return grads<float>(w, early, sms, st);
+}
 
 }  // namespace tca

@@ -245,6 +245,7 @@ def lora_ref(X, down, up, index, scale, base, out_dtype):
     X, down, up = (t.detach().double().cpu() for t in (X, down, up))
     L, R, K = down.shape
     M, N = up.shape[1], X.shape[1]
+    part = 2.0 ** -17 if out_dtype == BF16 else 2.0 ** -21
     idx = torch.zeros(N, dtype=torch.long) if index is None else index.cpu().long()
     Y = torch.zeros(M, N, dtype=torch.float64) if base is None else base.detach().double().cpu().clone()
     tol = U * Y.abs()
@@ -258,15 +259,15 @@ def lora_ref(X, down, up, index, scale, base, out_dtype):
         H[:, at] = h
         d, da = up[a] @ h, up[a].abs() @ h.abs()
         Y[:, at] += d
-        tol[:, at] += lora_sum_error(K) * (up[a].abs() @ ha) + lora_sum_error(R) * da + 2 * U * Y[:, at].abs()
+        tol[:, at] += lora_sum_error(K) * (up[a].abs() @ ha) + lora_sum_error(R, part) * da + 2 * U * Y[:, at].abs()
     tol = tol + TINY
     return Y, tol + half_step(Y.abs() + tol, out_dtype), H
 
 
-def lora_sum_error(n):
+def lora_sum_error(n, parts=2.0 ** -21):
     """A sum of n products: the tensor cores may cut (not round) at each of up to n / 4 + 64 partial sums, a full step
-    each; an intermediate is held in two parts of its type, at worst two bf16s: 2^-17."""
-    return 2 * U * (n / 4 + 64) + 2.0 ** -17
+    each; an intermediate is held in parts of its type: 22 bits or more of it, 2^-17 where a bf16 result needs no more."""
+    return 2 * U * (n / 4 + 64) + parts
 
 
 def lora_grads_ref(X, down, up, index, scale, dY, base=None):
@@ -274,8 +275,9 @@ def lora_grads_ref(X, down, up, index, scale, dY, base=None):
     X, down, up, dY = (t.detach().double().cpu() for t in (X, down, up, dY))
     L, R, K = down.shape
     M, N = up.shape[1], X.shape[1]
-    # With 16-bit factors the fp32 operands of the gradients' products are rounded to TF32 (10 bits after the point).
-    tf = 0.0 if dt == F32 else 2.0 ** -11
+    # With bf16 factors the fp32 operands of the gradients' products are rounded to TF32 (10 bits after the point), and the
+    # intermediate of dX is held in two parts.
+    tf, part = (2.0 ** -11, 2.0 ** -17) if dt == BF16 else (0.0, 2.0 ** -21)
     idx = torch.zeros(N, dtype=torch.long) if index is None else index.cpu().long()
     dX = torch.zeros(K, N, dtype=torch.float64) if base is None else base.double().cpu().clone()
     dD, dU = torch.zeros_like(down), torch.zeros_like(up)
@@ -291,7 +293,7 @@ def lora_grads_ref(X, down, up, index, scale, dY, base=None):
         e_p = (lora_sum_error(M) + tf) * abs(s) * (up[a].abs().T @ g.abs())
         d = down[a].T @ p
         dX[:, at] += d
-        eX[:, at] += down[a].abs().T @ (e_p + (lora_sum_error(R) + tf) * p.abs()) + 2 * U * dX[:, at].abs()
+        eX[:, at] += down[a].abs().T @ (e_p + lora_sum_error(R, part) * p.abs()) + 2 * U * dX[:, at].abs()
         n = at.numel()
         # The columns of other adapters in between count as zero terms of the sums.
         dD[a] = p @ x.T
