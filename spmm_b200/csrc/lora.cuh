@@ -264,11 +264,13 @@ __device__ __forceinline__ void store_four(T *p, const float (&y)[4])
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 
-// Of a tile's columns: their adapters (-1: none, or past the end), and those that occur, by their first columns.
+// Of a tile's columns: their adapters (-1: none, or past the end), and those that occur, by their first columns; for each of
+// those, where there are several, which blocks of 8 columns hold any of its columns, and which others' beside them.
 template <int TN>
 struct TileColumns {
     __align__(16) int ids[TN];
     int list[TN], count;
+    unsigned char some[TN], mixed[TN];  // TN / 8 bits each
     // `meanwhile` runs while the indices are on their way.
     template <typename F>
     __device__ __forceinline__ void load(const Columns &c, long long t0, long long N, F &&meanwhile)
@@ -292,6 +294,19 @@ struct TileColumns {
             if (lane == 0) count = n;
         }
         __syncthreads();
+        if (count > 1) {
+            for (int d = threadIdx.x; d < count; d += THREADS) {
+                const int a = list[d];
+                unsigned has = 0u, other = 0u;
+                for (int t = 0; t < TN; ++t) {
+                    has |= (unsigned)(ids[t] == a) << (t >> 3);
+                    other |= (unsigned)(ids[t] != a && ids[t] >= 0) << (t >> 3);
+                }
+                some[d] = (unsigned char)has;
+                mixed[d] = (unsigned char)other;
+            }
+            __syncthreads();
+        }
     }
 };
 
@@ -442,20 +457,10 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
             fill_next();
             const unsigned char *in = ring + at * Q::STAGE, *f = in + KS * Q::IN_PITCH;
             if (++at == Q::STAGES) at = 0;
-            const int a = list[d];
+            const int a = list[d], this_d = d;
             const bool first = d == 0;
             if (++d == nd) d = 0;
-            // Which blocks of 8 columns hold columns of adapter a, and which others beside them.
-            unsigned some = ~0u, mixed = 0u;
-            if (nd > 1) {
-                some = 0u;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const int o = ids[b * 8 + (lane & 7)];
-                    if (__any_sync(~0u, o == a)) some |= 1u << b;
-                    if (__any_sync(~0u, o != a && o >= 0)) mixed |= 1u << b;
-                }
-            }
+            const unsigned some = nd > 1 ? tile.some[this_d] : ~0u, mixed = nd > 1 ? tile.mixed[this_d] : 0u;
             // acc += part, or in a mixed block only for adapter a's columns.
             auto add = [&](auto &&product) {
                 if (some == ~0u && !mixed) {
@@ -990,15 +995,14 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
         for (int pass = 0; pass < nd; ++pass) {
             // The thread's columns of this pass's adapter; pairs of blocks with any.
             const int a = list[pass];
+            const unsigned blocks = nd > 1 ? tile.some[pass] : ~0u;
             unsigned mine = 0u, some = 0u;
 #pragma unroll
             for (int b = 0; b < PAIRS; ++b) {
                 const int4 id = *(const int4 *)(ids + b * 16 + 4 * q);
-                const unsigned m = (id.x == a) | (id.y == a) << 1 | (id.z == a) << 2 | (id.w == a) << 3;
-                mine |= m << (b * 4);
-                some |= (unsigned)(m != 0u) << b;
+                mine |= ((id.x == a) | (id.y == a) << 1 | (id.z == a) << 2 | (id.w == a) << 3) << (b * 4);
+                some |= (unsigned)((blocks >> (2 * b) & 3u) != 0u) << b;
             }
-            some = __reduce_or_sync(~0u, some);
             // F2's slices alternate between two buffers: the next pass's (or chunk's) is fetched during this one.
             const bool more = pass + 1 < nd || chunk + 1 < chunks;
             const int next_pass = pass + 1 < nd ? pass + 1 : 0, next_chunk = pass + 1 < nd ? chunk : chunk + 1;
