@@ -397,12 +397,13 @@ typedef struct tcaspmm_adapters {
 /* Bytes of the buffer tcaspmm_lora works in (device memory, 16-byte aligned).
  * With keep it leaves scale * down * X there for the backward pass (opaque);
  * without, the buffer is scratch, and 0 bytes where none is needed. */
-size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t K, int64_t N, tcaspmm_dtype dt, int keep);
+size_t tcaspmm_lora_hidden_bytes(int64_t count, int64_t rank, int64_t M, int64_t K, int64_t N, tcaspmm_dtype dt,
+                                 int keep);
 /* Y[:, t] = base[:, t] + scale[a] * up[a] * (down[a] * X[:, t]), a = index[t];
  * Y = base where column t has no adapter.  X is K x N in dt; base (M x N, or NULL
  * = 0: usually the C of an execute call) and Y are in y_dt, and Y may be base
- * itself (same ld).  hidden: tcaspmm_lora_hidden_bytes(rank, K, N, dt, keep)
- * bytes. */
+ * itself (same ld).  hidden: tcaspmm_lora_hidden_bytes(count, rank, M, K, N, dt,
+ * keep) bytes. */
 tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *dX, int64_t ldx, int64_t N, const void *dBase,
                             int64_t ldbase, void *dY, int64_t ldy, tcaspmm_dtype y_dt, void *hidden, int keep,
                             void *stream);

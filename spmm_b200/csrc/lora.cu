@@ -48,9 +48,9 @@ bool aligned(const void *p, int64_t ld, int type, int bytes)
 
 using namespace tca;
 
-extern "C" size_t tcaspmm_lora_hidden_bytes(int64_t rank, int64_t K, int64_t N, tcaspmm_dtype dt, int keep)
+extern "C" size_t tcaspmm_lora_hidden_bytes(int64_t count, int64_t rank, int64_t M, int64_t K, int64_t N, tcaspmm_dtype dt, int keep)
 {
-    if (rank < 1 || N < 1 || !dtype_valid(dt) || (!keep && by_token(K, N))) return 0;
+    if (rank < 1 || N < 1 || !dtype_valid(dt) || (!keep && by_token(count, rank, M, K, N))) return 0;
     return Hidden::bytes(rank, N, type_code(dt));
 }
 
@@ -65,7 +65,7 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
         return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld or NULL pointer",
                     (long long)ldx, (long long)ldbase, (long long)ldy);
     if (N == 0) return TCASPMM_OK;
-    const bool tokens = !keep && by_token(ad->K, N);
+    const bool tokens = !keep && by_token(ad->count, ad->rank, ad->M, ad->K, N);
     if (!tokens && (!hidden || (uintptr_t)hidden % 16)) return fail(TCASPMM_ERR_INVALID_ARG, "lora: hidden must be a 16-byte aligned device pointer");
     const int ft = type_code(ad->dt), yt = type_code(y_dt);
     ApplyParams p = {};

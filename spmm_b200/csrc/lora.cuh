@@ -1053,7 +1053,7 @@ __device__ __forceinline__ float load_base(const ApplyParams &p, long long i)
 }
 
 template <typename T, int VEC1, int VEC2>
-__global__ void __launch_bounds__(THREADS) lora_token(const ApplyParams p)
+__global__ void __launch_bounds__(THREADS, 4) lora_token(const ApplyParams p)
 {
     constexpr int AHEAD = 4;  // rows of U in flight a thread
     extern __shared__ __align__(16) float xs[];  // the block's part of the column
@@ -1461,9 +1461,15 @@ tcaspmm_status expand(const ApplyParams &p, int sms, cudaStream_t st)
     return expand_parts<TF, TRANS, sizeof(TF) == 2 ? 2 : 1>(p, sms, st);
 }
 
-// Where the forward pass takes column by column: up to this many, when a column's part fits in shared memory.
-constexpr int TOKEN_MOST = 64;
-inline bool by_token(long long K, long long N) { return N <= TOKEN_MOST && K <= 8ll * 8192; }
+// Where the forward pass goes column by column: up to 64 columns, or 256 where tiles of 64 may hold many adapters, within the
+// work that its reads of the factors from L2 are worth.  Measured (fp16, columns one by one against tiles): 64 columns of 64
+// adapters of rank 16, 4096 x 1024: 9 and 61 us, 256 of them 29 and 80; 64 columns of rank 64, 4096 x 4096, 8 adapters: 40 and
+// 56 us, 128 of them more than 80 and 56; 64 columns of rank 8, 512 x 512, one adapter: 6.2 and 7.7 us, 128 of them 10.8 and 7.5.
+inline bool by_token(long long L, long long R, long long M, long long K, long long N)
+{
+    const long long work = N * R * (K + M);
+    return K <= 8ll * 8192 && (N <= 64 ? work <= 40ll << 20 : N <= 256 && L >= 16 && work <= 24ll << 20);
+}
 
 template <typename TF>
 tcaspmm_status token(ApplyParams p, cudaStream_t st)

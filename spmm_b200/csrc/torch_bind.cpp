@@ -281,14 +281,14 @@ struct Adapters {
     }
 };
 
-int64_t hidden_bytes(const Tensor &x, int64_t R, bool keep)
+int64_t hidden_bytes(const Tensor &x, int64_t L, int64_t R, int64_t M, bool keep)
 {
-    return (int64_t)tcaspmm_lora_hidden_bytes(R, x.size(0), x.size(1), code(x.scalar_type()), keep);
+    return (int64_t)tcaspmm_lora_hidden_bytes(L, R, M, x.size(0), x.size(1), code(x.scalar_type()), keep);
 }
 
-Tensor hidden_buffer(const Tensor &x, int64_t R, bool keep)
+Tensor hidden_buffer(const Tensor &x, int64_t L, int64_t R, int64_t M, bool keep)
 {
-    const int64_t size = hidden_bytes(x, R, keep);
+    const int64_t size = hidden_bytes(x, L, R, M, keep);
     return size || keep ? at::empty({size}, x.options().dtype(at::kByte)) : Tensor();
 }
 
@@ -317,7 +317,7 @@ Tensor lora_call(const Tensor &x, const Tensor &down, const Tensor &up, const Ma
     if (out) check_with(x, *out, "out");
     const c10::cuda::CUDAGuard guard(x.device());
     if (!out) Y = Matrix(at::empty({a.M, a.N}, x.options().dtype(type)), "out");
-    const Tensor hidden = hidden_buffer(x, a.R, H != nullptr);
+    const Tensor hidden = hidden_buffer(x, a.L, a.R, a.M, H != nullptr);
     check(tcaspmm_lora(a.args(), a.X.ptr(), a.X.ld, a.N, base.ptr(), base.ld, Y.ptr(), Y.ld, code(type), ptr(hidden),
                        H != nullptr, at::cuda::getCurrentCUDAStream().stream()));
     if (H) *H = hidden;
@@ -356,7 +356,7 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
     check_shape(dy, "dY", {a.M, a.N});
     TORCH_CHECK_VALUE(dy.scalar_type() == at::kFloat || dy.scalar_type() == x.scalar_type(), "dY must be float32 or X's type ",
                       x.scalar_type(), ", not ", dy.scalar_type());
-    TORCH_CHECK_VALUE(H.scalar_type() == at::kByte && H.dim() == 1 && H.is_contiguous() && H.numel() == hidden_bytes(x, a.R, true),
+    TORCH_CHECK_VALUE(H.scalar_type() == at::kByte && H.dim() == 1 && H.is_contiguous() && H.numel() == hidden_bytes(x, a.L, a.R, a.M, true),
                       "H must be the tensor that lora returned with hidden");
     const Tensor b = given(base_);
     Matrix base;
@@ -375,7 +375,7 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
     Tensor dD = at::empty(need_down ? a.down.sizes() : at::IntArrayRef{0}, x.options());
     Tensor dU = at::empty(need_up ? a.up.sizes() : at::IntArrayRef{0}, x.options());
     Tensor P;
-    if (need_input || need_down) P = hidden_buffer(x, a.R, true);
+    if (need_input || need_down) P = hidden_buffer(x, a.L, a.R, a.M, true);
     check(tcaspmm_lora_backward(a.args(), dY.ptr(), dY.ld, code(dy.scalar_type()), a.X.ptr(), a.X.ld, a.N, H.data_ptr(),
                                 (const float *)base.ptr(), base.ld, need_input ? dX.data_ptr() : nullptr, a.N,
                                 need_down ? dD.data_ptr() : nullptr, need_up ? dU.data_ptr() : nullptr, ptr(P),

@@ -27,7 +27,7 @@ _sig("tcaspmm_layer_norm", [_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, C.
 _sig("tcaspmm_layer_norm_backward_workspace", [_i64, _i64, C.c_int], C.c_size_t)
 _sig("tcaspmm_layer_norm_backward", [_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, _vp, _vp, C.c_int, _vp, _i64, _vp, _vp,
                                      _i64, _i64, C.c_int, _vp, C.c_size_t, _vp])
-_sig("tcaspmm_lora_hidden_bytes", [_i64, _i64, _i64, C.c_int, C.c_int], C.c_size_t)
+_sig("tcaspmm_lora_hidden_bytes", [_i64, _i64, _i64, _i64, _i64, C.c_int, C.c_int], C.c_size_t)
 _sig("tcaspmm_lora", [C.POINTER(_Adapters), _vp, _i64, _i64, _vp, _i64, _vp, _i64, C.c_int, _vp, C.c_int, _vp])
 _sig("tcaspmm_lora_backward", [C.POINTER(_Adapters), _vp, _i64, C.c_int, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
                                _vp, _vp, _vp])
@@ -35,9 +35,9 @@ _sig("tcaspmm_lora_backward", [C.POINTER(_Adapters), _vp, _i64, C.c_int, _vp, _i
 _OPS: dict = {}
 
 
-def hidden_bytes(rank: int, K: int, N: int, dt) -> int:
+def hidden_bytes(count: int, rank: int, M: int, K: int, N: int, dt) -> int:
     """Size of the buffer that lora returns with hidden."""
-    return lib.tcaspmm_lora_hidden_bytes(rank, K, N, int(as_dtype(dt)), 1)
+    return lib.tcaspmm_lora_hidden_bytes(count, rank, M, K, N, int(as_dtype(dt)), 1)
 
 
 def _op(name: str):
@@ -59,8 +59,8 @@ def _register_shapes() -> None:
 
     fake = torch.library.register_fake
 
-    def hidden(X, down):
-        return X.new_empty(hidden_bytes(down.shape[1], X.shape[0], X.shape[1], X.dtype), dtype=torch.uint8)
+    def hidden(X, up):
+        return X.new_empty(hidden_bytes(up.shape[0], up.shape[2], up.shape[1], X.shape[0], X.shape[1], X.dtype), dtype=torch.uint8)
 
     @fake("tcaspmm::layer_norm")
     def _(X, weight, bias, eps, dim, out_dtype):
@@ -83,11 +83,11 @@ def _register_shapes() -> None:
 
     @fake("tcaspmm::lora_hidden")
     def _(X, down, up, index, scale, base):
-        return X.new_empty((up.shape[1], X.shape[1]), dtype=torch.float32 if base is None else base.dtype), hidden(X, down)
+        return X.new_empty((up.shape[1], X.shape[1]), dtype=torch.float32 if base is None else base.dtype), hidden(X, up)
 
     @fake("tcaspmm::lora_into")
     def _(X, down, up, index, scale, base, out):
-        return hidden(X, down)
+        return hidden(X, up)
 
     @fake("tcaspmm::lora_backward")
     def _(dY, X, down, up, H, index, scale, base, need_input, need_down, need_up):

@@ -226,7 +226,7 @@ def _spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torc
 
 @_spmm_lora.register_fake
 def _(crow, col, val, X, down, up, index, scale):
-    size = dense.hidden_bytes(down.shape[1], X.shape[0], X.shape[1], X.dtype)
+    size = dense.hidden_bytes(up.shape[0], up.shape[2], up.shape[1], X.shape[0], X.shape[1], X.dtype)
     return X.new_empty((crow.shape[0] - 1, X.shape[1]), dtype=torch.float32), X.new_empty(size, dtype=torch.uint8)
 
 

@@ -415,29 +415,35 @@ def test_lora_wide_range_intermediate(dt):
     y, tol, h = lora_ref(X, down, up, None, scale, base, F32)
     assert float(h.abs().max()) > 65504
     close(T.lora(X, down, up, None, scale, base), y, tol)
+    close(T.lora(X, down, up, None, scale, base, hidden=True)[0], y, tol)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("N", [9, 90])
-def test_lora_of_views_in_place_and_without_base(dt, N):
+@pytest.mark.parametrize("hidden", [False, True])
+def test_lora_of_views_in_place_and_without_base(dt, N, hidden):
+    def lora(*args, **kw):
+        got = T.lora(*args, hidden=hidden, **kw)
+        return got[0] if hidden else got
+
     X, down, up, index, scale, base = lora_inputs(120, 70, N, 16, 3, dt)
     y, tol, _ = lora_ref(X, down, up, index, scale, base, F32)
     pad = torch.zeros(75, N + 13, device="cuda", dtype=dt)
     pad[2:72, 5:5 + N] = X
-    close(T.lora(pad[2:72, 5:5 + N], down, up, index, scale, base), y, tol)
-    close(T.lora(X.T.contiguous().T, down.transpose(1, 2).contiguous().transpose(1, 2), up, index, scale, base), y, tol)
+    close(lora(pad[2:72, 5:5 + N], down, up, index, scale, base), y, tol)
+    close(lora(X.T.contiguous().T, down.transpose(1, 2).contiguous().transpose(1, 2), up, index, scale, base), y, tol)
     out = torch.full((122, N + 7), 7.0, device="cuda")
     view = out[1:121, 3:3 + N]
-    assert T.lora(X, down, up, index, scale, base, out=view) is view
+    assert lora(X, down, up, index, scale, base, out=view) is view
     close(view, y, tol)
     view.fill_(7.0)
     assert torch.equal(out, torch.full_like(out, 7.0))  # nothing beside it was written
     view.copy_(base)
-    T.lora(X, down, up, index, scale, view, out=view)
+    lora(X, down, up, index, scale, view, out=view)
     close(view, y, tol)
     y0, tol0, _ = lora_ref(X, down, up, index, None, None, F32)
-    close(T.lora(X, down, up, index), y0, tol0)
+    close(lora(X, down, up, index), y0, tol0)
 
 
 @pytest.mark.gpu
@@ -567,7 +573,7 @@ def test_spmm_lora_is_the_product_and_its_adapters():
     X, down, up, index, scale, _ = lora_inputs(150, 96, 70, 16, 3, F16)
     C0 = torch.ops.tcaspmm.spmm(crow, col, val, X)
     Y = torch_op.spmm_lora(crow, col, val, X, down, up, index, scale)
-    assert torch.equal(Y, T.lora(X, down, up, index, scale, C0))
+    assert torch.equal(Y, T.lora(X, down, up, index, scale, C0, hidden=True)[0])
     with pytest.raises(ValueError, match="up"):
         torch_op.spmm_lora(crow, col, val, X, down, up[:, :149], index, scale)
     torch_op.clear_plan_cache()
@@ -697,7 +703,7 @@ def test_lora_refuses():
                            ((X, down, up, idx, sc, base), dict(out=torch.zeros(5, 4).T), "contiguous")]:
         with pytest.raises(ValueError, match=word):
             T.lora(*args, **kw)
-    H = torch.zeros(dense.hidden_bytes(3, 6, 5, F32), dtype=torch.uint8)
+    H = torch.zeros(dense.hidden_bytes(2, 3, 4, 6, 5, F32), dtype=torch.uint8)
     for args, word in [((base.half(), X, down, up, H), "dY"), ((base[:3], X, down, up, H), "shape"),
                        ((base, X, down, up, H[:-1]), "H must"), ((base, X, down, up, H.float()), "H must"),
                        ((base, X, down, up, H, idx, sc, X.half()), "base"), ((base, X, down, up, H), "CUDA")]:
