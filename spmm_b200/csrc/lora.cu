@@ -26,7 +26,7 @@ tcaspmm_status check(const tcaspmm_adapters *ad, int64_t N, const char *who)
         return fail(TCASPMM_ERR_INVALID_ARG, "%s: bad sizes count=%lld rank=%lld M=%lld K=%lld N=%lld", who, (long long)ad->count,
                     (long long)ad->rank, (long long)ad->M, (long long)ad->K, (long long)N);
     if (ad->rank > MAX_RANK) return fail(TCASPMM_ERR_UNSUPPORTED, "%s: rank %lld is above %lld", who, (long long)ad->rank, (long long)MAX_RANK);
-    if (ad->count > INT_MAX || N > INT_MAX - 65535 || ad->M > INT_MAX - 65535 || ad->K > INT_MAX - 65535)
+    if (ad->count > INT_MAX - 65535 || N > INT_MAX - 65535 || ad->M > INT_MAX - 65535 || ad->K > INT_MAX - 65535)
         return fail(TCASPMM_ERR_UNSUPPORTED, "%s: adapters, M, K and N must be below 2^31 - 65535", who);
     if (ad->index && ad->index_bytes != 4 && ad->index_bytes != 8)
         return fail(TCASPMM_ERR_INVALID_ARG, "%s: index_bytes must be 4 or 8, not %d", who, ad->index_bytes);

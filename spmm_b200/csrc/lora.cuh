@@ -1467,8 +1467,9 @@ tcaspmm_status expand(const ApplyParams &p, int sms, cudaStream_t st)
 // 56 us, 128 of them more than 80 and 56; 64 columns of rank 8, 512 x 512, one adapter: 6.2 and 7.7 us, 128 of them 10.8 and 7.5.
 inline bool by_token(long long L, long long R, long long M, long long K, long long N)
 {
+    if (N > 256 || K > 8ll * 8192) return false;
     const long long work = N * R * (K + M);
-    return K <= 8ll * 8192 && (N <= 64 ? work <= 40ll << 20 : N <= 256 && L >= 16 && work <= 24ll << 20);
+    return (N <= 64 ? work <= 40ll << 20 : L >= 16 && work <= 24ll << 20);
 }
 
 template <typename TF>

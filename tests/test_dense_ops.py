@@ -104,7 +104,7 @@ def norm_inputs(rows, cols, dim, dt, pdt, seed=0):
 
 
 NORM_SHAPES = [(1, 1), (1, 7), (5, 1), (3, 8), (64, 512), (33, 1000), (7, 5003), (300, 64), (129, 24), (2, 20000), (1000, 31),
-               (2049, 17), (513, 264), (4100, 130), (20000, 3), (9, 4096)]
+               (2049, 17), (513, 264), (4100, 130), (20000, 3), (9, 4096), (3, 12000), (3, 9001), (70001, 5), (6000, 33)]
 
 
 @pytest.mark.gpu
@@ -656,6 +656,62 @@ def test_training_step_captured():
 
 
 @pytest.mark.gpu
+def test_registered_operators():
+    """Schemas and fake tensors agree with what the operators do."""
+    check = ("test_schema", "test_faketensor")
+    X, w, b = norm_inputs(12, 16, 1, BF16, F32)
+    ops = torch.ops.tcaspmm
+    for dim in (0, 1):
+        p = w if dim == 1 else w[:12]
+        torch.library.opcheck(ops.layer_norm.default, (X, p, p, 1e-5, dim, F32), test_utils=check)
+        torch.library.opcheck(ops.layer_norm_stats.default, (X, p, None, 1e-5, dim, BF16), test_utils=check)
+        _, mean, rstd = T.layer_norm(X, dim=dim, stats=True)
+        torch.library.opcheck(ops.layer_norm_backward.default, (X, X, mean, rstd, None, dim, F32, True, False, True), test_utils=check)
+    X, down, up, index, scale, base = lora_inputs(20, 12, 16, 4, 2, F16)
+    torch.library.opcheck(ops.lora.default, (X, down, up, index, scale, base), test_utils=check)
+    torch.library.opcheck(ops.lora_hidden.default, (X, down, up, None, None, None), test_utils=("test_faketensor",))
+    torch.library.opcheck(ops.lora_into.default, (X, down, up, index, scale, base, base.clone()), test_utils=("test_faketensor",))
+    _, H = T.lora(X, down, up, index, scale, base, hidden=True)
+    torch.library.opcheck(ops.lora_backward.default, (base, X, down, up, H, index, scale, None, True, True, False), test_utils=check)
+
+
+@pytest.mark.gpu
+def test_calls_overlap_on_two_streams():
+    """Calls share nothing: the same results when many run on two streams at once, in either order."""
+    args = [lora_inputs(300, 200, n, 16, 5, F16, seed=n) for n in (500, 40, 130, 700)]
+    norms = [norm_inputs(300, c, 0, F16, F32, seed=c) for c in (400, 33, 64, 256)]
+    want = [(T.lora(*a), T.layer_norm(*n, 1e-5, 0)) for a, n in zip(args, norms)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], {}
+    for turn in range(6):
+        for k in range(4):
+            s = (turn + k) % 2
+            with torch.cuda.stream(streams[s]):
+                got[turn, k] = (T.lora(*args[k]), T.layer_norm(*norms[k], 1e-5, 0))
+    torch.cuda.synchronize()
+    for (_, k), (y, z) in got.items():
+        assert torch.equal(y, want[k][0]) and torch.equal(z, want[k][1])
+
+
+@pytest.mark.gpu
+def test_lora_past_32_bit_offsets():
+    """A base of more than 2^31 elements: columns at both ends of the last rows."""
+    M, N = 34000, 65600
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("needs 14 GB")
+    X = torch.randn(16, N, device="cuda").to(BF16)
+    down, up = torch.randn(1, 4, 16, device="cuda").to(BF16), torch.randn(1, M, 4, device="cuda").to(BF16)
+    out = torch.empty(M, N, device="cuda", dtype=BF16)
+    T.lora(X, down, up, out=out)
+    for rows, cols in [(slice(0, 40), slice(0, 40)), (slice(M - 40, M), slice(N - 40, N)), (slice(M - 40, M), slice(0, 40))]:
+        y, tol, _ = lora_ref(X[:, cols], down, up[:, rows], None, None, None, BF16)
+        close(out[rows, cols], y, tol)
+    Y = T.layer_norm(out, dim=1)
+    y, tol, *_ = norm_ref(out[M - 3:], None, None, 1e-5, 1, BF16)
+    close(Y[M - 3:], y, tol)
+
+
+@pytest.mark.gpu
 def test_on_another_device():
     if torch.cuda.device_count() < 2:
         pytest.skip("one GPU")
@@ -746,7 +802,7 @@ def test_c_entries_refuse_bad_arguments():
     for kw in [dict(dt=9), dict(yt=9), dict(count=-1), dict(rank=0), dict(M=-1), dict(K=-1), dict(n=-1), dict(index_bytes=2),
                dict(down=None), dict(up=None), dict(x=None), dict(y=None), dict(ldx=7), dict(ldy=7), dict(base=p, ldb=7), dict(h=None), dict(h=p + 4)]:
         assert lora(**kw) == INV, kw
-    for kw in [dict(rank=257), dict(count=2 ** 31), dict(M=2 ** 31 - 1), dict(n=2 ** 31 - 1, ldx=2 ** 31, ldy=2 ** 31)]:
+    for kw in [dict(rank=257), dict(count=2 ** 31 - 1), dict(M=2 ** 31 - 1), dict(n=2 ** 31 - 1, ldx=2 ** 31, ldy=2 ** 31)]:
         assert lora(**kw) == UNS, kw
     assert lib.tcaspmm_lora(None, p, 8, 8, None, 8, p, 8, 0, p, 1, None) == INV
 
