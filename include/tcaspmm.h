@@ -352,7 +352,8 @@ tcaspmm_status tcaspmm_spmm_csr_noalloc(const int32_t *d_row_ptr, const int32_t 
  * on `stream` (capturable) and share no state, so calls may overlap on any
  * streams and from any threads as long as no output or workspace of one is used
  * by another.  Sums are fp32 and their order is fixed: results are
- * bit-identical from run to run.  No counterpart in the reference. */
+ * bit-identical from run to run.  fp32 adapters use the tensor cores with split
+ * operands, which keeps fp32's precision.  No counterpart in the reference. */
 
 /* Layer norm of the rows x cols matrix X: of each row (dim 1: a node's features,
  * the layout of a graph product's C) or of each column (dim 0: a token's

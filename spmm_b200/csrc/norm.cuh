@@ -6,13 +6,17 @@
 //   mean = sum x / n    rstd = 1 / sqrt(sum (x - mean)^2 / n + eps)    xh = (x - mean) rstd    y = w xh + b
 //   g = w dy            dx = rstd (g - mean(g) - xh mean(g xh))        dw = sum dy xh          db = sum dy
 //
-// Every pass is bound by memory: the vector is read once, held as it came (registers, or shared memory), and summed twice there (the mean
-// first, then the squared differences from it, so that a large mean costs no precision).  Rows: a part of a warp, a warp or a
-// block per row, whichever leaves a thread at most 16 elements.  Columns: a cluster of up to 8
-// blocks shares a strip of 16-64 columns, each block holds a part of the strip's rows, and the blocks exchange their sums
-// through distributed shared memory, so that reads stay coalesced along the rows.  The weight's gradient is summed by each
-// thread over the vectors it meets (its features stay the same), by block through shared memory, and over the blocks by a
-// second kernel, in a fixed order.
+// Every pass is bound by memory: the vector is read once, held as it came (registers, or shared memory), and summed twice there
+// (the mean first, then the squared differences from it, so that a large mean costs no precision).  Rows: a part of a warp, a
+// warp or a block per row, whichever leaves a thread at most 16 elements.  Columns: a cluster of up to 8 blocks shares a strip
+// of 16-64 columns, each block holds a part of the strip's rows, and the blocks exchange their sums through distributed shared
+// memory, so that reads stay coalesced along the rows.  The weight's gradient is summed by each thread over the vectors it
+// meets (its features stay the same), by block through shared memory, and over the blocks by a second kernel, in a fixed order.
+//
+// Measured (one B200, whose copy of large arrays reaches 6.5 TB/s): rows, 2^20 x 128 fp32, forward 168 us (6.4 TB/s), backward
+// 259 us (6.2 TB/s); 4096 x 8192 bf16, forward 40 us, backward 65 us; 100003 x 233 fp32 to bf16, whose rows allow no vectors,
+// 35 us (4.0 TB/s; about two thirds of the issue slots busy).  Columns, 4096 x 8192 bf16, forward 42 us (3.2 TB/s), backward
+// 80 us (2.5 TB/s): there the sums, the exchange between blocks and the unpacking of 16-bit elements take as long as memory.
 #pragma once
 
 #include <algorithm>
@@ -176,7 +180,9 @@ __device__ __forceinline__ void row_sum(float (&v)[COUNT], int lanes, float (*s)
 // ------------------------------------------------------------------ columns
 //
 // A cluster's block holds its part of a strip's rows in shared memory (asynchronous copies where the rows' alignment allows
-// them, 16 bytes a thread), so that several blocks an SM load, sum and write at the same time.
+// them, 16 bytes a thread), so that several blocks an SM load, sum and write at the same time: three of 64 KB.  The same
+// strips in registers, one block of 512 threads an SM, took 103 us forward and 123 us backward on 4096 x 8192 bf16 (42 and 80
+// here), for want of bytes on their way while a block was summing.
 constexpr int STRIP_THREADS = 256;
 constexpr int STRIP_WARPS = STRIP_THREADS / 32;
 constexpr int STRIP_MAX = 64;  // columns of a strip at most
