@@ -87,10 +87,15 @@ inline tcaspmm_status with_type(int code, F &&f)
     return f(__nv_bfloat16{});
 }
 
+inline int size_of(int code) { return code == 0 ? 4 : 2; }
+
+// Elements of the type of `code` may lie at p.
+inline bool pointer_ok(const void *p, int code) { return (uintptr_t)p % size_of(code) == 0; }
+
 // A matrix argument: an inner extent of `cols`, a leading dimension of `ld`, and a pointer unless it is empty.
-inline bool matrix_ok(const void *p, int64_t rows, int64_t cols, int64_t ld)
+inline bool matrix_ok(const void *p, int64_t rows, int64_t cols, int64_t ld, int code)
 {
-    return ld >= cols && (p != nullptr || rows == 0 || cols == 0);
+    return ld >= cols && (p != nullptr || rows == 0 || cols == 0) && pointer_ok(p, code);
 }
 
 }  // namespace tca

@@ -32,10 +32,11 @@ tcaspmm_status check(const tcaspmm_adapters *ad, int64_t N, const char *who)
         return fail(TCASPMM_ERR_INVALID_ARG, "%s: index_bytes must be 4 or 8, not %d", who, ad->index_bytes);
     if (ad->count > 0 && ((!ad->down && ad->K > 0) || (!ad->up && ad->M > 0)))
         return fail(TCASPMM_ERR_INVALID_ARG, "%s: NULL factor", who);
+    const int type = type_code(ad->dt);
+    if (!pointer_ok(ad->down, type) || !pointer_ok(ad->up, type) || !pointer_ok(ad->scale, 0) || (uintptr_t)ad->index % (ad->index ? ad->index_bytes : 1))
+        return fail(TCASPMM_ERR_INVALID_ARG, "%s: a misaligned factor, index or scale", who);
     return TCASPMM_OK;
 }
-
-int size_of(int type) { return type == 0 ? 4 : 2; }
 
 // Rows of an array start where `bytes`-byte accesses may.
 bool aligned(const void *p, int64_t ld, int type, int bytes)
@@ -61,13 +62,13 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
     const tcaspmm_status s = check(ad, N, "lora");
     if (s != TCASPMM_OK) return s;
     if (!dtype_valid(y_dt)) return fail(TCASPMM_ERR_INVALID_ARG, "lora: unknown dtype %d", (int)y_dt);
-    if (!matrix_ok(dX, ad->K, N, ldx) || !matrix_ok(dY, ad->M, N, ldy) || (dBase && ldbase < N))
-        return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld or NULL pointer",
+    const int ft = type_code(ad->dt), yt = type_code(y_dt);
+    if (!matrix_ok(dX, ad->K, N, ldx, ft) || !matrix_ok(dY, ad->M, N, ldy, yt) || (dBase && !matrix_ok(dBase, ad->M, N, ldbase, yt)))
+        return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld, NULL or misaligned pointer",
                     (long long)ldx, (long long)ldbase, (long long)ldy);
     if (N == 0) return TCASPMM_OK;
     const bool tokens = !keep && by_token(ad->count, ad->rank, ad->M, ad->K, N);
     if (!tokens && (!hidden || (uintptr_t)hidden % 16)) return fail(TCASPMM_ERR_INVALID_ARG, "lora: hidden must be a 16-byte aligned device pointer");
-    const int ft = type_code(ad->dt), yt = type_code(y_dt);
     ApplyParams p = {};
     p.F1 = ad->down;
     p.F2 = ad->up;
@@ -89,6 +90,9 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
     p.vec_in = aligned(dX, ldx, ft, 16);
     p.vec_f1 = aligned(ad->down, ad->K, ft, 16);
     p.vec_f2 = aligned(ad->up, ad->rank, ft, 16);
+    p.word_in = aligned(dX, ldx, ft, 4);
+    p.word_f1 = aligned(ad->down, ad->K, ft, 4);
+    p.word_f2 = aligned(ad->up, ad->rank, ft, 4);
     p.vec_base = aligned(dBase, ldbase, yt, 4 * size_of(yt));
     p.vec_out = aligned(dY, ldy, yt, 4 * size_of(yt));
     const auto run = ft == 0 ? lora_forward_f32 : ft == 1 ? lora_forward_f16 : lora_forward_bf16;
@@ -106,10 +110,10 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
     if (!dtype_valid(dy_dt)) return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: unknown dtype %d", (int)dy_dt);
     const int ft = type_code(ad->dt), gt = type_code(dy_dt);
     if (gt != 0 && gt != ft) return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: dY must be fp32 or of the factors' type");
-    if (!matrix_ok(dDY, ad->M, N, lddy) || (ddown && !matrix_ok(dX, ad->K, N, ldx)) || (dBase && ldbase < N) ||
-        (dDX && lddx < N))
+    if (!matrix_ok(dDY, ad->M, N, lddy, gt) || (ddown && !matrix_ok(dX, ad->K, N, ldx, ft)) || (dBase && !matrix_ok(dBase, ad->K, N, ldbase, 0)) ||
+        (dDX && !matrix_ok(dDX, ad->K, N, lddx, ft)) || !pointer_ok(ddown, ft) || !pointer_ok(dup, ft))
         return fail(TCASPMM_ERR_INVALID_ARG,
-                    "lora_backward: bad leading dimension lddy=%lld ldx=%lld ldbase=%lld lddx=%lld or NULL pointer",
+                    "lora_backward: bad leading dimension lddy=%lld ldx=%lld ldbase=%lld lddx=%lld, NULL or misaligned pointer",
                     (long long)lddy, (long long)ldx, (long long)ldbase, (long long)lddx);
     if (N > 0 && ((dup && !hidden) || ((dDX || ddown) && !scratch) || (uintptr_t)hidden % 16 || (uintptr_t)scratch % 16))
         return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: hidden and scratch must be 16-byte aligned device pointers");
@@ -136,6 +140,9 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
         p.vec_in = aligned(dDY, lddy, gt, 16);
         p.vec_f1 = aligned(ad->up, ad->rank, ft, 16);
         p.vec_f2 = aligned(ad->down, ad->K, ft, 16);
+        p.word_in = aligned(dDY, lddy, gt, 4);
+        p.word_f1 = aligned(ad->up, ad->rank, ft, 4);
+        p.word_f2 = aligned(ad->down, ad->K, ft, 4);
         p.vec_base = aligned(dBase, ldbase, 0, 16);
         p.vec_out = aligned(dDX, lddx, ft, 4 * size_of(ft));
         const auto run = ft == 0 ? lora_input_grad_f32 : ft == 1 ? lora_input_grad_f16 : lora_input_grad_bf16;
@@ -147,8 +154,8 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
     w.R = (int)ad->rank;
     w.N = N;
     // The first needs nothing of this call; the second what dX's first kernel has made.
-    w.p[0] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), (const float *)hidden, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
-    w.p[1] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), (const float *)scratch, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
+    w.p[0] = GradProblem{dDY, lddy, gt == 0, aligned(dDY, lddy, gt, 16), aligned(dDY, lddy, gt, 4), (const float *)hidden, ad->M, ad->M > 0 ? dup : nullptr, ad->rank, 1, 0};
+    w.p[1] = GradProblem{dX, ldx, ft == 0, aligned(dX, ldx, ft, 16), aligned(dX, ldx, ft, 4), (const float *)scratch, ad->K, ad->K > 0 ? ddown : nullptr, 1, ad->K, 0};
     const auto run = ft == 0 ? lora_factor_grads_f32 : ft == 1 ? lora_factor_grads_f16 : lora_factor_grads_bf16;
     return run(w, (dDX || ddown) && N > 0, sm_count(), st);  // early only behind kernels of this call
 }

@@ -76,6 +76,7 @@ struct ApplyParams {
     int outtype;
     void *hidden;  // S (Hidden)
     int vec_in, vec_f1, vec_f2, vec_base, vec_out;  // what alignment allows
+    int word_in, word_f1, word_f2;                  // rows start on 4 bytes
     long long per1;  // rows of In for each block of a cluster
     int chunks;      // of EXP_ROWS rows of Out for each block
 };
@@ -105,7 +106,7 @@ struct GradProblem {
     const void *Z;
     long long ldz;
     int z32;  // Z is fp32 (else the factors' type)
-    int vec;
+    int vec, word;  // what alignment allows: 16 bytes, 4 bytes
     const float *S;  // rows of Hidden's pitch
     long long n;
     void *G;  // or NULL: left out
@@ -134,6 +135,11 @@ __device__ __forceinline__ void copy16(void *dst, const void *src, int valid)
 __device__ __forceinline__ void copy8(void *dst, const void *src, int valid)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
+}
+// 4 bytes, those past `valid` as zeros.
+__device__ __forceinline__ void copy4(void *dst, const void *src, int valid)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -250,6 +256,42 @@ __device__ __forceinline__ void store_four(T *p, const float (&y)[4])
         uint2 bits;
         memcpy(&bits, u, sizeof bits);
         *(uint2 *)p = bits;
+    }
+}
+
+// A tile of ROWS x COLS elements whose rows are not 16-byte aligned, of which `rows` x `cols` exist (the rest: zeros), by
+// COUNT threads: 4-byte asynchronous copies where rows start on 4 bytes (`words`; always in fp32), else element by element, BATCH
+// loads in flight a thread (as many as leave the kernel's registers alone).
+template <typename T, int ROWS, int COLS, int PITCH, int COUNT, int BATCH>
+__device__ __forceinline__ void copy_loose(unsigned char *to, const T *from, long long ld, int rows, int cols, bool words, int thread)
+{
+    constexpr int PER = 4 / (int)sizeof(T);  // elements of a word
+    static_assert(ROWS * COLS % (COUNT * PER) == 0, "whole rounds of the threads");
+    if (words) {
+        constexpr int ROUNDS = ROWS * COLS / PER / COUNT;
+#pragma unroll BATCH
+        for (int k = 0; k < ROUNDS; ++k) {
+            const int at = (thread + k * COUNT) * PER, r = at / COLS, c = at % COLS;
+            const int left = r < rows ? cols - c : 0, valid = left <= 0 ? 0 : left >= PER ? 4 : (int)sizeof(T);
+            copy4(to + r * PITCH + c * (int)sizeof(T), valid ? from + r * ld + c : from, valid);
+        }
+    } else if constexpr (sizeof(T) == 2) {
+        constexpr int ROUNDS = ROWS * COLS / COUNT;
+        static_assert(ROUNDS % BATCH == 0, "whole batches");
+#pragma unroll 1
+        for (int k0 = 0; k0 < ROUNDS; k0 += BATCH) {
+            unsigned short v[BATCH];
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const int at = thread + (k0 + k) * COUNT, r = at / COLS, c = at % COLS;
+                v[k] = r < rows && c < cols ? __ldg((const unsigned short *)from + r * ld + c) : (unsigned short)0;
+            }
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                const int at = thread + (k0 + k) * COUNT;
+                *(unsigned short *)(to + at / COLS * PITCH + at % COLS * 2) = v[k];
+            }
+        }
     }
 }
 
@@ -402,12 +444,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
                 }
             }
         } else {
-            for (int k = lane; k < KS * TN; k += 32) {
-                const int r = k / TN, c = k - r * TN;
-                TI v = from_float<TI>(0.0f);
-                if (r < rows && t0 + c < p.N) v = ((const TI *)p.In)[(i0 + r) * p.ldin + t0 + c];
-                *(TI *)(in + r * Q::IN_PITCH + c * sizeof(TI)) = v;
-            }
+            copy_loose<TI, KS, TN, Q::IN_PITCH, 32, 4>(in, (const TI *)p.In + i0 * p.ldin + t0, p.ldin, rows, (int)min((long long)TN, p.N - t0), p.word_in, lane);
         }
         const TF *F = (const TF *)p.F1 + (long long)a * p.R * p.n1 + (TRANS ? i0 * p.R : i0);
         if (p.vec_f1) {
@@ -428,12 +465,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
                 }
             }
         } else {
-            for (int k = lane; k < Q::F_ROWS * Q::F_COLS; k += 32) {
-                const int r = k / Q::F_COLS, c = k - r * Q::F_COLS;
-                TF v = from_float<TF>(0.0f);
-                if (TRANS ? (r < rows && c < p.R) : (r < p.R && c < rows)) v = F[r * f_ld + c];
-                *(TF *)(f + r * Q::F_PITCH + c * sizeof(TF)) = v;
-            }
+            copy_loose<TF, Q::F_ROWS, Q::F_COLS, Q::F_PITCH, 32, 4>(f, F, f_ld, TRANS ? rows : p.R, TRANS ? p.R : rows, p.word_f1, lane);
         }
     };
 
@@ -722,12 +754,7 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
                     copy16(f + r * Q::F_PITCH + c * (int)sizeof(TF), valid ? F + r * f_ld + c : (const TF *)p.F2, valid);
             }
         } else {
-            for (int k = lane; k < Q::F_ROWS * Q::F_COLS; k += 32) {
-                const int r = k / Q::F_COLS, c = k - r * Q::F_COLS;
-                TF v = from_float<TF>(0.0f);
-                if (TRANS ? (r < p.R && c < rows) : (r < rows && c < p.R)) v = F[r * f_ld + c];
-                *(TF *)(f + r * Q::F_PITCH + c * sizeof(TF)) = v;
-            }
+            copy_loose<TF, Q::F_ROWS, Q::F_COLS, Q::F_PITCH, 32, 2>(f, F, f_ld, TRANS ? p.R : rows, TRANS ? rows : p.R, p.word_f2, lane);
         }
     };
     auto rows_of = [&](int chunk) { return chunk >= chunks ? 0 : chunk == chunks - 1 ? last_rows : 16; };
@@ -1214,12 +1241,7 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                 copy16(z + (z_row + k * RS) * Q::PITCH + z_col * (int)sizeof(TZ), valid ? z_src + t0 + k * RS * p.ldz : (const TZ *)p.Z, valid);
             }
         } else {
-            for (int k = threadIdx.x; k < GRAD_ROWS * GRAD_CHUNK; k += 256) {
-                const int r = k / GRAD_CHUNK, c = k % GRAD_CHUNK;
-                TZ v = from_float<TZ>(0.0f);
-                if (r < j_left && c < cols) v = ((const TZ *)p.Z)[(j0 + r) * p.ldz + t0 + c];
-                *(TZ *)(z + r * Q::PITCH + c * sizeof(TZ)) = v;
-            }
+            copy_loose<TZ, GRAD_ROWS, GRAD_CHUNK, Q::PITCH, 256, 4>(z, (const TZ *)p.Z + j0 * p.ldz + t0, p.ldz, j_left, cols, p.word, threadIdx.x);
         }
         const int left = cols - s_col, bytes = left <= 0 ? 0 : left >= 4 ? 16 : left * 4;
 #pragma unroll
@@ -1316,7 +1338,7 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
 }
 
 template <typename TF, int RT>
-__global__ void __launch_bounds__(256) lora_grad(const GradParams w)
+__global__ void __launch_bounds__(256, RT <= 4 ? 2 : 0) lora_grad(const GradParams w)
 {
     using Q = GradShape<RT>;
     extern __shared__ __align__(16) unsigned char smem[];

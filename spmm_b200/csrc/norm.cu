@@ -345,15 +345,17 @@ extern "C" tcaspmm_status tcaspmm_layer_norm(const void *dX, int64_t ldx, tcaspm
     if (!dtype_valid(x_dt) || !dtype_valid(y_dt) || !dtype_valid(p_dt))
         return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: unknown dtype");
     if (dim != 0 && dim != 1) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: dim must be 0 or 1, not %d", dim);
-    if (rows < 0 || cols < 0 || !matrix_ok(dX, rows, cols, ldx) || !matrix_ok(dY, rows, cols, ldy))
-        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: bad sizes rows=%lld cols=%lld ldx=%lld ldy=%lld or NULL pointer",
+    const int xt = type_code(x_dt), yt = type_code(y_dt), pt = type_code(p_dt);
+    if (rows < 0 || cols < 0 || !matrix_ok(dX, rows, cols, ldx, xt) || !matrix_ok(dY, rows, cols, ldy, yt))
+        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: bad sizes rows=%lld cols=%lld ldx=%lld ldy=%lld, NULL or misaligned pointer",
                     (long long)rows, (long long)cols, (long long)ldx, (long long)ldy);
     if (!(eps >= 0.0) || std::isinf(eps)) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: eps must be finite and not negative");
     if (!mean != !rstd) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: mean and rstd go together");
+    if (!pointer_ok(weight, pt) || !pointer_ok(bias, pt) || !pointer_ok(mean, 0) || !pointer_ok(rstd, 0))
+        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: misaligned weight, bias, mean or rstd");
     const long long vecs = dim == 1 ? rows : cols, n = dim == 1 ? cols : rows;
     if (vecs == 0) return TCASPMM_OK;
     if (n == 0) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: the normalised dimension is empty");
-    const int xt = type_code(x_dt), yt = type_code(y_dt), pt = type_code(p_dt);
     NormParams p{dX, ldx, dY, ldy, yt, weight, bias, pt, 0, mean, rstd, vecs, n, (float)eps};
     return with_type(xt, [&](auto t) {
         using T = decltype(t);
@@ -387,20 +389,22 @@ extern "C" tcaspmm_status tcaspmm_layer_norm_backward(const void *dDY, int64_t l
     if (!dtype_valid(x_dt) || !dtype_valid(dy_dt) || !dtype_valid(p_dt))
         return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: unknown dtype");
     if (dim != 0 && dim != 1) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: dim must be 0 or 1, not %d", dim);
-    if (rows < 0 || cols < 0 || !matrix_ok(dX, rows, cols, ldx) || !matrix_ok(dDY, rows, cols, lddy) ||
-        (dDX && lddx < cols))
+    const int xt = type_code(x_dt), gt = type_code(dy_dt), pt = type_code(p_dt);
+    if (rows < 0 || cols < 0 || !matrix_ok(dX, rows, cols, ldx, xt) || !matrix_ok(dDY, rows, cols, lddy, gt) ||
+        (dDX && !matrix_ok(dDX, rows, cols, lddx, xt)))
         return fail(TCASPMM_ERR_INVALID_ARG,
-                    "layer_norm_backward: bad sizes rows=%lld cols=%lld ldx=%lld lddy=%lld lddx=%lld or NULL pointer",
+                    "layer_norm_backward: bad sizes rows=%lld cols=%lld ldx=%lld lddy=%lld lddx=%lld, NULL or misaligned pointer",
                     (long long)rows, (long long)cols, (long long)ldx, (long long)lddy, (long long)lddx);
     const long long vecs = dim == 1 ? rows : cols, n = dim == 1 ? cols : rows;
     if (n == 0) return vecs == 0 ? TCASPMM_OK : fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: the normalised dimension is empty");
     if (vecs > 0 && (!mean || !rstd)) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: mean and rstd are needed");
+    if (!pointer_ok(mean, 0) || !pointer_ok(rstd, 0) || !pointer_ok(weight, pt) || !pointer_ok(dweight, pt) || !pointer_ok(dbias, pt))
+        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: misaligned mean, rstd, weight, dweight or dbias");
     const bool params = dweight || dbias;
     const size_t need = params ? tcaspmm_layer_norm_backward_workspace(rows, cols, dim) : 0;
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: a workspace of %zu bytes, 16-byte aligned, is needed", need);
     const cudaStream_t st = (cudaStream_t)stream;
-    const int xt = type_code(x_dt), gt = type_code(dy_dt), pt = type_code(p_dt);
     NormGradParams p{dDY, lddy, gt, dX, ldx, mean, rstd, weight, pt, 0, dDX, lddx, params ? (float *)workspace : nullptr, vecs, n};
     long long parts = 0;
     if (vecs > 0 && (dDX || params)) {

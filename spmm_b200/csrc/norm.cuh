@@ -285,7 +285,6 @@ __device__ float block_sum(float v, float *s)
 // ------------------------------------------------------------------ launches
 unsigned blocks_of(long long n) { return (unsigned)std::min<long long>(n, INT_MAX); }
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-int size_of(int type) { return type == 0 ? 4 : 2; }
 
 tcaspmm_status launched(const char *what)
 {

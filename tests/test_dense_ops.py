@@ -333,7 +333,7 @@ def lora_inputs(M, K, N, R, L, dt, ydt=F32, mix="runs", seed=0, index_dtype=torc
 
 LORA_SHAPES = [(1, 1, 1, 1, 1), (5, 3, 2, 1, 2), (64, 64, 1, 16, 4), (100, 72, 33, 8, 3), (257, 515, 70, 12, 5), (512, 256, 300, 16, 2),
                (96, 1000, 64, 64, 3), (130, 96, 200, 128, 2), (48, 40, 90, 200, 2), (1024, 2050, 9, 32, 9), (2048, 520, 130, 5, 3),
-               (40, 200, 700, 24, 4)]
+               (40, 200, 700, 24, 4), (131, 262, 333, 6, 3)]
 
 
 @pytest.mark.gpu
@@ -812,6 +812,37 @@ def test_c_entries_refuse_bad_arguments():
     for kw in [dict(dyt=9), dict(dy=None), dict(lddy=7), dict(x=None), dict(ldx=7), dict(h=None), dict(base=p, ldb=7), dict(lddx=7),
                dict(s=None), dict(rank=0)]:
         assert lback(**kw) == INV, kw
+
+
+def test_c_entries_refuse_misaligned_pointers():
+    """An element's own alignment is asked of every pointer, on the host: no device is needed."""
+    lib, p, INV = T.lib, 4096, T.Status.INVALID_ARG
+
+    def norm(x=p, y=p, w=p, b=p, m=p, r=p, t=0):
+        return lib.tcaspmm_layer_norm(x, 8, t, y, 8, t, w, b, t, m, r, 4, 8, 1, 1e-5, None)
+
+    def back(dy=p, x=p, m=p, r=p, w=p, dx=p, dw=p, db=p, t=0):
+        return lib.tcaspmm_layer_norm_backward(dy, 8, t, x, 8, t, m, r, w, t, dx, 8, dw, db, 4, 8, 1, p, 1 << 30, None)
+
+    def ad(t, wide, **kw):
+        d = dict(down=p, up=p, index=p, scale=p, count=2, rank=4, M=8, K=8, dt=t, index_bytes=8 if wide else 4)
+        d.update(kw)
+        return C.byref(dense._Adapters(*(d[n] for n, _ in dense._Adapters._fields_)))
+
+    def lora(x=p, base=p, y=p, t=0, wide=True, **kw):
+        return lib.tcaspmm_lora(ad(t, wide, **kw), x, 8, 8, base, 8, y, 8, t, p, 1, None)
+
+    def lback(dy=p, x=p, base=p, dx=p, dd=p, du=p, t=0, wide=True, **kw):
+        return lib.tcaspmm_lora_backward(ad(t, wide, **kw), dy, 8, t, x, 8, 8, p, base, 8, dx, 8, dd, du, p, None)
+
+    for call, names in [(norm, ["x", "y", "w", "b", "m", "r"]), (back, ["dy", "x", "m", "r", "w", "dx", "dw", "db"]),
+                        (lora, ["x", "base", "y", "down", "up", "scale", "index"]),
+                        (lback, ["dy", "x", "base", "dx", "dd", "du", "down", "up", "scale", "index"])]:
+        for name in names:
+            for t, off in [(0, 1), (0, 2), (1, 1), (2, 1)]:
+                assert call(**{name: p + off}, t=t) == INV, (call.__name__, name, t)
+                assert "aligned" in T.last_error()
+    assert lora(index=p + 4) == INV
 
 
 def test_adapters_struct_matches_the_header(tmp_path):
