@@ -351,7 +351,8 @@ tcaspmm_status tcaspmm_spmm_csr_noalloc(const int32_t *d_row_ptr, const int32_t 
  * take matrices in device memory of the current device, allocate nothing, launch
  * on `stream` (capturable) and share no state, so calls may overlap on any
  * streams and from any threads as long as no output or workspace of one is used
- * by another.  Sums are fp32 and their order is fixed: results are
+ * by another.  An output shares no memory with another argument, unless its entry
+ * says so.  Sums are fp32 and their order is fixed: results are
  * bit-identical from run to run.  fp32 adapters use the tensor cores with split
  * operands, which keeps fp32's precision.  No counterpart in the reference. */
 
@@ -412,7 +413,7 @@ tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *dX, int64_t 
  * dt, with dBase an fp32 K x N matrix (usually A^T dY) or NULL; ddown and dup in
  * dt, zeros for adapters without columns.  Any of the three may be NULL.  hidden
  * is what the forward pass left with keep (for dup); scratch is another buffer of
- * that size (for dX and ddown). */
+ * that size (for dX and ddown).  dX may be base itself (fp32, same ld). */
 tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, const void *dDY, int64_t lddy, tcaspmm_dtype dy_dt,
                                      const void *dX, int64_t ldx, int64_t N, const void *hidden, const float *dBase,
                                      int64_t ldbase, void *dDX, int64_t lddx, void *ddown, void *dup, void *scratch,

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cstring>
+#include <initializer_list>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -96,6 +97,34 @@ inline bool pointer_ok(const void *p, int code) { return (uintptr_t)p % size_of(
 inline bool matrix_ok(const void *p, int64_t rows, int64_t cols, int64_t ld, int code)
 {
     return ld >= cols && (p != nullptr || rows == 0 || cols == 0) && pointer_ok(p, code);
+}
+
+// The memory of a matrix (or, with one row, of an array) that is passed as an argument.
+struct Extent {
+    const char *p;
+    int64_t rows, bytes, pitch;  // of a row, and from one to the next
+    Extent(const void *at, int64_t r, int64_t cols, int64_t ld, int size)
+        : p((const char *)at), rows(at && cols > 0 ? r : 0), bytes(cols * size), pitch(ld * size)
+    {
+    }
+    const char *end() const { return p + (rows - 1) * pitch + bytes; }
+};
+
+// Whether two share memory; of two windows of one wider matrix that lie side by side, none is shared.
+inline bool overlap(const Extent &a, const Extent &b)
+{
+    if (a.rows <= 0 || b.rows <= 0 || a.end() <= b.p || b.end() <= a.p) return false;
+    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return true;
+    const int64_t d = ((b.p - a.p) % a.pitch + a.pitch) % a.pitch;
+    return d < a.bytes || a.pitch - d < b.bytes;
+}
+
+// Whether an output shares memory with any of the other arguments.
+inline bool overlaps_any(const Extent &out, std::initializer_list<Extent> others)
+{
+    for (const Extent &o : others)
+        if (overlap(out, o)) return true;
+    return false;
 }
 
 }  // namespace tca

@@ -66,6 +66,11 @@ extern "C" tcaspmm_status tcaspmm_lora(const tcaspmm_adapters *ad, const void *d
     if (!matrix_ok(dX, ad->K, N, ldx, ft) || !matrix_ok(dY, ad->M, N, ldy, yt) || (dBase && !matrix_ok(dBase, ad->M, N, ldbase, yt)))
         return fail(TCASPMM_ERR_INVALID_ARG, "lora: bad leading dimension ldx=%lld ldbase=%lld ldy=%lld, NULL or misaligned pointer",
                     (long long)ldx, (long long)ldbase, (long long)ldy);
+    const int fs = size_of(ft), ys = size_of(yt);
+    const Extent Y(dY, ad->M, N, ldy, ys), down(ad->down, ad->count * ad->rank, ad->K, ad->K, fs), up(ad->up, ad->count * ad->M, ad->rank, ad->rank, fs);
+    if (overlaps_any(Y, {Extent(dX, ad->K, N, ldx, fs), down, up}) ||
+        (!(dBase == dY && ldbase == ldy) && overlap(Y, Extent(dBase, ad->M, N, ldbase, ys))))
+        return fail(TCASPMM_ERR_INVALID_ARG, "lora: Y shares memory with an input (it may be base itself, with base's ld)");
     if (N == 0) return TCASPMM_OK;
     const bool tokens = !keep && by_token(ad->count, ad->rank, ad->M, ad->K, N);
     if (!tokens && (!hidden || (uintptr_t)hidden % 16)) return fail(TCASPMM_ERR_INVALID_ARG, "lora: hidden must be a 16-byte aligned device pointer");
@@ -115,6 +120,15 @@ extern "C" tcaspmm_status tcaspmm_lora_backward(const tcaspmm_adapters *ad, cons
         return fail(TCASPMM_ERR_INVALID_ARG,
                     "lora_backward: bad leading dimension lddy=%lld ldx=%lld ldbase=%lld lddx=%lld, NULL or misaligned pointer",
                     (long long)lddy, (long long)ldx, (long long)ldbase, (long long)lddx);
+    const int fs = size_of(ft);
+    const int64_t LR = ad->count * ad->rank;
+    const Extent X(ddown ? dX : nullptr, ad->K, N, ldx, fs), DY(dDY, ad->M, N, lddy, size_of(gt)), DX(dDX, ad->K, N, lddx, fs);
+    const Extent down(ad->down, LR, ad->K, ad->K, fs), up(ad->up, ad->count * ad->M, ad->rank, ad->rank, fs);
+    const Extent base(dBase, ad->K, N, ldbase, 4), gdown(ddown, LR, ad->K, ad->K, fs), gup(dup, ad->count * ad->M, ad->rank, ad->rank, fs);
+    const bool in_place = ft == 0 && dBase == dDX && ldbase == lddx;
+    if (overlaps_any(DX, {X, DY, down, up, gdown, gup}) || (!in_place && overlap(DX, base)) || overlaps_any(gdown, {X, DY, down, up, base, gup}) ||
+        overlaps_any(gup, {X, DY, down, up, base}))
+        return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: an output shares memory with another argument (dX may be an fp32 base itself)");
     if (N > 0 && ((dup && !hidden) || ((dDX || ddown) && !scratch) || (uintptr_t)hidden % 16 || (uintptr_t)scratch % 16))
         return fail(TCASPMM_ERR_INVALID_ARG, "lora_backward: hidden and scratch must be 16-byte aligned device pointers");
     const cudaStream_t st = (cudaStream_t)stream;

@@ -354,6 +354,9 @@ extern "C" tcaspmm_status tcaspmm_layer_norm(const void *dX, int64_t ldx, tcaspm
     if (!pointer_ok(weight, pt) || !pointer_ok(bias, pt) || !pointer_ok(mean, 0) || !pointer_ok(rstd, 0))
         return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: misaligned weight, bias, mean or rstd");
     const long long vecs = dim == 1 ? rows : cols, n = dim == 1 ? cols : rows;
+    if (overlaps_any(Extent(dY, rows, cols, ldy, size_of(yt)), {Extent(dX, rows, cols, ldx, size_of(xt)), Extent(weight, 1, n, n, size_of(pt)),
+                                                                Extent(bias, 1, n, n, size_of(pt))}))
+        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: Y shares memory with an input");
     if (vecs == 0) return TCASPMM_OK;
     if (n == 0) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: the normalised dimension is empty");
     NormParams p{dX, ldx, dY, ldy, yt, weight, bias, pt, 0, mean, rstd, vecs, n, (float)eps};
@@ -400,6 +403,9 @@ extern "C" tcaspmm_status tcaspmm_layer_norm_backward(const void *dDY, int64_t l
     if (vecs > 0 && (!mean || !rstd)) return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: mean and rstd are needed");
     if (!pointer_ok(mean, 0) || !pointer_ok(rstd, 0) || !pointer_ok(weight, pt) || !pointer_ok(dweight, pt) || !pointer_ok(dbias, pt))
         return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: misaligned mean, rstd, weight, dweight or dbias");
+    if (overlaps_any(Extent(dDX, rows, cols, lddx, size_of(xt)), {Extent(dX, rows, cols, ldx, size_of(xt)), Extent(dDY, rows, cols, lddy, size_of(gt)),
+                                                                  Extent(weight, 1, n, n, size_of(pt))}))
+        return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: dX shares memory with an input");
     const bool params = dweight || dbias;
     const size_t need = params ? tcaspmm_layer_norm_backward_workspace(rows, cols, dim) : 0;
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))

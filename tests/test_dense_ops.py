@@ -845,6 +845,57 @@ def test_c_entries_refuse_misaligned_pointers():
     assert lora(index=p + 4) == INV
 
 
+def test_c_entries_refuse_outputs_over_inputs():
+    """Refused on the host: no device is needed.  The two in-place forms and windows side by side are on the GPU below."""
+    lib, INV = T.lib, T.Status.INVALID_ARG
+    at = lambda k: 65536 * (k + 1)  # noqa: E731  (far from one another)
+
+    def norm(x=at(0), y=at(1), w=at(2), b=at(3), ldx=8, ldy=8):
+        return lib.tcaspmm_layer_norm(x, ldx, 0, y, ldy, 0, w, b, 0, None, None, 4, 8, 1, 1e-5, None)
+
+    # The same, a few elements on, the last element, another pitch, a window that runs into its neighbour.
+    for kw in [dict(y=at(0)), dict(y=at(0) + 4), dict(y=at(0) + 4 * 31), dict(y=at(0) - 4 * 31), dict(y=at(0), ldy=9),
+               dict(y=at(0) + 28, ldx=16, ldy=16), dict(y=at(2)), dict(y=at(3) - 4)]:
+        assert norm(**kw) == INV and "shares memory" in T.last_error(), kw
+
+    def back(dy=at(0), x=at(1), w=at(2), dx=at(3)):
+        return lib.tcaspmm_layer_norm_backward(dy, 8, 0, x, 8, 0, at(4), at(5), w, 0, dx, 8, None, None, 4, 8, 1, None, 0, None)
+
+    for kw in [dict(dx=at(0)), dict(dx=at(1)), dict(dx=at(2))]:
+        assert back(**kw) == INV and "shares memory" in T.last_error(), kw
+
+    def ad(down=at(10), up=at(11)):
+        return C.byref(dense._Adapters(down, up, at(12), None, 2, 4, 8, 8, 0, 4))
+
+    def lora(x=at(0), base=at(1), y=at(2), ldb=8, ldy=8, **kw):
+        return lib.tcaspmm_lora(ad(**kw), x, 8, 8, base, ldb, y, ldy, 0, at(3), 1, None)
+
+    for kw in [dict(y=at(0)), dict(y=at(1) + 4), dict(y=at(1), ldb=9), dict(y=at(10)), dict(y=at(11))]:
+        assert lora(**kw) == INV and "shares memory" in T.last_error(), kw
+
+    def lback(dy=at(0), x=at(1), base=at(2), dx=at(3), dd=at(4), du=at(5), **kw):
+        return lib.tcaspmm_lora_backward(ad(**kw), dy, 8, 0, x, 8, 8, at(6), base, 8, dx, 8, dd, du, at(7), None)
+
+    for kw in [dict(dx=at(0)), dict(dx=at(1)), dict(dx=at(2) + 4), dict(dx=at(4)), dict(dx=at(10)), dict(dd=at(0)), dict(dd=at(10)),
+               dict(dd=at(5)), dict(du=at(11)), dict(du=at(2)), dict(du=at(1))]:
+        assert lback(**kw) == INV and "shares memory" in T.last_error(), kw
+
+
+@pytest.mark.gpu
+def test_lora_in_place_and_beside_its_base():
+    """Y as base itself, and Y and base as neighbouring windows of one matrix: the same bits as a new Y."""
+    X, down, up, index, scale, base = lora_inputs(200, 96, 150, 16, 3, F32, F32, "runs")
+    want = T.lora(X, down, up, index, scale, base)
+    both = torch.zeros(200, 304, device="cuda")
+    both[:, :150] = base
+    got = T.lora(X, down, up, index, scale, both[:, :150], out=both[:, 150:300])
+    assert torch.equal(got, want) and torch.equal(both[:, :150], base) and not both[:, 300:].any()
+    assert torch.equal(T.lora(X, down, up, index, scale, both[:, :150], out=both[:, :150]), want)
+    for out in (both[:, 1:151], both[:, 149:299]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            T.lora(X, down, up, index, scale, both[:, :150], out=out)
+
+
 def test_adapters_struct_matches_the_header(tmp_path):
     import os
     import shutil
