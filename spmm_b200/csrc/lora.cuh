@@ -302,10 +302,11 @@ __device__ __forceinline__ void copy_loose(unsigned char *to, const T *from, lon
 // with all R x TN sums in the warp's registers.  The sums are joined over warps, then over blocks through distributed shared
 // memory, in a fixed order.  With several adapters among a tile's columns the product runs once for each, and a column keeps
 // its own adapter's.  It does R products for each element of In, so the tensor cores' legacy form (mma.sync, 8 cycles an
-// instruction for each quarter of an SM, measured: 580 TFLOP/s in 16 bits, 290 in TF32) is enough: In's bytes take as long as
-// the products of rank 90 in 16 bits.  Measured: K 1024, 8192 columns, rank 64, bf16: 15 us (17 MB of In), 25 us with tiles of
-// two adapters among them, which take about twice as long as the others; of a step's 1700 cycles most go to issuing its copies
-// and waiting for one another's results, with 8 warps an SM.
+// instruction for each quarter of an SM, measured; at 1.9 GHz 576 TFLOP/s in 16 bits, 288 in TF32) is enough: In's bytes take
+// as long as the products of rank 90 in 16 bits.  Measured: K 1024, 8192 columns, rank 64, bf16 (17 MB of In): 16.6 us where
+// every tile has one adapter, 24.3 us where some have two, which take twice as long as the others.  Of a warp's 14200 cycles for
+// its 8 steps 5300 are fragments and products, 3200 the issue of copies, 100 waits between steps and the rest the first fill;
+// joining the sums takes another 7000.
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 
@@ -670,12 +671,12 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
 // memory; F2's slices come a chunk ahead and base two (asynchronous copies), the first of them before the block waits for the
 // kernel that makes S (programmatic dependent launch), so that the start of this kernel hides behind the end of that
 // one.  Columns are dealt to the matrix instruction so that a thread's results of two blocks of 8 lie side by side: base and
-// Out move 16 bytes a thread.  In 16 bits S's parts are multiplied one by one (a 16-bit Out needs two), so that an fp32
-// Out is as exact as fp32 sums of exact products.  With several adapters among the columns the product runs once for each, for the pairs of blocks that have
-// any of its columns.  Bound by base and Out: R / 8 products a byte.
-// Measured: M 4096, 8192 columns, rank 64, bf16 factors, fp32 base and Out (268 MB): 64 us with two parts of S, 70 us with
-// three.  Chunks were measured at 1, 2, 3, 4, 5, 8 and 16 a block: 87, 73, 67, 66, 67, 66, 63 us where every tile has one
-// adapter, 89, 78, 75, 76, 79, 84, 98 us where some have two.
+// Out move 16 bytes a thread.  In 16 bits S's parts are multiplied one by one (a 16-bit Out needs two), so that an fp32 Out is
+// as exact as fp32 sums of exact products.  With several adapters among the columns the product runs once for each, for the
+// pairs of blocks that have any of its columns.  Bound by base and Out: R / 8 products a byte.
+// Measured: M 4096, 8192 columns, rank 64, bf16 factors, fp32 base and Out (268 MB), three parts of S, at 1, 2, 3, 4, 5, 8 and
+// 16 chunks a block: 96, 77, 73, 70, 72, 72, 70 us (3.7 TB/s at 3) where every tile has one adapter, 97, 85, 81, 82, 86, 91,
+// 108 us where some have two, whose blocks end last.  Two parts of S took 6 us less.
 constexpr int EXP_COLS = 64;
 constexpr int EXP_ROWS = WARPS * 16;
 constexpr int EXP_PAIRS = EXP_COLS / 16;
@@ -1191,8 +1192,8 @@ __global__ void __launch_bounds__(THREADS, 4) lora_token(const ApplyParams p)
 // R of S.  Columns of other adapters count as zeros in both operands (an infinity there meets a zero nowhere).
 // The blocks' sums are joined through distributed shared memory in a fixed order.  Both products of a backward pass are one
 // launch, dU first: it may start while dX is still being made.  Measured: K = M = 2048, 4096 columns, rank 32, three adapters,
-// bf16 beside fp32 dY: 36 us for both (50 MB); one product alone 24 us, of which the look at the indices takes 2 us, the
-// chunks 4 us and the join 3 us a block, 1.3 blocks an SM in turn.
+// bf16 beside fp32 dY: 37 us for both after dX (50 MB); dU alone 23 us, of which a block's look at the indices takes 2 us, its
+// chunks 4 us and the join 3 us, 1.3 blocks in turn for each of an SM's two places.
 constexpr int GRAD_ROWS = 128;
 constexpr int GRAD_CHUNK = 32;
 constexpr int GRAD_SCAN = 128;  // chunks looked over at once
