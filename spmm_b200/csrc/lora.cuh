@@ -174,13 +174,6 @@ __device__ __forceinline__ void mma8(float (&d)[4], const unsigned (&a)[4], unsi
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ unsigned to_tf32(float x)
-{
-    unsigned r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
-}
-
 // x = hi + lo up to 2^-21 |x|, both TF32 values: the upper 10 bits after the point, and what is left.
 __device__ __forceinline__ void split_tf32(float x, unsigned &hi, unsigned &lo)
 {
@@ -205,26 +198,18 @@ __device__ __forceinline__ void split16(float x, T (&part)[PARTS<T>])
     }
 }
 
-// Operands of a product as TF32.  16-bit values are exact in it.  An fp32 one is rounded (2^-11) beside bf16 factors, whose
-// results have an eighth of its bits; beside fp16 and fp32 factors it is split in two, and of two split ones the product of
-// both low parts (2^-21) is left out, which keeps fp32's precision.
+// Operands of a product as TF32.  16-bit values are exact in it; an fp32 one is split in two, and of two split ones the product
+// of both low parts (2^-21) is left out.
 template <bool SPLIT> struct Operand;
 template <> struct Operand<false> {
     unsigned v;
-    template <typename T> __device__ __forceinline__ void of(T x)
-    {
-        if constexpr (sizeof(T) == 2)
-            v = __float_as_uint(to_float(x));
-        else
-            v = to_tf32(x);
-    }
+    template <typename T> __device__ __forceinline__ void of(T x) { v = __float_as_uint(to_float(x)); }
 };
 template <> struct Operand<true> {
     unsigned v, lo;
     __device__ __forceinline__ void of(float x) { split_tf32(x, v, lo); }
 };
-// Whether an operand of type T is split beside factors of type TF.
-template <typename TF, typename T> constexpr bool IS_SPLIT = sizeof(T) == 4 && !std::is_same<TF, __nv_bfloat16>::value;
+template <typename T> constexpr bool IS_SPLIT = sizeof(T) == 4;
 
 template <bool SA, bool SB>
 __device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SA> (&a)[4], const Operand<SB> &b0, const Operand<SB> &b1)
@@ -359,7 +344,7 @@ struct TileColumns {
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
 struct ShrinkShape {
     static constexpr bool M16 = sizeof(TF) == 2 && sizeof(TI) == 2;  // 16-bit matrix instructions (else TF32)
-    static constexpr bool SA = IS_SPLIT<TF, TF>, SB = IS_SPLIT<TF, TI>;
+    static constexpr bool SA = IS_SPLIT<TF>, SB = IS_SPLIT<TI>;
     static constexpr int KS = sizeof(TF) == 4 ? 8 : 16;  // rows of In a step
     static constexpr int RP = RT * 16;
     // Row pitches in bytes, padded so that a matrix fragment's rows fall into different banks (ranks above 128, whose ring
@@ -1214,7 +1199,7 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                                            float (&acc)[RT * 2][4])
 {
     using Q = GradShape<RT>;
-    constexpr bool SA = IS_SPLIT<TF, TZ>, SB = IS_SPLIT<TF, float>;
+    constexpr bool SA = IS_SPLIT<TZ>, SB = true;
     __shared__ unsigned members[GRAD_SCAN];  // which columns of a chunk are the adapter's
     __shared__ unsigned char list[GRAD_SCAN];
     __shared__ int count, seen;

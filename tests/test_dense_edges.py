@@ -1,0 +1,45 @@
+"""Layer norm and low-rank adapters where the arithmetic, autograd and the build can go wrong at the edges.
+
+Values are chosen so that the formula's result is known exactly, or the bound stands beside the check.
+"""
+import pytest
+import torch
+
+import spmm_b200 as T
+from test_dense_ops import BF16, F16, F32
+
+
+# ------------------------------------------------------------------ precision
+def _adapter(down, up, X, dY, dt, N, at=(0, 1)):
+    """One adapter from nested lists; X and dY hold a few columns, put at `at` among N that are zero otherwise."""
+    D, Up = torch.tensor([down]).to(dt).cuda(), torch.tensor([up]).to(dt).cuda()
+    x, g = torch.tensor(X), torch.tensor(dY)
+    Xn, Gn = torch.zeros(x.shape[0], N), torch.zeros(g.shape[0], N)
+    for k, t in enumerate(at[:x.shape[1]]):
+        Xn[:, t], Gn[:, t] = x[:, k], g[:, k]
+    return Xn.to(dt).cuda(), D, Up, Gn.cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("N,at", [(2, (0, 1)), (70, (3, 66))])
+def test_gradients_keep_the_bits_of_fp32_operands(dt, N, at):
+    """An fp32 dY and the fp32 intermediates H and P are not rounded to the tensor cores' 10 bits: what is left where two
+    terms cancel is exact."""
+    e, f = 2.0 ** -13, 2.0 ** -12
+    # dU = (1 + e) h - h with h = 1: dY's low part.
+    X, D, Up, G = _adapter([[1.0]], [[1.0]], [[1.0, 1.0]], [[1 + e, -1.0]], dt, N, at)
+    H = T.lora(X, D, Up, hidden=True)[1]
+    assert float(T.lora_backward(G, X, D, Up, H)[2]) == e
+    # dU = h0 - h1 with h0 = 1 + f, h1 = 1: H's low part.
+    X, D, Up, G = _adapter([[1.0, f]], [[1.0]], [[1.0, 1.0], [1.0, 0.0]], [[1.0, -1.0]], dt, N, at)
+    H = T.lora(X, D, Up, hidden=True)[1]
+    assert float(T.lora_backward(G, X, D, Up, H)[2]) == f
+    # dD = p0 - p1 with p0 = 1 + f, p1 = 1: P's low part.
+    X, D, Up, G = _adapter([[1.0]], [[1.0], [f]], [[1.0, -1.0]], [[1.0, 1.0], [1.0, 0.0]], dt, N, at)
+    H = T.lora(X, D, Up, hidden=True)[1]
+    assert float(T.lora_backward(G, X, D, Up, H)[1]) == f
+    # p = (1 + e) - 1, dX = p: dY's low part in the product with up.
+    X, D, Up, G = _adapter([[1.0]], [[1.0], [-1.0]], [[1.0, 0.0]], [[1 + e, 0.0], [1.0, 0.0]], dt, N, at)
+    H = T.lora(X, D, Up, hidden=True)[1]
+    assert float(T.lora_backward(G, X, D, Up, H)[0][0, at[0]]) == e
