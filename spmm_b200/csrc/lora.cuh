@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
 // memory; F2's slices come a chunk ahead and base two (asynchronous copies), the first of them before the block waits for the
 // kernel that makes S (programmatic dependent launch), so that the start of this kernel hides behind the end of that
 // one.  Columns are dealt to the matrix instruction so that a thread's results of two blocks of 8 lie side by side: base and
-// Out move 16 bytes a thread.  In 16 bits S's parts are multiplied one by one (a 16-bit Out needs two), so that an fp32 Out is
+// Out move 16 bytes a thread.  In 16 bits S's parts are multiplied one by one, so that Out is, before its own rounding,
 // as exact as fp32 sums of exact products.  With several adapters among the columns the product runs once for each, for the
 // pairs of blocks that have any of its columns.  Bound by base and Out: R / 8 products a byte.
 // Measured: M 4096, 8192 columns, rank 64, bf16 factors, fp32 base and Out (268 MB), three parts of S, at 1, 2, 3, 4, 5, 8 and
@@ -666,8 +666,9 @@ constexpr int EXP_COLS = 64;
 constexpr int EXP_ROWS = WARPS * 16;
 constexpr int EXP_PAIRS = EXP_COLS / 16;
 
-template <typename TF, int RT, bool TRANS, int COUNT>  // COUNT: S's parts that are multiplied
+template <typename TF, int RT, bool TRANS>
 struct ExpandShape {
+    static constexpr int COUNT = sizeof(TF) == 2 ? PARTS<TF> : 1;  // S's parts
     static constexpr int RP = RT * 16;
     static constexpr int F_ROWS = TRANS ? RP : 16;
     static constexpr int F_COLS = TRANS ? 16 : RP;
@@ -688,10 +689,11 @@ struct ExpandShape {
     static_assert(BYTES <= ROOM, "F2's slices do not fit");
 };
 
-template <typename TF, int RT, bool TRANS, int COUNT>
+template <typename TF, int RT, bool TRANS>
 __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const ApplyParams p)
 {
-    using Q = ExpandShape<TF, RT, TRANS, COUNT>;
+    using Q = ExpandShape<TF, RT, TRANS>;
+    constexpr int COUNT = Q::COUNT;
     constexpr bool HALF = std::is_same<TF, __half>::value;
     constexpr int PAIRS = EXP_PAIRS, RP = Q::RP;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -1451,13 +1453,13 @@ tcaspmm_status shrink(ApplyParams p, int sms, cudaStream_t st)
     });
 }
 
-template <typename TF, bool TRANS, int COUNT>
-tcaspmm_status expand_parts(ApplyParams p, int sms, cudaStream_t st)
+template <typename TF, bool TRANS>
+tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
 {
     return with_rank(p.R, [&](auto rt) {
         constexpr int RT = rt.value;
-        using Q = ExpandShape<TF, RT, TRANS, COUNT>;
-        const auto kernel = lora_expand<TF, RT, TRANS, COUNT>;
+        using Q = ExpandShape<TF, RT, TRANS>;
+        const auto kernel = lora_expand<TF, RT, TRANS>;
         const long long across = ceil_div(p.N, EXP_COLS), chunks = ceil_div(p.n2, EXP_ROWS);
         if (chunks == 0) return TCASPMM_OK;
         // As many chunks a block as leave every SM eight blocks (those with several adapters take longer).
@@ -1468,14 +1470,6 @@ tcaspmm_status expand_parts(ApplyParams p, int sms, cudaStream_t st)
         const tcaspmm_status s = allow_shared("lora launch", (const void *)kernel, Q::BYTES, done);
         return s != TCASPMM_OK ? s : launch("lora launch", kernel, dim3((unsigned)blocks), 0, true, Q::BYTES, st, p);
     });
-}
-
-template <typename TF, bool TRANS>
-tcaspmm_status expand(const ApplyParams &p, int sms, cudaStream_t st)
-{
-    if constexpr (std::is_same<TF, __nv_bfloat16>::value && !TRANS)
-        if (p.outtype == 0) return expand_parts<TF, TRANS, 3>(p, sms, st);
-    return expand_parts<TF, TRANS, sizeof(TF) == 2 ? 2 : 1>(p, sms, st);
 }
 
 // Where the forward pass goes column by column: up to 64 columns, or 256 where tiles of 64 may hold many adapters, within the

@@ -43,3 +43,20 @@ def test_gradients_keep_the_bits_of_fp32_operands(dt, N, at):
     X, D, Up, G = _adapter([[1.0]], [[1.0], [-1.0]], [[1.0, 0.0]], [[1 + e, 0.0], [1.0, 0.0]], dt, N, at)
     H = T.lora(X, D, Up, hidden=True)[1]
     assert float(T.lora_backward(G, X, D, Up, H)[0][0, at[0]]) == e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("N", [1, 70])
+def test_intermediate_keeps_its_bits_for_16_bit_results(dt, N):
+    """S = down X (and P) is a sum, held in fp32's bits also where the result is 16-bit: what cancels there is exact."""
+    e = 2.0 ** -20
+    # P = (1 + 2^-9 + e, 1 + 2^-9), dX = their difference.
+    X, D, Up, G = _adapter([[1.0], [-1.0]], [[1.0, 0.0], [0.0, 1.0]], [[0.0]], [[1 + 2.0 ** -9 + e], [1 + 2.0 ** -9]], dt, N)
+    H = T.lora(X, D, Up, hidden=True)[1]
+    assert float(T.lora_backward(G, X, D, Up, H)[0][0, 0]) == e
+    # H the same, through the forward product, into a result of the factors' type.
+    X, D, Up, _ = _adapter([[1.0, 2.0 ** -9, e], [1.0, 2.0 ** -9, 0.0]], [[1.0, -1.0]], [[1.0], [1.0], [1.0]], [[0.0]], dt, N)
+    for hidden in (False, True):
+        Y = T.lora(X, D, Up, None, None, torch.zeros(1, N, device="cuda", dtype=dt), hidden=hidden)
+        assert float((Y[0] if hidden else Y)[0, 0]) == e
