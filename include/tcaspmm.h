@@ -353,8 +353,9 @@ tcaspmm_status tcaspmm_spmm_csr_noalloc(const int32_t *d_row_ptr, const int32_t 
  * streams and from any threads as long as no output or workspace of one is used
  * by another.  An output shares no memory with another argument, unless its entry
  * says so.  Sums are fp32 and their order is fixed: results are
- * bit-identical from run to run.  fp32 adapters use the tensor cores with split
- * operands, which keeps fp32's precision.  No counterpart in the reference. */
+ * bit-identical from run to run.  fp32 adapters use the tensor cores with operands
+ * split in two, rounded to nearest: a product is off by at most 2^-21, and results
+ * are about as exact as plain fp32 sums.  No counterpart in the reference. */
 
 /* Layer norm of the rows x cols matrix X: of each row (dim 1: a node's features,
  * the layout of a graph product's C) or of each column (dim 0: a token's

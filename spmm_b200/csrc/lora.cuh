@@ -174,15 +174,6 @@ __device__ __forceinline__ void mma8(float (&d)[4], const unsigned (&a)[4], unsi
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo up to 2^-21 |x|, both TF32 values: the upper 10 bits after the point, and what is left.
-__device__ __forceinline__ void split_tf32(float x, unsigned &hi, unsigned &lo)
-{
-    const unsigned b = __float_as_uint(x);
-    const bool special = (b & 0x7f800000u) == 0x7f800000u;  // infinities and NaN stay whole
-    hi = special ? __float_as_uint(x + x) : b & 0xffffe000u;
-    lo = special ? 0u : __float_as_uint(x - __uint_as_float(hi));
-}
-
 // x as a sum of PARTS values of type T, each the nearest to what the ones before leave: 24 bits of x in three bf16 parts, 22 in
 // two fp16 ones.  Kept below the type's largest value, the first ones are finite, and an infinity or NaN comes back whole from
 // the last.
@@ -198,29 +189,59 @@ __device__ __forceinline__ void split16(float x, T (&part)[PARTS<T>])
     }
 }
 
-// Operands of a product as TF32.  16-bit values are exact in it; an fp32 one is split in two, and of two split ones the product
-// of both low parts (2^-21) is left out.
+// Operands of a product as TF32 (10 bits after the point; the instruction ignores the bits behind them).  16-bit values are exact
+// in it.  An fp32 x is split in two, x = v + lo up to 2^-23 |x|, each to the nearest: lo is at most 2^-11 |x|, of either sign, so
+// that what is left out averages out: of two split operands the product of both low parts, 2^-22.  A product is off by at most
+// 2^-21.  (Parts cut toward zero, 2^-10 and 2^-21, had three times the plain fp32 sums' error.)
 template <bool SPLIT> struct Operand;
 template <> struct Operand<false> {
     unsigned v;
-    template <typename T> __device__ __forceinline__ void of(T x) { v = __float_as_uint(to_float(x)); }
 };
 template <> struct Operand<true> {
     unsigned v, lo;
-    __device__ __forceinline__ void of(float x) { split_tf32(x, v, lo); }
 };
 template <typename T> constexpr bool IS_SPLIT = sizeof(T) == 4;
 
-template <bool SA, bool SB>
-__device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SA> (&a)[4], const Operand<SB> &b0, const Operand<SB> &b1)
+template <typename T, int COUNT>
+__device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T>> (&o)[COUNT])
+{
+    if constexpr (!IS_SPLIT<T>) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) o[i].v = __float_as_uint(to_float(x[i]));
+    } else {
+        // What would round to infinity, infinities and NaN: one branch for all of them (integer additions instead of the
+        // conversion instruction, which is several times slower: 36 and 60 us for one of lora_grad's products).
+        bool usual = true;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) usual = usual && fabsf(x[i]) < 3.402e38f;
+        if (usual) {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                o[i].v = (__float_as_uint(x[i]) + 0x1000u) & 0xffffe000u;
+                o[i].lo = __float_as_uint(x[i] - __uint_as_float(o[i].v)) + 0x1000u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                const bool finite = fabsf(x[i]) <= 3.4028234663852886e38f;
+                const unsigned b = __float_as_uint(x[i]);
+                o[i].v = !finite ? __float_as_uint(x[i] + x[i]) : (fabsf(x[i]) < 3.402e38f ? b + 0x1000u : b) & 0xffffe000u;
+                o[i].lo = finite ? __float_as_uint(x[i] - __uint_as_float(o[i].v)) + 0x1000u : 0u;
+            }
+        }
+    }
+}
+
+template <bool SA>
+__device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SA> (&a)[4], const Operand<true> (&b)[2])
 {
     const unsigned hi[4] = {a[0].v, a[1].v, a[2].v, a[3].v};
     if constexpr (SA) {
         const unsigned lo[4] = {a[0].lo, a[1].lo, a[2].lo, a[3].lo};
-        mma8(d, lo, b0.v, b1.v);
+        mma8(d, lo, b[0].v, b[1].v);
     }
-    if constexpr (SB) mma8(d, hi, b0.lo, b1.lo);
-    mma8(d, hi, b0.v, b1.v);
+    mma8(d, hi, b[0].lo, b[1].lo);
+    mma8(d, hi, b[0].v, b[1].v);
 }
 
 // A 16-bit element of type code 1 (fp16) or 2 (bf16).
@@ -344,7 +365,6 @@ struct TileColumns {
 template <typename TF, typename TI, int RT, int TN, bool TRANS>
 struct ShrinkShape {
     static constexpr bool M16 = sizeof(TF) == 2 && sizeof(TI) == 2;  // 16-bit matrix instructions (else TF32)
-    static constexpr bool SA = IS_SPLIT<TF>, SB = IS_SPLIT<TI>;
     static constexpr int KS = sizeof(TF) == 4 ? 8 : 16;  // rows of In a step
     static constexpr int RP = RT * 16;
     // Row pitches in bytes, padded so that a matrix fragment's rows fall into different banks (ranks above 128, whose ring
@@ -536,24 +556,28 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
             } else {
 #pragma unroll
                 for (int k = 0; k < KS; k += 8) {
-                    Operand<Q::SA> A[RT][4];
+                    Operand<IS_SPLIT<TF>> A[RT][4];
 #pragma unroll
-                    for (int m = 0; m < RT; ++m)
+                    for (int m = 0; m < RT; ++m) {
+                        TF v[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int r = m * 16 + g + (e & 1) * 8, i = k + q + (e >> 1) * 4;
-                            A[m][e].of(*(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF)));
+                            v[e] = *(const TF *)(TRANS ? f + i * Q::F_PITCH + r * sizeof(TF) : f + r * Q::F_PITCH + i * sizeof(TF));
                         }
-                    Operand<Q::SB> B8[2];
+                        operands(v, A[m]);
+                    }
+                    Operand<true> B8[2];
                     int have = -1;
                     add([&](int m, int b, float (&to)[4]) {
                         if (have != b) {
+                            TI v[2];
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                B8[e].of(*(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI)));
+                            for (int e = 0; e < 2; ++e) v[e] = *(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI));
+                            operands(v, B8);
                             have = b;
                         }
-                        mma8_any(to, A[m], B8[0], B8[1]);
+                        mma8_any(to, A[m], B8);
                     });
                 }
             }
@@ -818,21 +842,23 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
 #pragma unroll 2
             for (int k = 0; k < RP; k += 8) {
                 Operand<true> A[4];
+                float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int j = g + (e & 1) * 8, r = k + q + (e >> 1) * 4;
-                    A[e].of(*(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4));
+                    v[e] = *(const float *)(TRANS ? f + r * Q::F_PITCH + j * 4 : f + j * Q::F_PITCH + r * 4);
                 }
+                operands(v, A);
 #pragma unroll
                 for (int b = 0; b < PAIRS; ++b) {
                     if (!all.value && !(some >> b & 1)) continue;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const unsigned char *s = sh + (k + q) * Q::S_PITCH + (b * 16 + 4 * (g >> 1) + 2 * h + (g & 1)) * 4;
+                        const float w[2] = {*(const float *)s, *(const float *)(s + 4 * Q::S_PITCH)};
                         Operand<true> B[2];
-                        B[0].of(*(const float *)s);
-                        B[1].of(*(const float *)(s + 4 * Q::S_PITCH));
-                        mma8_any(sum[b][h], A, B[0], B[1]);
+                        operands(w, B);
+                        mma8_any(sum[b][h], A, B);
                     }
                 }
             }
@@ -1201,7 +1227,6 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                                            float (&acc)[RT * 2][4])
 {
     using Q = GradShape<RT>;
-    constexpr bool SA = IS_SPLIT<TZ>, SB = true;
     __shared__ unsigned members[GRAD_SCAN];  // which columns of a chunk are the adapter's
     __shared__ unsigned char list[GRAD_SCAN];
     __shared__ int count, seen;
@@ -1290,28 +1315,32 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
             const auto multiply = [&](auto mixed) {
 #pragma unroll
                 for (int k = 0; k < GRAD_CHUNK; k += 8) {
-                    Operand<SA> A[4];
                     const bool in[2] = {!mixed.value || (member >> (k + q) & 1), !mixed.value || (member >> (k + q + 4) & 1)};
+                    Operand<IS_SPLIT<TZ>> A[4];
+                    TZ u[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const TZ v = *(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ));
-                        A[e].of(in[e >> 1] ? v : from_float<TZ>(0.0f));
+                        u[e] = *(const TZ *)(z + (g + (e & 1) * 8) * Q::PITCH + (k + q + (e >> 1) * 4) * sizeof(TZ));
+                        if (!in[e >> 1]) u[e] = from_float<TZ>(0.0f);
                     }
+                    operands(u, A);
 #pragma unroll
                     for (int b = 0; b < RT * 2; ++b) {
-                        Operand<SB> B[2];
+                        Operand<true> B[2];
+                        float v[2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float v = *(const float *)(s + (b * 8 + g) * Q::PITCH + (k + q + e * 4) * 4);
-                            B[e].of(in[e] ? v : 0.0f);
+                            v[e] = *(const float *)(s + (b * 8 + g) * Q::PITCH + (k + q + e * 4) * 4);
+                            if (!in[e]) v[e] = 0.0f;
                         }
+                        operands(v, B);
                         if constexpr (sizeof(TF) == 4) {  // long sums are kept outside the tensor cores, which cut them
                             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma8_any(part, A, B[0], B[1]);
+                            mma8_any(part, A, B);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) acc[b][e] += part[e];
                         } else {
-                            mma8_any(acc[b], A, B[0], B[1]);
+                            mma8_any(acc[b], A, B);
                         }
                     }
                 }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import spmm_b200 as T
-from test_dense_ops import BF16, F16, F32
+from test_dense_ops import BF16, F16, F32, U
 
 
 # ------------------------------------------------------------------ precision
@@ -60,3 +60,17 @@ def test_intermediate_keeps_its_bits_for_16_bit_results(dt, N):
     for hidden in (False, True):
         Y = T.lora(X, D, Up, None, None, torch.zeros(1, N, device="cuda", dtype=dt), hidden=hidden)
         assert float((Y[0] if hidden else Y)[0, 0]) == e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 70])
+def test_fp32_products_are_rounded_to_nearest(N):
+    """fp32 operands in two TF32 parts.  Rounded to nearest a part leaves at most 2^-11, so that the product of both low parts,
+    left out, is at most 2^-22, and each operand is held to 2^-23: a product is off by at most 2^-21 = 8 units of 2^-24.  The
+    one step of 8 products adds three instructions that may cut 2 units each; the second product (up = 1: only S's own 2
+    units) three more: 22 units.  Parts cut toward zero lose 28 of each product here."""
+    x = 1 + 2.0 ** -10 - 2.0 ** -23
+    X, D, Up = torch.full((8, N), x).cuda(), torch.full((1, 1, 8), x).cuda(), torch.ones(1, 1, 1).cuda()
+    Y = T.lora(X, D, Up, hidden=True)[0].double().cpu()
+    ref = 8 * x * x
+    assert float((Y - ref).abs().max()) <= 22 * U * ref
