@@ -858,7 +858,10 @@ __global__ void __launch_bounds__(THREADS, RT <= 4 ? 2 : 1) lora_expand(const Ap
                         const float w[2] = {*(const float *)s, *(const float *)(s + 4 * Q::S_PITCH)};
                         Operand<true> B[2];
                         operands(w, B);
-                        mma8_any(sum[b][h], A, B);
+                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the tensor cores cut their sums: kept outside
+                        mma8_any(part, A, B);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum[b][h][e] += part[e];
                     }
                 }
             }

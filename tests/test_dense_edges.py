@@ -74,3 +74,24 @@ def test_fp32_products_are_rounded_to_nearest(N):
     Y = T.lora(X, D, Up, hidden=True)[0].double().cpu()
     ref = 8 * x * x
     assert float((Y - ref).abs().max()) <= 22 * U * ref
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("trans", [False, True])
+def test_fp32_sums_over_the_rank_are_kept_outside_the_tensor_cores(trans):
+    """2^24, then 31 steps that add 1.5 each: every addition rounded to nearest is off by at most half a step, 1, so the sum by
+    31 at most; sums cut at every step never move from 2^24 and are 46.5 off."""
+    R, N = 256, 5
+    row = torch.zeros(R)
+    row[8::8] = 1.5
+    row[0] = 2.0 ** 24
+    ones = torch.ones(R)
+    if trans:  # dX = down^T P, P = up^T dY = 1
+        D, Up = row.reshape(1, R, 1).cuda(), ones.reshape(1, 1, R).cuda()
+        X, G = torch.zeros(1, N).cuda(), torch.ones(1, N).cuda()
+        H = T.lora(X, D, Up, hidden=True)[1]
+        got = T.lora_backward(G, X, D, Up, H)[0]
+    else:
+        D, Up = ones.reshape(1, R, 1).cuda(), row.reshape(1, 1, R).cuda()
+        got = T.lora(torch.ones(1, N).cuda(), D, Up, hidden=True)[0]
+    assert float((got.double().cpu() - (2.0 ** 24 + 46.5)).abs().max()) <= 31
