@@ -174,25 +174,47 @@ __device__ __forceinline__ void mma8(float (&d)[4], const unsigned (&a)[4], unsi
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x as a sum of PARTS values of type T, each the nearest to what the ones before leave: 24 bits of x in three bf16 parts, 22 in
-// two fp16 ones.  Kept below the type's largest value, the first ones are finite, and an infinity or NaN comes back whole from
-// the last.
+// A 16-bit element of type code 1 (fp16) or 2 (bf16).
+__device__ __forceinline__ float as_float(unsigned bits, int type)
+{
+    return type == 1 ? __half2float(__ushort_as_half((unsigned short)bits)) : __bfloat162float(__ushort_as_bfloat16((unsigned short)bits));
+}
+
+// x as a sum of PARTS values of type T: all 24 bits of it in three bf16 parts, 22 in two fp16 ones.  The parts have x's sign and
+// none is zero unless x is (a first part that would leave nothing gives up its last bit), so that an infinite factor times each
+// of them is what it is times x.  An infinity or NaN is the last part, behind ones.
 template <typename T> constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
 template <typename T>
 __device__ __forceinline__ void split16(float x, T (&part)[PARTS<T>])
 {
-    constexpr float MOST = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
+    const bool finite = fabsf(x) <= 3.4028234663852886e38f;
 #pragma unroll
-    for (int i = 0; i < PARTS<T>; ++i) {
-        part[i] = from_float<T>(i + 1 < PARTS<T> ? fminf(fmaxf(x, -MOST), MOST) : x);
-        x -= to_float(part[i]);
+    for (int i = 0; i + 1 < PARTS<T>; ++i) {
+        unsigned short bits;
+        if constexpr (std::is_same<T, __half>::value)
+            bits = __half_as_ushort(__float2half_rz(x));
+        else
+            bits = (unsigned short)(__float_as_uint(x) >> 16);
+        const auto value = [&] { return as_float(bits, std::is_same<T, __half>::value ? 1 : 2); };
+        if (!finite)
+            bits = (unsigned short)((__float_as_uint(x) >> 16 & 0x8000u) | (std::is_same<T, __half>::value ? 0x3c00u : 0x3f80u));
+        else if (value() == x && (bits & 0x7fffu))
+            --bits;
+        memcpy(&part[i], &bits, 2);
+        if (finite) x -= value();
     }
+    part[PARTS<T> - 1] = from_float<T>(x);
 }
 
 // Operands of a product as TF32 (10 bits after the point; the instruction ignores the bits behind them).  16-bit values are exact
-// in it.  An fp32 x is split in two, x = v + lo up to 2^-23 |x|, each to the nearest: lo is at most 2^-11 |x|, of either sign, so
-// that what is left out averages out: of two split operands the product of both low parts, 2^-22.  A product is off by at most
-// 2^-21.  (Parts cut toward zero, 2^-10 and 2^-21, had three times the plain fp32 sums' error.)
+// in it; an fp32 x is split in two, x = v + lo, both in integer additions (the conversion instruction took lora_grad's product with
+// both operands split from 37 to 60 us).  A product is off by at most 2^-21.
+//  - Beside another split one v and lo are rounded to nearest, up to 2^-23 |x|: lo is at most 2^-11 |x|, of either sign, so that
+//    what is left out, the product of both low parts, 2^-22, averages out.  (Parts cut toward zero, 2^-10 and 2^-21, had three
+//    times the plain fp32 sums' error.)  An infinity or NaN is lo beside a one of its sign: lo times the other's v is what x is
+//    times the other, and the one times the other's parts is finite or the same infinity.
+//  - Beside a whole one v is the next value below |x|, cut, so that lo has x's sign and is zero only where x is (up to 2^-22 |x|):
+//    an infinite whole operand times each part is what it is times x.  An infinity is v beside the largest finite lo, a NaN is v.
 template <bool SPLIT> struct Operand;
 template <> struct Operand<false> {
     unsigned v;
@@ -202,32 +224,30 @@ template <> struct Operand<true> {
 };
 template <typename T> constexpr bool IS_SPLIT = sizeof(T) == 4;
 
-template <typename T, int COUNT>
+template <bool BOTH = true, typename T, int COUNT>  // BOTH: the other operand is split too
 __device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T>> (&o)[COUNT])
 {
-    if constexpr (!IS_SPLIT<T>) {
+    constexpr float MOST = 3.4028234663852886e38f;
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) o[i].v = __float_as_uint(to_float(x[i]));
-    } else {
-        // What would round to infinity, infinities and NaN: one branch for all of them (integer additions instead of the
-        // conversion instruction, which is several times slower: 36 and 60 us for one of lora_grad's products).
-        bool usual = true;
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i) usual = usual && fabsf(x[i]) < 3.402e38f;
-        if (usual) {
-#pragma unroll
-            for (int i = 0; i < COUNT; ++i) {
-                o[i].v = (__float_as_uint(x[i]) + 0x1000u) & 0xffffe000u;
-                o[i].lo = __float_as_uint(x[i] - __uint_as_float(o[i].v)) + 0x1000u;
+    for (int i = 0; i < COUNT; ++i) {
+        if constexpr (!IS_SPLIT<T>) {
+            o[i].v = __float_as_uint(to_float(x[i]));
+        } else if constexpr (BOTH) {
+            const unsigned b = __float_as_uint(x[i]);
+            unsigned v = b;
+            if (fabsf(x[i]) < 3.402e38f) v += 0x1000u;  // beyond: cut, it would round to infinity
+            v &= 0xffffe000u;
+            unsigned lo = __float_as_uint(x[i] - __uint_as_float(v)) + 0x1000u;
+            if (!(fabsf(x[i]) <= MOST)) {
+                v = (b & 0x80000000u) | 0x3f800000u;
+                lo = __float_as_uint(x[i] + x[i]);  // a NaN's payload may lie in the bits that are ignored
             }
+            o[i].v = v;
+            o[i].lo = lo;
         } else {
-#pragma unroll
-            for (int i = 0; i < COUNT; ++i) {
-                const bool finite = fabsf(x[i]) <= 3.4028234663852886e38f;
-                const unsigned b = __float_as_uint(x[i]);
-                o[i].v = !finite ? __float_as_uint(x[i] + x[i]) : (fabsf(x[i]) < 3.402e38f ? b + 0x1000u : b) & 0xffffe000u;
-                o[i].lo = finite ? __float_as_uint(x[i] - __uint_as_float(o[i].v)) + 0x1000u : 0u;
-            }
+            o[i].v = __float_as_uint(x[i] * 0.99999994f) & 0xffffe000u;  // times 1 - 2^-24: the next of fp32 below |x|
+            const float left = fminf(fabsf(x[i] - __uint_as_float(o[i].v)), MOST);  // infinity - infinity becomes finite
+            o[i].lo = ((__float_as_uint(x[i]) & 0x80000000u) | __float_as_uint(left)) + 0x1000u;
         }
     }
 }
@@ -242,12 +262,6 @@ __device__ __forceinline__ void mma8_any(float (&d)[4], const Operand<SA> (&a)[4
     }
     mma8(d, hi, b[0].lo, b[1].lo);
     mma8(d, hi, b[0].v, b[1].v);
-}
-
-// A 16-bit element of type code 1 (fp16) or 2 (bf16).
-__device__ __forceinline__ float as_float(unsigned bits, int type)
-{
-    return type == 1 ? __half2float(__ushort_as_half((unsigned short)bits)) : __bfloat162float(__ushort_as_bfloat16((unsigned short)bits));
 }
 
 template <typename T>
@@ -574,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
                             TI v[2];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) v[e] = *(const TI *)(in + (k + q + e * 4) * Q::IN_PITCH + (b * 8 + g) * sizeof(TI));
-                            operands(v, B8);
+                            operands<IS_SPLIT<TF>>(v, B8);
                             have = b;
                         }
                         mma8_any(to, A[m], B8);
@@ -1336,7 +1350,7 @@ __device__ __forceinline__ void grad_block(const GradProblem &p, const GradParam
                             v[e] = *(const float *)(s + (b * 8 + g) * Q::PITCH + (k + q + e * 4) * 4);
                             if (!in[e]) v[e] = 0.0f;
                         }
-                        operands(v, B);
+                        operands<IS_SPLIT<TZ>>(v, B);
                         if constexpr (sizeof(TF) == 4) {  // long sums are kept outside the tensor cores, which cut them
                             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             mma8_any(part, A, B);

@@ -95,3 +95,67 @@ def test_fp32_sums_over_the_rank_are_kept_outside_the_tensor_cores(trans):
         D, Up = ones.reshape(1, R, 1).cuda(), row.reshape(1, 1, R).cuda()
         got = T.lora(torch.ones(1, N).cuda(), D, Up, hidden=True)[0]
     assert float((got.double().cpu() - (2.0 ** 24 + 46.5)).abs().max()) <= 31
+
+
+# ------------------------------------------------------------------ infinities
+def _same(got, ref, size):
+    """Infinities by sign, NaN, and finite values within 2^-15 of the sum of their terms' magnitudes (two products in turn of at
+    most 20 terms: 2 U (20 / 4 + 64) < 2^-16 each) and half a step of a 16-bit result."""
+    step = torch.finfo(got.dtype).eps / 2
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), ref.isnan()), (got, ref)
+    inf = ref.isinf()
+    assert torch.equal(got.isinf(), inf) and torch.equal(got[inf], ref[inf]), (got, ref)
+    fin = ref.isfinite()
+    assert bool(((got - ref).abs() <= 2.0 ** -15 * size + step * ref.abs())[fin].all())
+
+
+def _product(a, b, own):
+    """(a @ b over the columns `own`, the same of magnitudes), IEEE rules for infinities."""
+    a, b = a[:, own], b[own]
+    terms = a[:, :, None] * b[None]
+    return terms.sum(1), torch.where(terms.isfinite(), terms.abs(), 0.0).sum(1)
+
+
+INF = float("inf")
+PLACES = [("X", (4, 3), INF), ("X", (0, 3), -INF), ("down", (1, 2, 3), INF), ("up", (2, 5, 0), -INF), ("up", (0, 1, 2), INF),
+          ("dY", (5, 3), INF), ("dY", (2, 2), -INF)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("N", [6, 80])
+@pytest.mark.parametrize("name,place,value", PLACES)
+@pytest.mark.parametrize("g16", [False, True])
+def test_infinities_are_those_of_the_formula(dt, N, name, place, value, g16):
+    """One infinity among values that 16 bits and TF32 hold exactly (so that low parts are nothing): every result is the
+    infinity, NaN or finite value of the formula, whichever kernel computes it."""
+    M, K, R, L = 12, 10, 3, 4
+    g = torch.Generator().manual_seed(5)
+    pick = lambda *s: torch.tensor([0.5, 1.0, 2.0, 1.0, 4.0])[torch.randint(0, 5, s, generator=g)]  # noqa: E731
+    t = {"X": pick(K, N), "down": pick(L, R, K), "up": pick(L, M, R), "dY": pick(M, N)}
+    t["up"][:, 7] *= -1
+    t["down"][:, :, 6] *= -1
+    t[name][place] = value
+    index = (torch.arange(N) % L).int()
+    dev = {k: v.to(F32 if k == "dY" and not g16 else dt).cuda() for k, v in t.items()}
+    X, down, up, dY = (t[k].double() for k in ("X", "down", "up", "dY"))
+    Y, dX = torch.zeros(M, N).double(), torch.zeros(K, N).double()
+    sY, sX, dD, dU = Y.clone(), dX.clone(), torch.zeros_like(down), torch.zeros_like(up)
+    sD, sU = dD.clone(), dU.clone()
+    for a in range(L):
+        at = (index == a).nonzero().flatten()
+        h, hs = _product(down[a], X[:, at], slice(None))
+        p, ps = _product(up[a].T, dY[:, at], slice(None))
+        Y[:, at] = _product(up[a], h, slice(None))[0]
+        sY[:, at] = _product(up[a].abs(), hs, slice(None))[1]
+        dX[:, at] = _product(down[a].T, p, slice(None))[0]
+        sX[:, at] = _product(down[a].T.abs(), ps, slice(None))[1]
+        dD[a], dU[a] = _product(p, X[:, at].T, slice(None))[0], _product(dY[:, at], h.T, slice(None))[0]
+        sD[a], sU[a] = _product(ps, X[:, at].T.abs(), slice(None))[1], _product(dY[:, at].abs(), hs.T, slice(None))[1]
+    args = (dev["X"], dev["down"], dev["up"], index.cuda())
+    _same(T.lora(*args), Y, sY)
+    got, H = T.lora(*args, hidden=True)
+    _same(got, Y, sY)
+    for got, ref, size in zip(T.lora_backward(dev["dY"], *args[:3], H, args[3]), (dX, dD, dU), (sX, sD, sU)):
+        _same(got, ref, size)
