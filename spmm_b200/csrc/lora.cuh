@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cstring>
 #include <type_traits>
@@ -187,7 +188,7 @@ template <typename T> constexpr int PARTS = std::is_same<T, __half>::value ? 2 :
 template <typename T>
 __device__ __forceinline__ void split16(float x, T (&part)[PARTS<T>])
 {
-    const bool finite = fabsf(x) <= 3.4028234663852886e38f;
+    const bool finite = fabsf(x) <= FLT_MAX;
 #pragma unroll
     for (int i = 0; i + 1 < PARTS<T>; ++i) {
         unsigned short bits;
@@ -227,7 +228,6 @@ template <typename T> constexpr bool IS_SPLIT = sizeof(T) == 4;
 template <bool BOTH = true, typename T, int COUNT>  // BOTH: the other operand is split too
 __device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T>> (&o)[COUNT])
 {
-    constexpr float MOST = 3.4028234663852886e38f;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
         if constexpr (!IS_SPLIT<T>) {
@@ -238,7 +238,7 @@ __device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T
             if (fabsf(x[i]) < 3.402e38f) v += 0x1000u;  // beyond: cut, it would round to infinity
             v &= 0xffffe000u;
             unsigned lo = __float_as_uint(x[i] - __uint_as_float(v)) + 0x1000u;
-            if (!(fabsf(x[i]) <= MOST)) {
+            if (!(fabsf(x[i]) <= FLT_MAX)) {
                 v = (b & 0x80000000u) | 0x3f800000u;
                 lo = __float_as_uint(x[i] + x[i]);  // a NaN's payload may lie in the bits that are ignored
             }
@@ -246,7 +246,7 @@ __device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T
             o[i].lo = lo;
         } else {
             o[i].v = __float_as_uint(x[i] * 0.99999994f) & 0xffffe000u;  // times 1 - 2^-24: the next of fp32 below |x|
-            const float left = fminf(fabsf(x[i] - __uint_as_float(o[i].v)), MOST);  // infinity - infinity becomes finite
+            const float left = fminf(fabsf(x[i] - __uint_as_float(o[i].v)), FLT_MAX);  // infinity - infinity becomes finite
             o[i].lo = ((__float_as_uint(x[i]) & 0x80000000u) | __float_as_uint(left)) + 0x1000u;
         }
     }
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
         if (keep) h.s()[r * h.pitch + t0 + c] = v;
         if (HALF) {
             slot[SLOT + r * PITCH + c] = v;
-            most = fmaxf(most, fabsf(v));
+            if (fabsf(v) <= FLT_MAX) most = fmaxf(most, fabsf(v));
         } else if (sizeof(TF) == 2 && keep) {
             TF part[PARTS<TF>];
             split16<TF>(v, part);
@@ -671,9 +671,9 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
     if (HALF) {
         atomicMax(&colmax[c], __float_as_int(most));  // the order does not matter
         __syncthreads();
-        // The column's largest value goes to [2^13, 2^14); zeros and infinities stay.
+        // The column's largest finite value goes to [2^13, 2^14), whatever stands beside it; zeros stay.
         const int e = (colmax[c] >> 23) - 127;
-        const int shift = e == -127 || e == 128 ? 0 : max(-100, min(100, e - 13));
+        const int shift = e == -127 ? 0 : max(-126, e - 13);
         const float down = __int_as_float((127 - shift) << 23);
         if (keep) {
             for (int r = r_first; r < p.R; r += r_step) {

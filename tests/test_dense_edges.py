@@ -159,3 +159,19 @@ def test_infinities_are_those_of_the_formula(dt, N, name, place, value, g16):
     _same(got, Y, sY)
     for got, ref, size in zip(T.lora_backward(dev["dY"], *args[:3], H, args[3]), (dX, dD, dU), (sX, sD, sU)):
         _same(got, ref, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [False, True])
+def test_fp16_intermediate_beside_an_infinity_and_at_the_end_of_the_range(hidden):
+    """H's parts are scaled by the column's largest finite value: a finite value past fp16's range beside an infinity stays
+    finite, and so does one near the end of fp32's range."""
+    def lora(*a):
+        return T.lora(*a, hidden=True)[0] if hidden else T.lora(*a)
+
+    down = torch.tensor([[[INF, 0.0], [0.0, 8.0]]]).half().cuda()  # h = (inf, 480000)
+    up, X = torch.tensor([[[1.0, -1.0]]]).half().cuda(), torch.tensor([[1.0], [60000.0]]).half().cuda()
+    assert float(lora(X, down, up)) == INF
+    one = torch.ones(1, 1, 1).half().cuda()
+    for e in (118, 127):
+        assert float(lora(torch.ones(1, 1).half().cuda(), one, one, None, torch.tensor([2.0 ** e]).cuda())) == 2.0 ** e
