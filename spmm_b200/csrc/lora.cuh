@@ -331,12 +331,12 @@ constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 
 // Of a tile's columns: their adapters (-1: none, or past the end), and those that occur, by their first columns; for each of
-// those, where there are several, which blocks of 8 columns hold any of its columns, and which others' beside them.
+// those, where there are several, which blocks of 8 columns hold any of its columns.
 template <int TN>
 struct TileColumns {
     __align__(16) int ids[TN];
     int list[TN], count;
-    unsigned char some[TN], mixed[TN];  // TN / 8 bits each
+    unsigned char some[TN];  // TN / 8 bits
     // `meanwhile` runs while the indices are on their way.
     template <typename F>
     __device__ __forceinline__ void load(const Columns &c, long long t0, long long N, F &&meanwhile)
@@ -363,13 +363,9 @@ struct TileColumns {
         if (count > 1) {
             for (int d = threadIdx.x; d < count; d += THREADS) {
                 const int a = list[d];
-                unsigned has = 0u, other = 0u;
-                for (int t = 0; t < TN; ++t) {
-                    has |= (unsigned)(ids[t] == a) << (t >> 3);
-                    other |= (unsigned)(ids[t] != a && ids[t] >= 0) << (t >> 3);
-                }
+                unsigned has = 0u;
+                for (int t = 0; t < TN; ++t) has |= (unsigned)(ids[t] == a) << (t >> 3);
                 some[d] = (unsigned char)has;
-                mixed[d] = (unsigned char)other;
             }
             __syncthreads();
         }
@@ -515,10 +511,10 @@ __global__ void __launch_bounds__(THREADS, RT * TN <= 128 ? 2 : 1) lora_shrink(c
             const int a = list[d], this_d = d;
             const bool first = d == 0;
             if (++d == nd) d = 0;
-            const unsigned some = nd > 1 ? tile.some[this_d] : ~0u, mixed = nd > 1 ? tile.mixed[this_d] : 0u;
-            // acc += part, or in a mixed block only for adapter a's columns.
+            const unsigned some = nd > 1 ? tile.some[this_d] : ~0u;
+            // acc += part; with several adapters, only in the blocks with any of adapter a's columns, and only for these.
             auto add = [&](auto &&product) {
-                if (some == ~0u && !mixed) {
+                if (nd == 1) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
