@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import spmm_b200 as T
-from test_dense_ops import BF16, F16, F32, U
+from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref
 
 
 # ------------------------------------------------------------------ precision
@@ -175,3 +175,15 @@ def test_fp16_intermediate_beside_an_infinity_and_at_the_end_of_the_range(hidden
     one = torch.ones(1, 1, 1).half().cuda()
     for e in (118, 127):
         assert float(lora(torch.ones(1, 1).half().cuda(), one, one, None, torch.tensor([2.0 ** e]).cuda())) == 2.0 ** e
+
+
+# ------------------------------------------------------------------ which kernels
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,R,L", [(96, 72, 64, 16, 64), (130, 96, 200, 8, 40), (61, 35, 256, 5, 16), (40, 50, 65, 3, 33)])
+@pytest.mark.parametrize("dt,ydt", [(F32, F32), (F16, F32), (BF16, F32), (BF16, BF16), (F16, F16), (F32, F16)])
+def test_lora_many_adapters(M, K, N, R, L, dt, ydt):
+    """Up to 64 adapters among a tile's columns, and up to 256 columns one by one."""
+    X, down, up, index, scale, base = lora_inputs(M, K, N, R, L, dt, ydt, "each", seed=N)
+    y, tol, _ = lora_ref(X, down, up, index, scale, base, ydt)
+    close(T.lora(X, down, up, index, scale, base), y, tol)
+    close(T.lora(X, down, up, index, scale, base, hidden=True)[0], y, tol)
