@@ -67,6 +67,13 @@ Tensor given(const MaybeTensor &t) { return t.has_value() && t->defined() ? *t :
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 
+// The operators have no forward-mode derivatives; a tangent would be dropped without a word.
+void refuse_tangents(const char *name, std::initializer_list<Tensor> inputs)
+{
+    for (const Tensor &t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name, " has no forward-mode derivatives");
+}
+
 template <typename F>
 auto op(const char *name)
 {
@@ -214,6 +221,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 
 Tensor layer_norm_autograd(const Tensor &X, const MaybeTensor &weight, const MaybeTensor &bias, double eps, int64_t dim, ScalarType out)
 {
+    refuse_tangents("layer_norm", {X, given(weight), given(bias)});
     if (at::GradMode::is_enabled() && (wants_grad(X) || wants_grad(given(weight)) || wants_grad(given(bias))))
         return NormFunction::apply(X, weight, bias, eps, dim, out);
     static const auto run = op<NormOp>("tcaspmm::layer_norm");
@@ -427,6 +435,7 @@ struct LoraFunction : torch::autograd::Function<LoraFunction> {
 Tensor lora_autograd(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
                      const MaybeTensor &base)
 {
+    refuse_tangents("lora", {X, down, up, given(scale), given(base)});
     const bool grad = at::GradMode::is_enabled();
     TORCH_CHECK_VALUE(!grad || !wants_grad(given(scale)), "the adapters' scale is a constant: it has no gradient");
     if (grad && (wants_grad(X) || wants_grad(down) || wants_grad(up) || wants_grad(given(base))))

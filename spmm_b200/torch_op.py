@@ -212,11 +212,18 @@ layer_norm = dense.layer_norm
 lora = dense.lora
 
 
+def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """spmm_lora has no forward mode: a tangent would be dropped without a word."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("spmm_lora has no forward-mode derivatives")
+
+
 @torch.library.custom_op("tcaspmm::spmm_lora", mutates_args=())
 def _spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torch.Tensor, down: torch.Tensor,
                up: torch.Tensor, index: Optional[torch.Tensor],
                scale: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
     """(A @ X with each column's adapter beside it, the adapters' H): the plan's product, then the adapters in place."""
+    _refuse_tangents(X, down, up, scale)
     M = crow.shape[0] - 1
     if tuple(up.shape[1:2]) != (M,):
         raise ValueError(f"up must have shape (L, {M}, R), not {tuple(up.shape)}")
@@ -261,7 +268,8 @@ _spmm_lora.register_autograd(_backward_spmm_lora, setup_context=_setup_spmm_lora
 def spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torch.Tensor, down: torch.Tensor,
               up: torch.Tensor, index: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A @ X + each column's low-rank adapter, fp32: a frozen pruned weight with the adapters that train (or serve)
-    beside it.  Gradients for X, down and up."""
+    beside it.  Gradients for X, down and up; no forward mode."""
+    _refuse_tangents(X, down, up, scale)
     return torch.ops.tcaspmm.spmm_lora(crow, col, val, X, down, up, index, scale)[0]
 
 

@@ -4,8 +4,11 @@ Values are chosen so that the formula's result is known exactly, or the bound st
 """
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 
 import spmm_b200 as T
+from spmm_b200 import torch_op
 from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref
 
 
@@ -187,3 +190,32 @@ def test_lora_many_adapters(M, K, N, R, L, dt, ydt):
     y, tol, _ = lora_ref(X, down, up, index, scale, base, ydt)
     close(T.lora(X, down, up, index, scale, base), y, tol)
     close(T.lora(X, down, up, index, scale, base, hidden=True)[0], y, tol)
+
+
+# ------------------------------------------------------------------ autograd
+def _fake_args():
+    """X, weight, bias of a norm; X, down, up, index, scale, base of adapters: CUDA tensors without data."""
+    z = lambda *s, **k: torch.zeros(*s, device="cuda", **k)  # noqa: E731
+    return (z(6, 5), z(5), z(5)), (z(6, 5), z(2, 3, 6), z(2, 4, 3), z(5, dtype=torch.int32), z(2), z(4, 5))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """A tangent would be dropped without a word: whichever input has one, the call raises."""
+    with FakeTensorMode(), torch.set_grad_enabled(grad):
+        norm, lora = _fake_args()
+        csr = [torch.zeros(5, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), torch.zeros(0)]
+        for f, args, which in [(torch_op.layer_norm, norm, (0, 1, 2)), (torch_op.lora, lora, (0, 1, 2, 4, 5)),
+                               (lambda *a: T.layer_norm(*a, stats=True), norm, (0, 1)),
+                               (lambda *a: T.lora(*a, hidden=True), lora, (0, 2)),
+                               (lambda *a: T.lora(*a, out=a[5].clone()), lora, (0, 1, 2, 5)),
+                               (lambda *a: torch_op.spmm_lora(*csr, *a[:5]), lora, (0, 1, 2))]:
+            f(*args)
+            for k in which:
+                with forward_ad.dual_level():
+                    dual = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+                    with pytest.raises(NotImplementedError, match="forward"):
+                        f(*args[:k], dual, *args[k + 1:])
+        for f, args in ((torch_op.layer_norm, norm), (torch_op.lora, lora), (lambda *a: torch_op.spmm_lora(*csr, *a[:5]), lora)):
+            with pytest.raises(NotImplementedError, match="forward"):
+                torch.func.jvp(lambda x: f(x, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
