@@ -394,6 +394,8 @@ std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor 
 using LoraOp = Tensor(const Tensor &, const Tensor &, const Tensor &, const MaybeTensor &, const MaybeTensor &, const MaybeTensor &);
 using LoraHiddenOp = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const MaybeTensor &,
                                                 const MaybeTensor &, const MaybeTensor &);
+using LoraIntoOp = Tensor(const Tensor &, const Tensor &, const Tensor &, const MaybeTensor &, const MaybeTensor &, const MaybeTensor &,
+                          const Tensor &);
 using LoraGradOp = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                                                       const MaybeTensor &, const MaybeTensor &, const MaybeTensor &, bool, bool, bool);
 
@@ -431,6 +433,26 @@ struct LoraFunction : torch::autograd::Function<LoraFunction> {
         return out;
     }
 };
+
+// `out` gets a new version, so that autograd sees what it saved change.
+Tensor lora_into_versioned(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
+                           const MaybeTensor &base, const Tensor &out)
+{
+    static const auto run = op<LoraIntoOp>("tcaspmm::lora_into");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor H = run.call(X, down, up, index, scale, base, out);
+    if (!out.is_inference()) torch::autograd::impl::bump_version(out);
+    return H;
+}
+
+Tensor lora_into_autograd(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
+                          const MaybeTensor &base, const Tensor &out)
+{
+    refuse_tangents("lora", {X, down, up, given(scale), given(base), out});
+    static const auto run = op<LoraIntoOp>("tcaspmm::lora_into");
+    const at::AutoDispatchBelowAutograd below;
+    return run.call(X, down, up, index, scale, base, out);
+}
 
 Tensor lora_autograd(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
                      const MaybeTensor &base)
@@ -485,5 +507,10 @@ TORCH_LIBRARY_IMPL(tcaspmm, Autograd, m)
     m.impl("layer_norm_backward", torch::autograd::autogradNotImplementedFallback());
     m.impl("lora_hidden", torch::autograd::autogradNotImplementedFallback());
     m.impl("lora_backward", torch::autograd::autogradNotImplementedFallback());
-    m.impl("lora_into", torch::autograd::autogradNotImplementedFallback());
+    m.impl("lora_into", lora_into_autograd);
+}
+
+TORCH_LIBRARY_IMPL(tcaspmm, ADInplaceOrView, m)
+{
+    m.impl("lora_into", lora_into_versioned);
 }

@@ -219,3 +219,26 @@ def test_forward_mode_is_refused(grad):
         for f, args in ((torch_op.layer_norm, norm), (torch_op.lora, lora), (lambda *a: torch_op.spmm_lora(*csr, *a[:5]), lora)):
             with pytest.raises(NotImplementedError, match="forward"):
                 torch.func.jvp(lambda x: f(x, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
+
+
+def test_out_is_seen_to_change():
+    """A tensor written through out= gets a new version."""
+    with FakeTensorMode():
+        _, (X, down, up, index, scale, base) = _fake_args()
+        C = base.clone()
+        for k, hidden in enumerate((False, True, False)):
+            assert C._version == k
+            T.lora(X, down, up, index, scale, C, out=C, hidden=hidden)
+        assert C._version == 3
+        T.lora(X, down, up, index, scale, base, out=C)
+        assert C._version == 4 and base._version == 0
+
+
+@pytest.mark.gpu
+def test_backward_refuses_what_out_overwrote():
+    X, down, up, index, scale, base = lora_inputs(20, 12, 16, 4, 2, F32)
+    C = base.requires_grad_(True).exp()  # its backward pass reads C
+    with torch.no_grad():
+        T.lora(X, down, up, index, scale, C, out=C)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        C.sum().backward()
