@@ -449,6 +449,9 @@ Tensor lora_into_autograd(const Tensor &X, const Tensor &down, const Tensor &up,
                           const MaybeTensor &base, const Tensor &out)
 {
     refuse_tangents("lora", {X, down, up, given(scale), given(base), out});
+    for (const Tensor &t : {X, down, up, given(scale), given(base), out})  // as torch's own out= forms
+        TORCH_CHECK(!at::GradMode::is_enabled() || !wants_grad(t),
+                    "lora with out does not support automatic differentiation, but one of the arguments requires grad");
     static const auto run = op<LoraIntoOp>("tcaspmm::lora_into");
     const at::AutoDispatchBelowAutograd below;
     return run.call(X, down, up, index, scale, base, out);
@@ -502,7 +505,7 @@ TORCH_LIBRARY_IMPL(tcaspmm, Autograd, m)
 {
     m.impl("layer_norm", layer_norm_autograd);
     m.impl("lora", lora_autograd);
-    // The parts have no derivatives of their own: differentiating through one raises.
+    // The parts have no derivatives of their own: differentiating through one raises, and out= is refused at once.
     m.impl("layer_norm_stats", torch::autograd::autogradNotImplementedFallback());
     m.impl("layer_norm_backward", torch::autograd::autogradNotImplementedFallback());
     m.impl("lora_hidden", torch::autograd::autogradNotImplementedFallback());

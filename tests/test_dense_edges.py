@@ -242,3 +242,17 @@ def test_backward_refuses_what_out_overwrote():
         T.lora(X, down, up, index, scale, C, out=C)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         C.sum().backward()
+
+
+def test_out_has_no_gradients():
+    """As torch's own out= forms: an argument that requires a gradient is refused in grad mode."""
+    with FakeTensorMode():
+        _, args = _fake_args()
+        for hidden in (False, True):
+            for k in (0, 1, 2, 4, 5, 6):
+                a = [t.clone() for t in (*args, args[5])]
+                a[k].requires_grad_(True)
+                with pytest.raises(RuntimeError, match="requires grad"):
+                    T.lora(*a[:6], out=a[6], hidden=hidden)
+                with torch.no_grad():
+                    T.lora(*a[:6], out=a[6], hidden=hidden)
