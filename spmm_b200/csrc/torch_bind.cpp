@@ -346,13 +346,13 @@ std::tuple<Tensor, Tensor> lora_hidden(const Tensor &X, const Tensor &down, cons
     return {Y, H};
 }
 
-// Into `out`, which may be base; returns H.
+// Into `out`, which may be base; returns H, or an empty tensor where it is not kept (few columns then go one by one).
 Tensor lora_into(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
-                 const MaybeTensor &base, const Tensor &out)
+                 const MaybeTensor &base, const Tensor &out, bool keep)
 {
     Tensor H;
-    lora_call(X, down, up, index, scale, base, &out, &H);
-    return H;
+    lora_call(X, down, up, index, scale, base, &out, keep ? &H : nullptr);
+    return keep ? H : at::empty({0}, X.options().dtype(at::kByte));
 }
 
 std::tuple<Tensor, Tensor, Tensor> lora_backward(const Tensor &dy, const Tensor &x, const Tensor &down, const Tensor &up, const Tensor &H,
@@ -395,7 +395,7 @@ using LoraOp = Tensor(const Tensor &, const Tensor &, const Tensor &, const Mayb
 using LoraHiddenOp = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const MaybeTensor &,
                                                 const MaybeTensor &, const MaybeTensor &);
 using LoraIntoOp = Tensor(const Tensor &, const Tensor &, const Tensor &, const MaybeTensor &, const MaybeTensor &, const MaybeTensor &,
-                          const Tensor &);
+                          const Tensor &, bool);
 using LoraGradOp = std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                                                       const MaybeTensor &, const MaybeTensor &, const MaybeTensor &, bool, bool, bool);
 
@@ -436,17 +436,17 @@ struct LoraFunction : torch::autograd::Function<LoraFunction> {
 
 // `out` gets a new version, so that autograd sees what it saved change.
 Tensor lora_into_versioned(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
-                           const MaybeTensor &base, const Tensor &out)
+                           const MaybeTensor &base, const Tensor &out, bool keep)
 {
     static const auto run = op<LoraIntoOp>("tcaspmm::lora_into");
     const at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor H = run.call(X, down, up, index, scale, base, out);
+    const Tensor H = run.call(X, down, up, index, scale, base, out, keep);
     if (!out.is_inference()) torch::autograd::impl::bump_version(out);
     return H;
 }
 
 Tensor lora_into_autograd(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
-                          const MaybeTensor &base, const Tensor &out)
+                          const MaybeTensor &base, const Tensor &out, bool keep)
 {
     refuse_tangents("lora", {X, down, up, given(scale), given(base), out});
     for (const Tensor &t : {X, down, up, given(scale), given(base), out})  // as torch's own out= forms
@@ -454,7 +454,7 @@ Tensor lora_into_autograd(const Tensor &X, const Tensor &down, const Tensor &up,
                     "lora with out does not support automatic differentiation, but one of the arguments requires grad");
     static const auto run = op<LoraIntoOp>("tcaspmm::lora_into");
     const at::AutoDispatchBelowAutograd below;
-    return run.call(X, down, up, index, scale, base, out);
+    return run.call(X, down, up, index, scale, base, out, keep);
 }
 
 Tensor lora_autograd(const Tensor &X, const Tensor &down, const Tensor &up, const MaybeTensor &index, const MaybeTensor &scale,
@@ -481,7 +481,8 @@ TORCH_LIBRARY_FRAGMENT(tcaspmm, m)
           "bool need_input, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)");
     m.def("lora(Tensor X, Tensor down, Tensor up, Tensor? index, Tensor? scale, Tensor? base) -> Tensor");
     m.def("lora_hidden(Tensor X, Tensor down, Tensor up, Tensor? index, Tensor? scale, Tensor? base) -> (Tensor, Tensor)");
-    m.def("lora_into(Tensor X, Tensor down, Tensor up, Tensor? index, Tensor? scale, Tensor? base, Tensor(a!) out) -> Tensor");
+    m.def("lora_into(Tensor X, Tensor down, Tensor up, Tensor? index, Tensor? scale, Tensor? base, Tensor(a!) out, "
+          "bool keep=True) -> Tensor");
     m.def("lora_backward(Tensor dY, Tensor X, Tensor down, Tensor up, Tensor H, Tensor? index, Tensor? scale, Tensor? base, "
           "bool need_input, bool need_down, bool need_up) -> (Tensor, Tensor, Tensor)");
 }

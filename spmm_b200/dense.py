@@ -86,8 +86,8 @@ def _register_shapes() -> None:
         return X.new_empty((up.shape[1], X.shape[1]), dtype=torch.float32 if base is None else base.dtype), hidden(X, up)
 
     @fake("tcaspmm::lora_into")
-    def _(X, down, up, index, scale, base, out):
-        return hidden(X, up)
+    def _(X, down, up, index, scale, base, out, keep=True):
+        return hidden(X, up) if keep else X.new_empty(0, dtype=torch.uint8)
 
     @fake("tcaspmm::lora_backward")
     def _(dY, X, down, up, H, index, scale, base, need_input, need_down, need_up):
@@ -130,7 +130,7 @@ def lora(X, down, up, index=None, scale=None, base=None, *, out=None, hidden: bo
     hidden, returns (Y, H) with scale * down @ X as lora_backward takes it (an opaque buffer).  (No autograd with out or
     hidden.)"""
     if out is not None:
-        H = _op("lora_into")(X, down, up, index, scale, base, out)
+        H = _op("lora_into")(X, down, up, index, scale, base, out, hidden)
         return (out, H) if hidden else out
     return _op("lora_hidden" if hidden else "lora")(X, down, up, index, scale, base)
 

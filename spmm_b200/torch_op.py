@@ -220,25 +220,27 @@ def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
 
 @torch.library.custom_op("tcaspmm::spmm_lora", mutates_args=())
 def _spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torch.Tensor, down: torch.Tensor,
-               up: torch.Tensor, index: Optional[torch.Tensor],
-               scale: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(A @ X with each column's adapter beside it, the adapters' H): the plan's product, then the adapters in place."""
+               up: torch.Tensor, index: Optional[torch.Tensor], scale: Optional[torch.Tensor],
+               keep: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(A @ X with each column's adapter beside it, the adapters' H or, without keep, an empty tensor): the plan's product,
+    then the adapters in place."""
     _refuse_tangents(X, down, up, scale)
     M = crow.shape[0] - 1
     if tuple(up.shape[1:2]) != (M,):
         raise ValueError(f"up must have shape (L, {M}, R), not {tuple(up.shape)}")
     Y = spmm(crow, col, val, X)
-    return dense.lora(X, down, up, index, scale, Y, out=Y, hidden=True)
+    H = dense._op("lora_into")(X, down, up, index, scale, Y, Y, keep)
+    return Y, H
 
 
 @_spmm_lora.register_fake
-def _(crow, col, val, X, down, up, index, scale):
-    size = dense.hidden_bytes(up.shape[0], up.shape[2], up.shape[1], X.shape[0], X.shape[1], X.dtype)
+def _(crow, col, val, X, down, up, index, scale, keep=True):
+    size = dense.hidden_bytes(up.shape[0], up.shape[2], up.shape[1], X.shape[0], X.shape[1], X.dtype) if keep else 0
     return X.new_empty((crow.shape[0] - 1, X.shape[1]), dtype=torch.float32), X.new_empty(size, dtype=torch.uint8)
 
 
 def _setup_spmm_lora(ctx, inputs, output):
-    crow, col, val, X, down, up, index, scale = inputs
+    crow, col, val, X, down, up, index, scale, _ = inputs
     ctx.mark_non_differentiable(output[1])
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(crow, col, val, X, down, up, index, scale, output[1])
@@ -248,7 +250,7 @@ def _backward_spmm_lora(ctx, dY, *_):
     if ctx.needs_input_grad[7]:
         raise ValueError("the adapters' scale is a constant: it has no gradient")
     if dY is None:
-        return (None,) * 8
+        return (None,) * 9
     crow, col, val, X = ctx.saved_tensors[:4]
     needed = [bool(n) for n in ctx.needs_input_grad[3:6]]
     base = torch.ops.tcaspmm.spmm_t(crow, col, val, dY.to(X.dtype), X.shape[0]) if needed[0] else None
@@ -259,7 +261,7 @@ def _backward_spmm_lora(ctx, dY, *_):
     if any(needed):
         grads = dense.lora_backward(dY, X, down, up, H, index, scale, base, need_input=needed[0], need_down=needed[1],
                                     need_up=needed[2])
-    return (None, None, None, *grads, None, None)
+    return (None, None, None, *grads, None, None, None)
 
 
 _spmm_lora.register_autograd(_backward_spmm_lora, setup_context=_setup_spmm_lora)
@@ -270,7 +272,8 @@ def spmm_lora(crow: torch.Tensor, col: torch.Tensor, val: torch.Tensor, X: torch
     """A @ X + each column's low-rank adapter, fp32: a frozen pruned weight with the adapters that train (or serve)
     beside it.  Gradients for X, down and up; no forward mode."""
     _refuse_tangents(X, down, up, scale)
-    return torch.ops.tcaspmm.spmm_lora(crow, col, val, X, down, up, index, scale)[0]
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (X, down, up, scale))
+    return torch.ops.tcaspmm.spmm_lora(crow, col, val, X, down, up, index, scale, keep)[0]
 
 
 class LayerNorm(torch.nn.Module):

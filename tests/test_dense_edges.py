@@ -8,7 +8,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
 
 import spmm_b200 as T
-from spmm_b200 import torch_op
+from spmm_b200 import dense, torch_op
 from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref
 
 
@@ -190,6 +190,69 @@ def test_lora_many_adapters(M, K, N, R, L, dt, ydt):
     y, tol, _ = lora_ref(X, down, up, index, scale, base, ydt)
     close(T.lora(X, down, up, index, scale, base), y, tol)
     close(T.lora(X, down, up, index, scale, base, hidden=True)[0], y, tol)
+
+
+def _allocations(f):
+    f()
+    n = [torch.cuda.memory_stats()["allocation.all.allocated"]]
+    f()
+    return torch.cuda.memory_stats()["allocation.all.allocated"] - n[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,ydt", [(F32, F32), (F16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("M,K,N,R,L", [(300, 200, 1, 16, 3), (120, 70, 9, 5, 3), (96, 72, 64, 16, 64), (130, 96, 200, 8, 40),
+                                       (90, 60, 300, 8, 3)])
+def test_out_takes_the_same_kernels_and_keeps_nothing_unasked(M, K, N, R, L, dt, ydt):
+    """A result in place, or in a window, has the bits of a new one; nothing is allocated where few columns go one by one."""
+    X, down, up, index, scale, base = lora_inputs(M, K, N, R, L, dt, ydt, "each", seed=3)
+    want = T.lora(X, down, up, index, scale, base)
+    window = torch.full((M + 2, N + 5), 7.0, device="cuda").to(ydt)
+    view = window[1:-1, 3:3 + N]
+    assert torch.equal(T.lora(X, down, up, index, scale, base, out=view), want)
+    view.fill_(7.0)
+    assert bool((window == 7.0).all())
+    C = base.clone()
+    assert torch.equal(T.lora(X, down, up, index, scale, C, out=C), want)
+    scratch = int(N == 300)  # the tiles' own, given back
+    assert _allocations(lambda: T.lora(X, down, up, index, scale, C, out=C)) == scratch
+    kept = base.clone()
+    assert T.lora(X, down, up, index, scale, kept, out=kept, hidden=True)[1].numel() == dense.hidden_bytes(L, R, M, K, N, dt)
+
+
+@pytest.mark.gpu
+def test_adapted_product_without_gradients_keeps_nothing():
+    """A @ X and its adapters, 64 tokens of 64 adapters: without gradients the bits of the product with lora in place, and no
+    allocation beside the product's own; with gradients the same up to the order of sums, and H."""
+    M, K, N, R, L = 192, 128, 64, 16, 64
+    A = T.gen_uniform(M, K, 0.3, 0)
+    csr = [torch.from_numpy(a) for a in (A.row_ptr, A.col, A.values())]
+    X, down, up, index, scale, _ = lora_inputs(M, K, N, R, L, F16, F32, "each", seed=9)
+    adapters = torch_op.LowRankAdapters(L, R, M, K, device="cuda", dtype=F16)
+    with torch.no_grad():
+        adapters.down.copy_(down)
+        adapters.up.copy_(up)
+    block = torch_op.AdaptedProduct(*csr, adapters)
+    C = torch.ops.tcaspmm.spmm(*csr, X)
+    want = T.lora(X, down, up, index, adapters.scale, C)
+    with torch.no_grad():
+        Y = block(X, index)
+        assert torch.equal(Y, want)
+        n = _allocations(lambda: torch.ops.tcaspmm.spmm(*csr, X))
+        assert _allocations(lambda: block(X, index)) == n
+    for p in adapters.parameters():  # nothing to train: nothing kept in grad mode either
+        p.requires_grad_(False)
+    assert _allocations(lambda: block(X, index)) == n
+    for p in adapters.parameters():
+        p.requires_grad_(True)
+    Z = block(X, index)
+    assert Z.requires_grad and torch.equal(Z, T.lora(X, down, up, index, adapters.scale, C, hidden=True)[0])
+    dY = torch.randn(M, N, generator=torch.Generator().manual_seed(1)).cuda()
+    got = torch.autograd.grad(Z, [adapters.down, adapters.up], dY)
+    H = T.lora(X, down, up, index, adapters.scale, C, hidden=True)[1]
+    for a, b in zip(got, T.lora_backward(dY, X, down, up, H, index, adapters.scale)[1:]):
+        assert torch.equal(a, b)
+    torch_op.clear_plan_cache()
 
 
 # ------------------------------------------------------------------ autograd
