@@ -319,3 +319,17 @@ def test_out_has_no_gradients():
                     T.lora(*a[:6], out=a[6], hidden=hidden)
                 with torch.no_grad():
                     T.lora(*a[:6], out=a[6], hidden=hidden)
+
+
+@pytest.mark.gpu
+def test_registered_autograd():
+    """The operators' registrations for autograd, by torch's own checks."""
+    X, w, b = (t.requires_grad_(True) for t in (torch.randn(12, 16, device="cuda"), torch.ones(16, device="cuda"), torch.ones(16, device="cuda")))
+    ops = torch.ops.tcaspmm
+    check = ("test_schema", "test_autograd_registration", "test_faketensor")
+    torch.library.opcheck(ops.layer_norm.default, (X, w, b, 1e-5, 1, F32), test_utils=check)
+    X, down, up, index, scale, base = lora_inputs(20, 12, 16, 4, 2, F32)
+    leaves = [t.requires_grad_(True) for t in (X, down, up)]
+    torch.library.opcheck(ops.lora.default, (*leaves, index, scale, base), test_utils=check)
+    with torch.no_grad():
+        torch.library.opcheck(ops.lora_into.default, (X.detach(), down.detach(), up.detach(), index, scale, base, base.clone()), test_utils=check)
