@@ -46,7 +46,7 @@ def _op(name: str):
         import torch
 
         if not os.path.exists(TORCH_PATH):
-            raise ImportError(f"{TORCH_PATH} is missing: build it with `make -C spmm_b200/csrc`")
+            raise ImportError(f"{TORCH_PATH} is missing: build it with `make -C spmm_b200/csrc torch`")
         torch.ops.load_library(TORCH_PATH)
         _register_shapes()
         for k in ("layer_norm", "layer_norm_stats", "layer_norm_backward", "lora", "lora_hidden", "lora_into", "lora_backward"):

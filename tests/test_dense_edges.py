@@ -2,6 +2,10 @@
 
 Values are chosen so that the formula's result is known exactly, or the bound stands beside the check.
 """
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -10,6 +14,9 @@ from torch.autograd import forward_ad
 import spmm_b200 as T
 from spmm_b200 import dense, torch_op
 from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref
+
+
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 
 
 # ------------------------------------------------------------------ precision
@@ -333,3 +340,23 @@ def test_registered_autograd():
     torch.library.opcheck(ops.lora.default, (*leaves, index, scale, base), test_utils=check)
     with torch.no_grad():
         torch.library.opcheck(ops.lora_into.default, (X.detach(), down.detach(), up.detach(), index, scale, base, base.clone()), test_utils=check)
+
+
+# ------------------------------------------------------------------ without the torch operators
+def _make(*args):
+    return subprocess.run(["make", "-C", os.path.join(ROOT, "spmm_b200", "csrc"), *args], capture_output=True, text=True)
+
+
+@pytest.mark.parametrize("python", ["no-such-python", "false"])
+def test_make_without_torch(python):
+    """The C library and the driver need no torch: where $(PYTHON) has none, only the torch operators are left out."""
+    plan = _make("-n", "-B", f"PYTHON={python}")
+    assert plan.returncode == 0, plan.stderr
+    assert "libtcaspmm.so" in plan.stdout and "bin/test" in plan.stdout
+    assert "torch_bind.cpp" not in plan.stdout and "torch_bind.cpp" in _make("-n", "-B", f"PYTHON={sys.executable}").stdout
+
+
+def test_make_torch_says_what_is_missing(tmp_path):
+    """Asked for by name, the torch operators are an error without torch."""
+    got = _make(f"LIB={tmp_path}", "-o", f"{tmp_path}/libtcaspmm.so", "PYTHON=false", "torch")
+    assert got.returncode != 0 and "no torch in false" in got.stderr
