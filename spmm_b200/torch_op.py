@@ -207,7 +207,10 @@ spmm_fused.register_autograd(_backward_fused, setup_context=_setup_fused)
 
 
 # ------------------------------------------- layer norm and low-rank adapters
-dense._op("layer_norm")  # loads the operators
+try:
+    dense._op("layer_norm")  # loads the operators
+except (ImportError, OSError):
+    pass  # not built, or for another torch: the first call says so, and the products above need none of it
 layer_norm = dense.layer_norm
 lora = dense.lora
 

@@ -15,7 +15,6 @@ import spmm_b200 as T
 from spmm_b200 import dense, torch_op
 from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref
 
-
 ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 
 
@@ -360,3 +359,20 @@ def test_make_torch_says_what_is_missing(tmp_path):
     """Asked for by name, the torch operators are an error without torch."""
     got = _make(f"LIB={tmp_path}", "-o", f"{tmp_path}/libtcaspmm.so", "PYTHON=false", "torch")
     assert got.returncode != 0 and "no torch in false" in got.stderr
+
+
+@pytest.mark.parametrize("broken", [False, True])
+def test_import_without_the_torch_operators(tmp_path, broken):
+    """Without libtcaspmm_torch.so, or with one that does not load, torch_op's sparse operators are there; the norm's and the
+    adapters' first call raises."""
+    path = tmp_path / "libtcaspmm_torch.so"
+    if broken:
+        path.write_bytes(b"not a library")
+    code = (f"import spmm_b200.dense as d; d.TORCH_PATH = {str(path)!r}\n"
+            "import torch, spmm_b200.torch_op as t\n"
+            "assert torch.ops.tcaspmm.spmm and torch.ops.tcaspmm.spmm_fused and t.GCNAggregate\n"
+            "for call in (lambda: t.layer_norm(torch.zeros(2, 2)), lambda: t.lora(*[torch.zeros(1, 1, 1)] * 3)):\n"
+            "    try:\n        call()\n    except (ImportError, OSError) as e:\n        assert 'libtcaspmm_torch.so' in str(e)\n"
+            "    else:\n        raise SystemExit('no error')\n")
+    got = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout + got.stderr
