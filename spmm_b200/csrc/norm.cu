@@ -307,19 +307,31 @@ tcaspmm_status forward(const NormParams &p, int dim, cudaStream_t st)
                 constexpr int N = nch.value, ROWS = N * VEC * (int)sizeof(T) <= 16 ? 4 : N * VEC * (int)sizeof(T) <= 32 ? 2 : 1;
                 // One wave of blocks, each with its share of the rows; of the shortest rows, whose weights are few, blocks of
                 // four turns (2^20 x 128 fp32: 162 us, in one wave 203 us; 2^19 x 256 fp16 the other way, 105 and 125 us).
-                if (r.lanes) {
-                    static std::atomic<int> known[2];
-                    const bool whole = r.lanes == 32;
-                    const auto kernel = whole ? norm_rows_fwd<T, VEC, N, ROWS, 32, false> : norm_rows_fwd<T, VEC, N, ROWS, 0, false>;
-                    const long long wave = (long long)resident((const void *)kernel, 256, 0, known[whole]) * sm_count();
+                const auto launch = [&](auto kernel, std::atomic<int> &known) {
+                    const long long wave = (long long)resident((const void *)kernel, 256, 0, known) * sm_count();
                     const long long turns = ceil_div(p.vecs, 256 / r.lanes * ROWS);
                     const long long blocks = std::min(turns, N * VEC <= 4 ? std::max(wave, ceil_div(turns, 4)) : wave);
                     kernel<<<blocks_of(blocks), 256, 0, st>>>(p, r.lanes);
-                } else {
-                    const long long fit = (long long)std::max(1, 1024 / r.threads) * sm_count();
-                    norm_rows_fwd<T, VEC, N, 1, 0, true><<<blocks_of(std::min(p.vecs, fit)), r.threads, 0, st>>>(p, 32);
+                    return launched("layer_norm launch");
+                };
+                if (r.lanes == 32) {
+                    static std::atomic<int> known;
+                    return launch(norm_rows_fwd<T, VEC, N, ROWS, 32, false>, known);
                 }
-                return launched("layer_norm launch");
+                if constexpr (N == 1) {  // a part of a warp: one chunk a thread
+                    if (r.lanes) {
+                        static std::atomic<int> known;
+                        return launch(norm_rows_fwd<T, VEC, N, ROWS, 0, false>, known);
+                    }
+                }
+                if constexpr (N * VEC * 4 >= FWD_MOST) {  // a block: a quarter of the most, or more
+                    if (!r.lanes) {
+                        const long long fit = (long long)std::max(1, 1024 / r.threads) * sm_count();
+                        norm_rows_fwd<T, VEC, N, 1, 0, true><<<blocks_of(std::min(p.vecs, fit)), r.threads, 0, st>>>(p, 32);
+                        return launched("layer_norm launch");
+                    }
+                }
+                return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm: no kernel for rows of %lld", p.n);
             });
         }
     } else {

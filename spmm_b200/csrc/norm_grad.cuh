@@ -332,15 +332,29 @@ tcaspmm_status backward(const NormGradParams &p, int dim, long long *parts, cuda
             return with_chunks<BWD_MOST / VEC>(r.nch, [&](auto nch) {
                 constexpr int N = nch.value;
                 const size_t shared = r.lanes ? sizeof(float) * 2 * r.lanes * VEC * N : 0;
-                if (r.lanes == 32)
+                if (r.lanes == 32) {
                     norm_rows_bwd<T, G, VEC, N, 32, 256><<<(unsigned)grid, 256, shared, st>>>(p, 32);
-                else if (r.lanes)
-                    norm_rows_bwd<T, G, VEC, N, 0, 256><<<(unsigned)grid, 256, shared, st>>>(p, r.lanes);
-                else if (r.threads <= 512)
-                    norm_rows_bwd<T, G, VEC, N, 0, 512><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
-                else
-                    norm_rows_bwd<T, G, VEC, N, 0, 1024><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
-                return launched("layer_norm_backward launch");
+                    return launched("layer_norm_backward launch");
+                }
+                if constexpr (N == 1) {  // a part of a warp: one chunk a thread
+                    if (r.lanes) {
+                        norm_rows_bwd<T, G, VEC, N, 0, 256><<<(unsigned)grid, 256, shared, st>>>(p, r.lanes);
+                        return launched("layer_norm_backward launch");
+                    }
+                }
+                if constexpr (N * VEC * 4 >= BWD_MOST) {  // a block: a quarter of the most, or more
+                    if (!r.lanes && r.threads <= 512) {
+                        norm_rows_bwd<T, G, VEC, N, 0, 512><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
+                        return launched("layer_norm_backward launch");
+                    }
+                }
+                if constexpr (N * VEC == BWD_MOST) {  // more than 512 threads: the most
+                    if (!r.lanes) {
+                        norm_rows_bwd<T, G, VEC, N, 0, 1024><<<(unsigned)grid, r.threads, 0, st>>>(p, 32);
+                        return launched("layer_norm_backward launch");
+                    }
+                }
+                return fail(TCASPMM_ERR_INVALID_ARG, "layer_norm_backward: no kernel for rows of %lld", p.n);
             });
         }
     } else {

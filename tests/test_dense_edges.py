@@ -13,7 +13,8 @@ from torch.autograd import forward_ad
 
 import spmm_b200 as T
 from spmm_b200 import dense, torch_op
-from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref
+from test_dense_ops import BF16, F16, F32, U, close, lora_inputs, lora_ref, test_norm_and_its_gradients as check_norm
+
 
 ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 
@@ -259,6 +260,15 @@ def test_adapted_product_without_gradients_keeps_nothing():
     for a, b in zip(got, T.lora_backward(dY, X, down, up, H, index, adapters.scale)[1:]):
         assert torch.equal(a, b)
     torch_op.clear_plan_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [16, 20, 32, 33, 64, 65, 100, 128, 129, 200, 256, 257, 333, 512, 513, 600, 1025, 1500, 2048, 2049, 3001,
+                                  4096, 4097, 6000, 6001, 8192, 8193, 12001, 16384, 16385])
+@pytest.mark.parametrize("dt,out,pdt", [(F32, F32, F32), (F16, F32, F16), (BF16, BF16, F32)])
+def test_norm_of_every_row_plan(cols, dt, out, pdt):
+    """Widths on both sides of each change of a row's threads and chunks, aligned and odd."""
+    check_norm(5, cols, 1, dt, out, pdt)
 
 
 # ------------------------------------------------------------------ autograd
