@@ -34,6 +34,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <cstring>
 #include <mutex>
 
 #include <cuda_bf16.h>
@@ -74,6 +75,21 @@ struct NoallocParams {
     int cstride;   // floats per carry row (ncols rounded up to 4)
     float *carry;  // device address of g_noalloc_carry
 };
+
+// A nonzero's value.  16-bit ones are loaded as integers: the headers' __ldg of a 16-bit float is an assembly statement without
+// side effects, which the compiler may execute ahead of the condition that guards it, past the end of the caller's array.
+template <typename T>
+__device__ __forceinline__ float load_value(const T *p)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __ldg(p);
+    } else {
+        const unsigned short bits = __ldg(reinterpret_cast<const unsigned short *>(p));
+        T v;
+        memcpy(&v, &bits, 2);
+        return to_f<T>(v);
+    }
+}
 
 // Last row r in [0, M) with row_ptr[r] <= j (rows are empty-tolerant).
 __device__ __forceinline__ int row_of(const int32_t *row_ptr, int M, int j)
@@ -139,7 +155,7 @@ __global__ void __launch_bounds__(256) noalloc_chunks(const NoallocParams p)
             for (int u = 0; u < 8; ++u) {
                 const bool ok = j + u < j1;
                 cc[u] = ok ? __ldg(p.col + j + u) : 0;
-                vv[u] = ok ? to_f<T>(__ldg(val + j + u)) : 0.0f;
+                vv[u] = ok ? load_value(val + j + u) : 0.0f;
             }
             Raw<T, VEC> rb[8];
 #pragma unroll
