@@ -1218,8 +1218,8 @@ __global__ void __launch_bounds__(THREADS, 4) lora_token(const ApplyParams p)
 // R of S.  Columns of other adapters count as zeros in both operands (an infinity there meets a zero nowhere).
 // The blocks' sums are joined through distributed shared memory in a fixed order.  Both products of a backward pass are one
 // launch, dU first: it may start while dX is still being made.  Measured: K = M = 2048, 4096 columns, rank 32, three adapters,
-// bf16 beside fp32 dY: 37 us for both after dX (50 MB); dU alone 23 us, of which a block's look at the indices takes 2 us, its
-// chunks 4 us and the join 3 us, 1.3 blocks in turn for each of an SM's two places.
+// bf16 beside fp32 dY: 52 us for both after dX (50 MB); dU alone, both of whose operands are split, 37 us (23 us when they were
+// rounded to TF32).  The splits take as many issue slots as the rest: 45% of the active cycles are busy, the tensor pipe 20%.
 constexpr int GRAD_ROWS = 128;
 constexpr int GRAD_CHUNK = 32;
 constexpr int GRAD_SCAN = 128;  // chunks looked over at once
@@ -1517,7 +1517,9 @@ tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
 // Where the forward pass goes column by column: up to 64 columns, or 256 where tiles of 64 may hold many adapters, within the
 // work that its reads of the factors from L2 are worth.  Measured (fp16, columns one by one against tiles): 64 columns of 64
 // adapters of rank 16, 4096 x 1024: 9 and 61 us, 256 of them 29 and 80; 64 columns of rank 64, 4096 x 4096, 8 adapters: 40 and
-// 56 us, 128 of them more than 80 and 56; 64 columns of rank 8, 512 x 512, one adapter: 6.2 and 7.7 us, 128 of them 10.8 and 7.5.
+// 56 us, 128 of them more than 80 and 56; 64 columns of rank 8, 512 x 512, one adapter: 6.2 and 7.7 us, 128 of them 10.8 and 7.5.  fp32, whose tiles
+// take longer still: 64 columns of 64 adapters of rank 16, 4096 x 1024: 11 and 132 us; 64 of rank 64, 5120 x 5120, 8 adapters: 41
+// and 194 us, one adapter: 40 and 40 us; 256 columns of 16 adapters of rank 16, 4096 x 2048: 39 and 107 us.
 inline bool by_token(long long L, long long R, long long M, long long K, long long N)
 {
     if (N > 256 || K > 8ll * 8192) return false;

@@ -306,7 +306,7 @@ tcaspmm_status forward(const NormParams &p, int dim, cudaStream_t st)
             return with_chunks<FWD_MOST / VEC>(r.nch, [&](auto nch) {
                 constexpr int N = nch.value, ROWS = N * VEC * (int)sizeof(T) <= 16 ? 4 : N * VEC * (int)sizeof(T) <= 32 ? 2 : 1;
                 // One wave of blocks, each with its share of the rows; of the shortest rows, whose weights are few, blocks of
-                // four turns (2^20 x 128 fp32: 162 us, in one wave 203 us; 2^19 x 256 fp16 the other way, 105 and 125 us).
+                // four turns (2^20 x 128 fp32: 167 us, in one wave a quarter more; 2^19 x 256 fp16 the other way, a fifth more).
                 const auto launch = [&](auto kernel, std::atomic<int> &known) {
                     const long long wave = (long long)resident((const void *)kernel, 256, 0, known) * sm_count();
                     const long long turns = ceil_div(p.vecs, 256 / r.lanes * ROWS);

@@ -13,10 +13,14 @@
 // memory, so that reads stay coalesced along the rows.  The weight's gradient is summed by each thread over the vectors it
 // meets (its features stay the same), by block through shared memory, and over the blocks by a second kernel, in a fixed order.
 //
-// Measured (one B200, whose copy of large arrays reaches 6.5 TB/s): rows, 2^20 x 128 fp32, forward 168 us (6.4 TB/s), backward
-// 259 us (6.2 TB/s); 4096 x 8192 bf16, forward 40 us, backward 65 us; 100003 x 233 fp32 to bf16, whose rows allow no vectors,
-// 35 us (4.0 TB/s; about two thirds of the issue slots busy).  Columns, 4096 x 8192 bf16, forward 42 us (3.2 TB/s), backward
-// 80 us (2.5 TB/s): there the sums, the exchange between blocks and the unpacking of 16-bit elements take as long as memory.
+// Measured (one B200, whose copy of large arrays reaches 6.5 TB/s): rows, 2^20 x 128 fp32, forward 167 us (6.4 TB/s), backward
+// 258 us (6.2 TB/s); 4096 x 8192 bf16, forward 40 us, backward 65 us; 100003 x 233 fp32 to bf16, whose rows allow no vectors,
+// 36 us (3.9 TB/s; about two thirds of the issue slots busy).  Columns, 4096 x 8192 bf16, forward 42 us (3.2 TB/s), backward
+// 82 us (2.5 TB/s): there the sums, the exchange between blocks and the unpacking of 16-bit elements take as long as memory.
+// Wide rows leave a thread 64 registers, which is too few: the backward kernels of 8193 to 16384 elements spill 160 to 376 bytes a
+// thread, with one element a load 464 to 856, and with one element a load the forward kernel spills 168 to 196 from 2049 on.
+// 4096 x 16384 bf16: forward 81 us, backward 159 us; 4096 x 16383: 420 and 1250 us; 4096 x 8191: 196 and 158 us.  Rows past
+// 16384 elements are read two or three times, element by element: 4096 x 20000 bf16, 450 and 1100 us.
 #pragma once
 
 #include <algorithm>
@@ -181,7 +185,7 @@ __device__ __forceinline__ void row_sum(float (&v)[COUNT], int lanes, float (*s)
 //
 // A cluster's block holds its part of a strip's rows in shared memory (asynchronous copies where the rows' alignment allows
 // them, 16 bytes a thread), so that several blocks an SM load, sum and write at the same time: three of 64 KB.  The same
-// strips in registers, one block of 512 threads an SM, took 103 us forward and 123 us backward on 4096 x 8192 bf16 (42 and 80
+// strips in registers, one block of 512 threads an SM, took 103 us forward and 123 us backward on 4096 x 8192 bf16 (42 and 82
 // here), for want of bytes on their way while a block was summing.
 constexpr int STRIP_THREADS = 256;
 constexpr int STRIP_WARPS = STRIP_THREADS / 32;
