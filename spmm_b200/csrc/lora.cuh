@@ -216,6 +216,7 @@ __device__ __forceinline__ void split16(float x, T (&part)[PARTS<T>])
 //    times the other, and the one times the other's parts is finite or the same infinity.
 //  - Beside a whole one v is the next value below |x|, cut, so that lo has x's sign and is zero only where x is (up to 2^-22 |x|):
 //    an infinite whole operand times each part is what it is times x.  An infinity is v beside the largest finite lo, a NaN is v.
+//    (The last four values below fp32's end may round to infinity.)
 template <bool SPLIT> struct Operand;
 template <> struct Operand<false> {
     unsigned v;
@@ -233,11 +234,9 @@ __device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T
         if constexpr (!IS_SPLIT<T>) {
             o[i].v = __float_as_uint(to_float(x[i]));
         } else if constexpr (BOTH) {
-            const unsigned b = __float_as_uint(x[i]);
-            unsigned v = b;
-            if (fabsf(x[i]) < 3.402e38f) v += 0x1000u;  // beyond: cut, it would round to infinity
-            v &= 0xffffe000u;
-            unsigned lo = __float_as_uint(x[i] - __uint_as_float(v)) + 0x1000u;
+            const unsigned b = __float_as_uint(x[i]), half = fabsf(x[i]) < 3.402e38f ? 0x1000u : 0u;  // beyond: cut, not past infinity
+            unsigned v = (b + half) & 0xffffe000u;
+            unsigned lo = __float_as_uint(x[i] - __uint_as_float(v)) + half;
             if (!(fabsf(x[i]) <= FLT_MAX)) {
                 v = (b & 0x80000000u) | 0x3f800000u;
                 lo = __float_as_uint(x[i] + x[i]);  // a NaN's payload may lie in the bits that are ignored

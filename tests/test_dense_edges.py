@@ -187,6 +187,20 @@ def test_fp16_intermediate_beside_an_infinity_and_at_the_end_of_the_range(hidden
         assert float(lora(torch.ones(1, 1).half().cuda(), one, one, None, torch.tensor([2.0 ** e]).cuda())) == 2.0 ** e
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [False, True])
+def test_fp32_values_at_the_end_of_the_range(hidden):
+    """The largest values stay finite (both parts are cut there), beside ones that do not reach them: 2^-21 for each of two
+    products and a cut, 2^-23, for each of three instructions: 2 (2^-21 + 3 2^-23) < 2^-19."""
+    most = torch.finfo(F32).max
+    X = torch.tensor([[most, -most, 3.4e38, 1.0]]).cuda()
+    for down, up in ((1.0, 1.0), (0.25, 4.0), (-1.0, 1.0)):
+        Y = T.lora(X, torch.full((1, 1, 1), down).cuda(), torch.full((1, 1, 1), up).cuda(), hidden=hidden)
+        Y = (Y[0] if hidden else Y).double().cpu()
+        ref = X.double().cpu() * down * up
+        assert bool(((Y - ref).abs() <= 2.0 ** -19 * ref.abs()).all())
+
+
 # ------------------------------------------------------------------ which kernels
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,K,N,R,L", [(96, 72, 64, 16, 64), (130, 96, 200, 8, 40), (61, 35, 256, 5, 16), (40, 50, 65, 3, 33)])
