@@ -234,7 +234,8 @@ __device__ __forceinline__ void operands(const T (&x)[COUNT], Operand<IS_SPLIT<T
         if constexpr (!IS_SPLIT<T>) {
             o[i].v = __float_as_uint(to_float(x[i]));
         } else if constexpr (BOTH) {
-            const unsigned b = __float_as_uint(x[i]), half = fabsf(x[i]) < 3.402e38f ? 0x1000u : 0u;  // beyond: cut, not past infinity
+            const unsigned b = __float_as_uint(x[i]);
+            const unsigned half = fabsf(x[i]) < 3.402e38f ? 0x1000u : 0u;  // beyond: cut, not rounded to infinity
             unsigned v = (b + half) & 0xffffe000u;
             unsigned lo = __float_as_uint(x[i] - __uint_as_float(v)) + half;
             if (!(fabsf(x[i]) <= FLT_MAX)) {
@@ -1516,9 +1517,10 @@ tcaspmm_status expand(ApplyParams p, int sms, cudaStream_t st)
 // Where the forward pass goes column by column: up to 64 columns, or 256 where tiles of 64 may hold many adapters, within the
 // work that its reads of the factors from L2 are worth.  Measured (fp16, columns one by one against tiles): 64 columns of 64
 // adapters of rank 16, 4096 x 1024: 9 and 61 us, 256 of them 29 and 80; 64 columns of rank 64, 4096 x 4096, 8 adapters: 40 and
-// 56 us, 128 of them more than 80 and 56; 64 columns of rank 8, 512 x 512, one adapter: 6.2 and 7.7 us, 128 of them 10.8 and 7.5.  fp32, whose tiles
-// take longer still: 64 columns of 64 adapters of rank 16, 4096 x 1024: 11 and 132 us; 64 of rank 64, 5120 x 5120, 8 adapters: 41
-// and 194 us, one adapter: 40 and 40 us; 256 columns of 16 adapters of rank 16, 4096 x 2048: 39 and 107 us.
+// 56 us, 128 of them more than 80 and 56; 64 columns of rank 8, 512 x 512, one adapter: 6.2 and 7.7 us, 128 of them 10.8 and 7.5.
+// fp32, whose tiles take longer still: 64 columns of 64 adapters of rank 16, 4096 x 1024: 11 and 132 us; 64 of rank 64,
+// 5120 x 5120, 8 adapters: 41 and 194 us, one adapter: 40 and 40 us; 256 columns of 16 adapters of rank 16, 4096 x 2048: 39 and
+// 107 us.
 inline bool by_token(long long L, long long R, long long M, long long K, long long N)
 {
     if (N > 256 || K > 8ll * 8192) return false;
